@@ -17,7 +17,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libcoopt_amd.so")
 
 COOPT_OK, COOPT_EINVAL, COOPT_EHIP, COOPT_EWORKSPACE = 0, -1, -2, -3
-DT_F32, DT_BF16, DT_F16, DT_I8 = 0, 1, 2, 3
+DT_F32, DT_BF16, DT_F16, DT_I8, DT_I4 = 0, 1, 2, 3, 4
 
 _i, _i64, _f, _p, _sz = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
 
@@ -72,6 +72,13 @@ SIGNATURES = {
                                          _i64, _i64, _i64, _p, _i64, _p, _p, _i, _i, _i, _i, _i,
                                          _i64, _i, _i, _i64, _f, _p, _i64, _i64, _p, _sz, _p]),
     "coopt_verify_attention_window_rows": (_i, [_i, _i, _i, _i, _i, _i, _i, _i64]),
+    "coopt_qkv_norm_epilogue": (_i, [_i, _p, _i64, _p, _i, _i64, _p, _p, _f, _p, _p, _p, _i64, _i,
+                                     _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64,
+                                     _i64, _p, _i, _i, _i, _i, _i, _i64, _p]),
+    "coopt_window_attention_workspace": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i]),
+    "coopt_window_attention": (_i, [_i, _p, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64,
+                                    _i64, _i64, _p, _i64, _p, _p, _i, _i, _i, _i, _i, _i64, _i,
+                                    _i, _i64, _i, _i, _f, _p, _i64, _i64, _p, _sz, _p]),
     "coopt_accept_sample_workspace": (_sz, [_i, _i, _i]),
     "coopt_accept_sample": (_i, [_i, _p, _i64, _p, _i, _p, _i64, _p, _p, _p, _p, _p, _f, _i, _i,
                                  _i, _p, _p, _p, _p, _sz, _p]),
@@ -173,6 +180,26 @@ def require_cuda(*tensors):
         if t is not None and not t.is_cuda:
             raise CooptError("libcoopt_amd.so kernels take device tensors; got a CPU tensor "
                              "(there is no CPU fallback)")
+
+
+def require_one_device(*tensors):
+    """The device of the tensors, which must be one GPU (None entries are skipped)."""
+    require_cuda(*tensors)
+    dev = None
+    for t in tensors:
+        if t is not None:
+            if dev is not None and t.device != dev:
+                raise ValueError(f"tensors are on {dev} and {t.device}; one device is needed")
+            dev = t.device
+    return dev
+
+
+def call_on(dev, fn, *args):
+    """fn(*args) with `dev` the current device, on which the library launches."""
+    if dev.index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
 
 
 class WorkspaceCache:

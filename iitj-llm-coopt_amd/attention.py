@@ -15,6 +15,12 @@ max_seqlen_q <= 64 (speculative verify and decode), take the tuned path; longer 
 prefill chunks engine/engine.py:414-420 mixes into the same batch) run in query windows of
 64/(Hq/Hkv) rows, one block per window and KV head -- or, where the batch has windows enough to fill
 the GPU, of 128/(Hq/Hkv) rows in a kernel that stages K and V in LDS for the window's rows.
+
+window=W limits a query at position p to the keys above p - W, beside the first sink_tokens keys
+of its sequence, which stay visible (attention sinks): key k is seen iff k <= p and (k > p - W or
+k < sink_tokens).  Pages without a visible key are not read, so they may be freed and reused.
+INT4 caches (reshape_and_cache_flash(..., "int4")) are attended over as INT8 ones, with or
+without a window; their keys and values are code * scale, unrounded.
 """
 import functools
 import math
@@ -25,7 +31,7 @@ import torch
 from . import _lib
 
 __all__ = ["flash_attn_varlen_func", "paged_attention", "paged_attention_qkv",
-           "qkv_attention_supported", "workspace_bytes"]
+           "qkv_attention_supported", "window_workspace_bytes", "workspace_bytes"]
 
 _WS = _lib.WorkspaceCache()
 
@@ -43,9 +49,39 @@ def workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, head_dim: int
                                                   max_seqlen_q, max_seqlen_k)))
 
 
+@functools.lru_cache(maxsize=1024)
+def _window_workspace_bytes(*sizes):
+    return int(_lib.load().coopt_window_attention_workspace(*sizes))
+
+
+def _window_args(window, sink_tokens, max_seqlen_k):
+    """(window, sink_tokens) as the library takes them: 0 for no window, and neither past
+    max_seqlen_k, where a larger one sees no other keys."""
+    sinks = operator.index(sink_tokens)
+    if sinks < 0:
+        raise ValueError(f"sink_tokens must not be negative, got {sinks}")
+    if window is None:
+        if sinks:
+            raise ValueError("sink_tokens needs a window (without one every key is visible)")
+        return 0, 0
+    window = operator.index(window)
+    if window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    return min(window, max_seqlen_k), min(sinks, max_seqlen_k)
+
+
+def window_workspace_bytes(batch: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                           max_seqlen_q: int, max_seqlen_k: int, window=None,
+                           sink_tokens: int = 0) -> int:
+    """Bytes paged_attention needs with a window or over INT4 caches."""
+    sizes = tuple(map(operator.index, (batch, num_heads, num_kv_heads, head_dim, max_seqlen_q,
+                                       max_seqlen_k)))
+    return _window_workspace_bytes(*sizes, *_window_args(window, sink_tokens, sizes[-1]))
+
+
 def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, max_seqlen_q,
                     max_seqlen_k, softmax_scale=None, k_scale=None, v_scale=None, out=None,
-                    workspace=None):
+                    workspace=None, window=None, sink_tokens=0):
     """out [T, Hq, D] bf16 = causal paged attention; see the module docstring."""
     _lib.require_cuda(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table)
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(-1) != 1:
@@ -55,7 +91,8 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
             k_cache.dim() != 4 or k_cache.stride(-1) != 1:
         raise ValueError("k/v caches must be [num_blocks, block_size, Hkv, D] alike")
     NB, bs, Hkv, cD = k_cache.shape
-    if cD != D or Hq % Hkv:
+    int4 = k_cache.dtype == torch.uint8
+    if cD * (2 if int4 else 1) != D or Hq % Hkv:
         raise ValueError(f"q {tuple(q.shape)} does not match cache {tuple(k_cache.shape)}")
     B = seq_lens.numel()
     if cu_seqlens_q.numel() != B + 1:
@@ -68,18 +105,22 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
         raise ValueError("block_table must be [batch, width] int32, row-major")
     if k_cache.dtype == torch.bfloat16:
         code, ks, vs, sstr = _lib.DT_BF16, None, None, (0, 0, 0)
-    elif k_cache.dtype == torch.int8:
+    elif k_cache.dtype == torch.int8 or int4:
         if k_scale is None or v_scale is None:
-            raise ValueError("INT8 caches need k_scale and v_scale")
+            raise ValueError(f"{'INT4' if int4 else 'INT8'} caches need k_scale and v_scale")
         if k_scale.shape != (NB, bs, Hkv) or k_scale.dtype != torch.float16 or \
                 v_scale.shape != k_scale.shape or v_scale.stride() != k_scale.stride():
             raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
         _lib.require_cuda(k_scale, v_scale)
-        code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
+        code, ks, vs, sstr = _lib.DT_I4 if int4 else _lib.DT_I8, k_scale, v_scale, k_scale.stride()
     else:
         raise ValueError(f"unsupported cache dtype {k_cache.dtype}")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
+    if int4 or window is not None or sink_tokens:
+        return _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table,
+                                 int(max_seqlen_q), int(max_seqlen_k), float(softmax_scale), code, ks,
+                                 vs, sstr, out, workspace, window, sink_tokens)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
     elif out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
@@ -104,6 +145,50 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
         _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(workspace),
         workspace.numel() * workspace.element_size(), _lib.stream_handle(q.device)),
         "coopt_verify_attention")
+    return out
+
+
+def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, max_seqlen_q,
+                      max_seqlen_k, softmax_scale, code, ks, vs, sstr, out, workspace, window,
+                      sink_tokens):
+    """paged_attention's call with a window or over INT4 caches, its arguments checked there."""
+    T, Hq, D = q.shape
+    NB, bs, Hkv, _ = k_cache.shape
+    B = seq_lens.numel()
+    if v_cache.dtype != k_cache.dtype or (vs is not None and vs.dtype != torch.float16):
+        raise ValueError("k and v caches and their scales must be of one type")
+    if out is not None and (out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or
+                            out.stride(-1) != 1):
+        raise ValueError("out must be bf16 [T, Hq, D] with contiguous D")
+    if block_table.shape[1] * bs < max_seqlen_k:
+        raise ValueError(f"block_table holds {block_table.shape[1]} blocks of {bs} tokens a sequence, "
+                         f"max_seqlen_k is {max_seqlen_k}")
+    win, sinks = _window_args(window, sink_tokens, max_seqlen_k)
+    dev = _lib.require_one_device(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ks, vs,
+                                  out, workspace)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    if B == 0 or T == 0:
+        return out
+    need = _window_workspace_bytes(B, Hq, Hkv, D, max_seqlen_q, max_seqlen_k, win, sinks)
+    if workspace is None:
+        # a graph under capture gets a workspace of its own (from its memory pool), so that two
+        # graphs captured on one stream may replay at the same time
+        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev) \
+            if torch.cuda.is_current_stream_capturing() else _WS.get(need, dev)
+    elif workspace.numel() * workspace.element_size() < need:
+        raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} "
+                         f"bytes, {need} needed")
+    cu, sl = cu_seqlens_q.contiguous(), seq_lens.contiguous()
+    cs = k_cache.stride()
+    _lib.check(_lib.call_on(
+        dev, _lib.load().coopt_window_attention, code, _lib.ptr(q), q.stride(0), q.stride(1),
+        _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs),
+        sstr[0], sstr[1], sstr[2], _lib.ptr(block_table), block_table.stride(0), _lib.ptr(cu),
+        _lib.ptr(sl), B, Hq, Hkv, D, bs, NB, max_seqlen_q, max_seqlen_k, T, win, sinks,
+        softmax_scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(workspace),
+        workspace.numel() * workspace.element_size(), _lib.stream_handle(dev)),
+        "coopt_window_attention")
     return out
 
 
@@ -211,12 +296,15 @@ def paged_attention_qkv(qkv, positions, cos, sin, slot_mapping, k_cache, v_cache
 
 def flash_attn_varlen_func(q, k, v, cu_seqlens_q, max_seqlen_q, seqused_k, max_seqlen_k,
                            softmax_scale=None, causal=True, block_table=None, fa_version=2,
-                           k_scale=None, v_scale=None, out=None, workspace=None):
-    """Keyword-compatible with the vLLM call the reference makes (engine/model.py:244-247)."""
+                           k_scale=None, v_scale=None, out=None, workspace=None, window=None,
+                           sink_tokens=0):
+    """Keyword-compatible with the vLLM call the reference makes (engine/model.py:244-247);
+    window / sink_tokens as in the module docstring."""
     if not causal:
         raise ValueError("only causal=True is supported (the reference always passes it)")
     if block_table is None:
         raise ValueError("block_table is required: this is the paged-KV path")
     del fa_version
     return paged_attention(q, k, v, cu_seqlens_q, seqused_k, block_table, max_seqlen_q,
-                           max_seqlen_k, softmax_scale, k_scale, v_scale, out, workspace)
+                           max_seqlen_k, softmax_scale, k_scale, v_scale, out, workspace, window,
+                           sink_tokens)

@@ -24,6 +24,11 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 // Checks hipGetLastError() after a launch; records the message on failure.
 int check_launch(const char* what);
 
+// What a cache-writing entry point refuses in its cache arguments, or null (abi.hip).
+const char* cache_write_error(int cache_dtype, const void* k_cache, const void* v_cache,
+                              int64_t c_blk_stride, int64_t c_tok_stride, int64_t c_head_stride,
+                              const void* k_scale, const void* v_scale);
+
 }  // namespace coopt
 
 #define COOPT_REQUIRE(cond, msg)                                 \
@@ -33,6 +38,10 @@ int check_launch(const char* what);
       return COOPT_EINVAL;                                       \
     }                                                            \
   } while (0)
+
+// What a paged cache holds, as the kernels' template argument (kBf16 / kI8 are also the values
+// of the bool INT8 that kernels of those two take).
+constexpr int kBf16 = 0, kI8 = 1, kI4 = 2;
 
 // ---------------------------------------------------------------------------------------
 // Device side: number formats.  bf16 values travel as raw uint16_t bit patterns.
@@ -209,6 +218,20 @@ __device__ __forceinline__ uint32_t group_max_u32(uint32_t v) {
     const u32x2_pl_t r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     v = mx(r[0], r[1]);
   }
+  return v;
+}
+
+// Sum over aligned groups of `G` lanes, every lane of a group the same bits (each step adds a
+// lane's value to its partner's).
+template <int G>
+__device__ __forceinline__ float group_sum_f32(float v) {
+  static_assert(G >= 1 && G <= 64 && (G & (G - 1)) == 0, "G must be a power of two <= 64");
+  if constexpr (G >= 2) v += dpp_f32<dpp::kXor1>(v);
+  if constexpr (G >= 4) v += dpp_f32<dpp::kXor2>(v);
+  if constexpr (G >= 8) v += dpp_f32<dpp::kRowHalfMirror>(v);
+  if constexpr (G >= 16) v += dpp_f32<dpp::kRowMirror>(v);
+  if constexpr (G >= 32) v = add_xor16(v);
+  if constexpr (G >= 64) v = add_xor32(v);
   return v;
 }
 

@@ -13,7 +13,7 @@
 
 namespace {
 
-template <int G, bool INT8>
+template <int G, int KV>
 __global__ __launch_bounds__(256) void kv_write_kernel(
     const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t k_ts, int64_t k_hs,
     int64_t v_ts, int64_t v_hs, void* __restrict__ kc, void* __restrict__ vc, int64_t c_bs, int64_t c_ts, int64_t c_hs,
@@ -39,8 +39,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   const int64_t blk = bs_shift >= 0 ? slot >> bs_shift : slot / block_size;
   const int64_t off = bs_shift >= 0 ? slot & ((int64_t{1} << bs_shift) - 1) : slot % block_size;
 
-  const int64_t c_off = blk * c_bs + off * c_ts + h * c_hs + c * 8;
-  store_kv_chunk<G, INT8>(kr, vr, kc, vc, c_off, ks, vs, blk * s_bs + off * s_ts + h * s_hs, c);
+  const int64_t c_off = blk * c_bs + off * c_ts + h * c_hs + c * chunk_step<KV>();
+  store_kv_chunk<G, KV>(kr, vr, kc, vc, c_off, ks, vs, blk * s_bs + off * s_ts + h * s_hs, c);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -118,7 +118,7 @@ struct QkvChunk {
   }
 };
 
-template <int G, bool INT8, int KS>
+template <int G, int KV, int KS>
 __global__ __launch_bounds__(256) void qkv_epilogue_kernel(QkvArgs a) {
   // grid: x covers T tokens x G lanes (32-bit, checked by the host), y the q / k head
   const int lid = static_cast<int>(blockIdx.x) * 256 + static_cast<int>(threadIdx.x);
@@ -146,11 +146,12 @@ __global__ __launch_bounds__(256) void qkv_epilogue_kernel(QkvArgs a) {
   const uint4 vr = vc.get(a);
   const int64_t blk = a.bs_shift >= 0 ? slot >> a.bs_shift : slot / a.block_size;
   const int64_t off = a.bs_shift >= 0 ? slot & ((int64_t{1} << a.bs_shift) - 1) : slot % a.block_size;
-  store_kv_chunk<G, INT8>(yr, vr, a.kc, a.vc, blk * a.c_bs + off * a.c_ts + hk * a.c_hs + c * 8,
-                          a.k_scale, a.v_scale, blk * a.s_bs + off * a.s_ts + hk * a.s_hs, c);
+  store_kv_chunk<G, KV>(yr, vr, a.kc, a.vc,
+                        blk * a.c_bs + off * a.c_ts + hk * a.c_hs + c * chunk_step<KV>(),
+                        a.k_scale, a.v_scale, blk * a.s_bs + off * a.s_ts + hk * a.s_hs, c);
 }
 
-template <bool INT8>
+template <int KV>
 int launch_kv_write(int G, const uint16_t* k, const uint16_t* v, int64_t k_ts, int64_t k_hs,
                     int64_t v_ts, int64_t v_hs, void* kc, void* vc, int64_t c_bs, int64_t c_ts, int64_t c_hs, uint16_t* ks,
                     uint16_t* vs, int64_t s_bs, int64_t s_ts, int64_t s_hs, const int64_t* slot,
@@ -161,7 +162,7 @@ int launch_kv_write(int G, const uint16_t* k, const uint16_t* v, int64_t k_ts, i
   const int bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1;
 #define COOPT_KVW(GV)                                                                         \
   case GV:                                                                                    \
-    hipLaunchKernelGGL((kv_write_kernel<GV, INT8>), grid, dim3(256), 0, stream, k, v, k_ts, k_hs, \
+    hipLaunchKernelGGL((kv_write_kernel<GV, KV>), grid, dim3(256), 0, stream, k, v, k_ts, k_hs, \
                        v_ts, v_hs, kc, vc, c_bs, c_ts, c_hs, ks, vs, s_bs, s_ts, s_hs, slot, T, \
                        bs_shift, block_size, num_slots);                                      \
     break;
@@ -876,8 +877,8 @@ extern "C" int coopt_qkv_epilogue(int cache_dtype, const void* qkv, int64_t qkv_
                                   int Hq, int Hkv, int D, int block_size, int64_t num_blocks,
                                   coopt_stream_t stream) {
   coopt::clear_error();
-  COOPT_REQUIRE(cache_dtype == COOPT_DT_BF16 || cache_dtype == COOPT_DT_I8,
-                "cache_dtype must be COOPT_DT_BF16 or COOPT_DT_I8");
+  COOPT_REQUIRE(cache_dtype == COOPT_DT_BF16 || cache_dtype == COOPT_DT_I8 || cache_dtype == COOPT_DT_I4,
+                "cache_dtype must be COOPT_DT_BF16, COOPT_DT_I8 or COOPT_DT_I4");
   COOPT_REQUIRE(T >= 0 && Hq > 0 && Hkv > 0 && block_size > 0 && num_blocks > 0 && max_pos > 0,
                 "bad sizes");
   COOPT_REQUIRE(D == 64 || D == 128 || D == 256, "D must be 64, 128 or 256");
@@ -900,17 +901,11 @@ extern "C" int coopt_qkv_epilogue(int cache_dtype, const void* qkv, int64_t qkv_
                 "cos/sin rows must be 16-byte aligned with at least D/2 entries");
   COOPT_REQUIRE(coopt::aligned16(q_out) && q_tok_stride % 8 == 0 && q_head_stride % 8 == 0,
                 "q_out rows must be 16-byte aligned");
-  const bool int8 = cache_dtype == COOPT_DT_I8;
-  if (int8) {
-    COOPT_REQUIRE(k_scale && v_scale, "INT8 cache needs k_scale and v_scale");
-    COOPT_REQUIRE((reinterpret_cast<uintptr_t>(k_cache) & 7u) == 0 &&
-                      (reinterpret_cast<uintptr_t>(v_cache) & 7u) == 0 && c_blk_stride % 8 == 0 &&
-                      c_tok_stride % 8 == 0 && c_head_stride % 8 == 0,
-                  "INT8 cache rows must be 8-byte aligned");
-  } else {
-    COOPT_REQUIRE(coopt::aligned16(k_cache) && coopt::aligned16(v_cache) &&
-                      c_blk_stride % 8 == 0 && c_tok_stride % 8 == 0 && c_head_stride % 8 == 0,
-                  "bf16 cache rows must be 16-byte aligned");
+  const bool int8 = cache_dtype == COOPT_DT_I8, int4 = cache_dtype == COOPT_DT_I4;
+  if (const char* bad = coopt::cache_write_error(cache_dtype, k_cache, v_cache, c_blk_stride, c_tok_stride,
+                                                 c_head_stride, k_scale, v_scale)) {
+    coopt::set_error(std::string(__func__) + ": " + bad);
+    return COOPT_EINVAL;
   }
   QkvArgs a{static_cast<const uint16_t*>(qkv), qkv_tok_stride, part, ks, slice_stride, positions,
             static_cast<const uint16_t*>(cos), static_cast<const uint16_t*>(sin), table_stride,
@@ -929,8 +924,9 @@ extern "C" int coopt_qkv_epilogue(int cache_dtype, const void* qkv, int64_t qkv_
   const int kbound = kb <= 8 ? kb : 0;
 #define COOPT_QKV_KS(GV, KSV)                                                                   \
   case KSV:                                                                                     \
-    if (int8) hipLaunchKernelGGL((qkv_epilogue_kernel<GV, true, KSV>), grid, dim3(256), 0, st, a); \
-    else hipLaunchKernelGGL((qkv_epilogue_kernel<GV, false, KSV>), grid, dim3(256), 0, st, a);    \
+    if (int4) hipLaunchKernelGGL((qkv_epilogue_kernel<GV, kI4, KSV>), grid, dim3(256), 0, st, a); \
+    else if (int8) hipLaunchKernelGGL((qkv_epilogue_kernel<GV, kI8, KSV>), grid, dim3(256), 0, st, a); \
+    else hipLaunchKernelGGL((qkv_epilogue_kernel<GV, kBf16, KSV>), grid, dim3(256), 0, st, a);    \
     break;
 #define COOPT_QKV(GV)          \
   case GV:                     \
@@ -960,8 +956,8 @@ extern "C" int coopt_kv_write(int cache_dtype, const void* k, const void* v, int
                               int64_t s_tok_stride, int64_t s_head_stride,
                               const int64_t* slot_mapping, int T, int Hkv, int D, int block_size,
                               int64_t num_blocks, coopt_stream_t stream) {
-  COOPT_REQUIRE(cache_dtype == COOPT_DT_BF16 || cache_dtype == COOPT_DT_I8,
-                "cache_dtype must be COOPT_DT_BF16 or COOPT_DT_I8");
+  COOPT_REQUIRE(cache_dtype == COOPT_DT_BF16 || cache_dtype == COOPT_DT_I8 || cache_dtype == COOPT_DT_I4,
+                "cache_dtype must be COOPT_DT_BF16, COOPT_DT_I8 or COOPT_DT_I4");
   COOPT_REQUIRE(T >= 0 && Hkv > 0 && block_size > 0 && num_blocks > 0, "bad sizes");
   COOPT_REQUIRE(D % 8 == 0 && D >= 8 && D <= 512 && ((D / 8) & (D / 8 - 1)) == 0,
                 "D must be 8 * a power of two, at most 512");
@@ -970,37 +966,22 @@ extern "C" int coopt_kv_write(int cache_dtype, const void* k, const void* v, int
   COOPT_REQUIRE(coopt::aligned16(k) && coopt::aligned16(v) && k_tok_stride % 8 == 0 &&
                     k_head_stride % 8 == 0 && v_tok_stride % 8 == 0 && v_head_stride % 8 == 0,
                 "k/v rows must be 16-byte aligned (strides multiples of 8 elements)");
-  const bool int8 = cache_dtype == COOPT_DT_I8;
-  if (int8) {
-    COOPT_REQUIRE(k_scale && v_scale, "INT8 cache needs k_scale and v_scale");
-    COOPT_REQUIRE((reinterpret_cast<uintptr_t>(k_cache) & 7u) == 0 &&
-                      (reinterpret_cast<uintptr_t>(v_cache) & 7u) == 0 && c_blk_stride % 8 == 0 &&
-                      c_tok_stride % 8 == 0 && c_head_stride % 8 == 0,
-                  "INT8 cache rows must be 8-byte aligned");
-    COOPT_REQUIRE((reinterpret_cast<uintptr_t>(k_scale) & 1u) == 0 &&
-                      (reinterpret_cast<uintptr_t>(v_scale) & 1u) == 0,
-                  "scales must be 2-byte aligned");
-  } else {
-    COOPT_REQUIRE(coopt::aligned16(k_cache) && coopt::aligned16(v_cache) &&
-                      c_blk_stride % 8 == 0 && c_tok_stride % 8 == 0 && c_head_stride % 8 == 0,
-                  "bf16 cache rows must be 16-byte aligned");
+  if (const char* bad = coopt::cache_write_error(cache_dtype, k_cache, v_cache, c_blk_stride, c_tok_stride,
+                                                 c_head_stride, k_scale, v_scale)) {
+    coopt::set_error(std::string(__func__) + ": " + bad);
+    return COOPT_EINVAL;
   }
   coopt::clear_error();
   const int64_t num_slots = num_blocks * block_size;
   auto s = static_cast<hipStream_t>(stream);
   const auto* kp = static_cast<const uint16_t*>(k);
   const auto* vp = static_cast<const uint16_t*>(v);
-  if (int8)
-    return launch_kv_write<true>(D / 8, kp, vp, k_tok_stride, k_head_stride, v_tok_stride,
-                                 v_head_stride, k_cache, v_cache,
-                                 c_blk_stride, c_tok_stride, c_head_stride,
-                                 static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale),
-                                 s_blk_stride, s_tok_stride, s_head_stride, slot_mapping, T, Hkv,
-                                 block_size, num_slots, s);
-  return launch_kv_write<false>(D / 8, kp, vp, k_tok_stride, k_head_stride, v_tok_stride,
-                                v_head_stride, k_cache, v_cache,
-                                c_blk_stride, c_tok_stride, c_head_stride, nullptr, nullptr, 0, 0,
-                                0, slot_mapping, T, Hkv, block_size, num_slots, s);
+  const auto launch = cache_dtype == COOPT_DT_BF16 ? launch_kv_write<kBf16>
+                      : cache_dtype == COOPT_DT_I8 ? launch_kv_write<kI8> : launch_kv_write<kI4>;
+  return launch(D / 8, kp, vp, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride, k_cache,
+                v_cache, c_blk_stride, c_tok_stride, c_head_stride, static_cast<uint16_t*>(k_scale),
+                static_cast<uint16_t*>(v_scale), s_blk_stride, s_tok_stride, s_head_stride,
+                slot_mapping, T, Hkv, block_size, num_slots, s);
 }
 
 extern "C" int coopt_quantize(int bits, int in_dtype, const void* x, int64_t rows, int D, void* q,

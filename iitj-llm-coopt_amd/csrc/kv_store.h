@@ -1,5 +1,6 @@
 // Device helpers shared by the kernels that write the paged KV cache: the symmetric absmax
-// INT8 quantiser, the per-chunk KV store, and neox RoPE on one 16-byte chunk of a head vector.
+// INT8 / INT4 quantiser, the per-chunk KV store, and neox RoPE on one 16-byte chunk of a head
+// vector.
 //
 // Quantisation follows kv_tier_manager.quantize (engine/kv_tier_manager.py:21-31) as torch
 // executes it on a GPU tensor:
@@ -119,25 +120,53 @@ __device__ __forceinline__ QuantPair quant_pair8(const uint4& a, const uint4& b)
   return QuantPair{make_uint4(p0.x, p0.y, p1.x, p1.y), f32_to_f16(s32)};
 }
 
+// Bytes lane c of a group lies past a vector's first in a cache of kind KV, in the units of the
+// cache's strides (elements of 2 bytes, INT8 codes, or bytes of two INT4 codes).
+template <int KV>
+constexpr int chunk_step() { return KV == kI4 ? 4 : 8; }
+
+// The INT4 codes of the group's vector (element e of the chunk in nibble e, offset by +8, as
+// coopt_quantize packs them) at the lane's place, and its fp16 scale.
+template <int G>
+__device__ __forceinline__ void store_chunk_i4(const uint32_t (&w)[4], uint8_t* dst, uint16_t* scale, int c) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+  amax = group_max_u32<G>(amax);
+  const float s32 = quant_scale<7>(bf16_to_f32(static_cast<uint16_t>(amax)));
+  int code[8];
+  quant_codes8<7>(w, s32, code);
+  uint32_t word = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) word |= static_cast<uint32_t>(code[e] + 8) << (4 * e);
+  __builtin_nontemporal_store(word, reinterpret_cast<uint32_t*>(dst));
+  if (c == 0) *scale = f32_to_f16(s32);
+}
+
 // ---------------------------------------------------------------------------------------
 // KV write.  One lane per 16-byte chunk (8 bf16) of a (token, head) vector; G = D/8 lanes
 // (an aligned power-of-two group inside the wave) cover one vector, and each lane handles
 // the same chunk of K and of V, so every load and store is a 16- or 8-byte access.
 // ---------------------------------------------------------------------------------------
 // Lane c of a G-lane group stores elements [8c, 8c + 8) of one (token, head) K and V vector
-// at cache element offset c_off: bf16 as is, or INT8 codes with the group's fp16 scale at
-// s_off (kv_tier_manager.quantize(x, 8) per vector, engine/kv_tier_manager.py:21-31).
+// at cache offset c_off (chunk_step units): bf16 as is, or INT8 / INT4 codes with the group's fp16
+// scale at s_off (kv_tier_manager.quantize(x, 8 or 4) per vector, engine/kv_tier_manager.py:21-31).
 // The K / V words are nontemporal stores (a group writes whole 128- or 256-byte rows).
 // Alternated with plain stores on MI355X: the KV write of 65536 tokens 84.3 -> 69.0 us, the
 // step's fused draft attention launch 16.9 -> 16.4 us, the fused target launch unchanged
 // (its block reads its new keys back after a barrier either way).
-template <int G, bool INT8>
+template <int G, int KV>
 __device__ __forceinline__ void store_kv_chunk(uint4 kr, uint4 vr, void* kc, void* vc,
                                                int64_t c_off, uint16_t* ks, uint16_t* vs,
                                                int64_t s_off, int c) {
   typedef uint32_t u32x4_st __attribute__((ext_vector_type(4)));
   typedef uint32_t u32x2_st __attribute__((ext_vector_type(2)));
-  if constexpr (!INT8) {
+  if constexpr (KV == kI4) {
+    const uint32_t kw[4] = {kr.x, kr.y, kr.z, kr.w};
+    const uint32_t vw[4] = {vr.x, vr.y, vr.z, vr.w};
+    store_chunk_i4<G>(kw, static_cast<uint8_t*>(kc) + c_off, ks + s_off, c);
+    store_chunk_i4<G>(vw, static_cast<uint8_t*>(vc) + c_off, vs + s_off, c);
+  } else if constexpr (KV == kBf16) {
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4_st, kr),
                                 reinterpret_cast<u32x4_st*>(static_cast<uint16_t*>(kc) + c_off));
     __builtin_nontemporal_store(__builtin_bit_cast(u32x4_st, vr),
@@ -167,6 +196,29 @@ __device__ __forceinline__ void store_kv_chunk(uint4 kr, uint4 vr, void* kc, voi
       ks[s_off] = f32_to_f16(ksc);
       vs[s_off] = f32_to_f16(vsc);
     }
+  }
+}
+
+// The same for one vector: its chunk xr at c_off of `cache`, its scale at s_off of `scale`.
+template <int G, int KV>
+__device__ __forceinline__ void store_chunk(uint4 xr, void* cache, int64_t c_off, uint16_t* scale,
+                                            int64_t s_off, int c) {
+  typedef uint32_t u32x4_st __attribute__((ext_vector_type(4)));
+  typedef uint32_t u32x2_st __attribute__((ext_vector_type(2)));
+  const uint32_t w[4] = {xr.x, xr.y, xr.z, xr.w};
+  if constexpr (KV == kBf16) {
+    __builtin_nontemporal_store(__builtin_bit_cast(u32x4_st, xr),
+                                reinterpret_cast<u32x4_st*>(static_cast<uint16_t*>(cache) + c_off));
+  } else if constexpr (KV == kI4) {
+    store_chunk_i4<G>(w, static_cast<uint8_t*>(cache) + c_off, scale + s_off, c);
+  } else {
+    uint32_t amax = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+    const float s32 = quant_scale<127>(bf16_to_f32(static_cast<uint16_t>(group_max_u32<G>(amax))));
+    const uint2 q = quant_pack8_i8(w, s32);
+    __builtin_nontemporal_store(u32x2_st{q.x, q.y}, reinterpret_cast<u32x2_st*>(static_cast<int8_t*>(cache) + c_off));
+    if (c == 0) scale[s_off] = f32_to_f16(s32);
   }
 }
 

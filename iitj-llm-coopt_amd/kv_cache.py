@@ -5,19 +5,22 @@ Drop-in surfaces (reference paths under mohsinmubarak/iitj-llm-coopt):
   reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype, k_scale,
                           v_scale)                         engine/model.py:242-243 (vLLM op)
   qkv_rope_and_cache(qkv, positions, cos, sin, ...)        engine/model.py:238-243 in one launch
+  qkv_norm_rope_and_cache(qkv, q_weight, k_weight, ...)    the same with normed q and k heads
 
 Cache layouts.  bf16 ("auto"): k_cache/v_cache [num_blocks, block_size, Hkv, D] bf16, possibly
 a strided per-layer view of a block-major buffer (engine/elastic.py:74-77).  INT8 ("int8"):
 int8 codes of the same shape plus fp16 scales [num_blocks, block_size, Hkv] passed as
 k_scale/v_scale -- per (token, head) vector, exactly what quantize(cache[blocks], 8) produces
-(engine/kv_tier_manager.py:99; SwappedKV shapes :46-49).
+(engine/kv_tier_manager.py:99; SwappedKV shapes :46-49).  INT4 ("int4"): uint8 [num_blocks,
+block_size, Hkv, D/2], two codes a byte, with the same scales: what quantize(cache[blocks], 4)
+produces.
 """
 import torch
 
 from . import _lib
 
 __all__ = ["quantize", "dequantize", "reshape_and_cache_flash", "allocate_kv_cache",
-           "qkv_rope_and_cache"]
+           "qkv_rope_and_cache", "qkv_norm_rope_and_cache"]
 
 
 def quantize(x: torch.Tensor, bits: int):
@@ -87,7 +90,32 @@ def allocate_kv_cache(num_blocks: int, block_size: int, num_kv_heads: int, head_
                 torch.zeros(store, dtype=torch.int8, device=device).transpose(1, 2),
                 torch.zeros(sstore, dtype=torch.float16, device=device).transpose(1, 2),
                 torch.zeros(sstore, dtype=torch.float16, device=device).transpose(1, 2))
-    raise ValueError(f"kv_cache_dtype must be 'auto' or 'int8', got {kv_cache_dtype!r}")
+    if kv_cache_dtype == "int4":
+        if head_dim % 2:
+            raise ValueError("'int4' caches need an even head_dim")
+        store = (num_blocks, num_kv_heads, block_size, head_dim // 2)
+        # zeros, as in the other caches: two codes of 0, offset by +8
+        return (torch.full(store, 0x88, dtype=torch.uint8, device=device).transpose(1, 2),
+                torch.full(store, 0x88, dtype=torch.uint8, device=device).transpose(1, 2),
+                torch.zeros(store[:3], dtype=torch.float16, device=device).transpose(1, 2),
+                torch.zeros(store[:3], dtype=torch.float16, device=device).transpose(1, 2))
+    raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
+
+
+def _scale_args(k_cache, k_scale, v_scale, kv_cache_dtype):
+    """The strides of the scale caches of an "int8" or "int4" cache, checked."""
+    if k_scale is None or v_scale is None:
+        raise ValueError(f"{kv_cache_dtype!r} caches need k_scale and v_scale scale caches")
+    if k_scale.shape != k_cache.shape[:3] or k_scale.dtype != torch.float16 or \
+            v_scale.dtype != torch.float16 or k_scale.stride() != v_scale.stride() or \
+            v_scale.shape != k_scale.shape:
+        raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
+    return k_scale.stride()
+
+
+def _check_int4(k_cache, v_cache):
+    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+        raise ValueError("'int4' caches hold two codes a byte in uint8")
 
 
 def _check_cache_pair(k_cache, v_cache):
@@ -104,7 +132,7 @@ def reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype
     kv_cache_dtype "auto": bf16 caches, k_scale/v_scale ignored (the reference passes fp32
     ones, engine/model.py:129).  "int8": int8 code caches; k_scale/v_scale are the fp16
     [num_blocks, block_size, Hkv] scale caches and each written vector is quantised in the
-    same kernel.
+    same kernel.  "int4": the same with uint8 caches of two codes a byte.
     """
     _lib.require_cuda(k, v, k_cache, v_cache, slot_mapping)
     _check_cache_pair(k_cache, v_cache)
@@ -114,7 +142,7 @@ def reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype
         raise ValueError("k and v must be bf16")
     T, Hkv, D = k.shape
     NB, bs, cH, cD = k_cache.shape
-    if (cH, cD) != (Hkv, D):
+    if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
         raise ValueError(f"cache heads/dim {(cH, cD)} != k's {(Hkv, D)}")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
         raise ValueError("slot_mapping must be int64 with one entry per token")
@@ -132,8 +160,12 @@ def reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype
                 k_scale.stride() != v_scale.stride() or v_scale.shape != k_scale.shape:
             raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
         code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
+    elif kv_cache_dtype == "int4":
+        _check_int4(k_cache, v_cache)
+        sstr = _scale_args(k_cache, k_scale, v_scale, "int4")
+        code, ks, vs = _lib.DT_I4, k_scale, v_scale
     else:
-        raise ValueError(f"kv_cache_dtype must be 'auto' or 'int8', got {kv_cache_dtype!r}")
+        raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
     _lib.require_cuda(ks, vs)
     lib = _lib.load()
     cs = k_cache.stride()
@@ -170,7 +202,7 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
     _lib.require_cuda(positions, cos, sin, k_cache, v_cache, slot_mapping)
     _check_cache_pair(k_cache, v_cache)
     NB, bs, cH, cD = k_cache.shape
-    if (cH, cD) != (Hkv, D):
+    if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
         raise ValueError(f"cache heads/dim {(cH, cD)} != ({Hkv}, {D})")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
         raise ValueError("slot_mapping must be int64 with one entry per token")
@@ -185,8 +217,13 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
         if k_scale is None or v_scale is None or k_scale.stride() != v_scale.stride():
             raise ValueError("'int8' caches need alike k_scale and v_scale scale caches")
         code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
+    elif kv_cache_dtype == "int4":
+        _check_int4(k_cache, v_cache)
+        sstr = _scale_args(k_cache, k_scale, v_scale, "int4")
+        _lib.require_cuda(k_scale, v_scale)
+        code, ks, vs = _lib.DT_I4, k_scale, v_scale
     else:
-        raise ValueError(f"kv_cache_dtype must be 'auto' or 'int8', got {kv_cache_dtype!r}")
+        raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
     if q_out is None:
         q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
     positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
@@ -200,4 +237,78 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
         _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1],
         sstr[2], _lib.ptr(slot_mapping), T, Hq, Hkv, D, bs, NB,
         _lib.stream_handle(dev)), "coopt_qkv_epilogue")
+    return q_out
+
+
+def qkv_norm_rope_and_cache(qkv, q_weight, k_weight, eps, positions, cos, sin, k_cache, v_cache,
+                            slot_mapping, num_heads, num_kv_heads, head_dim, kv_cache_dtype="auto",
+                            k_scale=None, v_scale=None, q_out=None):
+    """qkv_rope_and_cache for models that norm their query and key heads: in one launch, every q
+    and k head vector x becomes RoPE(x * rsqrt(mean(x^2) + eps) * weight), computed in fp32 and
+    rounded to bf16 once; k and v go to the paged cache and q [T, num_heads, head_dim] is returned.
+
+    q_weight, k_weight: bf16 [head_dim].  `qkv` is the projection's bf16 output [T, (Hq + 2 Hkv) D]
+    or its fused.LinearPartials.  kv_cache_dtype "auto", "int8" or "int4", as in
+    reshape_and_cache_flash; rows with slot < 0 write no cache entry.  head_dim 64, 128 or 256."""
+    from .fused import LinearPartials
+
+    Hq, Hkv, D = int(num_heads), int(num_kv_heads), int(head_dim)
+    width = (Hq + 2 * Hkv) * D
+    part = qkv if isinstance(qkv, LinearPartials) else None
+    if part is not None:
+        if part.n != width:
+            raise ValueError(f"partials are {part.n} wide, expected {width}")
+        T, qkv_t = part.rows, part.buf
+    else:
+        if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
+            raise ValueError(f"qkv must be bf16 [T, {width}] with contiguous rows")
+        T, qkv_t = qkv.shape[0], qkv
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype != torch.bfloat16 or w.shape != (D,) or w.stride(0) != 1:
+            raise ValueError(f"{name} must be bf16 [{D}], contiguous")
+    _check_cache_pair(k_cache, v_cache)
+    NB, bs, cH, cD = k_cache.shape
+    if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
+        raise ValueError(f"cache heads/dim {(cH, cD)} != ({Hkv}, {D})")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
+        raise ValueError("slot_mapping must be int64 with one entry per token")
+    if positions.dtype != torch.int64 or positions.numel() != T:
+        raise ValueError("positions must be int64 with one entry per token")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride() or \
+            cos.shape[0] < 1 or cos.shape[1] < D // 2 or cos.dtype != torch.bfloat16 or \
+            sin.dtype != torch.bfloat16 or cos.stride(1) != 1:
+        raise ValueError("cos/sin tables must be bf16 [max_pos, >= D/2] alike")
+    if kv_cache_dtype == "auto":
+        if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
+            raise ValueError("'auto' caches are bf16")
+        code, ks, vs, sstr = _lib.DT_BF16, None, None, (0, 0, 0)
+    elif kv_cache_dtype in ("int8", "int4"):
+        if kv_cache_dtype == "int4":
+            _check_int4(k_cache, v_cache)
+        elif k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
+            raise ValueError("'int8' caches hold int8 codes")
+        sstr = _scale_args(k_cache, k_scale, v_scale, kv_cache_dtype)
+        code, ks, vs = _lib.DT_I8 if kv_cache_dtype == "int8" else _lib.DT_I4, k_scale, v_scale
+    else:
+        raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
+    if q_out is not None and (q_out.shape != (T, Hq, D) or q_out.dtype != torch.bfloat16 or
+                              q_out.stride(-1) != 1):
+        raise ValueError("q_out must be bf16 [T, Hq, D] with contiguous D")
+    dev = _lib.require_one_device(qkv_t, q_weight, k_weight, positions, cos, sin, k_cache, v_cache,
+                                  slot_mapping, ks, vs, q_out)
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+    if T == 0:
+        return q_out
+    positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
+    cs = k_cache.stride()
+    _lib.check(_lib.call_on(
+        dev, _lib.load().coopt_qkv_norm_epilogue, code, None if part is not None else _lib.ptr(qkv_t),
+        0 if part is not None else qkv_t.stride(0), None if part is None else _lib.ptr(part.buf),
+        0 if part is None else part.ks, 0 if part is None else part.rows_padded * part.n,
+        _lib.ptr(q_weight), _lib.ptr(k_weight), float(eps), _lib.ptr(positions), _lib.ptr(cos),
+        _lib.ptr(sin), cos.stride(0), cos.shape[0], _lib.ptr(q_out), q_out.stride(0),
+        q_out.stride(1), _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks),
+        _lib.ptr(vs), sstr[0], sstr[1], sstr[2], _lib.ptr(slot_mapping), T, Hq, Hkv, D, bs, NB,
+        _lib.stream_handle(dev)), "coopt_qkv_norm_epilogue")
     return q_out

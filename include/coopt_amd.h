@@ -73,7 +73,8 @@ enum {
   COOPT_DT_F32 = 0,
   COOPT_DT_BF16 = 1,
   COOPT_DT_F16 = 2,
-  COOPT_DT_I8 = 3
+  COOPT_DT_I8 = 3,
+  COOPT_DT_I4 = 4 /* caches only: two codes a byte, as coopt_quantize(bits 4) packs them */
 };
 
 /* Message describing the last failed call on this thread ("" if none). */
@@ -93,6 +94,9 @@ int coopt_hip_runtime_version(int* version);
  *                              k_scale/v_scale are fp16 [NB, block_size, Hkv]; each (token, head)
  *                              vector is quantised as kv_tier_manager.quantize(x, 8) does
  *                              (engine/kv_tier_manager.py:21-31), codes and scales bit-exact.
+ *               COOPT_DT_I4:   k_cache/v_cache are uint8 [NB, block_size, Hkv, D/2], two codes a
+ *                              byte, as kv_tier_manager.quantize(x, 4) gives them, with the same
+ *                              fp16 scales; cache strides count bytes, rows 4-byte aligned.
  *   cache strides (c_blk, c_tok, c_head, 1) may describe a strided per-layer view of a
  *   block-major buffer (engine/elastic.py:74-77); scale strides (s_blk, s_tok, s_head).
  *   slot_mapping [T] int64.  A slot < 0 or >= num_blocks * block_size is skipped (padding).
@@ -131,6 +135,28 @@ int coopt_qkv_epilogue(int cache_dtype, const void* qkv, int64_t qkv_tok_stride,
                        int64_t s_tok_stride, int64_t s_head_stride,
                        const int64_t* slot_mapping, int T, int Hq, int Hkv, int D,
                        int block_size, int64_t num_blocks, coopt_stream_t stream);
+
+/*
+ * coopt_qkv_epilogue with the query and key heads normed first, in the same pass: for every
+ * query or key head vector x
+ *   y = x * rsqrt(mean(x^2) + eps) * weight    q_weight / k_weight [D] bf16, one for all heads
+ *   z = RoPE(y)                                as coopt_rope
+ * in fp32 and rounded to bf16 once, after the rotation; v goes to the cache as it is.  No
+ * counterpart in the reference, whose models norm no heads.  INT8 / INT4 caches hold the codes
+ * of the rounded z and v (coopt_kv_write).  The other arguments are coopt_qkv_epilogue's;
+ * partials are reduced and rounded to bf16 before the norm.  D in {64, 128, 256}.
+ */
+int coopt_qkv_norm_epilogue(int cache_dtype, const void* qkv, int64_t qkv_tok_stride,
+                            const float* part, int ks, int64_t slice_stride,
+                            const void* q_weight, const void* k_weight, float eps,
+                            const int64_t* positions, const void* cos, const void* sin,
+                            int64_t table_stride, int max_pos, void* q_out, int64_t q_tok_stride,
+                            int64_t q_head_stride, void* k_cache, void* v_cache,
+                            int64_t c_blk_stride, int64_t c_tok_stride, int64_t c_head_stride,
+                            void* k_scale, void* v_scale, int64_t s_blk_stride,
+                            int64_t s_tok_stride, int64_t s_head_stride,
+                            const int64_t* slot_mapping, int T, int Hq, int Hkv, int D,
+                            int block_size, int64_t num_blocks, coopt_stream_t stream);
 
 /*
  * Symmetric absmax codec over contiguous rows, kv_tier_manager.quantize / dequantize
@@ -289,6 +315,38 @@ int coopt_verify_attention_rows(int kv_dtype,
  * are not cut into windows. */
 int coopt_verify_attention_window_rows(int kv_dtype, int B, int Hq, int Hkv, int D,
                                        int max_seqlen_q, int max_seqlen_k, int64_t total_q);
+
+/*
+ * Paged attention with a sliding window, and over INT4 caches: coopt_verify_attention where query
+ * row j of sequence b, at position p = seq_lens[b] - n_b + j, sees key k iff
+ *   k <= p  and  (k > p - window  or  k < sink_tokens).
+ * No counterpart in the reference.
+ *   window       keys a row sees at most, its own included, beside the first sink_tokens of its
+ *                sequence; 0: all of them (sink_tokens 0 then)
+ *   kv_dtype     COOPT_DT_BF16, COOPT_DT_I8 or COOPT_DT_I4.  INT8 keys are bf16(code * scale), as
+ *                coopt_verify_attention attends over them; INT4 keys and values are code * scale,
+ *                unrounded.  INT4 caches are uint8 [NB, block_size, Hkv, D/2], strides in bytes.
+ *   total_q      query rows of the call (0: unknown); decides how long items are cut, nothing else
+ * Pages that hold no visible key are not read: their block ids may be anything (ids outside the
+ * pool are clamped to it), and what a key or value that a row does not see holds, infinities and NaN
+ * included, does not reach that row.  Rows that see no key are written as zeros.
+ * The other arguments, and the limits on shapes and alignment, are coopt_verify_attention's.
+ */
+size_t coopt_window_attention_workspace(int B, int Hq, int Hkv, int D, int max_seqlen_q,
+                                        int max_seqlen_k, int window, int sink_tokens);
+int coopt_window_attention(int kv_dtype,
+                           const void* q, int64_t q_tok_stride, int64_t q_head_stride,
+                           const void* k_cache, const void* v_cache,
+                           int64_t c_blk_stride, int64_t c_tok_stride, int64_t c_head_stride,
+                           const void* k_scale, const void* v_scale,
+                           int64_t s_blk_stride, int64_t s_tok_stride, int64_t s_head_stride,
+                           const int32_t* block_table, int64_t bt_stride,
+                           const int32_t* cu_seqlens_q, const int32_t* seq_lens,
+                           int B, int Hq, int Hkv, int D, int block_size, int64_t num_blocks,
+                           int max_seqlen_q, int max_seqlen_k, int64_t total_q, int window,
+                           int sink_tokens, float softmax_scale, void* out, int64_t o_tok_stride,
+                           int64_t o_head_stride, void* workspace, size_t workspace_bytes,
+                           coopt_stream_t stream);
 
 /*
  * The qkv epilogue and the verification attention of one layer in one launch: replaces
