@@ -219,7 +219,7 @@ def test_a_step_through_all_of_them(dev):
         K, V = (OC_values(caches[i][blk, off].cpu().numpy(), caches[2 + i][blk, off].cpu().numpy(), "int4")
                 for i in range(2))
         ref, tol = closed_form(q.double().cpu().numpy(), K, V, D ** -0.5, window, sinks, "int4",
-                               caches[2][blk, off].double().cpu().numpy())
+                               caches[2][blk, off].double().cpu().numpy(), caches[3][blk, off].double().cpu().numpy())
         assert (np.abs(out.double().cpu().numpy() - ref) <= tol).all(), n
         # the values of the new tokens are within half a step of a 4-bit code of what came in
         new = x.view(n, Hq + 2 * Hkv, D)[:, Hq + Hkv:].double().cpu().numpy()

@@ -8,7 +8,11 @@ u_p: a probability rounded to 16 bits next to its value (bf16 caches 2^-8; codes
 an INT8 value of the definition is itself rounded to bf16, which the kernel need not do (2^-8).
 ds: the error of a score: a product of D terms summed in fp32 in any order, D 2^-24 sum |q||k|,
 where a 4-bit key enters as code plus 24 (so |k| + 24 s), and 2^-22 of the score for the exponent.
-Both numerator and sum move by ds (2 ds).  2^-18 covers the fp32 sums over up to 2^6 tiles.
+Both numerator and sum move by ds (2 ds).  2^-18 A covers the fp32 sums over up to 2^6 tiles, each
+a rounding of 2^-24 of the magnitudes summed so far.  A 4-bit value is summed as code plus 8, and 8
+times the sum of w s is taken off at the end: the magnitudes summed are |v| + 8 s, not |v| alone, so
+there the last term is 2^-18 sum_k w_k (|v_k| + 8 s_k).  (Where every code of an element is 0, |v| is
+0 and these roundings, up to 64 * 2^-24 * 8 s, are all of the error.)
 """
 import numpy as np
 import pytest
@@ -21,8 +25,9 @@ from oracle import codec as OC
 pytestmark = pytest.mark.gpu
 
 
-def closed_form(q, K, V, scale, window, sinks, kv, s_k):
-    """float64 (out, tol) of one sequence: q [n, Hq, D], K / V [L, Hkv, D], s_k [L, Hkv] or None."""
+def closed_form(q, K, V, scale, window, sinks, kv, s_k, s_v):
+    """float64 (out, tol) of one sequence: q [n, Hq, D], K / V [L, Hkv, D], their scales s_k, s_v
+    [L, Hkv] (None for bf16)."""
     n, Hq, D = q.shape
     L, Hkv, _ = K.shape
     out, tol = np.zeros((n, Hq, D)), np.zeros((n, Hq, D))
@@ -46,7 +51,9 @@ def closed_form(q, K, V, scale, window, sinks, kv, s_k):
                 mag = mag + 24 * s_k[see, g] * np.abs(q[j, h]).sum()
             ds = (D * 2.0 ** -24 * mag * scale).max() + 2.0 ** -22 * np.abs(s).max()
             u_p = {"auto": 2.0 ** -8, "int8": 2.0 ** -11 + 2.0 ** -8, "int4": 2.0 ** -11}[kv]
-            tol[j, h] = 2.0 ** -8 * np.abs(out[j, h]) + (u_p + 2 * ds + 2.0 ** -18) * (w @ np.abs(Vs))
+            A = w @ np.abs(Vs)
+            summed = A + (8 * (w @ s_v[see, g]) if kv == "int4" else 0)
+            tol[j, h] = 2.0 ** -8 * np.abs(out[j, h]) + (u_p + 2 * ds) * A + 2.0 ** -18 * summed
     return out, tol
 
 
@@ -63,7 +70,7 @@ class Setup:
         nb = sum(widths) + 3
         perm = rng.permutation(nb)
         self.table_np = np.full((len(seqs), max(max(widths), 1) + 1), -7, np.int32)
-        self.K, self.V, self.sk = [], [], []
+        self.K, self.V, self.sk, self.sv = [], [], [], []
         store = {"head": (nb, Hkv, bs, D), "token": (nb, bs, Hkv, D), "padded": (nb, bs + 1, Hkv + 2, D + 32)}[layout]
 
         def view(t, last):
@@ -107,8 +114,7 @@ class Setup:
                     v = OC_values(c, s, kv)
                     vals.append(v)
                     s = torch.from_numpy(np.asarray(s, np.float16))
-                    if i == 0:
-                        self.sk.append(s.double().numpy())
+                    (self.sk, self.sv)[i].append(s.double().numpy())
                     if poison:
                         s[torch.from_numpy(hidden)] = float("nan")
                     self.caches[i][blk, off] = torch.from_numpy(c)
@@ -121,6 +127,7 @@ class Setup:
             self.V.append(vals[1])
             if kv == "auto":
                 self.sk.append(None)
+                self.sv.append(None)
 
         def move(t):     # to the GPU with its strides
             if t is None:
@@ -155,7 +162,7 @@ class Setup:
         row, worst = 0, 0.0
         for b, (n, L) in enumerate(self.seqs):
             ref, tol = closed_form(q[row:row + n], self.K[b], self.V[b], self.D ** -0.5, self.window,
-                                   self.sinks, self.kv, self.sk[b])
+                                   self.sinks, self.kv, self.sk[b], self.sv[b])
             d = np.abs(o[row:row + n] - ref)
             assert np.isfinite(o[row:row + n]).all(), f"{note} sequence {b}: not finite"
             if d.size:

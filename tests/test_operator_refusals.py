@@ -36,7 +36,7 @@ def test_window_attention_refuses(lib):
                      (dict(k=None), "null"), (dict(q=8), "aligned"), (dict(qts=4097), "aligned"),
                      (dict(k=8), "aligned"), (dict(cts=520), "aligned"), (dict(ks=None), "k_scale"),
                      (dict(kv=_lib.DT_I8, vs=None), "k_scale"), (dict(ks=17), "k_scale"), (dict(nb=0), "num_blocks"),
-                     (dict(B=70000), "65535"), (dict(B=-1), "Hq")):
+                     (dict(B=70000, wsb=1 << 40), "65535"), (dict(B=-1), "Hq")):
         assert what in refused(attention(lib, **kw)), (kw, _lib.last_error())
     assert attention(lib, B=0) == _lib.COOPT_OK
     assert attention(lib, wsb=8) == _lib.COOPT_EWORKSPACE
