@@ -365,7 +365,7 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
 
 // ---- INT4 operands: the code + 8, n, of a nibble enters a product as 16 + n (K: bf16, exact, n in
 // mantissa bits 3..6) or n 2^-20 (V: fp16, n in bits 4..7 of a subnormal, which the matrix cores
-// take as it is), and the 24 or 8 too much comes off the sums: the score MFMAs' accumulators start
+// take as it is; from bits 0..3, n 2^-24, its products lose their last bits), and the 24 or 8 too much comes off the sums: the score MFMAs' accumulators start
 // at -24 sum_d q[d], and the scale of the key multiplies the score; V's products with the
 // probabilities P' leave 8 sum P' too much, which one more MFMA of P' against ones counts.
 // (Subtracting in the operands instead costs V a packed fp16 add per two values; bf16 has none.)
@@ -393,12 +393,16 @@ __device__ __forceinline__ u32x4_t permute_q8(u32x4_t q) {
   return u32x4_t{(q[0] & 0xffffu) | (q[2] << 16), (q[0] >> 16) | (q[2] & 0xffff0000u),
                  (q[1] & 0xffffu) | (q[3] << 16), (q[1] >> 16) | (q[3] & 0xffff0000u)};
 }
-// n 2^-20 of nibble dt of two keys' dwords, as fp16 (x0's in the low half); hi0 / hi1: the dwords
-// shifted left by 4, whose bytes hold the even nibbles high.
+// n 2^-20 of nibble dt of two keys' dwords as fp16, x0's in the low half; even / odd: i4_nibbles of
+// the dwords.
+struct I4Nibbles {
+  uint32_t even, odd;  // the nibbles in the upper halves of the bytes
+};
+__device__ __forceinline__ I4Nibbles i4_nibbles(uint32_t x) { return {(x << 4) & 0xf0f0f0f0u, x & 0xf0f0f0f0u}; }
 template <int DT>
-__device__ __forceinline__ uint32_t v_pair_i4(uint32_t x0, uint32_t x1, uint32_t hi0, uint32_t hi1) {
+__device__ __forceinline__ uint32_t v_pair_i4(const I4Nibbles& x0, const I4Nibbles& x1) {
   constexpr uint32_t b = DT / 2, sel = 0x0c000c00u | ((4 + b) << 16) | b;
-  return (DT & 1 ? __builtin_amdgcn_perm(x1, x0, sel) : __builtin_amdgcn_perm(hi1, hi0, sel)) & 0x00f000f0u;
+  return DT & 1 ? __builtin_amdgcn_perm(x1.odd, x0.odd, sel) : __builtin_amdgcn_perm(x1.even, x0.even, sel);
 }
 
 
@@ -886,14 +890,14 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     // score phase's registers ----
     u32x4_t va[kDt];
     auto build_va_i4 = [&]() {
-      uint32_t hi[8];
+      I4Nibbles x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) hi[j] = raw.v[j][0] << 4;
+      for (int j = 0; j < 8; ++j) x[j] = i4_nibbles(raw.v[j][0]);
       each<kDt>([&](auto dt) {
         constexpr int DT = decltype(dt)::value;
 #pragma unroll
         for (int e2 = 0; e2 < 4; ++e2)
-          va[DT][e2] = v_pair_i4<DT>(raw.v[2 * e2][0], raw.v[2 * e2 + 1][0], hi[2 * e2], hi[2 * e2 + 1]);
+          va[DT][e2] = v_pair_i4<DT>(x[2 * e2], x[2 * e2 + 1]);
       });
     };
     auto build_va = [&]() {
@@ -1702,15 +1706,15 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
     if constexpr (INT4) {
       // the codes themselves (64 + n less 72: exact in fp16); every wave reads them, so the bias
       // comes off here
-      uint32_t hi[4];
+      I4Nibbles x[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) hi[j] = vx[j][0] << 4;
+      for (int j = 0; j < 4; ++j) x[j] = i4_nibbles(vx[j][0]);
       each<kDt>([&](auto dt) {
         constexpr int DT = decltype(dt)::value;
         u32x2_t va;
 #pragma unroll
         for (int e2 = 0; e2 < 2; ++e2) {
-          const uint32_t n = v_pair_i4<DT>(vx[2 * e2][0], vx[2 * e2 + 1][0], hi[2 * e2], hi[2 * e2 + 1]) | 0x54005400u;
+          const uint32_t n = v_pair_i4<DT>(x[2 * e2], x[2 * e2 + 1]) | 0x54005400u;
           va[e2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(f16x2_t, n) - f16x2_t{72.0f16, 72.0f16});
         }
         vd[DT * 128] = va;

@@ -31,6 +31,7 @@ extern "C" int coopt_window_attention(
   coopt::clear_error();
   COOPT_REQUIRE(window >= 0 && sink_tokens >= 0, "window and sink_tokens must not be negative");
   COOPT_REQUIRE(window > 0 || sink_tokens == 0, "sink_tokens needs a window");
+  COOPT_REQUIRE(softmax_scale >= 0.0f && softmax_scale < 1e30f, "softmax_scale must be finite and not negative");
   // positions, windows and tile ends stay inside 32 bits
   COOPT_REQUIRE(max_seqlen_q < (1 << 29) && max_seqlen_k < (1 << 30), "max_seqlen_q/k out of range");
   return attention_impl<true>("coopt_window_attention", nullptr, clamp_window(window, max_seqlen_k),

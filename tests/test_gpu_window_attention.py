@@ -12,7 +12,8 @@ Both numerator and sum move by ds (2 ds).  2^-18 A covers the fp32 sums over up 
 a rounding of 2^-24 of the magnitudes summed so far.  A 4-bit value is summed as code plus 8, and 8
 times the sum of w s is taken off at the end: the magnitudes summed are |v| + 8 s, not |v| alone, so
 there the last term is 2^-18 sum_k w_k (|v_k| + 8 s_k).  (Where every code of an element is 0, |v| is
-0 and these roundings, up to 64 * 2^-24 * 8 s, are all of the error.)
+0 and these roundings, up to 64 * 2^-24 * 8 s, are all of the error.)  Its operand is a subnormal
+number of the matrix cores, whose products keep 2^-20 of the largest: four such tiles make 2^-18.
 """
 import numpy as np
 import pytest
@@ -289,6 +290,36 @@ def test_scores_far_apart_and_large_scales(dev, kv):
         if mag == 1000.0:     # keep scores in range: only the values are large
             s.q.mul_(1e-3)
         s.check(s.run(), f"magnitude {mag}")
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("magnitude", [0.0, 1e-30, 1e6])
+def test_queries_of_any_magnitude(dev, kv, magnitude):
+    """Queries of zeros (every visible key weighs the same), of tiny numbers, and so large that one
+    key takes all the weight (scores up to 10^7; the call takes them below 2^30, where the rounded
+    maximum of a row is still within a softmax exponent of the score itself)."""
+    for seqs in ([(2, 300), (1, 40)], [(50, 300)]):
+        s = Setup(dev, seqs, 8, 2, 128, kv, 100, 4, seed=6)
+        s.q.mul_(magnitude)
+        if magnitude < 1:
+            s.check(s.run(), f"queries times {magnitude}")
+            continue
+        # scores of 1e7: the largest one's value, half a bf16 step off (4-bit and INT8 values are
+        # code * scale, INT8's rounded to bf16 in the definition only: one more half step)
+        out, row = s.run().double().cpu().numpy(), 0
+        q = s.q.double().cpu().numpy()
+        for b, (n, L) in enumerate(seqs):
+            for j in range(n):
+                p, k = L - n + j, np.arange(L)
+                see = (k <= p) & ((k > p - 100) | (k < 4))
+                for h in range(8):
+                    score = np.where(see, s.K[b][:, h // 4] @ q[row, h], -np.inf)
+                    best = np.sort(score)[-2:]
+                    if best[1] - best[0] < 1e-5 * np.abs(best).max():
+                        continue     # a tie within the scores' own error
+                    want = s.V[b][score.argmax(), h // 4]
+                    assert (np.abs(out[row, h] - want) <= 2.0 ** -7 * np.abs(want) + 2.0 ** -18 * 8 * np.abs(want).max()).all()
+                row += 1
 
 
 @pytest.mark.parametrize("kv", KINDS)

@@ -20,12 +20,12 @@ def refused(rc):
 
 def attention(lib, **kw):
     a = dict(kv=_lib.DT_I4, q=16, qts=4096, qhs=128, k=16, v=16, cbs=8192, cts=512, chs=64, ks=16, vs=16, B=2, Hq=32,
-             Hkv=8, D=128, bs=16, nb=64, mq=5, mk=100, bt=16, win=0, sinks=0, out=16, ws=16, wsb=1 << 30)
+             Hkv=8, D=128, bs=16, nb=64, mq=5, mk=100, bt=16, win=0, sinks=0, scale=0.088, out=16, ws=16, wsb=1 << 30)
     a.update(kw)
     return lib.coopt_window_attention(a["kv"], a["q"], a["qts"], a["qhs"], a["k"], a["v"], a["cbs"], a["cts"],
                                       a["chs"], a["ks"], a["vs"], 128, 8, 1, 16, a["bt"], 16, 16, a["B"], a["Hq"],
                                       a["Hkv"], a["D"], a["bs"], a["nb"], a["mq"], a["mk"], 0, a["win"], a["sinks"],
-                                      0.088, a["out"], 4096, 128, a["ws"], a["wsb"], None)
+                                      a["scale"], a["out"], 4096, 128, a["ws"], a["wsb"], None)
 
 
 def test_window_attention_refuses(lib):
@@ -36,7 +36,9 @@ def test_window_attention_refuses(lib):
                      (dict(k=None), "null"), (dict(q=8), "aligned"), (dict(qts=4097), "aligned"),
                      (dict(k=8), "aligned"), (dict(cts=520), "aligned"), (dict(ks=None), "k_scale"),
                      (dict(kv=_lib.DT_I8, vs=None), "k_scale"), (dict(ks=17), "k_scale"), (dict(nb=0), "num_blocks"),
-                     (dict(B=70000, wsb=1 << 40), "65535"), (dict(B=-1), "Hq")):
+                     (dict(B=70000, wsb=1 << 40), "65535"), (dict(B=-1), "Hq"), (dict(scale=-1.0), "softmax_scale"), (dict(scale=float("nan")), "softmax_scale"),
+                     (dict(scale=float("inf")), "softmax_scale"), (dict(mk=1 << 30), "out of range"),
+                     (dict(mq=1 << 29), "out of range")):
         assert what in refused(attention(lib, **kw)), (kw, _lib.last_error())
     assert attention(lib, B=0) == _lib.COOPT_OK
     assert attention(lib, wsb=8) == _lib.COOPT_EWORKSPACE
