@@ -161,6 +161,11 @@ def stream_handle(device=None) -> int:
     return _raw_stream(torch.cuda.current_device() if index is None else index)
 
 
+def raw_stream(index: int) -> int:
+    """stream_handle of GPU `index`, given as its number."""
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -194,11 +199,25 @@ def require_one_device(*tensors):
     return dev
 
 
-def call_on(dev, fn, *args):
-    """fn(*args) with `dev` the current device, on which the library launches."""
-    if dev.index == torch.cuda.current_device():
+_entries = {}
+
+
+def entry(name):
+    """The library's function `name` (load()'s lock and attribute lookup once a name)."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(load(), name)
+    return fn
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def call_on(index, fn, *args):
+    """fn(*args) with GPU `index` the current device, on which the library launches."""
+    if index == _current_device():
         return fn(*args)
-    with torch.cuda.device(dev):
+    with torch.cuda.device(index):
         return fn(*args)
 
 

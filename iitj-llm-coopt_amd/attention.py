@@ -83,6 +83,10 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
                     max_seqlen_k, softmax_scale=None, k_scale=None, v_scale=None, out=None,
                     workspace=None, window=None, sink_tokens=0):
     """out [T, Hq, D] bf16 = causal paged attention; see the module docstring."""
+    if window is not None or sink_tokens or k_cache.dtype is torch.uint8:
+        return _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, max_seqlen_q,
+                                 max_seqlen_k, softmax_scale, k_scale, v_scale, out, workspace, window,
+                                 sink_tokens)
     _lib.require_cuda(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table)
     if q.dtype != torch.bfloat16 or q.dim() != 3 or q.stride(-1) != 1:
         raise ValueError("q must be bf16 [T, Hq, D] with contiguous D")
@@ -91,8 +95,7 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
             k_cache.dim() != 4 or k_cache.stride(-1) != 1:
         raise ValueError("k/v caches must be [num_blocks, block_size, Hkv, D] alike")
     NB, bs, Hkv, cD = k_cache.shape
-    int4 = k_cache.dtype == torch.uint8
-    if cD * (2 if int4 else 1) != D or Hq % Hkv:
+    if cD != D or Hq % Hkv:
         raise ValueError(f"q {tuple(q.shape)} does not match cache {tuple(k_cache.shape)}")
     B = seq_lens.numel()
     if cu_seqlens_q.numel() != B + 1:
@@ -105,22 +108,18 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
         raise ValueError("block_table must be [batch, width] int32, row-major")
     if k_cache.dtype == torch.bfloat16:
         code, ks, vs, sstr = _lib.DT_BF16, None, None, (0, 0, 0)
-    elif k_cache.dtype == torch.int8 or int4:
+    elif k_cache.dtype == torch.int8:
         if k_scale is None or v_scale is None:
-            raise ValueError(f"{'INT4' if int4 else 'INT8'} caches need k_scale and v_scale")
+            raise ValueError("INT8 caches need k_scale and v_scale")
         if k_scale.shape != (NB, bs, Hkv) or k_scale.dtype != torch.float16 or \
                 v_scale.shape != k_scale.shape or v_scale.stride() != k_scale.stride():
             raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
         _lib.require_cuda(k_scale, v_scale)
-        code, ks, vs, sstr = _lib.DT_I4 if int4 else _lib.DT_I8, k_scale, v_scale, k_scale.stride()
+        code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
     else:
         raise ValueError(f"unsupported cache dtype {k_cache.dtype}")
     if softmax_scale is None:
         softmax_scale = 1.0 / math.sqrt(D)
-    if int4 or window is not None or sink_tokens:
-        return _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table,
-                                 int(max_seqlen_q), int(max_seqlen_k), float(softmax_scale), code, ks,
-                                 vs, sstr, out, workspace, window, sink_tokens)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
     elif out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or out.stride(-1) != 1:
@@ -148,47 +147,92 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
     return out
 
 
+_WINDOW_KINDS = {torch.bfloat16: (_lib.DT_BF16, 1), torch.int8: (_lib.DT_I8, 1),
+                 torch.uint8: (_lib.DT_I4, 2)}   # code, elements a unit of the cache holds
+
+
 def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, max_seqlen_q,
-                      max_seqlen_k, softmax_scale, code, ks, vs, sstr, out, workspace, window,
+                      max_seqlen_k, softmax_scale, k_scale, v_scale, out, workspace, window,
                       sink_tokens):
-    """paged_attention's call with a window or over INT4 caches, its arguments checked there."""
+    """paged_attention's call with a window or over INT4 caches."""
+    if q.dim() != 3 or q.dtype is not torch.bfloat16 or k_cache.dim() != 4:
+        raise ValueError("q must be bf16 [T, Hq, D], caches [num_blocks, block_size, Hkv, D]")
     T, Hq, D = q.shape
-    NB, bs, Hkv, _ = k_cache.shape
+    NB, bs, Hkv, cD = k_cache.shape
+    q0, q1, q2 = q.stride()
+    cs = k_cache.stride()
+    kind = _WINDOW_KINDS.get(k_cache.dtype)
+    if kind is None or v_cache.dtype is not k_cache.dtype:
+        raise ValueError(f"unsupported cache dtypes {k_cache.dtype}, {v_cache.dtype}")
+    code, per_unit = kind
+    if q2 != 1:
+        raise ValueError("q must be bf16 [T, Hq, D] with contiguous D")
+    if k_cache.shape != v_cache.shape or cs != v_cache.stride() or cs[3] != 1:
+        raise ValueError("k/v caches must be [num_blocks, block_size, Hkv, D] alike")
+    if cD * per_unit != D or Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"q {tuple(q.shape)} does not match cache {tuple(k_cache.shape)}")
     B = seq_lens.numel()
-    if v_cache.dtype != k_cache.dtype or (vs is not None and vs.dtype != torch.float16):
-        raise ValueError("k and v caches and their scales must be of one type")
-    if out is not None and (out.shape != (T, Hq, D) or out.dtype != torch.bfloat16 or
-                            out.stride(-1) != 1):
-        raise ValueError("out must be bf16 [T, Hq, D] with contiguous D")
-    if block_table.shape[1] * bs < max_seqlen_k:
+    if cu_seqlens_q.numel() != B + 1:
+        raise ValueError("cu_seqlens_q must have batch + 1 entries")
+    if cu_seqlens_q.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 or \
+            block_table.dtype is not torch.int32:
+        raise ValueError("cu_seqlens_q, seq_lens and block_table must be int32")
+    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.stride(1) != 1:
+        raise ValueError("block_table must be [batch, width] int32, row-major")
+    max_q, max_k = operator.index(max_seqlen_q), operator.index(max_seqlen_k)
+    if block_table.shape[1] * bs < max_k:
         raise ValueError(f"block_table holds {block_table.shape[1]} blocks of {bs} tokens a sequence, "
-                         f"max_seqlen_k is {max_seqlen_k}")
-    win, sinks = _window_args(window, sink_tokens, max_seqlen_k)
-    dev = _lib.require_one_device(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ks, vs,
-                                  out, workspace)
+                         f"max_seqlen_k is {max_k}")
+    win, sinks = _window_args(window, sink_tokens, max_k)
+    index = q.get_device()   # of every tensor; -1 on the CPU
+    alike = index >= 0 and index == k_cache.get_device() == v_cache.get_device() == \
+        cu_seqlens_q.get_device() == seq_lens.get_device() == block_table.get_device()
+    if code == _lib.DT_BF16:
+        ks = vs = s0 = s1 = s2 = 0
+    else:
+        if k_scale is None or v_scale is None:
+            raise ValueError(f"{'INT4' if per_unit == 2 else 'INT8'} caches need k_scale and v_scale")
+        if k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_scale.shape or \
+                k_scale.dtype is not torch.float16 or v_scale.dtype is not torch.float16 or \
+                v_scale.stride() != k_scale.stride():
+            raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
+        s0, s1, s2 = k_scale.stride()
+        alike = alike and index == k_scale.get_device() == v_scale.get_device()
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    if out is not None:
+        if out.shape != (T, Hq, D) or out.dtype is not torch.bfloat16 or out.stride(-1) != 1:
+            raise ValueError("out must be bf16 [T, Hq, D] with contiguous D")
+        alike = alike and index == out.get_device()
+    if workspace is not None:
+        alike = alike and index == workspace.get_device()
+    if not alike:
+        _lib.require_one_device(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table,
+                                k_scale if ks else None, v_scale if vs else None, out, workspace)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+        out = q.new_empty((T, Hq, D))
     if B == 0 or T == 0:
         return out
-    need = _window_workspace_bytes(B, Hq, Hkv, D, max_seqlen_q, max_seqlen_k, win, sinks)
+    stream = _lib.raw_stream(index)
+    need = _window_workspace_bytes(B, Hq, Hkv, D, max_q, max_k, win, sinks)
     if workspace is None:
         # a graph under capture gets a workspace of its own (from its memory pool), so that two
         # graphs captured on one stream may replay at the same time
-        workspace = torch.empty(max(need, 256), dtype=torch.uint8, device=dev) \
-            if torch.cuda.is_current_stream_capturing() else _WS.get(need, dev)
-    elif workspace.numel() * workspace.element_size() < need:
-        raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} "
-                         f"bytes, {need} needed")
-    cu, sl = cu_seqlens_q.contiguous(), seq_lens.contiguous()
-    cs = k_cache.stride()
+        workspace = q.new_empty((max(need, 256),), dtype=torch.uint8) \
+            if torch.cuda.is_current_stream_capturing() else _WS.get(need, q.device)
+        have = workspace.numel()
+    else:
+        have = workspace.numel() * workspace.element_size()
+        if have < need or not workspace.is_contiguous():
+            raise ValueError(f"workspace holds {have} bytes, {need} needed, contiguous")
+    cu = cu_seqlens_q if cu_seqlens_q.is_contiguous() else cu_seqlens_q.contiguous()
+    sl = seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
+    o0, o1, _ = out.stride()
     _lib.check(_lib.call_on(
-        dev, _lib.load().coopt_window_attention, code, _lib.ptr(q), q.stride(0), q.stride(1),
-        _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs),
-        sstr[0], sstr[1], sstr[2], _lib.ptr(block_table), block_table.stride(0), _lib.ptr(cu),
-        _lib.ptr(sl), B, Hq, Hkv, D, bs, NB, max_seqlen_q, max_seqlen_k, T, win, sinks,
-        softmax_scale, _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size(), _lib.stream_handle(dev)),
-        "coopt_window_attention")
+        index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
+        v_cache.data_ptr(), cs[0], cs[1], cs[2], ks, vs, s0, s1, s2, block_table.data_ptr(),
+        block_table.stride(0), cu.data_ptr(), sl.data_ptr(), B, Hq, Hkv, D, bs, NB, max_q, max_k, T, win,
+        sinks, 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, out.data_ptr(), o0, o1,
+        workspace.data_ptr(), have, stream), "coopt_window_attention")
     return out
 
 

@@ -77,9 +77,23 @@ constexpr int kThreads = 256;  // merge kernel
 // Waves per attention block: 8 (one block per CU at two waves per SIMD, i.e. at most 256
 // registers per lane) while the accumulators and two tile buffers fit that (RT <= 3), else 4.
 constexpr int waves_for(int RT) { return RT <= 3 ? 8 : 4; }
-// Blocks that share a CU: two with 4 waves at head dim 64 and bf16 (79 KB of LDS, at most 256 registers
-// asked for), where batches of many query windows take 0.63 to 0.8 of the time; see alone_lds.
-constexpr int blocks_per_cu(int D, int kv, int RT) { return D == 64 && kv == kBf16 && RT == 4 ? 2 : 1; }
+// Waves a SIMD is to hold: two blocks a CU with 4 waves at head dim 64 and bf16 (79 KB of LDS, at most 256
+// registers asked for), where batches of many query windows take 0.63 to 0.8 of the time; see alone_lds.
+constexpr int waves_per_simd(int D, int kv, int RT, bool win) {
+#ifdef W64
+  if (win && D == 64 && RT == 1) return W64;
+#endif
+  return D == 64 && kv == kBf16 && RT == 4 ? 2 : 1;
+}
+// Tile buffers of a wave: its loads in flight are this many less one.  A 4-bit tile is a quarter of a
+// bf16 one (4 KB at head dim 128), and it takes bytes in flight to cover the memory's latency.
+constexpr int tile_buffers(int D, int kv, int RT, bool sc, bool win) {
+#ifdef NB1
+  if (win && kv == kI4) return !sc ? (RT <= 2 ? 2 : 1) : RT == 1 ? (D == 128 ? NB1 : NB64) : RT == 2 ? NB2 : 1;
+#endif
+  if (win && kv == kI4) return RT > 2 ? 1 : !sc ? 2 : RT == 1 ? 4 : 3;
+  return RT <= 2 || (kv == kI8 && RT == 3 && !win) ? 2 : 1;
+}
 constexpr int kTileKeys = 32;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -244,6 +258,40 @@ __device__ __forceinline__ uint32_t take_out_not_finite(uint32_t x, uint32_t& an
   return x & ~(bad | (bad - (bad >> 15)));
 }
 
+// Loads at a wave-uniform base in four scalar registers plus a lane's 32-bit byte offset (buffer
+// instructions: the compiler neither copies the offset nor adds it up in 64 bits, as it does with
+// pointers whose lane parts it has moved out of the loop).  Untyped, no bound.
+typedef __amdgpu_buffer_rsrc_t buffer_t;
+__device__ __forceinline__ buffer_t buffer_at(const unsigned char* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned char*>(p), 0, -1, 0x00020000);
+}
+// BYTES 16, 8, 4 or 2 into dst; NT: nontemporal (see load_words)
+template <int BYTES, bool NT, typename T>
+__device__ __forceinline__ void buffer_load(buffer_t b, uint32_t off, T& dst) {
+  constexpr int aux = NT ? 2 : 0;
+  if constexpr (BYTES == 16) {
+    const u32x4_t x = __builtin_amdgcn_raw_buffer_load_b128(b, off, 0, aux);
+    dst[0] = x[0]; dst[1] = x[1]; dst[2] = x[2]; dst[3] = x[3];
+  } else if constexpr (BYTES == 8) {
+    const u32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(b, off, 0, aux);
+    dst[0] = x[0]; dst[1] = x[1];
+  } else if constexpr (BYTES == 4) {
+    dst[0] = __builtin_amdgcn_raw_buffer_load_b32(b, off, 0, aux);
+  } else {
+    dst[0] = __builtin_amdgcn_raw_buffer_load_b16(b, off, 0, aux);
+  }
+}
+
+// max of own and partner's value as max_xor16 / max_xor32, and of two values, one instruction each: a
+// median with infinity (fmaxf also quiets its operands, which are no signalling NaN here).
+__device__ __forceinline__ float max_med(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
+__device__ __forceinline__ float max_lanes_16_32(float v) {
+  u32x2_pl_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = max_med(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return max_med(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 __device__ __forceinline__ int64_t clamp_page(int32_t page, int64_t num_blocks) {
   return page < 0 ? 0 : (page >= num_blocks ? num_blocks - 1 : page);
 }
@@ -363,36 +411,82 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
   }
 }
 
-// ---- INT4 operands: the code + 8, n, of a nibble enters a product as 16 + n (K: bf16, exact, n in
-// mantissa bits 3..6) or n 2^-20 (V: fp16, n in bits 4..7 of a subnormal, which the matrix cores
-// take as it is; from bits 0..3, n 2^-24, its products lose their last bits), and the 24 or 8 too much comes off the sums: the score MFMAs' accumulators start
-// at -24 sum_d q[d], and the scale of the key multiplies the score; V's products with the
-// probabilities P' leave 8 sum P' too much, which one more MFMA of P' against ones counts.
-// (Subtracting in the operands instead costs V a packed fp16 add per two values; bf16 has none.)
-constexpr float kI4KBias = 24.0f, kI4VBias = 8.0f, kI4VUnit = 0x1p20f;
+// ---- INT4 operands.  The nibble n, code + 8, enters the products without a conversion: in the low
+// bits of an fp8 (e4m3) byte it is n 2^-9 (K), in bits 4..7 of an fp16 half word n 2^-20 (V), both
+// exact.  (From bits 0..3, n 2^-24, the products of V lose their last bits.)  The 8 too much comes off
+// the sums: the score accumulators start at -8 sum_d q[d], V's products with the probabilities P' leave
+// 8 sum P' too much, which one more MFMA of P' against ones counts.
+// K: three instructions per 8 codes.  The other operand is q as the sum of two e4m3 parts, a row times
+// the power of two that brings its largest value to [2^7, 2^8): 4 bits and then the 4 below them, all of
+// a bf16's 8, except that values under 2^-9 of the row's largest are rounded to 2^-17 of it.  The key's
+// scale multiplies the score, the row's power of two goes into its softmax scale.  At head dim 128 the
+// 128-term MFMA takes one part at a time, at 64 both at once (K twice in its operand).
+// Against K as bf16 16 + n, eight instructions and four MFMAs per 8 codes: measured below.
+constexpr float kI4Bias = 8.0f, kI4VUnit = 0x1p20f;
 
-// The constants of k_operand_i4 as registers (opaque to the compiler, which otherwise splits each
-// and-or into two instructions with a literal each).
-struct I4Const {
-  uint32_t mask = 0x00780078u, bits = 0x41804180u;  // bf16 16
-  __device__ __forceinline__ I4Const() { asm("" : "+s"(mask), "+v"(bits)); }
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
+struct F8Operand {  // of the 128-term MFMA: 32 bytes a lane
+  u32x4_t lo, hi;
 };
+__device__ __forceinline__ f32x4_t mfma_f8(const F8Operand& a, const F8Operand& b, f32x4_t c) {
+  const i32x8_t av = __builtin_bit_cast(i32x8_t, a), bv = __builtin_bit_cast(i32x8_t, b);
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 0, 0, 0, 0, 0, 0);
+}
+
+// The 16 codes of two dwords (element e of a dword's 8: its nibble e), even elements then odd ones.
+__device__ __forceinline__ u32x4_t k_bytes_i4(uint32_t x0, uint32_t x1) {
+  constexpr uint32_t m = 0x0f0f0f0fu;
+  return u32x4_t{x0 & m, (x0 >> 4) & m, x1 & m, (x1 >> 4) & m};
+}
+
+// The exponent of a row's power of two; amax: its largest |q| as bf16 bits.
+__device__ __forceinline__ int q_exponent_i4(uint32_t amax) { return min(134 - static_cast<int>(amax >> 7), 126); }
+// 8 elements of the row in the order of k_bytes_i4: the two parts.
+struct QBytes {
+  u32x2_t first, second;
+};
+__device__ __forceinline__ QBytes q_bytes_i4(u32x4_t q, int exponent) {
+  const float f = __builtin_ldexpf(1.0f, exponent);
+  QBytes r;
+#pragma unroll
+  for (int odd = 0; odd < 2; ++odd) {
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(odd ? q[e] & 0xffff0000u : q[e] << 16) * f;
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    r.first[odd] = static_cast<uint32_t>(w);
+    x[0] -= __builtin_amdgcn_cvt_f32_fp8(w, 0);
+    x[1] -= __builtin_amdgcn_cvt_f32_fp8(w, 1);
+    x[2] -= __builtin_amdgcn_cvt_f32_fp8(w, 2);
+    x[3] -= __builtin_amdgcn_cvt_f32_fp8(w, 3);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+    w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
+    r.second[odd] = static_cast<uint32_t>(w);
+  }
+  return r;
+}
+// What turns a row's sums into scores in the log2 domain.
+__device__ __forceinline__ float row_scale_i4(float scale_log2, int exponent) {
+  return __builtin_ldexpf(scale_log2, 9 - exponent);
+}
+// K of code 0 everywhere
+__device__ __forceinline__ F8Operand k_zero_i4() {
+  constexpr uint32_t e = 0x08080808u;
+  return F8Operand{u32x4_t{e, e, e, e}, u32x4_t{e, e, e, e}};
+}
 
 // x times the fp16 in the low (high) half of w, one v_fma_mix that converts the half in place.
 __device__ __forceinline__ float times_f16(float x, uint32_t w, int high) {
   return fmaf(x, static_cast<float>(__builtin_bit_cast(f16x2_t, w)[high]), 0.0f);
 }
 
-// The 8 codes of a dword as the K operand: word w holds elements w and w + 4, the order permute_q8
-// gives the other operand.
-__device__ __forceinline__ u32x4_t k_operand_i4(uint32_t x, const I4Const& c) {
-  return u32x4_t{((x << 3) & c.mask) | c.bits, ((x >> 1) & c.mask) | c.bits, ((x >> 5) & c.mask) | c.bits,
-                 ((x >> 9) & c.mask) | c.bits};
+// The fp16 pair (x0, x1) times the one in w, each product rounded once (v_fma_mixlo / mixhi).
+__device__ __forceinline__ uint32_t pair_times_f16(float x0, float x1, uint32_t w) {
+  return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(times_f16(x0, w, 0)),
+                                              static_cast<_Float16>(times_f16(x1, w, 1))});
 }
-__device__ __forceinline__ u32x4_t permute_q8(u32x4_t q) {
-  return u32x4_t{(q[0] & 0xffffu) | (q[2] << 16), (q[0] >> 16) | (q[2] & 0xffff0000u),
-                 (q[1] & 0xffffu) | (q[3] << 16), (q[1] >> 16) | (q[3] & 0xffff0000u)};
-}
+
 // n 2^-20 of nibble dt of two keys' dwords as fp16, x0's in the low half; even / odd: i4_nibbles of
 // the dwords.
 struct I4Nibbles {
@@ -445,14 +539,15 @@ __device__ void plan_item(const AttnArgs& a, int lane, int* out) {
 // (a run-time choice of input made the compiler wait for every earlier load where the two
 // input paths joined).
 template <int D, int KV, int RT, bool SC, int FUSED, bool WIN>
-__global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void verify_attn_kernel(
+__global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN)) void verify_attn_kernel(
     const int32_t* cu_p, const int32_t* sl_p, const int32_t* bt_p, int64_t bt_stride, int split,
     int bs_shift, int mode, AttnArgs a) {
   using Raw = RawTile<D, KV>;
   constexpr bool INT8 = KV == kI8, INT4 = KV == kI4, CODES = KV != kBf16;
   constexpr int kWaves = waves_for(RT);
   constexpr int kBlock = 64 * kWaves;
-  constexpr bool DB = RT <= 2 || (CODES && RT == 3 && (SC || !WIN));
+  constexpr int kBufs = tile_buffers(D, KV, RT, SC, WIN);
+  constexpr bool DB = kBufs == 2;
   constexpr int kKs = D / 32;   // k-steps of the score MFMA
   constexpr int kDt = D / 16;   // d-tiles of the output = V elements per lane per key
   constexpr int kElt = Raw::kElt;
@@ -482,6 +577,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   __shared__ float sm_M[kRows];
   __shared__ float sm_L[kRows];
   __shared__ int sm_plan[4];
+  __shared__ int sm_exp[INT4 ? kRows : 1];  // INT4: the rows' q_exponent_i4
   float* osh = reinterpret_cast<float*>(lds + kOOff);
   const int tid = threadIdx.x, lane = tid & 63, grp = lane >> 4, l16 = lane & 15;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -508,8 +604,14 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
                        const int L, const int32_t pg0, const int32_t pg1) {
   const const_i32_ptr table = (const_i32_ptr)(bt_p + static_cast<int64_t>(b) * bt_stride);
   const int k_begin = sidx * split;
-  int64_t first_pg0 = clamp_page(pg0, a.num_blocks);
-  int64_t first_pg1 = clamp_page(pg1, a.num_blocks);
+  // WIN: the host keeps page numbers and block strides within 32 bits, which halves the loop's
+  // scalar arithmetic
+  using Page = std::conditional_t<WIN, uint32_t, int64_t>;
+  auto in_pool = [&](int32_t page) -> Page {
+    if constexpr (WIN) return static_cast<uint32_t>(min(max(page, 0), static_cast<int32_t>(a.num_blocks) - 1));
+    else return clamp_page(page, a.num_blocks);
+  };
+  Page first_pg0 = in_pool(pg0), first_pg1 = in_pool(pg1);
   if (n <= 0) return;
   // WIN: k_begin, k_end and the tiles count the keys that are left (Visible)
   Visible vis{0, 0};
@@ -626,8 +728,20 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
       for (int it = 0; it < kQIter; ++it) {
         const int idx = it * kBlock + tid;
         const int r = idx / kQCh, c = idx % kQCh;
-        if (r < kRows)
-          *reinterpret_cast<u32x4_t*>(qsh + r * kQPitch + c * 16) = INT4 ? permute_q8(qreg[it]) : qreg[it];
+        if constexpr (INT4) {  // D / 8 adjacent lanes hold a row; its parts, D bytes each, one after the other
+          uint32_t amax = 0;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) amax = max_u16x2(amax, qreg[it][e] & 0x7fff7fffu);
+          const int exponent = q_exponent_i4(group_max_u32<kQCh>(max(amax & 0xffffu, amax >> 16)));
+          const QBytes q = q_bytes_i4(qreg[it], exponent);
+          if (r < kRows) {
+            if (c == 0) sm_exp[r] = exponent;
+            *reinterpret_cast<u32x2_t*>(qsh + r * kQPitch + c * 8) = q.first;
+            *reinterpret_cast<u32x2_t*>(qsh + r * kQPitch + D + c * 8) = q.second;
+          }
+          continue;
+        }
+        if (r < kRows) *reinterpret_cast<u32x4_t*>(qsh + r * kQPitch + c * 16) = qreg[it];
       }
     }
     __syncthreads();
@@ -644,11 +758,10 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   // contraction map of the K loads)
   const unsigned char* qlds = qsh + l16 * kQPitch;
   auto q_byte = [&](int ks) {
-    if constexpr (INT4) return 2 * (D / 4 * grp + 8 * ks);
     return INT8 ? 2 * (64 * (ks >> 1) + 16 * grp + 8 * (ks & 1)) : 2 * (32 * ks + 8 * grp);
   };
 
-  constexpr int kAcc = INT4 ? kDt + 1 : kDt;  // INT4: the last one sums P' (see kI4VBias)
+  constexpr int kAcc = INT4 ? kDt + 1 : kDt;  // INT4: the last one sums P' (INT4 operands)
   f32x4_t o[RT][kAcc];
   float m_run[RT], l_run[RT];
 #pragma unroll
@@ -658,22 +771,30 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
 #pragma unroll
     for (int dt = 0; dt < kAcc; ++dt) o[rt][dt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   }
-  const I4Const i4;
-  f32x4_t score0[RT];  // INT4: what the score accumulators start at (kI4KBias)
+  // INT4: what the score accumulators start at, the rows' scales of the sums in the log2 domain
+  // (one register each where the accumulators leave no more)
+  std::conditional_t<(RT <= 2), f32x4_t, float> score0[RT];
+  float row_scale[RT];
+  // and part `part` of the lane's Q operand (head dim 64: of both)
+  constexpr int kParts = D / 64;
+  auto q_operand = [&](int rt, int part) {
+    const unsigned char* src = qlds + rt * 16 * kQPitch + (D == 128 ? part * D + grp * 32 : grp * 16);
+    return F8Operand{*reinterpret_cast<const u32x4_t*>(src), *reinterpret_cast<const u32x4_t*>(src + (D == 128 ? 16 : D))};
+  };
   auto start_scores = [&]() {
     if constexpr (INT4) {
-      constexpr uint32_t one = 0x3f803f80u;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
         f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int ks = 0; ks < kKs; ++ks)
-          sum = mfma_bf16(u32x4_t{one, one, one, one},
-                          *reinterpret_cast<const u32x4_t*>(qlds + rt * 16 * kQPitch + q_byte(ks)), sum);
-        score0[rt] = sum * -kI4KBias;
+        for (int part = 0; part < kParts; ++part) sum = mfma_f8(k_zero_i4(), q_operand(rt, part), sum);
+        if constexpr (RT <= 2) score0[rt] = -sum;
+        else score0[rt] = -sum[0];
+        row_scale[rt] = row_scale_i4(a.scale_log2, sm_exp[rt * 16 + l16]);
       }
     }
   };
+  auto scale_log2 = [&](int rt) { return INT4 ? row_scale[rt] : score_scale; };
   // INT8: the wave's V-scale reference exponent e_v (wave-uniform).  The PV operand is
   // fp16(p * s_v * 2^-e_v); o and l are kept relative to 2^(m_run + e_v), so e_v enters the
   // exponent of p and the row maxima the merge sees, and cancels in o / l.
@@ -693,7 +814,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   // of key kb (sub-tile 0) and of key kb + 16 (sub-tile 1); keys past the end are clamped to
   // L - 1, which stays in the page of its 16-key sub-tile.
   auto page_of = [&](int key) {
-    return clamp_page(table[min(key, L - 1) >> bs_shift], a.num_blocks);
+    return in_pool(table[min(key, L - 1) >> bs_shift]);
   };
 
   if constexpr (WIN) {  // the pages were looked up for the tile's place without the gap
@@ -734,8 +855,59 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   // a full tile: every key < L
   // INT8: the scales are issued first, so the V-scale check of a loaded tile (vcheck) waits
   // only for them and leaves the tile's K/V loads in flight.
-  auto load_full = [&](Raw& raw, int t, int64_t pg0, int64_t pg1) {
+  const unsigned char* const khead = kbase + kElt * head_off;
+  const unsigned char* const vhead = vbase + kElt * head_off;
+  const unsigned char* const kshead = reinterpret_cast<const unsigned char*>(a.ks + shead_off);
+  const unsigned char* const vshead = reinterpret_cast<const unsigned char*>(a.vs + shead_off);
+  auto load_full_win = [&](Raw& raw, int t, Page pg0, Page pg1) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
+    const uint32_t c_blk = kElt * static_cast<uint32_t>(a.c_bs), s_blk = 2 * static_cast<uint32_t>(a.s_bs);
+    auto at = [](uint32_t pg, uint32_t blk, uint32_t in_page) { return static_cast<uint64_t>(pg) * blk + in_page; };
+    if constexpr (CODES) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        const uint32_t tok0 = (kb + kt * 16) & bs_mask;
+        const uint64_t off = at(kt ? pg1 : pg0, s_blk, tok0 * (SC ? 2u : 2u * s_ts));
+        const buffer_t ksp = buffer_at(kshead + off), vsp = buffer_at(vshead + off);
+        auto four = [&](buffer_t sp) {
+          u32x2_t x;
+          if constexpr (SC) {
+            buffer_load<8, false>(sp, grp * 8u, x);
+          } else {
+            uint32_t vh[4][1];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) buffer_load<2, false>(sp, 2u * ((grp * 4 + i) * s_ts), vh[i]);
+            x = u32x2_t{vh[0][0] | (vh[1][0] << 16), vh[2][0] | (vh[3][0] << 16)};
+          }
+          return x;
+        };
+        if constexpr (INT4) {
+          raw.ks4[kt] = four(ksp);
+        } else {
+          uint32_t x[1];
+          buffer_load<2, false>(ksp, 2u * (SC ? l16 : l16 * s_ts), x);
+          raw.ks[kt] = x[0];
+        }
+        raw.vs[kt] = four(vsp);
+      }
+    }
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const uint32_t tok0 = (kb + kt * 16) & bs_mask;
+      const uint64_t off = at(kt ? pg1 : pg0, c_blk, kElt * tok0 * static_cast<uint32_t>(c_ts));
+      const buffer_t kp = buffer_at(khead + off), vp = buffer_at(vhead + off);
+#pragma unroll
+      for (int c = 0; c < Raw::kKVec; ++c)
+        buffer_load<(Raw::kKBytes < 16 ? 8 : 16), false>(kp, k_lane + 64 * c, raw.k[kt][c]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        buffer_load<Raw::kVBytes, (Raw::kVBytes >= 8)>(vp, v_lane[i], raw.v[kt * 4 + i]);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // the loads go out before the tile in hand is computed
+  };
+  auto load_full = [&](Raw& raw, int t, Page pg0, Page pg1) {
+    if constexpr (WIN) return load_full_win(raw, t, pg0, pg1);
+    const int kb = k_begin + t * kTileKeys;
     if constexpr (CODES) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -746,21 +918,14 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
         if constexpr (SC) {
           uint32_t ko2 = l16 * 2, vo2 = grp * 8;
           asm volatile("" : "+v"(ko2), "+v"(vo2));
-          if constexpr (INT4)
-            raw.ks4[kt] = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const unsigned char*>(ksp + tok0) + vo2);
-          else
-            raw.ks[kt] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const unsigned char*>(ksp + tok0) + ko2);
+          raw.ks[kt] = *reinterpret_cast<const uint16_t*>(reinterpret_cast<const unsigned char*>(ksp + tok0) + ko2);
           raw.vs[kt] = *reinterpret_cast<const u32x2_t*>(reinterpret_cast<const unsigned char*>(vsp + tok0) + vo2);
         } else {
-          auto four = [&](const uint16_t* sp) {
-            uint32_t vh[4];
+          raw.ks[kt] = ksp[(tok0 + l16) * s_ts];
+          uint32_t vh[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) vh[i] = sp[(tok0 + grp * 4 + i) * s_ts];
-            return u32x2_t{vh[0] | (vh[1] << 16), vh[2] | (vh[3] << 16)};
-          };
-          if constexpr (INT4) raw.ks4[kt] = four(ksp);
-          else raw.ks[kt] = ksp[(tok0 + l16) * s_ts];
-          raw.vs[kt] = four(vsp);
+          for (int i = 0; i < 4; ++i) vh[i] = vsp[(tok0 + grp * 4 + i) * s_ts];
+          raw.vs[kt] = u32x2_t{vh[0] | (vh[1] << 16), vh[2] | (vh[3] << 16)};
         }
       }
     }
@@ -773,7 +938,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     }
   };
   // the split's last tile when it ends inside a tile: keys clamped to L - 1
-  auto load_partial = [&](Raw& raw, int t, int64_t pg0, int64_t pg1) {
+  auto load_partial = [&](Raw& raw, int t, Page pg0, Page pg1) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
@@ -940,11 +1105,30 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     f32x4_t acc[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      if constexpr (INT4) acc[rt][0] = acc[rt][1] = score0[rt];
+      if constexpr (INT4 && RT <= 2) acc[rt][0] = acc[rt][1] = score0[rt];
+      else if constexpr (INT4) acc[rt][0] = acc[rt][1] = f32x4_t{score0[rt], score0[rt], score0[rt], score0[rt]};
       else acc[rt][0] = acc[rt][1] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
+    if constexpr (INT4) {
+      F8Operand kop[2];
 #pragma unroll
-    for (int ks = 0; ks < kKs; ++ks) {
+      for (int kt = 0; kt < 2; ++kt) {
+        const auto& x = raw.k[kt][0];
+        kop[kt].lo = k_bytes_i4(x[0], x[1]);
+        if constexpr (D == 128) kop[kt].hi = k_bytes_i4(x[2], x[3]);
+        else kop[kt].hi = kop[kt].lo;
+      }
+#pragma unroll
+      for (int part = 0; part < kParts; ++part)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const F8Operand qop = q_operand(rt, part);
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = mfma_f8(kop[kt], qop, acc[rt][kt]);
+        }
+    }
+#pragma unroll
+    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks) {
       u32x4_t qop[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -964,7 +1148,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
             kop[2 * h + 1] = dequant_pair(__builtin_amdgcn_perm(k64, ux, 0x04030402u), sk, skb);
           }
         } else if constexpr (INT4) {
-          kop = k_operand_i4(raw.k[kt][0][ks], i4);
+          kop = u32x4_t{0, 0, 0, 0};  // not reached: no steps
         } else {
           kop = raw.k[kt][ks];
         }
@@ -988,6 +1172,13 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     // sums), and the accumulators are rescaled only on those rare raises (one branch per
     // tile, taken by the whole wave).
     constexpr float kSlack = 8.0f;
+    // WIN: the lane's maximum of the row, formed where the scores are the sums' own (known not to need
+    // quieting) or masked
+    float lane_max[RT];
+    auto max8 = [](const float (&x)[2][4]) {
+      return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                   fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+    };
     float sv[RT][2][4];  // raw scores (the scale is applied in the exponent); masked -inf
     if (open) {  // one uniform branch for the whole tile
 #pragma unroll
@@ -996,6 +1187,10 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sv[rt][kt][i] = acc[rt][kt][i];
+      if constexpr (WIN) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lane_max[rt] = max8(sv[rt]);
+      }
     } else {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -1009,15 +1204,19 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
             else
               sv[rt][kt][i] = (key > lim[rt] || key >= k_end) ? -INFINITY : acc[rt][kt][i];
           }
+      if constexpr (WIN) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) lane_max[rt] = max8(sv[rt]);
+      }
     }
     float m_tile[RT];
     bool raise_any = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      float tmax = fmaxf(fmaxf(fmaxf(sv[rt][0][0], sv[rt][0][1]), fmaxf(sv[rt][0][2], sv[rt][0][3])),
-                         fmaxf(fmaxf(sv[rt][1][0], sv[rt][1][1]), fmaxf(sv[rt][1][2], sv[rt][1][3])));
-      tmax = max_xor32(max_xor16(tmax));
-      m_tile[rt] = tmax * score_scale;
+      float tmax;
+      if constexpr (WIN) tmax = max_lanes_16_32(lane_max[rt]);
+      else tmax = max_xor32(max_xor16(max8(sv[rt])));
+      m_tile[rt] = tmax * scale_log2(rt);
       raise_any |= m_tile[rt] > m_run[rt] + kSlack;
     }
     if (__builtin_amdgcn_ballot_w64(raise_any)) {
@@ -1042,7 +1241,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], score_scale, -m_use));
+          p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], scale_log2(rt), -m_use));
           psum += p[kt][i];
         }
       l_run[rt] += psum;
@@ -1051,14 +1250,14 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            if constexpr (WIN) p[kt][i] = times_f16(p[kt][i], raw.vs[kt][i >> 1], i & 1);
-            else p[kt][i] *= scale_of(raw.vs[kt], i);
-          }
-        pb[rt][0] = pack_f16x2(p[0][0], p[0][1]);
-        pb[rt][1] = pack_f16x2(p[0][2], p[0][3]);
-        pb[rt][2] = pack_f16x2(p[1][0], p[1][1]);
-        pb[rt][3] = pack_f16x2(p[1][2], p[1][3]);
+          for (int i = 0; i < 4; ++i)
+            if constexpr (!WIN) p[kt][i] *= scale_of(raw.vs[kt], i);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int kt = w >> 1, i = 2 * (w & 1);
+          if constexpr (WIN) pb[rt][w] = pair_times_f16(p[kt][i], p[kt][i + 1], raw.vs[kt][i >> 1]);
+          else pb[rt][w] = pack_f16x2(p[kt][i], p[kt][i + 1]);
+        }
       } else {
         pb[rt][0] = pack_bf16x2(p[0][0], p[0][1]);
         pb[rt][1] = pack_bf16x2(p[0][2], p[0][3]);
@@ -1090,7 +1289,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   // bit-reproducible: each wave's sum covers the same keys on every call); the wave whose
   // sequence reaches nfull also takes the split's partial tile.
   const int nfull = (k_end - k_begin) / kTileKeys;
-  auto pages = [&](int t, int64_t& p0, int64_t& p1) {
+  auto pages = [&](int t, Page& p0, Page& p1) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
     p0 = page_of(kb);
     p1 = page_of(kb + 16);
@@ -1103,14 +1302,48 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     own_partial |= v == nfull;
     return v;
   };
-  if constexpr (DB) {
+  if constexpr (kBufs > 2) {
+    // A ring of buffers: the loads of the wave's next kBufs - 1 tiles are in flight while one is
+    // computed (unconditional loads, as below).
+    Raw ring[kBufs];
+    const int tlast = nfull - 1;
+    Page nx0 = 0, nx1 = 0;
+    if (wave < nfull) {
+      load_full(ring[0], wave, first_pg0, first_pg1);
+#pragma unroll
+      for (int i = 1; i < kBufs - 1; ++i) {
+        pages(min(wave + i * kWaves, tlast), nx0, nx1);
+        load_full(ring[i], min(wave + i * kWaves, tlast), nx0, nx1);
+      }
+      pages(min(wave + (kBufs - 1) * kWaves, tlast), nx0, nx1);
+    }
+    stage_q();
+    start_scores();
+    own_partial = nfull % kWaves == wave;
+    if (wave < nfull) {
+      int t = wave;
+      vcheck(ring[0], t);
+      for (bool more = true; more;) {
+#pragma unroll
+        for (int i = 0; i < kBufs; ++i) {
+          load_full(ring[(i + kBufs - 1) % kBufs], min(t + (kBufs - 1) * kWaves, tlast), nx0, nx1);
+          pages(min(t + kBufs * kWaves, tlast), nx0, nx1);
+          compute_tile(ring[i], t);
+          t += kWaves;
+          vcheck(ring[(i + 1) % kBufs], min(t, tlast));
+          more = t < nfull;
+          if (!more) break;
+        }
+      }
+    }
+  } else if constexpr (DB) {
     // Loads inside the loop are unconditional (an index past the last full tile repeats it,
     // already cached, and is never computed), so each compute waits only for its own
     // buffer's loads and the other buffer's stay in flight.
     Raw bufA, bufB;
     const int tlast = nfull - 1;
     int tA = wave;
-    int64_t nx0 = 0, nx1 = 0;  // pages of the wave's next tile to load
+    Page nx0 = 0, nx1 = 0;  // pages of the wave's next tile to load
     // fused: a first tile holding keys this launch writes ([L - n, L)) loads after the barrier
     const bool defer = fused && k_begin + (tA + 1) * kTileKeys > L - n;
     if (tA < nfull && !defer) load_full(bufA, tA, first_pg0, first_pg1);
@@ -1140,7 +1373,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
     }
   } else {
     Raw buf;
-    int64_t nx0 = 0, nx1 = 0;
+    Page nx0 = 0, nx1 = 0;
     int t = wave;
     if (t < nfull) {
       nx0 = first_pg0;
@@ -1159,7 +1392,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
   }
   if (nfull < ntiles && own_partial) {
     Raw buf;
-    int64_t p0, p1;
+    Page p0, p1;
     pages(nfull, p0, p1);
     load_partial(buf, nfull, p0, p1);
     vcheck(buf, nfull);
@@ -1179,7 +1412,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), blocks_per_cu(D, KV, RT)) void 
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int dt = 0; dt < kDt; ++dt) o[rt][dt] = o[rt][dt] * kI4VUnit - o[rt][kDt] * kI4VBias;
+      for (int dt = 0; dt < kDt; ++dt) o[rt][dt] = o[rt][dt] * kI4VUnit - o[rt][kDt] * kI4Bias;
   }
   // ---- merge the waves ----
   // the wave's o and l are relative to 2^(m_run + e_v) (e_v = 0 for bf16 KV)
@@ -1484,8 +1717,10 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
   using Raw = RawTile<D, KV>;
   constexpr bool INT8 = KV == kI8, INT4 = KV == kI4, CODES = KV != kBf16;
   constexpr int kKs = D / 32, kDt = D / 16, kElt = Raw::kElt, kKVec = Raw::kKVec;
-  constexpr int kKFrag = kStageKeys / 16 * kKs, kVFrag = kStageKeys / 32 * kDt;
-  __shared__ u32x4_t lk[2][kKFrag * 64];
+  constexpr int kKSub = INT4 ? D / 64 : kKs;  // 16-byte K chunks a lane and sub-tile (INT4: fp8 bytes)
+  constexpr int kKFrag = kStageKeys / 16 * kKSub, kVFrag = kStageKeys / 32 * kDt;
+  // two stages; at the end a wave's sums (2 kDt + 1 chunks, more than INT4's stages)
+  __shared__ u32x4_t lk[2][(kKFrag > kDt ? kKFrag : kDt + 1) * 64];
   __shared__ u32x4_t lv[2][kVFrag * 64];
   __shared__ uint16_t lsv[2][kStageKeys];
   __shared__ uint16_t lsk[INT4 ? 2 : 1][kStageKeys];
@@ -1553,21 +1788,43 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
       const int d = INT4   ? D / 4 * grp + 8 * ks
                     : INT8 ? 64 * (ks >> 1) + 16 * grp + 8 * (ks & 1) : 32 * ks + 8 * grp;
       qop[rt][ks] = r < R ? *reinterpret_cast<const u32x4_t*>(a.q + qoff + d) : u32x4_t{0, 0, 0, 0};
-      if constexpr (INT4) qop[rt][ks] = permute_q8(qop[rt][ks]);
     }
   }
-  const I4Const i4;
-  float score0[2];  // INT4: what the score accumulators start at (kI4KBias)
+  // INT4: the two parts of the rows as operands, what the score accumulators start at, and the rows'
+  // scales of the sums in the log2 domain
+  constexpr int kParts = D / 64;
+  F8Operand q8[2][kParts];
+  float score0[2], row_scale[2];
   if constexpr (INT4) {
-    constexpr uint32_t one = 0x3f803f80u;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) amax = max_u16x2(amax, qop[rt][ks][e] & 0x7fff7fffu);
+      amax = max(amax & 0xffffu, amax >> 16);
+      amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 16, 64)));
+      amax = max(amax, static_cast<uint32_t>(__shfl_xor(static_cast<int>(amax), 32, 64)));
+      const int exponent = q_exponent_i4(amax);
+      row_scale[rt] = row_scale_i4(a.scale_log2, exponent);
+      QBytes b[kKs];  // of 8 elements each: D / 4 adjacent ones a lane
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks) b[ks] = q_bytes_i4(qop[rt][ks], exponent);
+      auto four = [](u32x2_t x, u32x2_t y) { return u32x4_t{x[0], x[1], y[0], y[1]}; };
+      if constexpr (D == 128) {
+        q8[rt][0] = F8Operand{four(b[0].first, b[1].first), four(b[2].first, b[3].first)};
+        q8[rt][1] = F8Operand{four(b[0].second, b[1].second), four(b[2].second, b[3].second)};
+      } else {
+        q8[rt][0] = F8Operand{four(b[0].first, b[1].first), four(b[0].second, b[1].second)};
+      }
       f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) sum = mfma_bf16(u32x4_t{one, one, one, one}, qop[rt][ks], sum);
-      score0[rt] = sum[0] * -kI4KBias;
+      for (int part = 0; part < kParts; ++part) sum = mfma_f8(k_zero_i4(), q8[rt][part], sum);
+      score0[rt] = -sum[0];
     }
   }
+  auto scale_log2 = [&](int rt) { return INT4 ? row_scale[rt] : a.scale_log2; };
   const int first_lim = L - n + row0 / a.G;                        // of the wave's first row
   const int last_lim = L - n + (min(row0 + 32, R) - 1) / a.G;      // and of its last
 
@@ -1647,7 +1904,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
   auto block_open = [&](int kb) { return kb + 31 <= L - n && (kb + 32 <= a.sinks || kb >= L - a.window); };
   auto store_stage = [&](const Staged& st, int s) {
     const int buf = s & 1;
-    u32x4_t* const kd = &lk[buf][wave * kKs * 64 + lane];
+    u32x4_t* const kd = &lk[buf][wave * kKSub * 64 + lane];
     if constexpr (INT8) {
       const float sk = f16_to_f32(static_cast<uint16_t>(st.ks));
       const float skb = -1152.0f * sk;
@@ -1664,7 +1921,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
       }
     } else if constexpr (INT4) {
 #pragma unroll
-      for (int ks = 0; ks < kKs; ++ks) kd[ks * 64] = k_operand_i4(st.k[0][ks], i4);
+      for (int c = 0; c < kParts; ++c) kd[c * 64] = k_bytes_i4(st.k[0][2 * c], st.k[0][2 * c + 1]);
       if (l16 == 0) *reinterpret_cast<u32x2_t*>(&lsk[buf][wave * 16 + grp * 4]) = st.ks4;
     } else {
 #pragma unroll
@@ -1757,7 +2014,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
   auto tile_seen = [&](int kb) { return kb <= last_lim && (kb < a.sinks || kb + 31 > first_lim - a.window); };
   auto compute_tile = [&](int s, int t0) {
     const int kb = stage_key(s) + 32 * t0, buf = s & 1;
-    const u32x4_t* const fk = &lk[buf][t0 * 2 * kKs * 64 + lane];
+    const u32x4_t* const fk = &lk[buf][t0 * 2 * kKSub * 64 + lane];
     const u32x4_t* const fv = &lv[buf][t0 * kDt * 64 + lane];
     f32x4_t acc[2][kSub];
 #pragma unroll
@@ -1768,8 +2025,18 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         else acc[rt][kt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
       }
     __builtin_amdgcn_sched_barrier(0);
+    if constexpr (INT4) {
 #pragma unroll
-    for (int ks = 0; ks < kKs; ++ks)
+      for (int kt = 0; kt < kSub; ++kt) {
+        const F8Operand kop{fk[kt * kKSub * 64], fk[(kt * kKSub + kKSub - 1) * 64]};
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+          for (int rt = 0; rt < 2; ++rt) acc[rt][kt] = mfma_f8(kop, q8[rt][part], acc[rt][kt]);
+      }
+    }
+#pragma unroll
+    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks)
 #pragma unroll
       for (int kt = 0; kt < kSub; ++kt) {
         const u32x4_t kop = fk[(kt * kKs + ks) * 64];
@@ -1777,9 +2044,9 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         for (int rt = 0; rt < 2; ++rt) acc[rt][kt] = mfma_bf16(kop, qop[rt][ks], acc[rt][kt]);
       }
     // two k-steps' fragments ahead of the MFMAs that take them (0x100: LDS reads, 8: MFMAs)
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * kSub, 0);
+    if constexpr (!INT4) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kSub, 0);
 #pragma unroll
-    for (int ks = 0; ks < kKs; ++ks) {
+    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks) {
       __builtin_amdgcn_sched_group_barrier(0x008, 2 * kSub, 0);
       if (ks + 2 < kKs) __builtin_amdgcn_sched_group_barrier(0x100, kSub, 0);
     }
@@ -1877,7 +2144,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
       for (int kt = 0; kt < kSub; ++kt)
         tmax = fmaxf(tmax, fmaxf(fmaxf(acc[rt][kt][0], acc[rt][kt][1]), fmaxf(acc[rt][kt][2], acc[rt][kt][3])));
       tmax = max_xor32(max_xor16(tmax));
-      m_tile[rt] = tmax * a.scale_log2;
+      m_tile[rt] = tmax * scale_log2(rt);
       raise_any |= m_tile[rt] > m_run[rt] + kSlack;
     }
     if (__builtin_amdgcn_ballot_w64(raise_any)) {
@@ -1900,7 +2167,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
       for (int kt = 0; kt < kSub; ++kt) {
         float pr[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = exp2_fast(fmaf(acc[rt][kt][i], a.scale_log2, -m_use));
+        for (int i = 0; i < 4; ++i) pr[i] = exp2_fast(fmaf(acc[rt][kt][i], scale_log2(rt), -m_use));
         l_run[rt] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
         if constexpr (CODES) {
 #pragma unroll
@@ -1986,7 +2253,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
   }
   if (pair) {  // waves 2 and 3 hand their sums to waves 0 and 1
     constexpr int kWords = 2 * kDt + 1;
-    static_assert(kWords <= 2 * kKFrag && kWords <= 2 * kVFrag, "a wave's sums fit one staging array");
+    static_assert(kWords <= 2 * kVFrag, "a wave's sums fit one staging array");
     u32x4_t* const xch = (wave & 1 ? &lv[0][0] : &lk[0][0]) + lane;
     __syncthreads();
     if (tile == 1 && !idle) {
@@ -2325,6 +2592,9 @@ int attention_impl(const char* who, const FusedQkv* fz, int window, int sinks, i
     return COOPT_EWORKSPACE;
   }
   ATTN_REQUIRE(num_blocks > 0, "num_blocks must be positive");
+  ATTN_REQUIRE(!WIN || (num_blocks < (int64_t{1} << 31) && c_blk_stride >= 0 && s_blk_stride >= 0 &&
+                        c_blk_stride < (int64_t{1} << (codes ? 32 : 31)) && s_blk_stride < (int64_t{1} << 31)),
+               "pool or block stride out of range");
   // lanes address a page's rows with 32-bit byte offsets
   ATTN_REQUIRE(c_tok_stride > 0 && (block_size * c_tok_stride + D) * (codes ? 1 : 2) < (int64_t{1} << 31) &&
                    (!codes || (s_tok_stride >= 0 && block_size * s_tok_stride * 2 < (int64_t{1} << 31))),

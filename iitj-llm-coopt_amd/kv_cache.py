@@ -18,6 +18,7 @@ produces.
 import torch
 
 from . import _lib
+from .fused import LinearPartials
 
 __all__ = ["quantize", "dequantize", "reshape_and_cache_flash", "allocate_kv_cache",
            "qkv_rope_and_cache", "qkv_norm_rope_and_cache"]
@@ -184,8 +185,6 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
     return q [T, num_heads, head_dim].  `qkv` is the projection's bf16 output [T, (Hq + 2 Hkv)
     D] or its fused.LinearPartials (split-K partials, reduced here).  Bit for bit the same as
     rope_ + reshape_and_cache_flash on the reduced output."""
-    from .fused import LinearPartials
-
     Hq, Hkv, D = int(num_heads), int(num_kv_heads), int(head_dim)
     width = (Hq + 2 * Hkv) * D
     part = qkv if isinstance(qkv, LinearPartials) else None
@@ -240,6 +239,11 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
     return q_out
 
 
+_BF16 = torch.bfloat16
+_CACHE_KINDS = {"auto": (_lib.DT_BF16, torch.bfloat16, 1), "int8": (_lib.DT_I8, torch.int8, 1),
+                "int4": (_lib.DT_I4, torch.uint8, 2)}   # code, type, elements a unit of it holds
+
+
 def qkv_norm_rope_and_cache(qkv, q_weight, k_weight, eps, positions, cos, sin, k_cache, v_cache,
                             slot_mapping, num_heads, num_kv_heads, head_dim, kv_cache_dtype="auto",
                             k_scale=None, v_scale=None, q_out=None):
@@ -250,65 +254,77 @@ def qkv_norm_rope_and_cache(qkv, q_weight, k_weight, eps, positions, cos, sin, k
     q_weight, k_weight: bf16 [head_dim].  `qkv` is the projection's bf16 output [T, (Hq + 2 Hkv) D]
     or its fused.LinearPartials.  kv_cache_dtype "auto", "int8" or "int4", as in
     reshape_and_cache_flash; rows with slot < 0 write no cache entry.  head_dim 64, 128 or 256."""
-    from .fused import LinearPartials
-
     Hq, Hkv, D = int(num_heads), int(num_kv_heads), int(head_dim)
-    width = (Hq + 2 * Hkv) * D
-    part = qkv if isinstance(qkv, LinearPartials) else None
-    if part is not None:
-        if part.n != width:
-            raise ValueError(f"partials are {part.n} wide, expected {width}")
-        T, qkv_t = part.rows, part.buf
+    part = None
+    if isinstance(qkv, LinearPartials):
+        part, x, T, width, stride = qkv, qkv.buf, qkv.rows, qkv.n, 0
     else:
-        if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
-            raise ValueError(f"qkv must be bf16 [T, {width}] with contiguous rows")
-        T, qkv_t = qkv.shape[0], qkv
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w.dtype != torch.bfloat16 or w.shape != (D,) or w.stride(0) != 1:
-            raise ValueError(f"{name} must be bf16 [{D}], contiguous")
+        x = qkv
+        if x.dim() != 2 or x.dtype is not _BF16:
+            raise ValueError("qkv must be bf16 [T, (Hq + 2 Hkv) * D] with contiguous rows")
+        T, width = x.shape
+        stride, inner = x.stride()
+        if inner != 1 and width > 1:
+            raise ValueError("qkv must be bf16 [T, (Hq + 2 Hkv) * D] with contiguous rows")
+    if width != (Hq + 2 * Hkv) * D:
+        raise ValueError(f"qkv must be {(Hq + 2 * Hkv) * D} wide, got {width}")
+    kind = _CACHE_KINDS.get(kv_cache_dtype)
+    if kind is None:
+        raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
+    code, dtype, per_unit = kind
     _check_cache_pair(k_cache, v_cache)
     NB, bs, cH, cD = k_cache.shape
-    if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
-        raise ValueError(f"cache heads/dim {(cH, cD)} != ({Hkv}, {D})")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
-        raise ValueError("slot_mapping must be int64 with one entry per token")
-    if positions.dtype != torch.int64 or positions.numel() != T:
-        raise ValueError("positions must be int64 with one entry per token")
-    if cos.dim() != 2 or cos.shape != sin.shape or cos.stride() != sin.stride() or \
-            cos.shape[0] < 1 or cos.shape[1] < D // 2 or cos.dtype != torch.bfloat16 or \
-            sin.dtype != torch.bfloat16 or cos.stride(1) != 1:
-        raise ValueError("cos/sin tables must be bf16 [max_pos, >= D/2] alike")
-    if kv_cache_dtype == "auto":
-        if k_cache.dtype != torch.bfloat16 or v_cache.dtype != torch.bfloat16:
-            raise ValueError("'auto' caches are bf16")
-        code, ks, vs, sstr = _lib.DT_BF16, None, None, (0, 0, 0)
-    elif kv_cache_dtype in ("int8", "int4"):
-        if kv_cache_dtype == "int4":
-            _check_int4(k_cache, v_cache)
-        elif k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
-            raise ValueError("'int8' caches hold int8 codes")
-        sstr = _scale_args(k_cache, k_scale, v_scale, kv_cache_dtype)
-        code, ks, vs = _lib.DT_I8 if kv_cache_dtype == "int8" else _lib.DT_I4, k_scale, v_scale
+    if cH != Hkv or cD * per_unit != D:
+        raise ValueError(f"cache heads/dim {(cH, cD)} != ({Hkv}, {D // per_unit})")
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
+        raise ValueError(f"{kv_cache_dtype!r} caches hold {dtype}")
+    # one GPU for all of them (get_device() is -1 on the CPU; 0.04 us, a device object twice that)
+    index = x.get_device()
+    alike = index >= 0 and index == k_cache.get_device() == v_cache.get_device() == \
+        slot_mapping.get_device() == positions.get_device() == cos.get_device() == \
+        sin.get_device() == q_weight.get_device() == k_weight.get_device()
+    if code == _lib.DT_BF16:
+        ks = vs = s0 = s1 = s2 = 0
     else:
-        raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
-    if q_out is not None and (q_out.shape != (T, Hq, D) or q_out.dtype != torch.bfloat16 or
-                              q_out.stride(-1) != 1):
-        raise ValueError("q_out must be bf16 [T, Hq, D] with contiguous D")
-    dev = _lib.require_one_device(qkv_t, q_weight, k_weight, positions, cos, sin, k_cache, v_cache,
-                                  slot_mapping, ks, vs, q_out)
+        s0, s1, s2 = _scale_args(k_cache, k_scale, v_scale, kv_cache_dtype)
+        alike = alike and index == k_scale.get_device() == v_scale.get_device()
+        ks, vs = k_scale.data_ptr(), v_scale.data_ptr()
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w.dtype is not _BF16 or w.dim() != 1 or w.numel() != D or not w.is_contiguous():
+            raise ValueError(f"{name} must be bf16 [{D}], contiguous")
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.numel() != T:
+        raise ValueError("slot_mapping must be int64 with one entry per token")
+    if positions.dtype is not torch.int64 or positions.numel() != T:
+        raise ValueError("positions must be int64 with one entry per token")
+    if cos.dtype is not _BF16 or sin.dtype is not _BF16 or cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError("cos/sin tables must be bf16 [max_pos, >= D/2] alike")
+    rows, half = cos.shape
+    tab = cos.stride()
+    if tab != sin.stride() or tab[1] != 1 or half < D // 2 or rows < 1:
+        raise ValueError("cos/sin tables must be bf16 [max_pos, >= D/2] alike")
+    if q_out is not None:
+        if q_out.shape != (T, Hq, D) or q_out.dtype is not _BF16 or q_out.stride(-1) != 1:
+            raise ValueError("q_out must be bf16 [T, Hq, D] with contiguous D")
+        alike = alike and index == q_out.get_device()
+    if not alike:
+        _lib.require_one_device(x, q_weight, k_weight, positions, cos, sin, k_cache, v_cache, slot_mapping,
+                                k_scale if ks else None, v_scale if vs else None, q_out)
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+        q_out = cos.new_empty((T, Hq, D))
     if T == 0:
         return q_out
-    positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
-    cs = k_cache.stride()
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
+    c0, c1, c2, _ = k_cache.stride()
+    q0, q1, _ = q_out.stride()
     _lib.check(_lib.call_on(
-        dev, _lib.load().coopt_qkv_norm_epilogue, code, None if part is not None else _lib.ptr(qkv_t),
-        0 if part is not None else qkv_t.stride(0), None if part is None else _lib.ptr(part.buf),
-        0 if part is None else part.ks, 0 if part is None else part.rows_padded * part.n,
-        _lib.ptr(q_weight), _lib.ptr(k_weight), float(eps), _lib.ptr(positions), _lib.ptr(cos),
-        _lib.ptr(sin), cos.stride(0), cos.shape[0], _lib.ptr(q_out), q_out.stride(0),
-        q_out.stride(1), _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks),
-        _lib.ptr(vs), sstr[0], sstr[1], sstr[2], _lib.ptr(slot_mapping), T, Hq, Hkv, D, bs, NB,
-        _lib.stream_handle(dev)), "coopt_qkv_norm_epilogue")
+        index, _lib.entry("coopt_qkv_norm_epilogue"), code, 0 if part is not None else x.data_ptr(), stride,
+        0 if part is None else x.data_ptr(), 0 if part is None else part.ks,
+        0 if part is None else part.rows_padded * part.n, q_weight.data_ptr(), k_weight.data_ptr(),
+        eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), tab[0], rows, q_out.data_ptr(), q0,
+        q1, k_cache.data_ptr(), v_cache.data_ptr(), c0, c1, c2, ks, vs, s0, s1, s2,
+        slot_mapping.data_ptr(), T, Hq, Hkv, D, bs, NB, _lib.raw_stream(index)),
+        "coopt_qkv_norm_epilogue")
     return q_out

@@ -7,7 +7,9 @@ Tolerance, per output element, from the roundings the operator is allowed:
 u_p: a probability rounded to 16 bits next to its value (bf16 caches 2^-8; codes 2^-11, fp16);
 an INT8 value of the definition is itself rounded to bf16, which the kernel need not do (2^-8).
 ds: the error of a score: a product of D terms summed in fp32 in any order, D 2^-24 sum |q||k|,
-where a 4-bit key enters as code plus 24 (so |k| + 24 s), and 2^-22 of the score for the exponent.
+where a 4-bit key enters as code plus 8 (|k| + 24 s covers it), and 2^-22 of the score for the
+exponent.  Beside 4-bit keys q is the sum of two 4-bit numbers: its elements under 2^-9 of the row's
+largest are rounded to steps of 2^-17 of it, 2^-18 max|q| sum |k| at most.
 Both numerator and sum move by ds (2 ds).  2^-18 A covers the fp32 sums over up to 2^6 tiles, each
 a rounding of 2^-24 of the magnitudes summed so far.  A 4-bit value is summed as code plus 8, and 8
 times the sum of w s is taken off at the end: the magnitudes summed are |v| + 8 s, not |v| alone, so
@@ -51,6 +53,8 @@ def closed_form(q, K, V, scale, window, sinks, kv, s_k, s_v):
             if kv == "int4":
                 mag = mag + 24 * s_k[see, g] * np.abs(q[j, h]).sum()
             ds = (D * 2.0 ** -24 * mag * scale).max() + 2.0 ** -22 * np.abs(s).max()
+            if kv == "int4":
+                ds += 2.0 ** -18 * np.abs(q[j, h]).max() * np.abs(Ks).sum(1).max() * scale
             u_p = {"auto": 2.0 ** -8, "int8": 2.0 ** -11 + 2.0 ** -8, "int4": 2.0 ** -11}[kv]
             A = w @ np.abs(Vs)
             summed = A + (8 * (w @ s_v[see, g]) if kv == "int4" else 0)
