@@ -79,20 +79,9 @@ constexpr int kThreads = 256;  // merge kernel
 constexpr int waves_for(int RT) { return RT <= 3 ? 8 : 4; }
 // Waves a SIMD is to hold: two blocks a CU with 4 waves at head dim 64 and bf16 (79 KB of LDS, at most 256
 // registers asked for), where batches of many query windows take 0.63 to 0.8 of the time; see alone_lds.
-constexpr int waves_per_simd(int D, int kv, int RT, bool win) {
-#ifdef W64
-  if (win && D == 64 && RT == 1) return W64;
-#endif
+constexpr int waves_per_simd(int D, int kv, int RT, bool sc, bool win) {
+  if (win && D == 64 && RT == 1 && kv == kI4 && sc) return 4;
   return D == 64 && kv == kBf16 && RT == 4 ? 2 : 1;
-}
-// Tile buffers of a wave: its loads in flight are this many less one.  A 4-bit tile is a quarter of a
-// bf16 one (4 KB at head dim 128), and it takes bytes in flight to cover the memory's latency.
-constexpr int tile_buffers(int D, int kv, int RT, bool sc, bool win) {
-#ifdef NB1
-  if (win && kv == kI4) return !sc ? (RT <= 2 ? 2 : 1) : RT == 1 ? (D == 128 ? NB1 : NB64) : RT == 2 ? NB2 : 1;
-#endif
-  if (win && kv == kI4) return RT > 2 ? 1 : !sc ? 2 : RT == 1 ? 4 : 3;
-  return RT <= 2 || (kv == kI8 && RT == 3 && !win) ? 2 : 1;
 }
 constexpr int kTileKeys = 32;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -282,15 +271,24 @@ __device__ __forceinline__ void buffer_load(buffer_t b, uint32_t off, T& dst) {
   }
 }
 
-// max of own and partner's value as max_xor16 / max_xor32, and of two values, one instruction each: a
-// median with infinity (fmaxf also quiets its operands, which are no signalling NaN here).
-__device__ __forceinline__ float max_med(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, INFINITY); }
-__device__ __forceinline__ float max_lanes_16_32(float v) {
-  u32x2_pl_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = max_med(__uint_as_float(r[0]), __uint_as_float(r[1]));
-  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return max_med(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
+// Maxima of one instruction, medians with infinity: fmaxf also quiets each operand (a v_max of its own)
+// unless the compiler knows that it is no signalling NaN.  `inf` is kept from the compiler, which would
+// make the median an fmaxf again.
+struct Maxima {
+  float inf = INFINITY;
+  __device__ __forceinline__ Maxima() { asm("" : "+s"(inf)); }
+  __device__ __forceinline__ float of(float a, float b) const { return __builtin_amdgcn_fmed3f(a, b, inf); }
+  __device__ __forceinline__ float of8(const float (&x)[2][4]) const {
+    return of(of(of(x[0][0], x[0][1]), of(x[0][2], x[0][3])), of(of(x[1][0], x[1][1]), of(x[1][2], x[1][3])));
+  }
+  // over the four lanes 16 apart
+  __device__ __forceinline__ float of_groups(float v) const {
+    u32x2_pl_t r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return of(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  }
+};
 
 __device__ __forceinline__ int64_t clamp_page(int32_t page, int64_t num_blocks) {
   return page < 0 ? 0 : (page >= num_blocks ? num_blocks - 1 : page);
@@ -539,15 +537,14 @@ __device__ void plan_item(const AttnArgs& a, int lane, int* out) {
 // (a run-time choice of input made the compiler wait for every earlier load where the two
 // input paths joined).
 template <int D, int KV, int RT, bool SC, int FUSED, bool WIN>
-__global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN)) void verify_attn_kernel(
+__global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, WIN)) void verify_attn_kernel(
     const int32_t* cu_p, const int32_t* sl_p, const int32_t* bt_p, int64_t bt_stride, int split,
     int bs_shift, int mode, AttnArgs a) {
   using Raw = RawTile<D, KV>;
   constexpr bool INT8 = KV == kI8, INT4 = KV == kI4, CODES = KV != kBf16;
   constexpr int kWaves = waves_for(RT);
   constexpr int kBlock = 64 * kWaves;
-  constexpr int kBufs = tile_buffers(D, KV, RT, SC, WIN);
-  constexpr bool DB = kBufs == 2;
+  constexpr bool DB = RT <= 2 || (INT8 && RT == 3 && !WIN);
   constexpr int kKs = D / 32;   // k-steps of the score MFMA
   constexpr int kDt = D / 16;   // d-tiles of the output = V elements per lane per key
   constexpr int kElt = Raw::kElt;
@@ -781,7 +778,27 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
     const unsigned char* src = qlds + rt * 16 * kQPitch + (D == 128 ? part * D + grp * 32 : grp * 16);
     return F8Operand{*reinterpret_cast<const u32x4_t*>(src), *reinterpret_cast<const u32x4_t*>(src + (D == 128 ? 16 : D))};
   };
+  // Q operands of all row tiles, read before the next tile's loads go out so that their way from LDS
+  // is not waited for; with one row tile and registers to spare they stay there
+  struct QOperands {
+    F8Operand x[INT4 ? RT : 1][INT4 ? kParts : 1];
+  };
+  constexpr bool kQEarly = INT4 && RT <= 2;
+  constexpr bool kQKept = kQEarly && RT == 1 && D == 128;
+  QOperands q_kept;
+  auto read_q = [&]() {
+    QOperands q;
+    if constexpr (kQEarly) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) q.x[rt][part] = q_operand(rt, part);
+    }
+    return q;
+  };
+  auto tile_q = [&]() { return kQKept ? q_kept : read_q(); };
   auto start_scores = [&]() {
+    if constexpr (kQKept) q_kept = read_q();
     if constexpr (INT4) {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
@@ -1025,7 +1042,8 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
   auto tile_open = [&](int kb) {
     return kb + kTileKeys - 1 <= min_lim && (kb + kTileKeys <= a.sinks || kb >= L - a.window);
   };
-  auto compute_tile = [&](Raw& raw, int t) {
+  const Maxima maxima;
+  auto compute_tile = [&](Raw& raw, int t, const QOperands& q) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
     // every key of the tile inside the split and visible to every row: no masking
     const bool open = WIN ? tile_open(kb) : kb + kTileKeys <= k_end && kb + kTileKeys - 1 <= min_lim;
@@ -1122,7 +1140,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
       for (int part = 0; part < kParts; ++part)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          const F8Operand qop = q_operand(rt, part);
+          const F8Operand qop = kQEarly ? q.x[rt][part] : q_operand(rt, part);
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = mfma_f8(kop[kt], qop, acc[rt][kt]);
         }
@@ -1172,13 +1190,6 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
     // sums), and the accumulators are rescaled only on those rare raises (one branch per
     // tile, taken by the whole wave).
     constexpr float kSlack = 8.0f;
-    // WIN: the lane's maximum of the row, formed where the scores are the sums' own (known not to need
-    // quieting) or masked
-    float lane_max[RT];
-    auto max8 = [](const float (&x)[2][4]) {
-      return fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                   fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-    };
     float sv[RT][2][4];  // raw scores (the scale is applied in the exponent); masked -inf
     if (open) {  // one uniform branch for the whole tile
 #pragma unroll
@@ -1187,10 +1198,6 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sv[rt][kt][i] = acc[rt][kt][i];
-      if constexpr (WIN) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lane_max[rt] = max8(sv[rt]);
-      }
     } else {
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -1204,18 +1211,19 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
             else
               sv[rt][kt][i] = (key > lim[rt] || key >= k_end) ? -INFINITY : acc[rt][kt][i];
           }
-      if constexpr (WIN) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) lane_max[rt] = max8(sv[rt]);
-      }
     }
     float m_tile[RT];
     bool raise_any = false;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       float tmax;
-      if constexpr (WIN) tmax = max_lanes_16_32(lane_max[rt]);
-      else tmax = max_xor32(max_xor16(max8(sv[rt])));
+      if constexpr (WIN) {
+        tmax = maxima.of_groups(maxima.of8(sv[rt]));
+      } else {
+        tmax = fmaxf(fmaxf(fmaxf(sv[rt][0][0], sv[rt][0][1]), fmaxf(sv[rt][0][2], sv[rt][0][3])),
+                     fmaxf(fmaxf(sv[rt][1][0], sv[rt][1][1]), fmaxf(sv[rt][1][2], sv[rt][1][3])));
+        tmax = max_xor32(max_xor16(tmax));
+      }
       m_tile[rt] = tmax * scale_log2(rt);
       raise_any |= m_tile[rt] > m_run[rt] + kSlack;
     }
@@ -1242,8 +1250,10 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], scale_log2(rt), -m_use));
-          psum += p[kt][i];
+          if constexpr (!WIN) psum += p[kt][i];
         }
+      if constexpr (WIN)
+        psum = ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
       l_run[rt] += psum;
       if constexpr (CODES) {
         // P' = p * s_v of the lane's key j = 4 kt + i, in fp16 next to the fp16 codes
@@ -1302,41 +1312,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
     own_partial |= v == nfull;
     return v;
   };
-  if constexpr (kBufs > 2) {
-    // A ring of buffers: the loads of the wave's next kBufs - 1 tiles are in flight while one is
-    // computed (unconditional loads, as below).
-    Raw ring[kBufs];
-    const int tlast = nfull - 1;
-    Page nx0 = 0, nx1 = 0;
-    if (wave < nfull) {
-      load_full(ring[0], wave, first_pg0, first_pg1);
-#pragma unroll
-      for (int i = 1; i < kBufs - 1; ++i) {
-        pages(min(wave + i * kWaves, tlast), nx0, nx1);
-        load_full(ring[i], min(wave + i * kWaves, tlast), nx0, nx1);
-      }
-      pages(min(wave + (kBufs - 1) * kWaves, tlast), nx0, nx1);
-    }
-    stage_q();
-    start_scores();
-    own_partial = nfull % kWaves == wave;
-    if (wave < nfull) {
-      int t = wave;
-      vcheck(ring[0], t);
-      for (bool more = true; more;) {
-#pragma unroll
-        for (int i = 0; i < kBufs; ++i) {
-          load_full(ring[(i + kBufs - 1) % kBufs], min(t + (kBufs - 1) * kWaves, tlast), nx0, nx1);
-          pages(min(t + kBufs * kWaves, tlast), nx0, nx1);
-          compute_tile(ring[i], t);
-          t += kWaves;
-          vcheck(ring[(i + 1) % kBufs], min(t, tlast));
-          more = t < nfull;
-          if (!more) break;
-        }
-      }
-    }
-  } else if constexpr (DB) {
+  if constexpr (DB) {
     // Loads inside the loop are unconditional (an index past the last full tile repeats it,
     // already cached, and is never computed), so each compute waits only for its own
     // buffer's loads and the other buffer's stay in flight.
@@ -1355,16 +1331,18 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
       int tB = grab();
       pages(min(tB, tlast), nx0, nx1);
       for (;;) {
+        const QOperands qA = tile_q();
         load_full(bufB, min(tB, tlast), nx0, nx1);
         const int tA2 = tB < nfull ? grab() : nfull;
         pages(min(tA2, tlast), nx0, nx1);
-        compute_tile(bufA, tA);
+        compute_tile(bufA, tA, qA);
         vcheck(bufB, min(tB, tlast));
         if (tB >= nfull) break;
+        const QOperands qB = tile_q();
         load_full(bufA, min(tA2, tlast), nx0, nx1);
         const int tB2 = tA2 < nfull ? grab() : nfull;
         pages(min(tB2, tlast), nx0, nx1);
-        compute_tile(bufB, tB);
+        compute_tile(bufB, tB, qB);
         vcheck(bufA, min(tA2, tlast));
         if (tA2 >= nfull) break;
         tA = tA2;
@@ -1386,7 +1364,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
       const int tn = grab();
       if (tn < nfull) pages(tn, nx0, nx1);
       vcheck(buf, t);
-      compute_tile(buf, t);
+      compute_tile(buf, t, tile_q());
       t = tn;
     }
   }
@@ -1396,7 +1374,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
     pages(nfull, p0, p1);
     load_partial(buf, nfull, p0, p1);
     vcheck(buf, nfull);
-    compute_tile(buf, nfull);
+    compute_tile(buf, nfull, tile_q());
   }
   if constexpr (WIN) {
     if (__builtin_amdgcn_ballot_w64(not_finite != 0))
@@ -1588,9 +1566,12 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, WIN))
     // keys [0, L) end where the window's last row's causal limit does
     L = min(sl, a.max_seqlen_k) - (nall - j0 - n);
   } else {
-    b = blockIdx.z;
-    hkv = blockIdx.y;
-    sidx = blockIdx.x;
+    // WIN: KV heads first, splits last.  Blocks go to the XCDs and their CUs in turn; with the splits
+    // among the first, those that only the longest sequences have (the other sequences' end at once)
+    // all fall on the same ones.
+    b = WIN ? blockIdx.y : blockIdx.z;
+    hkv = WIN ? blockIdx.x : blockIdx.y;
+    sidx = WIN ? blockIdx.z : blockIdx.x;
     // every scalar the block's first loads depend on, in one round: the row range, the key
     // count and the first tile's pages, and the kernel-argument lines the Q / K / V (or
     // epilogue) addressing reads.  The empty asm keeps these loads from being spread over the
@@ -2306,16 +2287,18 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
 // are not split however few the items are (1 sequence, 8 KV heads, bf16, 1 row, 400 keys: 9.0 us
 // whole, the merge launch alone costs 3); past that a split may be as short as one round (717
 // keys: 11.6 us whole, 11.8 in splits of two rounds, 9.8 of one; 4096 keys: 13.2 and 11.7).
-constexpr int kWholeRounds = 2;
+// INT4 contexts of up to kWholeRoundsI4 rounds are not split either (1 sequence, 8 KV heads, 1 row of 128:
+// 600 keys 8.9 us whole, 10.6 split; 1000 keys 11.4 and 10.4; the merge's launch costs the host 3 more).
+constexpr int kWholeRounds = 2, kWholeRoundsI4 = 3;
 int target_blocks(int waves) { return waves == 8 ? 256 : 512; }
 
-int choose_split(int B, int Hkv, int max_seqlen_k, int waves) {
+int choose_split(int B, int Hkv, int max_seqlen_k, int waves, int whole_rounds) {
   const int64_t items = static_cast<int64_t>(B) * Hkv;
   const int64_t target = target_blocks(waves);
   const int64_t gran = 32 * waves;
   int64_t per = (static_cast<int64_t>(max_seqlen_k) * items + target - 1) / target;
   per = ((per + gran - 1) / gran) * gran;
-  if (max_seqlen_k <= kWholeRounds * gran && per < max_seqlen_k) per = kWholeRounds * gran;
+  if (max_seqlen_k <= whole_rounds * gran && per < max_seqlen_k) per = whole_rounds * gran;
   if (per > 65536) per = 65536;
   return static_cast<int>(per);
 }
@@ -2395,7 +2378,8 @@ bool prefill_is_faster(int B, int G, int Hkv, int D, int max_seqlen_q, int max_s
 
 // total_q: the call's query rows, 0 if unknown (one row for every sequence but the longest then);
 // it and int8 decide between the window kernels only, not any workspace.
-AttnShape attn_shape(int B, int G, int Hkv, int D, int max_seqlen_q, int max_seqlen_k, int64_t total_q, bool int8) {
+AttnShape attn_shape(int B, int G, int Hkv, int D, int max_seqlen_q, int max_seqlen_k, int64_t total_q, bool int8,
+                     int whole_rounds = kWholeRounds) {
   AttnShape s{};
   if (G * static_cast<int64_t>(max_seqlen_q) > kMaxRows) {
     // longer items run in query windows of kMaxRows (verify_attn_kernel: a wave's tiles are its
@@ -2411,7 +2395,7 @@ AttnShape attn_shape(int B, int G, int Hkv, int D, int max_seqlen_q, int max_seq
   }
   s.rmax = G * max_seqlen_q;
   const int waves = waves_for((s.rmax + 15) / 16);
-  s.split = choose_split(B, Hkv, max_seqlen_k, waves);
+  s.split = choose_split(B, Hkv, max_seqlen_k, waves, whole_rounds);
   s.max_splits = (max_seqlen_k + s.split - 1) / s.split;
   s.plan = B <= kPlanSeqs && static_cast<int64_t>(B) * Hkv > target_blocks(waves) &&
            s.max_splits == 1;
@@ -2631,7 +2615,9 @@ int attention_impl(const char* who, const FusedQkv* fz, int window, int sinks, i
   a.o_hs = o_head_stride;
   a.window = window;
   a.sinks = sinks;
-  const AttnShape shape = attn_shape(B, G, Hkv, D, max_seqlen_q, keys, total_q, codes);
+  // (more whole rounds: fewer splits than the workspace is sized for)
+  const AttnShape shape = attn_shape(B, G, Hkv, D, max_seqlen_q, keys, total_q, codes,
+                                     kv_dtype == COOPT_DT_I4 ? kWholeRoundsI4 : kWholeRounds);
   // grid limits: 2^32 work-items along x, 65535 blocks along z
   ATTN_REQUIRE(shape.nwin == 0 || static_cast<int64_t>(B) * shape.nwin * Hkv < (int64_t{1} << 24),
                "too many query windows for one launch");
@@ -2685,7 +2671,10 @@ int attention_impl(const char* who, const FusedQkv* fz, int window, int sinks, i
 
   const int RT = (a.rmax + 15) / 16;
   const dim3 grid = shape.nwin > 0 ? dim3(B * shape.nwin * Hkv)
-                    : (shape.plan ? dim3(B * Hkv) : dim3(a.max_splits, Hkv, B));
+                    : shape.plan   ? dim3(B * Hkv)
+                    : WIN          ? dim3(Hkv, B, a.max_splits)
+                                   : dim3(a.max_splits, Hkv, B);
+  ATTN_REQUIRE(!WIN || shape.nwin > 0 || shape.plan || a.max_splits <= 65535, "too many splits for one launch");
   auto s = static_cast<hipStream_t>(stream);
   // scale caches with consecutive tokens adjacent and 8-byte aligned groups of four
   const bool sc = codes && s_tok_stride == 1 && s_blk_stride % 4 == 0 && s_head_stride % 4 == 0 &&
