@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/coopt_amd.h"
+#include <initializer_list>
 
 #define COOPT_WAVE 64
 
@@ -28,6 +29,13 @@ int check_launch(const char* what);
 const char* cache_write_error(int cache_dtype, const void* k_cache, const void* v_cache,
                               int64_t c_blk_stride, int64_t c_tok_stride, int64_t c_head_stride,
                               const void* k_scale, const void* v_scale);
+
+// Every stride fits 32 bits: the kernels multiply them in one instruction.
+inline bool narrow_strides(std::initializer_list<int64_t> strides) {
+  for (const int64_t s : strides)
+    if (s < -(int64_t{1} << 31) || s >= (int64_t{1} << 31)) return false;
+  return true;
+}
 
 }  // namespace coopt
 
@@ -96,6 +104,8 @@ __device__ __forceinline__ float add_xor32(float v) {
 namespace dpp {
 constexpr int kXor1 = 0xB1;        // quad_perm [1,0,3,2]: lane i ^ 1
 constexpr int kXor2 = 0x4E;        // quad_perm [2,3,0,1]: lane i ^ 2
+constexpr int kXor3 = 0x1B;        // quad_perm [3,2,1,0]: lane i ^ 3
+constexpr int kRowRor8 = 0x128;    // lane i ^ 8 within the row
 constexpr int kRowShr1 = 0x111;    // lane i - 1 within the row
 constexpr int kRowShr2 = 0x112;
 constexpr int kRowShr4 = 0x114;
@@ -233,6 +243,17 @@ __device__ __forceinline__ float group_sum_f32(float v) {
   if constexpr (G >= 32) v = add_xor16(v);
   if constexpr (G >= 64) v = add_xor32(v);
   return v;
+}
+
+// v of lane i ^ (G / 2) of aligned groups of G = 8, 16 or 32 lanes.
+template <int G>
+__device__ __forceinline__ float group_other_half(float v) {
+  static_assert(G == 8 || G == 16 || G == 32, "G must be 8, 16 or 32");
+  if constexpr (G == 8) return dpp_f32<dpp::kXor3>(dpp_f32<dpp::kRowHalfMirror>(v));  // i ^ 7 ^ 3
+  else if constexpr (G == 16) return dpp_f32<dpp::kRowRor8>(v);
+  const uint32_t u = __float_as_uint(v);
+  const u32x2_pl_t r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return __uint_as_float(threadIdx.x & 16 ? r[0] : r[1]);
 }
 
 __device__ __forceinline__ float wave_max_f32(float v) {

@@ -29,8 +29,8 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   // The K and V chunks load with the slot (none depends on another); the empty asm takes all
   // three, so the compiler neither sinks the K / V loads past the slot test nor waits for the
   // slot before issuing them: one memory round trip instead of two.
-  const uint4 kr = *reinterpret_cast<const uint4*>(k + t * k_ts + h * k_hs + c * 8);
-  const uint4 vr = *reinterpret_cast<const uint4*>(v + t * v_ts + h * v_hs + c * 8);
+  const uint4 kr = *reinterpret_cast<const uint4*>(k + stride_mul<KV>(t, k_ts) + h * k_hs + c * 8);
+  const uint4 vr = *reinterpret_cast<const uint4*>(v + stride_mul<KV>(t, v_ts) + h * v_hs + c * 8);
   const int64_t slot = slot_mapping[t];
   asm volatile("" ::"v"(kr.x), "v"(kr.y), "v"(kr.z), "v"(kr.w), "v"(vr.x), "v"(vr.y), "v"(vr.z),
                "v"(vr.w), "v"(slot));
@@ -39,8 +39,10 @@ __global__ __launch_bounds__(256) void kv_write_kernel(
   const int64_t blk = bs_shift >= 0 ? slot >> bs_shift : slot / block_size;
   const int64_t off = bs_shift >= 0 ? slot & ((int64_t{1} << bs_shift) - 1) : slot % block_size;
 
-  const int64_t c_off = blk * c_bs + off * c_ts + h * c_hs + c * chunk_step<KV>();
-  store_kv_chunk<G, KV>(kr, vr, kc, vc, c_off, ks, vs, blk * s_bs + off * s_ts + h * s_hs, c);
+  const int64_t c_off =
+      stride_mul<KV>(blk, c_bs) + stride_mul<KV>(off, c_ts) + h * c_hs + c * chunk_step<KV>();
+  store_kv_chunk<G, KV>(kr, vr, kc, vc, c_off, ks, vs,
+                        stride_mul<KV>(blk, s_bs) + stride_mul<KV>(off, s_ts) + h * s_hs, c);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -970,6 +972,11 @@ extern "C" int coopt_kv_write(int cache_dtype, const void* k, const void* v, int
                                                  c_head_stride, k_scale, v_scale)) {
     coopt::set_error(std::string(__func__) + ": " + bad);
     return COOPT_EINVAL;
+  }
+  if (cache_dtype == COOPT_DT_I4) {
+    const bool narrow = num_blocks < (int64_t{1} << 31) &&
+                        coopt::narrow_strides({k_tok_stride, v_tok_stride, c_blk_stride, c_tok_stride, s_blk_stride, s_tok_stride});
+    COOPT_REQUIRE(narrow, "INT4 caches: strides and num_blocks must stay below 2^31");
   }
   coopt::clear_error();
   const int64_t num_slots = num_blocks * block_size;

@@ -97,6 +97,34 @@ __device__ __forceinline__ uint2 quant_pack8_i8(const uint32_t (&w)[4], float s3
   return make_uint2(lo, hi);
 }
 
+// quant_codes8<7> of the 8 bf16 elements in w[0..3], offset by +8, element e in nibble e of the
+// word: quant_pack8_i8's steps with +-7 and 1.5 * 2^23 + 8, whose sums hold code + 8 (1..15) in
+// their low nibble and nothing in the rest of their low byte.
+__device__ __forceinline__ uint32_t quant_pack8_i4(const uint32_t (&w)[4], float s32) {
+  constexpr float kMagic = 12582920.0f;  // 1.5 * 2^23 + 8
+  const float r32 = __builtin_amdgcn_rcpf(s32);
+  float x[8], f[8];
+  bool near = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = bf16_to_f32(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
+    const float q = fminf(fmaxf(x[e] * r32, -7.0f), 7.0f);
+    f[e] = q + kMagic;
+    near |= fabsf(q - (f[e] - kMagic)) >= 0.5f - kNearTie;
+  }
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = fminf(fmaxf(x[e] / s32, -7.0f), 7.0f) + kMagic;
+  }
+  uint32_t b[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) b[e] = __float_as_uint(f[e]);
+  // byte j of `even` / `odd`: element 2 j's / 2 j + 1's
+  const uint32_t even = __builtin_amdgcn_perm(b[2], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[6], b[4], 0x04000c0cu);
+  const uint32_t odd = __builtin_amdgcn_perm(b[3], b[1], 0x0c0c0400u) | __builtin_amdgcn_perm(b[7], b[5], 0x04000c0cu);
+  return even | (odd << 4);
+}
+
 // INT8 codes of two adjacent chunks (16 elements, words of a and b) of a vector covered by
 // G2 lanes, two chunks a lane: the codes and scale quant_chunk<2 G2, 8> gives the two chunks'
 // lanes, as one 16-byte word.  Every lane of the group must call it together.
@@ -125,6 +153,14 @@ __device__ __forceinline__ QuantPair quant_pair8(const uint4& a, const uint4& b)
 template <int KV>
 constexpr int chunk_step() { return KV == kI4 ? 4 : 8; }
 
+// index * stride of an address.  INT4 calls have both below 2^31 (narrow_strides, checked by the host): one
+// 32 x 32 product instead of four.
+template <int KV>
+__device__ __forceinline__ int64_t stride_mul(int64_t index, int64_t stride) {
+  if constexpr (KV == kI4) return static_cast<int64_t>(static_cast<int32_t>(index)) * static_cast<int32_t>(stride);
+  else return index * stride;
+}
+
 // The INT4 codes of the group's vector (element e of the chunk in nibble e, offset by +8, as
 // coopt_quantize packs them) at the lane's place, and its fp16 scale.
 template <int G>
@@ -134,11 +170,7 @@ __device__ __forceinline__ void store_chunk_i4(const uint32_t (&w)[4], uint8_t* 
   for (int i = 0; i < 4; ++i) amax = max(amax, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
   amax = group_max_u32<G>(amax);
   const float s32 = quant_scale<7>(bf16_to_f32(static_cast<uint16_t>(amax)));
-  int code[8];
-  quant_codes8<7>(w, s32, code);
-  uint32_t word = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) word |= static_cast<uint32_t>(code[e] + 8) << (4 * e);
+  const uint32_t word = quant_pack8_i4(w, s32);
   __builtin_nontemporal_store(word, reinterpret_cast<uint32_t*>(dst));
   if (c == 0) *scale = f32_to_f16(s32);
 }

@@ -32,22 +32,24 @@ struct QkNormArgs {
   uint16_t* v_scale;
   int64_t s_bs, s_ts, s_hs;
   const int64_t* slot_mapping;
-  int T, Hq, Hkv, block_size;
+  int Hq, Hkv, block_size, bs_shift;  // bs_shift: log2(block_size) of a power of two, else -1
   int64_t num_slots;
-  int blocks_per_token;
 };
 
+constexpr int kMaxThreads = 512;
+
 // A G-lane group (G = D/8) takes one (token, head) vector, lane c its elements [8c, 8c + 8).
-template <int G, int KV>
-__global__ __launch_bounds__(256) void qk_norm_kernel(QkNormArgs a) {
+template <int G, int KV, bool PART>
+__global__ __launch_bounds__(kMaxThreads) void qk_norm_kernel(QkNormArgs a) {
   constexpr int D = 8 * G;
-  const int t = static_cast<int>(blockIdx.x) / a.blocks_per_token;
-  const int lid = (static_cast<int>(blockIdx.x) - t * a.blocks_per_token) * 256 + static_cast<int>(threadIdx.x);
+  const int t = static_cast<int>(blockIdx.x);
+  const int lid = static_cast<int>(blockIdx.y * blockDim.x + threadIdx.x);
   const int h = lid / G, c = lid % G;
   if (h >= a.Hq + 2 * a.Hkv) return;  // whole groups leave together
   const int width = (a.Hq + 2 * a.Hkv) * D;
+  const int64_t slot = a.slot_mapping[t], pos = a.pos[t];
   uint4 xr;
-  if (a.part) {
+  if constexpr (PART) {
     const float* p = a.part + static_cast<int64_t>(t) * width + lid * 8;
     const float4 lo = sum_partials4(p, a.ks, a.slice), hi = sum_partials4(p + 4, a.ks, a.slice);
     xr = make_uint4(pack2_bf16(lo.x, lo.y), pack2_bf16(lo.z, lo.w), pack2_bf16(hi.x, hi.y), pack2_bf16(hi.z, hi.w));
@@ -56,7 +58,7 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(QkNormArgs a) {
   }
   uint4 yr = xr;
   if (h < a.Hq + a.Hkv) {
-    const RopeTab tab = rope_tab<G>(a.cos, a.sin, a.tab_stride, a.pos[t], a.max_pos, c);
+    const RopeTab tab = rope_tab<G>(a.cos, a.sin, a.tab_stride, pos, a.max_pos, c);
     const uint4 wr = *reinterpret_cast<const uint4*>((h < a.Hq ? a.qw : a.kw) + 8 * c);
     const uint32_t xw[4] = {xr.x, xr.y, xr.z, xr.w}, ww[4] = {wr.x, wr.y, wr.z, wr.w};
     const uint32_t cw[4] = {tab.cos.x, tab.cos.y, tab.cos.z, tab.cos.w};
@@ -74,30 +76,38 @@ __global__ __launch_bounds__(256) void qk_norm_kernel(QkNormArgs a) {
     for (int e = 0; e < 8; ++e) y[e] = y[e] * r * half(ww, e);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float other = __shfl_xor(y[e], G / 2, COOPT_WAVE);  // element i +- D/2
+      const float other = group_other_half<G>(y[e]);  // element i +- D/2
       const float turn = other * half(sw, e);
       z[e] = fmaf(y[e], half(cw, e), c < G / 2 ? -turn : turn);
     }
     yr = make_uint4(pack2_bf16(z[0], z[1]), pack2_bf16(z[2], z[3]), pack2_bf16(z[4], z[5]), pack2_bf16(z[6], z[7]));
     if (h < a.Hq) {
-      *reinterpret_cast<uint4*>(a.q_out + t * a.q_ts + h * a.q_hs + c * 8) = yr;
+      *reinterpret_cast<uint4*>(a.q_out + t * a.q_ts + static_cast<int64_t>(h) * static_cast<int32_t>(a.q_hs) + c * 8) = yr;
       return;
     }
   }
-  const int64_t slot = a.slot_mapping[t];
   if (slot < 0 || slot >= a.num_slots) return;  // padding rows write nothing
-  const int64_t blk = slot / a.block_size, off = slot % a.block_size;
+  const int64_t blk = a.bs_shift >= 0 ? slot >> a.bs_shift : slot / a.block_size;
+  const int64_t off = slot - blk * a.block_size;
   const bool is_k = h < a.Hq + a.Hkv;
-  const int hk = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
-  store_chunk<G, KV>(yr, is_k ? a.kc : a.vc, blk * a.c_bs + off * a.c_ts + hk * a.c_hs + c * chunk_step<KV>(),
-                     is_k ? a.k_scale : a.v_scale, blk * a.s_bs + off * a.s_ts + hk * a.s_hs, c);
+  const int64_t hk = is_k ? h - a.Hq : h - a.Hq - a.Hkv;
+  store_chunk<G, KV>(yr, is_k ? a.kc : a.vc,
+                     blk * a.c_bs + off * a.c_ts + hk * static_cast<int32_t>(a.c_hs) + c * chunk_step<KV>(),
+                     is_k ? a.k_scale : a.v_scale,
+                     blk * a.s_bs + off * a.s_ts + hk * static_cast<int32_t>(a.s_hs), c);
+}
+
+template <int G, int KV>
+void launch_kv(const QkNormArgs& a, dim3 grid, dim3 block, hipStream_t s) {
+  if (a.part) hipLaunchKernelGGL((qk_norm_kernel<G, KV, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((qk_norm_kernel<G, KV, false>), grid, block, 0, s, a);
 }
 
 template <int G>
-void launch(int cache_dtype, const QkNormArgs& a, dim3 grid, hipStream_t s) {
-  if (cache_dtype == COOPT_DT_BF16) hipLaunchKernelGGL((qk_norm_kernel<G, kBf16>), grid, dim3(256), 0, s, a);
-  else if (cache_dtype == COOPT_DT_I8) hipLaunchKernelGGL((qk_norm_kernel<G, kI8>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((qk_norm_kernel<G, kI4>), grid, dim3(256), 0, s, a);
+void launch(int cache_dtype, const QkNormArgs& a, dim3 grid, dim3 block, hipStream_t s) {
+  if (cache_dtype == COOPT_DT_BF16) launch_kv<G, kBf16>(a, grid, block, s);
+  else if (cache_dtype == COOPT_DT_I8) launch_kv<G, kI8>(a, grid, block, s);
+  else launch_kv<G, kI4>(a, grid, block, s);
 }
 
 }  // namespace
@@ -140,20 +150,24 @@ extern "C" int coopt_qkv_norm_epilogue(
     coopt::set_error(std::string(__func__) + ": " + bad);
     return COOPT_EINVAL;
   }
-  const int per_token = static_cast<int>((width / 8 + 255) / 256);
-  COOPT_REQUIRE(static_cast<int64_t>(T) * per_token < (int64_t{1} << 24), "too many rows for one launch");
+  COOPT_REQUIRE(coopt::narrow_strides({q_head_stride, c_head_stride, s_head_stride}),
+                "head strides must stay below 2^31");
+  const int lanes = static_cast<int>(width / 8);
+  const int blocks = (lanes + kMaxThreads - 1) / kMaxThreads;
+  const int threads = ((lanes + blocks - 1) / blocks + COOPT_WAVE - 1) / COOPT_WAVE * COOPT_WAVE;
+  COOPT_REQUIRE(static_cast<int64_t>(T) * blocks < (int64_t{1} << 22) && blocks < 65536, "too many rows for one launch");
   QkNormArgs a{static_cast<const uint16_t*>(qkv), qkv_tok_stride, part, ks, slice_stride,
                static_cast<const uint16_t*>(q_weight), static_cast<const uint16_t*>(k_weight), eps,
                positions, static_cast<const uint16_t*>(cos), static_cast<const uint16_t*>(sin),
                table_stride, max_pos, static_cast<uint16_t*>(q_out), q_tok_stride, q_head_stride,
                k_cache, v_cache, c_blk_stride, c_tok_stride, c_head_stride,
                static_cast<uint16_t*>(k_scale), static_cast<uint16_t*>(v_scale), s_blk_stride,
-               s_tok_stride, s_head_stride, slot_mapping, T, Hq, Hkv, block_size,
-               num_blocks * block_size, per_token};
-  const dim3 grid(static_cast<unsigned>(T) * static_cast<unsigned>(per_token));
+               s_tok_stride, s_head_stride, slot_mapping, Hq, Hkv, block_size,
+               (block_size & (block_size - 1)) == 0 ? __builtin_ctz(block_size) : -1, num_blocks * block_size};
+  const dim3 grid(static_cast<unsigned>(T), static_cast<unsigned>(blocks)), block(static_cast<unsigned>(threads));
   auto s = static_cast<hipStream_t>(stream);
-  if (D == 64) launch<8>(cache_dtype, a, grid, s);
-  else if (D == 128) launch<16>(cache_dtype, a, grid, s);
-  else launch<32>(cache_dtype, a, grid, s);
+  if (D == 64) launch<8>(cache_dtype, a, grid, block, s);
+  else if (D == 128) launch<16>(cache_dtype, a, grid, block, s);
+  else launch<32>(cache_dtype, a, grid, block, s);
   return coopt::check_launch("coopt_qkv_norm_epilogue");
 }

@@ -58,15 +58,16 @@ def dequantize(q: torch.Tensor, scale, bits: int, dtype=torch.bfloat16):
         return q
     if bits not in (8, 4):
         raise ValueError(f"bits must be 16, 8 or 4, got {bits}")
-    _lib.require_cuda(q, scale)
+    index = q.get_device()
+    if index < 0 or index != scale.get_device():
+        _lib.require_cuda(q, scale)
     qc, sc = q.contiguous(), scale.contiguous()
-    D = qc.shape[-1] * (2 if bits == 4 else 1)
-    rows = sc.numel()
-    out = torch.empty((*qc.shape[:-1], D), dtype=dtype, device=q.device)
-    lib = _lib.load()
-    _lib.check(lib.coopt_dequantize(bits, _lib.ptr(qc), _lib.ptr(sc), rows, D,
-                                    _lib.dt_code(dtype), _lib.ptr(out),
-                                    _lib.stream_handle(q.device)), "coopt_dequantize")
+    *lead, width = qc.shape
+    D = width * (2 if bits == 4 else 1)
+    out = qc.new_empty((*lead, D), dtype=dtype)
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_dequantize"), bits, qc.data_ptr(), sc.data_ptr(),
+                            sc.numel(), D, _lib.dt_code(dtype), out.data_ptr(), _lib.raw_stream(index)),
+               "coopt_dequantize")
     return out
 
 
@@ -135,46 +136,54 @@ def reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype
     [num_blocks, block_size, Hkv] scale caches and each written vector is quantised in the
     same kernel.  "int4": the same with uint8 caches of two codes a byte.
     """
-    _lib.require_cuda(k, v, k_cache, v_cache, slot_mapping)
+    # get_device() is -1 on the CPU; 0.04 us, a device object twice that
+    index = k.get_device()
+    alike = index >= 0 and index == v.get_device() == k_cache.get_device() == \
+        v_cache.get_device() == slot_mapping.get_device()
+    if not alike:
+        _lib.require_cuda(k, v, k_cache, v_cache, slot_mapping)
     _check_cache_pair(k_cache, v_cache)
     if k.shape != v.shape or k.dim() != 3 or k.stride(-1) != 1 or v.stride(-1) != 1:
         raise ValueError("k and v must be [T, Hkv, D] with contiguous D")
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16:
+    if k.dtype is not _BF16 or v.dtype is not _BF16:
         raise ValueError("k and v must be bf16")
     T, Hkv, D = k.shape
     NB, bs, cH, cD = k_cache.shape
-    if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
+    if cH != Hkv or cD != (D // 2 if kv_cache_dtype == "int4" else D):
         raise ValueError(f"cache heads/dim {(cH, cD)} != k's {(Hkv, D)}")
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T:
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.numel() != T:
         raise ValueError("slot_mapping must be int64 with one entry per token")
-    slot_mapping = slot_mapping.contiguous()
+    if not slot_mapping.is_contiguous():
+        slot_mapping = slot_mapping.contiguous()
     if kv_cache_dtype == "auto":
-        if k_cache.dtype != torch.bfloat16:
+        if k_cache.dtype is not _BF16:
             raise ValueError("'auto' caches are bf16")
-        code, ks, vs, sstr = _lib.DT_BF16, None, None, (0, 0, 0)
+        code, ks, vs, sstr = _lib.DT_BF16, 0, 0, (0, 0, 0)
     elif kv_cache_dtype == "int8":
-        if k_cache.dtype != torch.int8:
+        if k_cache.dtype is not torch.int8:
             raise ValueError("'int8' caches hold int8 codes")
         if k_scale is None or v_scale is None:
             raise ValueError("'int8' caches need k_scale and v_scale scale caches")
-        if k_scale.shape != (NB, bs, Hkv) or k_scale.dtype != torch.float16 or \
+        if k_scale.shape != (NB, bs, Hkv) or k_scale.dtype is not torch.float16 or \
                 k_scale.stride() != v_scale.stride() or v_scale.shape != k_scale.shape:
             raise ValueError("scale caches must be fp16 [num_blocks, block_size, Hkv] alike")
-        code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
+        _lib.require_cuda(k_scale, v_scale)
+        code, ks, vs, sstr = _lib.DT_I8, k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride()
     elif kv_cache_dtype == "int4":
         _check_int4(k_cache, v_cache)
         sstr = _scale_args(k_cache, k_scale, v_scale, "int4")
-        code, ks, vs = _lib.DT_I4, k_scale, v_scale
+        if not (alike and index == k_scale.get_device() == v_scale.get_device()):
+            _lib.require_one_device(k, v, k_cache, v_cache, slot_mapping, k_scale, v_scale)
+        code, ks, vs = _lib.DT_I4, k_scale.data_ptr(), v_scale.data_ptr()
     else:
         raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
-    _lib.require_cuda(ks, vs)
-    lib = _lib.load()
-    cs = k_cache.stride()
-    _lib.check(lib.coopt_kv_write(code, _lib.ptr(k), _lib.ptr(v), k.stride(0), k.stride(1),
-                                  v.stride(0), v.stride(1), _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2],
-                                  _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1], sstr[2],
-                                  _lib.ptr(slot_mapping), T, Hkv, D, bs, NB,
-                                  _lib.stream_handle(k.device)), "coopt_kv_write")
+    c0, c1, c2, _ = k_cache.stride()
+    k0, k1, _ = k.stride()
+    v0, v1, _ = v.stride()
+    _lib.check(_lib.call_on(
+        index, _lib.entry("coopt_kv_write"), code, k.data_ptr(), v.data_ptr(), k0, k1, v0, v1,
+        k_cache.data_ptr(), v_cache.data_ptr(), c0, c1, c2, ks, vs, sstr[0], sstr[1], sstr[2],
+        slot_mapping.data_ptr(), T, Hkv, D, bs, NB, _lib.raw_stream(index)), "coopt_kv_write")
 
 
 def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping, num_heads,
