@@ -25,6 +25,7 @@ without a window; their keys and values are code * scale, unrounded.
 import functools
 import math
 import operator
+import threading
 
 import torch
 
@@ -34,6 +35,8 @@ __all__ = ["flash_attn_varlen_func", "paged_attention", "paged_attention_qkv",
            "qkv_attention_supported", "window_workspace_bytes", "workspace_bytes"]
 
 _WS = _lib.WorkspaceCache()
+# held over a window or INT4 call's launches where they share _WS with another thread's on its stream
+_WS_LOCK = threading.Lock()
 
 
 @functools.lru_cache(maxsize=1024)   # a pure function of the sizes; 0.9 us through ctypes
@@ -214,11 +217,12 @@ def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, 
         return out
     stream = _lib.raw_stream(index)
     need = _window_workspace_bytes(B, Hq, Hkv, D, max_q, max_k, win, sinks)
+    shared = False
     if workspace is None:
         # a graph under capture gets a workspace of its own (from its memory pool), so that two
         # graphs captured on one stream may replay at the same time
-        workspace = q.new_empty((max(need, 256),), dtype=torch.uint8) \
-            if torch.cuda.is_current_stream_capturing() else _WS.get(need, q.device)
+        shared = not torch.cuda.is_current_stream_capturing()
+        workspace = _WS.get(need, q.device) if shared else q.new_empty((max(need, 256),), dtype=torch.uint8)
         have = workspace.numel()
     else:
         have = workspace.numel() * workspace.element_size()
@@ -227,18 +231,26 @@ def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, 
     cu = cu_seqlens_q if cu_seqlens_q.is_contiguous() else cu_seqlens_q.contiguous()
     sl = seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
     o0, o1, _ = out.stride()
-    _lib.check(_lib.call_on(
-        index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
-        v_cache.data_ptr(), cs[0], cs[1], cs[2], ks, vs, s0, s1, s2, block_table.data_ptr(),
-        block_table.stride(0), cu.data_ptr(), sl.data_ptr(), B, Hq, Hkv, D, bs, NB, max_q, max_k, T, win,
-        sinks, 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, out.data_ptr(), o0, o1,
-        workspace.data_ptr(), have, stream), "coopt_window_attention")
+    call = (index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
+            v_cache.data_ptr(), cs[0], cs[1], cs[2], ks, vs, s0, s1, s2, block_table.data_ptr(),
+            block_table.stride(0), cu.data_ptr(), sl.data_ptr(), B, Hq, Hkv, D, bs, NB, max_q, max_k, T,
+            win, sinks, 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, out.data_ptr(),
+            o0, o1, workspace.data_ptr(), have, stream)
+    if shared:
+        with _WS_LOCK:
+            rc = _lib.call_on(*call)
+    else:
+        rc = _lib.call_on(*call)
+    _lib.check(rc, "coopt_window_attention")
     return out
 
 
 def qkv_attention_supported(kv_cache_dtype, batch, num_heads, num_kv_heads, head_dim,
                             max_seqlen_q, max_seqlen_k) -> bool:
-    """Whether paged_attention_qkv takes this launch shape (coopt_verify_attention_qkv)."""
+    """Whether paged_attention_qkv takes this launch shape (coopt_verify_attention_qkv).  It takes
+    "auto" and "int8" caches, without a window."""
+    if kv_cache_dtype == "int4":
+        return False
     code = _lib.DT_I8 if kv_cache_dtype == "int8" else _lib.DT_BF16
     return bool(_lib.load().coopt_verify_attention_qkv_supported(
         code, batch, num_heads, num_kv_heads, head_dim, int(max_seqlen_q), int(max_seqlen_k)))

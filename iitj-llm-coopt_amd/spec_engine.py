@@ -27,12 +27,13 @@ import torch.nn.functional as F
 
 from . import _lib
 from .attention import (paged_attention, paged_attention_qkv, qkv_attention_supported,
-                        workspace_bytes)
+                        window_workspace_bytes, workspace_bytes)
 from .batch import row_slots
 from .fused import (LinearPartials, linear, linear_silu, pack_gate_up_weight, pack_linear_weight,
                     rms_norm, rope_,
                     row_major, silu_and_mul)
-from .kv_cache import allocate_kv_cache, qkv_rope_and_cache, reshape_and_cache_flash
+from .kv_cache import (allocate_kv_cache, qkv_norm_rope_and_cache, qkv_rope_and_cache,
+                       reshape_and_cache_flash)
 from .spec_decode import AcceptResult, accept
 
 __all__ = ["LlamaShape", "TARGET_LLAMA31_8B", "DRAFT_LLAMA32_1B", "RandomLlama", "PagedKV",
@@ -51,12 +52,15 @@ class LlamaShape:
     rope_theta: float = 500000.0
     eps: float = 1e-5
     tie_embeddings: bool = False
+    window: int | None = None    # attention sees the last `window` keys ...
+    sink_tokens: int = 0         # ... and these first ones
+    qk_norm: bool = False        # RMS norms of the query and key heads before the rotation
 
     def params(self) -> int:
         qkv = (self.heads + 2 * self.kv_heads) * self.head_dim * self.hidden
         o = self.heads * self.head_dim * self.hidden
         mlp = 3 * self.ffn * self.hidden
-        per_layer = qkv + o + mlp + 2 * self.hidden
+        per_layer = qkv + o + mlp + 2 * self.hidden + (2 * self.head_dim if self.qk_norm else 0)
         emb = self.vocab * self.hidden
         return self.layers * per_layer + emb * (1 if self.tie_embeddings else 2) + self.hidden
 
@@ -92,6 +96,9 @@ class RandomLlama:
                 "gate_up": w(2 * shape.ffn, H),
                 "down": w(H, shape.ffn),
             })
+            if shape.qk_norm:
+                self.layers[-1].update({k: torch.ones(D, device=self.device, dtype=dtype)
+                                        for k in ("q_norm", "k_norm")})
         if self.device.type == "cuda":
             self._pack()
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, D, 2, dtype=torch.float32) / D))
@@ -154,12 +161,11 @@ class RandomLlama:
             # cache and attends (ops.attend_qkv), or into the epilogue launch that writes q
             # and the cache, then attention
             qkv = ops.linear(h, L["qkv"], defer_reduce=True)
-            attend_qkv = getattr(ops, "attend_qkv", None)
+            attend_qkv = None if s.qk_norm or s.window is not None else getattr(ops, "attend_qkv", None)
             attn = None if attend_qkv is None else attend_qkv(
                 kv, li, qkv, pos, self.cos, self.sin, slots, meta, self.scale, H, Hkv, D)
             if attn is None:
-                q = ops.qkv_epilogue(kv, li, qkv, pos, self.cos, self.sin, slots, H, Hkv, D)
-                attn = ops.attend(kv, li, q, meta, self.scale)
+                attn = self.attend(ops, kv, li, L, qkv, pos, slots, meta)
             # gate_up + SiLU·mul is one launch at draft and verify row counts (linear_silu); o, down and
             # otherwise gate_up feed only the fused add + norm or SiLU, which reduce their
             # split-K partials as they read them
@@ -170,6 +176,20 @@ class RandomLlama:
         if keep_rows is not None:
             h = h.index_select(0, keep_rows)
         return ops.linear(h, self.lm_head, out=logits_out)
+
+    def attend(self, ops, kv, li, L, qkv, pos, slots, meta):
+        """The epilogue of layer li's qkv projection (rotation, with the head norms where the shape
+        has them, and the KV write), then attention over the cache."""
+        s = self.s
+        sizes = (s.heads, s.kv_heads, s.head_dim)
+        if s.qk_norm:
+            q = ops.qkv_norm_epilogue(kv, li, qkv, L["q_norm"], L["k_norm"], s.eps, pos, self.cos,
+                                      self.sin, slots, *sizes)
+        else:
+            q = ops.qkv_epilogue(kv, li, qkv, pos, self.cos, self.sin, slots, *sizes)
+        if s.window is None:
+            return ops.attend(kv, li, q, meta, self.scale)
+        return ops.attend(kv, li, q, meta, self.scale, s.window, s.sink_tokens)
 
 
 class PagedKV:
@@ -248,6 +268,12 @@ class HipOps:
         return qkv_rope_and_cache(qkv, pos, cos, sin, kc, vc, slots, H, Hkv, D, kv.kv_dtype,
                                   ks, vs)
 
+    def qkv_norm_epilogue(self, kv: "PagedKV", layer, qkv, q_norm, k_norm, eps, pos, cos, sin, slots,
+                          H, Hkv, D):
+        kc, vc, ks, vs = kv.layers[layer]
+        return qkv_norm_rope_and_cache(qkv, q_norm, k_norm, eps, pos, cos, sin, kc, vc, slots, H, Hkv,
+                                       D, kv.kv_dtype, ks, vs)
+
     def silu_mul(self, gate_up):
         return silu_and_mul(gate_up)
 
@@ -260,14 +286,18 @@ class HipOps:
     def linear(self, x, w, out=None, defer_reduce=False):
         return linear(x, w, out=out, defer_reduce=defer_reduce)
 
-    def attend(self, kv: PagedKV, layer, q, meta, scale):
+    def attend(self, kv: PagedKV, layer, q, meta, scale, window=None, sink_tokens=0):
         kc, vc, ks, vs = kv.layers[layer]
         cu, seq_lens, S, max_k = meta
         B = seq_lens.numel()
-        nb = workspace_bytes(B, q.shape[1], kc.shape[2], q.shape[2], S, max_k)
+        sizes = (B, q.shape[1], kc.shape[2], q.shape[2], S, max_k)
+        if window is None and kv.kv_dtype != "int4":
+            nb = workspace_bytes(*sizes)
+        else:
+            nb = window_workspace_bytes(*sizes, window, sink_tokens)
         ws = self.workspace(("attn", q.shape[2]), nb)
         return paged_attention(q, kc, vc, cu, seq_lens, kv.block_table[:B], S, max_k, scale, ks,
-                               vs, workspace=ws)
+                               vs, workspace=ws, window=window, sink_tokens=sink_tokens)
 
     def attend_qkv(self, kv: PagedKV, layer, qkv, pos, cos, sin, slots, meta, scale, H, Hkv, D):
         """qkv_epilogue + attend as one launch, or None where that launch does not take the
@@ -499,8 +529,9 @@ class SpecDecoder:
     @torch.inference_mode()
     def prefill(self, prompts: torch.Tensor, u_first: torch.Tensor):
         """prompts [B, P] int64.  Runs both models over the prompt (attention over the prompt
-        in fp32 SDPA, KV written through the paged write kernel), samples the first token
-        from the target and sets num_computed = P (engine/engine.py:427-436)."""
+        in fp32 SDPA, KV written through the paged write kernel; a model with a window or head
+        norms attends over its cache, as a step does), samples the first token from the target
+        and sets num_computed = P (engine/engine.py:427-436)."""
         B, P = prompts.shape
         if B != self.B:
             raise ValueError(f"{self.B} prompts expected")
@@ -527,21 +558,27 @@ class SpecDecoder:
         slots = (blk * kv.block_size + pos % kv.block_size).reshape(-1)
         x = F.embedding(ids.reshape(-1), model.embed)
         d = None
+        meta = None
+        if s.qk_norm or s.window is not None:
+            meta = (self._meta(B, P), torch.full((B,), P, dtype=torch.int32, device=ids.device), P, P)
         for li, L in enumerate(model.layers):
             h = self.ops.rms_norm(x if d is None else d, None if d is None else x, L["ln1"], s.eps)
             qkv = F.linear(h, row_major(L["qkv"]))
-            q = qkv[:, : H * D].view(T, H, D)
-            k = qkv[:, H * D: (H + Hkv) * D].view(T, Hkv, D)
-            v = qkv[:, (H + Hkv) * D:].view(T, Hkv, D)
-            self.ops.rope(q, k, flat_pos, model.cos, model.sin)
-            self.ops.write(kv, li, k, v, slots)
-            # prompt attention in fp32 (plain causal over the prompt; GQA expanded)
-            qf = q.reshape(B, P, H, D).transpose(1, 2).float()
-            kf = k.reshape(B, P, Hkv, D).transpose(1, 2).float().repeat_interleave(H // Hkv, 1)
-            vf = v.reshape(B, P, Hkv, D).transpose(1, 2).float().repeat_interleave(H // Hkv, 1)
-            a = F.scaled_dot_product_attention(qf.contiguous(), kf.contiguous(), vf.contiguous(),
-                                               is_causal=True, scale=model.scale)
-            attn = a.transpose(1, 2).reshape(T, H * D).to(x.dtype)
+            if meta is not None:
+                attn = model.attend(self.ops, kv, li, L, qkv, flat_pos, slots, meta).reshape(T, H * D)
+            else:
+                q = qkv[:, : H * D].view(T, H, D)
+                k = qkv[:, H * D: (H + Hkv) * D].view(T, Hkv, D)
+                v = qkv[:, (H + Hkv) * D:].view(T, Hkv, D)
+                self.ops.rope(q, k, flat_pos, model.cos, model.sin)
+                self.ops.write(kv, li, k, v, slots)
+                # prompt attention in fp32 (plain causal over the prompt; GQA expanded)
+                qf = q.reshape(B, P, H, D).transpose(1, 2).float()
+                kf = k.reshape(B, P, Hkv, D).transpose(1, 2).float().repeat_interleave(H // Hkv, 1)
+                vf = v.reshape(B, P, Hkv, D).transpose(1, 2).float().repeat_interleave(H // Hkv, 1)
+                a = F.scaled_dot_product_attention(qf.contiguous(), kf.contiguous(), vf.contiguous(),
+                                                   is_causal=True, scale=model.scale)
+                attn = a.transpose(1, 2).reshape(T, H * D).to(x.dtype)
             o = F.linear(attn, row_major(L["o"]))
             h = self.ops.rms_norm(o, x, L["ln2"], s.eps)
             d = F.linear(self.ops.silu_mul(F.linear(h, row_major(L["gate_up"]))), row_major(L["down"]))

@@ -109,3 +109,7 @@ def test_wrappers_refuse_cpu_tensors_and_odd_heads():
         M.allocate_kv_cache(2, 16, 2, 33, "int4", device="cpu")
     with pytest.raises(ValueError, match="'int4'"):
         M.allocate_kv_cache(2, 16, 2, 64, "int2", device="cpu")
+
+
+def test_the_fused_call_leaves_int4_caches_to_the_two_calls():
+    assert not M.qkv_attention_supported("int4", 1, 32, 8, 128, 1, 100)
