@@ -1811,6 +1811,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
 
   f32x4_t o[2][kDt];
   float m_run[2], l_run[2];
+  float sum_limit[2] = {-1.0f, -1.0f};  // WIN: what a lane's sum of probabilities may reach; -1: no reference yet
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) {
     m_run[rt] = -INFINITY;
@@ -2044,9 +2045,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         const u32x2_t k4 = *reinterpret_cast<const u32x2_t*>(&lsk[buf][t0 * 32 + kt * 16 + grp * 4]);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float sk = f16_to_f32(static_cast<uint16_t>(k4[i >> 1] >> (16 * (i & 1))));
-          acc[0][kt][i] *= sk;
-          acc[1][kt][i] *= sk;
+          acc[0][kt][i] = times_f16(acc[0][kt][i], k4[i >> 1], i & 1);
+          acc[1][kt][i] = times_f16(acc[1][kt][i], k4[i >> 1], i & 1);
         }
       }
     }
@@ -2081,6 +2081,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           const float f = exp2_fast(static_cast<float>(e_v - e_new));
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt) {
+            if constexpr (WIN) sum_limit[rt] *= f;
             l_run[rt] *= f;
 #pragma unroll
             for (int dt = 0; dt < kDt; ++dt) o[rt][dt] *= f;
@@ -2090,12 +2091,6 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         }
       }
     }
-    // bf16 probabilities: the reference is the running maximum itself (no slack), so the largest
-    // one is exactly 1; with the slack one reference for all keys was 2 % further from 64 bits than
-    // verify_attn_kernel's one per wave (2.10e-3 against 2.05e-3 relative in the batch above; like
-    // this 2.02e-3; the largest excess over seven batches, 600 + 100 rows and 2 items: 1.977e-3
-    // against 1.968e-3)
-    constexpr float kSlack = CODES || WIN ? 8.0f : 0.0f;
     if constexpr (WIN) {
       if (!tile_open(kb)) {
 #pragma unroll
@@ -2117,56 +2112,102 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           for (int i = 0; i < 4; ++i)
             if (kb + kt * 16 + grp * 4 + i > lim[rt]) acc[rt][kt][i] = -INFINITY;
     }
-    float m_tile[2];
-    bool raise_any = false;
+    u32x4_t pb[2][kSub / 2];
+    if constexpr (WIN) {
+      // The probabilities against the reference as it is, and the tile's maxima only if a lane's sum
+      // of them passes 2^8: no maximum, and no exchange between lanes, stands between most tiles'
+      // scores and their exponents (the measured window case 82.4 -> 79.6 us).  A lane adds 8 probabilities,
+      // so none passes 2^8: the slack of 8 of a test of the maxima.
+      float sum[2];
+      auto probabilities = [&]() {
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      float tmax = -INFINITY;
-      if constexpr (WIN) {
-        const float sv[2][4] = {{acc[rt][0][0], acc[rt][0][1], acc[rt][0][2], acc[rt][0][3]},
-                                {acc[rt][1][0], acc[rt][1][1], acc[rt][1][2], acc[rt][1][3]}};
-        tmax = maxima.of_groups(maxima.of8(sv));
-      } else {
+        for (int rt = 0; rt < 2; ++rt) {
+          const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) + (CODES ? static_cast<float>(e_v) : 0.0f);
+          float part[kSub];
+#pragma unroll
+          for (int kt = 0; kt < kSub; ++kt) {
+            float pr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) pr[i] = exp2_fast(fmaf(acc[rt][kt][i], scale_log2(rt), -m_use));
+            part[kt] = (pr[0] + pr[1]) + (pr[2] + pr[3]);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2)
+              pb[rt][kt >> 1][2 * (kt & 1) + (i >> 1)] =
+                  CODES ? pair_times_f16(pr[i], pr[i + 1], vs[kt][i >> 1]) : pack_bf16x2(pr[i], pr[i + 1]);
+          }
+          sum[rt] = part[0] + part[1];
+        }
+      };
+      probabilities();
+      if (__builtin_amdgcn_ballot_w64(sum[0] > sum_limit[0] || sum[1] > sum_limit[1])) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+          const float sv[2][4] = {{acc[rt][0][0], acc[rt][0][1], acc[rt][0][2], acc[rt][0][3]},
+                                  {acc[rt][1][0], acc[rt][1][1], acc[rt][1][2], acc[rt][1][3]}};
+          const float m_tile = maxima.of_groups(maxima.of8(sv)) * scale_log2(rt);
+          const bool raise = m_tile > m_run[rt];
+          const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < kDt; ++dt) o[rt][dt] *= alpha;
+          if (raise) m_run[rt] = m_tile;
+          if (m_run[rt] > -INFINITY) sum_limit[rt] = CODES ? exp2_fast(8.0f - static_cast<float>(e_v)) : 256.0f;
+        }
+        probabilities();
+      }
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) l_run[rt] += sum[rt];
+    } else {
+      // bf16 probabilities: the reference is the running maximum itself (no slack), so the largest
+      // one is exactly 1; with the slack one reference for all keys was 2 % further from 64 bits than
+      // verify_attn_kernel's one per wave (2.10e-3 against 2.05e-3 relative in the batch above; like
+      // this 2.02e-3; the largest excess over seven batches, 600 + 100 rows and 2 items: 1.977e-3
+      // against 1.968e-3)
+      constexpr float kSlack = CODES ? 8.0f : 0.0f;
+      float m_tile[2];
+      bool raise_any = false;
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        float tmax = -INFINITY;
 #pragma unroll
         for (int kt = 0; kt < kSub; ++kt)
           tmax = fmaxf(tmax, fmaxf(fmaxf(acc[rt][kt][0], acc[rt][kt][1]), fmaxf(acc[rt][kt][2], acc[rt][kt][3])));
         tmax = max_xor32(max_xor16(tmax));
+        m_tile[rt] = tmax * scale_log2(rt);
+        raise_any |= m_tile[rt] > m_run[rt] + kSlack;
       }
-      m_tile[rt] = tmax * scale_log2(rt);
-      raise_any |= m_tile[rt] > m_run[rt] + kSlack;
-    }
-    if (__builtin_amdgcn_ballot_w64(raise_any)) {
+      if (__builtin_amdgcn_ballot_w64(raise_any)) {
+#pragma unroll
+        for (int rt = 0; rt < 2; ++rt) {
+          const bool raise = m_tile[rt] > m_run[rt] + kSlack;
+          const float m_new = raise ? m_tile[rt] : m_run[rt];
+          const float alpha = raise ? exp2_fast(m_run[rt] - m_new) : 1.0f;
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < kDt; ++dt) o[rt][dt] *= alpha;
+          m_run[rt] = m_new;
+        }
+      }
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
-        const bool raise = m_tile[rt] > m_run[rt] + kSlack;
-        const float m_new = raise ? m_tile[rt] : m_run[rt];
-        const float alpha = raise ? exp2_fast(m_run[rt] - m_new) : 1.0f;
-        l_run[rt] *= alpha;
+        const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) + (CODES ? static_cast<float>(e_v) : 0.0f);
 #pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) o[rt][dt] *= alpha;
-        m_run[rt] = m_new;
-      }
-    }
-    u32x4_t pb[2][kSub / 2];
+        for (int kt = 0; kt < kSub; ++kt) {
+          float pr[4];
 #pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) + (CODES ? static_cast<float>(e_v) : 0.0f);
+          for (int i = 0; i < 4; ++i) pr[i] = exp2_fast(fmaf(acc[rt][kt][i], scale_log2(rt), -m_use));
+          l_run[rt] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
+          if constexpr (CODES) {
 #pragma unroll
-      for (int kt = 0; kt < kSub; ++kt) {
-        float pr[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pr[i] = exp2_fast(fmaf(acc[rt][kt][i], scale_log2(rt), -m_use));
-        l_run[rt] += (pr[0] + pr[1]) + (pr[2] + pr[3]);
-        if constexpr (CODES) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            pr[i] *= f16_to_f32(static_cast<uint16_t>(vs[kt][i >> 1] >> (16 * (i & 1))));
-          pb[rt][kt >> 1][2 * (kt & 1)] = pack_f16x2(pr[0], pr[1]);
-          pb[rt][kt >> 1][2 * (kt & 1) + 1] = pack_f16x2(pr[2], pr[3]);
-        } else {
-          const uint32_t p0 = pack_bf16x2(pr[0], pr[1]), p1 = pack_bf16x2(pr[2], pr[3]);
-          pb[rt][kt >> 1][2 * (kt & 1)] = p0;
-          pb[rt][kt >> 1][2 * (kt & 1) + 1] = p1;
+            for (int i = 0; i < 4; ++i)
+              pr[i] *= f16_to_f32(static_cast<uint16_t>(vs[kt][i >> 1] >> (16 * (i & 1))));
+            pb[rt][kt >> 1][2 * (kt & 1)] = pack_f16x2(pr[0], pr[1]);
+            pb[rt][kt >> 1][2 * (kt & 1) + 1] = pack_f16x2(pr[2], pr[3]);
+          } else {
+            const uint32_t p0 = pack_bf16x2(pr[0], pr[1]), p1 = pack_bf16x2(pr[2], pr[3]);
+            pb[rt][kt >> 1][2 * (kt & 1)] = p0;
+            pb[rt][kt >> 1][2 * (kt & 1) + 1] = p1;
+          }
         }
       }
     }
@@ -2183,7 +2224,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
   // Two register sets: stage s + 2 loads while stage s is computed and stage s + 1 waits in the
   // other set.  Loads past the last stage repeat it (cached), so no load sits under a branch.
   if (stages > 0) {
-    Staged sa, sb;
+    Staged sa;
     const int last = stages - 1;
     int64_t pg = page_of(0);
     auto load = [&](Staged& st, int s) {
@@ -2201,26 +2242,41 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           compute_tile(s, t);
         }
     };
-    load(sa, 0);
-    load(sb, 1);
-    store_stage(sa, 0);
-    __syncthreads();
-    int s = 0;
-    for (; s + 2 <= last; s += 2) {
-      load(sa, s + 2);
+    if constexpr (WIN) {
+      // one set: the tiles' work covers a stage's loads, and their registers hold the probabilities
+      load(sa, 0);
+      store_stage(sa, 0);
+      __syncthreads();
+      for (int s = 0; s < last; ++s) {
+        load(sa, s + 1);
+        compute(s);
+        store_stage(sa, s + 1);
+        __syncthreads();
+      }
+      compute(last);
+    } else {
+      Staged sb;
+      load(sa, 0);
+      load(sb, 1);
+      store_stage(sa, 0);
+      __syncthreads();
+      int s = 0;
+      for (; s + 2 <= last; s += 2) {
+        load(sa, s + 2);
+        compute(s);
+        store_stage(sb, s + 1);
+        __syncthreads();
+        load(sb, s + 3);
+        compute(s + 1);
+        store_stage(sa, s + 2);
+        __syncthreads();
+      }
       compute(s);
-      store_stage(sb, s + 1);
-      __syncthreads();
-      load(sb, s + 3);
-      compute(s + 1);
-      store_stage(sa, s + 2);
-      __syncthreads();
-    }
-    compute(s);
-    if (s < last) {
-      store_stage(sb, s + 1);
-      __syncthreads();
-      compute(s + 1);
+      if (s < last) {
+        store_stage(sb, s + 1);
+        __syncthreads();
+        compute(s + 1);
+      }
     }
   }
   if constexpr (WIN) {
