@@ -761,6 +761,11 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
   constexpr int kAcc = INT4 ? kDt + 1 : kDt;  // INT4: the last one sums P' (INT4 operands)
   f32x4_t o[RT][kAcc];
   float m_run[RT], l_run[RT];
+  constexpr bool kLazy = WIN && CODES;
+  bool ref_set = false;  // kLazy: the wave has had a tile
+  float sum_limit[RT];  // kLazy: what a lane's sum of a tile's probabilities may reach; -1: no reference yet
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) sum_limit[rt] = -1.0f;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     m_run[rt] = -INFINITY;
@@ -1027,6 +1032,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
         const float f = exp2_fast(static_cast<float>(e_v - e_new));
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+          if constexpr (kLazy) sum_limit[rt] *= f;
           l_run[rt] *= f;
 #pragma unroll
           for (int dt = 0; dt < kAcc; ++dt) o[rt][dt] *= f;
@@ -1212,67 +1218,117 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
               sv[rt][kt][i] = (key > lim[rt] || key >= k_end) ? -INFINITY : acc[rt][kt][i];
           }
     }
-    float m_tile[RT];
-    bool raise_any = false;
+    uint32_t pb[RT][4];
+    if constexpr (kLazy) {
+      // The probabilities against the reference as it is; the tile's maxima only if a lane's sum of
+      // them passes 2^kSlack (each is at most that sum), so no exchange between lanes stands between
+      // most tiles' scores and their exponents.  Over INT4 codes 61.5 -> 58.5 us (32 sequences of 5
+      // rows and 8192 keys, 32/8 heads of 128), 20.1 -> 20.7 us at 4 tiles a wave; bf16 tiles have no registers for it (20 rows: 28 spilled).
+      float sum[RT];
+      auto probabilities = [&]() {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float tmax;
-      if constexpr (WIN) {
-        tmax = maxima.of_groups(maxima.of8(sv[rt]));
-      } else {
-        tmax = fmaxf(fmaxf(fmaxf(sv[rt][0][0], sv[rt][0][1]), fmaxf(sv[rt][0][2], sv[rt][0][3])),
-                     fmaxf(fmaxf(sv[rt][1][0], sv[rt][1][1]), fmaxf(sv[rt][1][2], sv[rt][1][3])));
-        tmax = max_xor32(max_xor16(tmax));
+        for (int rt = 0; rt < RT; ++rt) {
+          const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) + static_cast<float>(e_v);
+          float p[2][4];
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], scale_log2(rt), -m_use));
+          sum[rt] = ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int kt = w >> 1, i = 2 * (w & 1);
+            // P' = p * s_v of the lane's key j = 4 kt + i, in fp16 next to the fp16 codes
+            pb[rt][w] = pair_times_f16(p[kt][i], p[kt][i + 1], raw.vs[kt][i >> 1]);
+          }
+        }
+      };
+      bool raise_any = !ref_set;  // uniform
+      if (ref_set) {
+        probabilities();
+        bool over = false;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) over |= sum[rt] > sum_limit[rt];
+        raise_any = __builtin_amdgcn_ballot_w64(over) != 0;
       }
-      m_tile[rt] = tmax * scale_log2(rt);
-      raise_any |= m_tile[rt] > m_run[rt] + kSlack;
-    }
-    if (__builtin_amdgcn_ballot_w64(raise_any)) {
+      if (raise_any) {
+        ref_set = true;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const float m_tile = maxima.of_groups(maxima.of8(sv[rt])) * scale_log2(rt);
+          const bool raise = m_tile > m_run[rt];
+          const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;  // 0 when raised from -inf
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < kAcc; ++dt) o[rt][dt] *= alpha;
+          if (raise) m_run[rt] = m_tile;
+          if (m_run[rt] > -INFINITY) sum_limit[rt] = exp2_fast(kSlack - static_cast<float>(e_v));
+        }
+        probabilities();
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) l_run[rt] += sum[rt];
+    } else {
+      float m_tile[RT];
+      bool raise_any = false;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        const bool raise = m_tile[rt] > m_run[rt] + kSlack;
-        const float m_new = raise ? m_tile[rt] : m_run[rt];
-        const float alpha = raise ? exp2_fast(m_run[rt] - m_new) : 1.0f;  // 0 when raised from -inf
-        l_run[rt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < kAcc; ++dt) o[rt][dt] *= alpha;
-        m_run[rt] = m_new;
-      }
-    }
-    uint32_t pb[RT][4];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) +
-                          (CODES ? static_cast<float>(e_v) : 0.0f);
-      float p[2][4], psum = 0.0f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], scale_log2(rt), -m_use));
-          if constexpr (!WIN) psum += p[kt][i];
+        float tmax;
+        if constexpr (WIN) {
+          tmax = maxima.of_groups(maxima.of8(sv[rt]));
+        } else {
+          tmax = fmaxf(fmaxf(fmaxf(sv[rt][0][0], sv[rt][0][1]), fmaxf(sv[rt][0][2], sv[rt][0][3])),
+                       fmaxf(fmaxf(sv[rt][1][0], sv[rt][1][1]), fmaxf(sv[rt][1][2], sv[rt][1][3])));
+          tmax = max_xor32(max_xor16(tmax));
         }
-      if constexpr (WIN)
-        psum = ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
-      l_run[rt] += psum;
-      if constexpr (CODES) {
-        // P' = p * s_v of the lane's key j = 4 kt + i, in fp16 next to the fp16 codes
+        m_tile[rt] = tmax * scale_log2(rt);
+        raise_any |= m_tile[rt] > m_run[rt] + kSlack;
+      }
+      if (__builtin_amdgcn_ballot_w64(raise_any)) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const bool raise = m_tile[rt] > m_run[rt] + kSlack;
+          const float m_new = raise ? m_tile[rt] : m_run[rt];
+          const float alpha = raise ? exp2_fast(m_run[rt] - m_new) : 1.0f;  // 0 when raised from -inf
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int dt = 0; dt < kAcc; ++dt) o[rt][dt] *= alpha;
+          m_run[rt] = m_new;
+        }
+      }
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const float m_use = (m_run[rt] == -INFINITY ? 0.0f : m_run[rt]) +
+                            (CODES ? static_cast<float>(e_v) : 0.0f);
+        float p[2][4], psum = 0.0f;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if constexpr (!WIN) p[kt][i] *= scale_of(raw.vs[kt], i);
+          for (int i = 0; i < 4; ++i) {
+            p[kt][i] = exp2_fast(fmaf(sv[rt][kt][i], scale_log2(rt), -m_use));
+            if constexpr (!WIN) psum += p[kt][i];
+          }
+        if constexpr (WIN)
+          psum = ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+        l_run[rt] += psum;
+        if constexpr (CODES) {
+          // P' = p * s_v of the lane's key j = 4 kt + i, in fp16 next to the fp16 codes
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const int kt = w >> 1, i = 2 * (w & 1);
-          if constexpr (WIN) pb[rt][w] = pair_times_f16(p[kt][i], p[kt][i + 1], raw.vs[kt][i >> 1]);
-          else pb[rt][w] = pack_f16x2(p[kt][i], p[kt][i + 1]);
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              p[kt][i] *= scale_of(raw.vs[kt], i);
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int kt = w >> 1, i = 2 * (w & 1);
+            pb[rt][w] = pack_f16x2(p[kt][i], p[kt][i + 1]);
+          }
+        } else {
+          pb[rt][0] = pack_bf16x2(p[0][0], p[0][1]);
+          pb[rt][1] = pack_bf16x2(p[0][2], p[0][3]);
+          pb[rt][2] = pack_bf16x2(p[1][0], p[1][1]);
+          pb[rt][3] = pack_bf16x2(p[1][2], p[1][3]);
         }
-      } else {
-        pb[rt][0] = pack_bf16x2(p[0][0], p[0][1]);
-        pb[rt][1] = pack_bf16x2(p[0][2], p[0][3]);
-        pb[rt][2] = pack_bf16x2(p[1][0], p[1][1]);
-        pb[rt][3] = pack_bf16x2(p[1][2], p[1][3]);
       }
     }
 
