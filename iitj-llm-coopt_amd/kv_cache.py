@@ -64,6 +64,8 @@ def dequantize(q: torch.Tensor, scale, bits: int, dtype=torch.bfloat16):
     qc, sc = q.contiguous(), scale.contiguous()
     *lead, width = qc.shape
     D = width * (2 if bits == 4 else 1)
+    if sc.numel() * width != qc.numel():
+        raise ValueError(f"scale must have one entry a vector, shape {tuple(lead)}, got {tuple(scale.shape)}")
     out = qc.new_empty((*lead, D), dtype=dtype)
     _lib.check(_lib.call_on(index, _lib.entry("coopt_dequantize"), bits, qc.data_ptr(), sc.data_ptr(),
                             sc.numel(), D, _lib.dt_code(dtype), out.data_ptr(), _lib.raw_stream(index)),

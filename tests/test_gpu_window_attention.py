@@ -16,6 +16,13 @@ times the sum of w s is taken off at the end: the magnitudes summed are |v| + 8 
 there the last term is 2^-18 sum_k w_k (|v_k| + 8 s_k).  (Where every code of an element is 0, |v| is
 0 and these roundings, up to 64 * 2^-24 * 8 s, are all of the error.)  Its operand is a subnormal
 number of the matrix cores, whose products keep 2^-20 of the largest: four such tiles make 2^-18.
+
+Codes again: the probabilities times the values' scales, P' = p s 2^-e in fp16, have steps of 2^-24
+below 2^-14 and are off by up to 2^-25 there, whatever they are themselves.  2^e <= 2^-6 S, S the
+sequence's largest scale, and p is 2^(score - r) with a reference r that one of the row's scores
+had, so sum p >= 1 and the output moves by at most 2^-25 2^e sum |c| / sum p <= 2^-31 S sum |c| over the
+codes c the row sees.  (Only where the row's heavy keys have codes of 0 is this not hidden by the
+terms above: one key with nearly all the weight and a 0 there leaves A the size of the light keys'.)
 """
 import numpy as np
 import pytest
@@ -59,6 +66,9 @@ def closed_form(q, K, V, scale, window, sinks, kv, s_k, s_v):
             A = w @ np.abs(Vs)
             summed = A + (8 * (w @ s_v[see, g]) if kv == "int4" else 0)
             tol[j, h] = 2.0 ** -8 * np.abs(out[j, h]) + (u_p + 2 * ds) * A + 2.0 ** -18 * summed
+            if kv != "auto":
+                codes = (np.abs(Vs) / np.maximum(s_v[see, g], 1e-30)[:, None]).sum(0)
+                tol[j, h] += 2.0 ** -31 * s_v[:, g].max() * codes
     return out, tol
 
 
@@ -260,13 +270,14 @@ def test_rows_that_see_nothing_are_zero(dev, kv):
     assert (o[:3] == 0).all() and (o[5:8] == 0).all() and (o[8:41] == 0).all()
 
 
-@pytest.mark.parametrize("rows", [4, 40])
-def test_infinities_and_nan_reach_only_the_rows_that_see_them(dev, rows):
+@pytest.mark.parametrize("rows,Hq,Hkv", [(4, 8, 2), (40, 8, 2), (300, 64, 8)])
+def test_infinities_and_nan_reach_only_the_rows_that_see_them(dev, rows, Hq, Hkv):
     """bf16 keys and values of partly visible positions: rows before them, and rows whose window
     has passed them, are as if the values were finite."""
-    s = Setup(dev, [(rows, 200)], 8, 2, 128, "auto", 50, 3, seed=3)
+    L = max(200, rows + 100)
+    s = Setup(dev, [(rows, L)], Hq, Hkv, 128, "auto", 50, 3, seed=3)
     clean = s.run().clone()
-    first = 200 - rows
+    first = L - rows
     places = [(0, first + 1, float("nan")), (1, first + 2, float("inf")), (1, first - 49, float("nan")),
               (1, first - 48, float("-inf")), (0, first - 47, float("inf"))]
     for which, key, value in places:
@@ -284,6 +295,83 @@ def test_infinities_and_nan_reach_only_the_rows_that_see_them(dev, rows):
                 g = got[j].float()
                 assert not torch.isfinite(g).any(), (which, key, value, j)
                 assert torch.isnan(g).all() if value != value else (g == value).all()
+
+
+def takes_staged_kernel(s, Hq, Hkv):
+    """Whether the call's windows fill the GPU: 128 rows a window, staged for four waves."""
+    most = min(s.max_q, 128) + (s.window or s.max_k) + s.sinks + 128
+    return _lib.load().coopt_verify_attention_window_rows(
+        _lib.DT_BF16 if s.kv == "auto" else _lib.DT_I8, len(s.seqs), Hq, Hkv, s.D, s.max_q, min(most, s.max_k), s.T) == 128
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv,window,sinks", [(kv, *w) for kv in KINDS for w in ((40, 4), (130, 70), (1000, 8))] +
+                         [("int4", None, 0)])
+def test_batches_that_fill_the_gpu(dev, kv, window, sinks, D):
+    """Chunks whole and continued beside short items, 64 query heads: the windows of 128 rows, among
+    them some of at most 64 rows, an empty one, and rows before the first key."""
+    s = Setup(dev, [(300, 300), (37, 400), (5, 333), (0, 10), (130, 131), (3, 1)], 64, 8, D, kv, window, sinks,
+              seed=sinks, outlier=0.01)
+    assert takes_staged_kernel(s, 64, 8)
+    s.check(s.run(), "full")
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_batches_of_more_sequences_than_a_wave(dev, kv):
+    """More than 64 sequences: blocks in grid order, short items alone and beside a chunk."""
+    short = [(1 + b % 2, 1 + 17 * b % 200) for b in range(70)]
+    s = Setup(dev, short, 8, 2, 64, kv, 60, 3, seed=8)
+    s.check(s.run(), "70 short")
+    s = Setup(dev, [(270, 290)] + [(1, 1 + 17 * b % 200) for b in range(69)], 64, 8, 64, kv, 60, 3, seed=9)
+    assert takes_staged_kernel(s, 64, 8)
+    s.check(s.run(), "70 with a chunk")
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_scores_that_climb_over_the_keys(dev, kv):
+    """Each tile's scores lie further above the ones before it, or below: the reference of a row's
+    exponents moves at every tile, by more and by less than it may lag behind, or never again."""
+    for seqs, Hq, Hkv in (([(3, 700), (1, 90)], 8, 2), ([(300, 420), (2, 64)], 64, 8)):
+        for climb in (0.02, 0.3, -0.3):
+            s = Setup(dev, seqs, Hq, Hkv, 128, kv, 350, 8, seed=12)
+            for b, (n, L) in enumerate(seqs):      # keys along the queries' common direction
+                scale = (climb * np.arange(L)).astype(np.float32)
+                d = np.ones((Hkv, 128), np.float32) / 8
+                x = s.K[b].astype(np.float32) * 0.05 + scale[:, None, None] * d
+                blk = torch.from_numpy(s.table_np[b, np.arange(L) // 16].astype(np.int64))
+                ok, off = (blk >= 0) & (blk < s.caches[0].shape[0]), torch.arange(L) % 16
+                if kv == "auto":
+                    y = torch.from_numpy(x).to(torch.bfloat16)
+                    s.K[b] = y.double().numpy()
+                    s.caches[0][blk[ok].to(dev), off[ok].to(dev)] = y[ok].to(dev)
+                else:
+                    c, sc = OC.quantize(x, 8 if kv == "int8" else 4)
+                    s.K[b], s.sk[b] = OC_values(c, sc, kv), np.asarray(sc, np.float16).astype(np.float64)
+                    s.caches[0][blk[ok].to(dev), off[ok].to(dev)] = torch.from_numpy(c)[ok].to(dev)
+                    s.scales[0][blk[ok].to(dev), off[ok].to(dev)] = torch.from_numpy(np.asarray(sc, np.float16))[ok].to(dev)
+            s.q.mul_(0.1).add_(1.0)
+            s.check(s.run(), f"climb {climb} {seqs[0][0]} rows")
+
+
+def test_two_threads_on_one_stream(dev):
+    """Calls whose parts go through the stream's shared workspace, from two threads at once."""
+    import threading
+    sets = [Setup(dev, [(2, 5000 + 37 * i)], 8, 2, 128, "int4", None, 0, seed=20 + i) for i in range(2)]
+    want = [s.run().clone() for s in sets]
+    torch.cuda.synchronize(dev)
+    bad = []
+
+    def work(i):
+        for _ in range(200):
+            if not torch.equal(sets[i].run(), want[i]):
+                bad.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, f"{len(bad)} of 400 calls"
 
 
 @pytest.mark.parametrize("kv", KINDS)
