@@ -172,7 +172,8 @@ __device__ __forceinline__ void store_chunk_i4(const uint32_t (&w)[4], uint8_t* 
   const float s32 = quant_scale<7>(bf16_to_f32(static_cast<uint16_t>(amax)));
   const uint32_t word = quant_pack8_i4(w, s32);
   __builtin_nontemporal_store(word, reinterpret_cast<uint32_t*>(dst));
-  if (c == 0) *scale = f32_to_f16(s32);
+  // a NaN among the elements (bits above an infinity's) makes the scale one, so it is read back
+  if (c == 0) *scale = amax > 0x7f80u ? uint16_t{0x7e00} : f32_to_f16(s32);
 }
 
 // ---------------------------------------------------------------------------------------

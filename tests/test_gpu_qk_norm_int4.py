@@ -56,6 +56,26 @@ def test_int4_write_is_the_codecs(dev, layout, D, bs):
         assert np.array_equal(got[0].cpu().numpy(), q) and np.array_equal(got[1].cpu().numpy(), scale)
 
 
+def test_int4_write_of_extreme_values_is_quantize(dev):
+    """Infinities, subnormals and the type's largest values: the bytes of quantize(x, 4).  A vector
+    with a NaN has a NaN for its scale."""
+    gen = torch.Generator(device=dev).manual_seed(2)
+    x = torch.randn(40, 2, 128, generator=gen, device=dev)
+    for i, v in enumerate((float("inf"), float("-inf"), float("nan"), 1e-40, 3.3e38, -3.3e38, 1e-38, 0.0)):
+        x[4 * i:4 * i + 2, 0, 7 * i] = v
+        x[4 * i + 2, 1] = v
+    x = x.to(torch.bfloat16)
+    kc, vc, ks, vs = M.allocate_kv_cache(3, 16, 2, 128, "int4", device=dev)
+    M.reshape_and_cache_flash(x, x.flip(0).contiguous(), kc, vc, torch.arange(40, device=dev), "int4", ks, vs)
+    for src, c, s in ((x, kc, ks), (x.flip(0).contiguous(), vc, vs)):
+        q, sc = M.quantize(src, 4)
+        t = torch.arange(40, device=dev)
+        c, s, nan = c[t // 16, t % 16], s[t // 16, t % 16], src.isnan().any(-1)
+        assert torch.equal(c[~nan], q[~nan]) and torch.equal(s[~nan], sc[~nan])
+        assert nan.sum() == 3 and s[nan].isnan().all()
+        assert M.dequantize(c, s, 4)[nan].isnan().all()
+
+
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_int4_rope_and_cache_is_rope_then_write(dev, D):
     Hq, Hkv, T, nb = 6, 3, 37, 4
