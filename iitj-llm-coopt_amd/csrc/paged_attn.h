@@ -56,6 +56,16 @@
 // [2^-14, 2^15] for every scale the fp16 scale cache can hold (up to 65504, i.e. |V| up to
 // 8.3e6): it is set from the largest V scale seen so far and enters the softmax exponent, so
 // it cancels in o / l like the running max does.
+// Windows and INT4 (WIN).  Row p sees key k iff k <= p and (k > p - window or k < sinks).  The keys no row
+// of a block sees lie in one gap: tiles are counted without it (Visible), so a call's time follows the keys
+// in sight, not the context, and pages inside the gap are not read.  Tiles that every row sees whole take
+// no mask.  A partly visible tile may hold keys that were never written: values and scales that are not
+// finite are taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly,
+// into the rows that do see them (add_not_finite).  INT4 operands: below.
+// Measured, 32/8 heads of 128: 32 sequences of 5 rows, 512-8192 keys, window 2048, bf16: 43.7 us, the
+// bytes at 5.8 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.7 (17.2 and a merge of
+// 3.5: four tiles a wave, each waiting for its own loads); 1 row, window 1024, bf16: 14.2, the host's time
+// for two launches.
 #pragma once
 
 #include <math.h>
@@ -419,7 +429,10 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
 // a bf16's 8, except that values under 2^-9 of the row's largest are rounded to 2^-17 of it.  The key's
 // scale multiplies the score, the row's power of two goes into its softmax scale.  At head dim 128 the
 // 128-term MFMA takes one part at a time, at 64 both at once (K twice in its operand).
-// Against K as bf16 16 + n, eight instructions and four MFMAs per 8 codes: measured below.
+// 32 sequences of 5 rows over 8192 keys (280 MB, 32/8 heads of 128): 70.3 us with K as bf16 16 + n (eight
+// instructions per 8 codes, two q loads a step), 61.5 like this, 58.5 with the maxima taken rarely (kLazy);
+// its loads alone take 55, a copy of the bytes 44.5.  What bounds it: the memory stream and, at 28 % of the
+// matrix cores' cycles, ten VALU instructions a MFMA beside it.
 constexpr float kI4Bias = 8.0f, kI4VUnit = 0x1p20f;
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
@@ -1743,6 +1756,14 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a) {
 // probabilities with ones: 67.4 us, and no longer a sum of 32-bit probabilities.)
 // Tried: 64 keys per softmax (66-72 us, but 50 instead of 42 us for 2000 keys of a verify item alone,
 // which two waves share below), one stage of loads in flight with an L2 touch ahead (72).
+// The WIN forms hold one stage of loads in flight, not two (the registers hold the probabilities), and
+// take a tile's maxima only where a lane's sum of probabilities passes 2^8.  2000 and 1000 tokens in a
+// window of 1024 with 16 items of 5 (bf16, 43 GFLOP): 79.6 us, 0.54 PFLOP/s, the matrix cores busy for a quarter
+// of the cycles; 1500 and 500 tokens with 16 items over an INT4 cache: 77.
+// Tried there: 8 waves of 16 rows a block (+4 %); the scores of a stage's second tile issued under the
+// first one's exponents (registers spill: 324 us); raised wave priority around the products (nothing).
+// Without stores, loads and barriers it still took 83 of 92 us then: the chain of a wave's own scores,
+// exponents and products, at two waves a SIMD, is what bounds it.
 // Blocks take every sequence's last window first, then every one's last but one, and so on
 // (B <= kPlanSeqs; larger batches run in grid order): a chunk's windows with most keys ahead of its
 // others, and no block without rows among them. Sequences are not ranked by their keys.
@@ -2454,6 +2475,9 @@ constexpr int kMaxRows = 64;
 // worst 1.22 (one chunk over its own keys). us, verify / prefill, bf16, 32/8 heads of 128: a chunk of 512
 // tokens over 512 keys 14.8 / 21.1, over 16384 240 / 438, with 16 items of 5 over 16384 713 / 449; 1024
 // over 4096 114 / 120; 2048 over 4096 197 / 143; 16 chunks of 256 over 4096 504 / 347.
+// WIN calls use it with the keys that a block may walk, INT4 as INT8: 56 batches with windows of 128 to 4096
+// or INT4 caches take 1.01 of the better kernel's time in the mean, 1.16 at worst (33 sequences of one
+// chunk of 656 tokens, 7 heads a KV head).
 // `one_round`: verify_attn_kernel's windows are estimated to run in one round (alone_lds).
 bool prefill_is_faster(int B, int G, int Hkv, int D, int max_seqlen_q, int max_seqlen_k, int64_t total_q,
                        bool int8, bool& one_round) {

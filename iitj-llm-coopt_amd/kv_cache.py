@@ -137,6 +137,8 @@ def reshape_and_cache_flash(k, v, k_cache, v_cache, slot_mapping, kv_cache_dtype
     ones, engine/model.py:129).  "int8": int8 code caches; k_scale/v_scale are the fp16
     [num_blocks, block_size, Hkv] scale caches and each written vector is quantised in the
     same kernel.  "int4": the same with uint8 caches of two codes a byte.
+    Tokens of one call have slots of their own: of two with the same, either's codes and either's
+    scale may stay.
     """
     # get_device() is -1 on the CPU; 0.04 us, a device object twice that
     index = k.get_device()
