@@ -234,7 +234,7 @@ def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, 
     call = (index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
             v_cache.data_ptr(), cs[0], cs[1], cs[2], ks, vs, s0, s1, s2, block_table.data_ptr(),
             block_table.stride(0), cu.data_ptr(), sl.data_ptr(), B, Hq, Hkv, D, bs, NB, max_q, max_k, T,
-            win, sinks, 1.0 / math.sqrt(D) if softmax_scale is None else softmax_scale, out.data_ptr(),
+            win, sinks, 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale), out.data_ptr(),
             o0, o1, workspace.data_ptr(), have, stream)
     if shared:
         with _WS_LOCK:

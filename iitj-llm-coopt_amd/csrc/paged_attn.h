@@ -1256,8 +1256,9 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
           }
         }
       };
-      bool raise_any = !ref_set;  // uniform
-      if (ref_set) {
+      const bool first = !ref_set;  // uniform
+      bool raise_any = first;
+      if (!first) {
         probabilities();
         bool over = false;
 #pragma unroll
@@ -1268,8 +1269,10 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
         ref_set = true;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+          // a row's reference follows its own sums only, whatever the block's other rows do
+          const bool own = first || max_xor32(max_xor16(sum[rt] > sum_limit[rt] ? 1.0f : 0.0f)) > 0.0f;
           const float m_tile = maxima.of_groups(maxima.of8(sv[rt])) * scale_log2(rt);
-          const bool raise = m_tile > m_run[rt];
+          const bool raise = own && m_tile > m_run[rt];
           const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;  // 0 when raised from -inf
           l_run[rt] *= alpha;
 #pragma unroll
@@ -2221,8 +2224,10 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         for (int rt = 0; rt < 2; ++rt) {
           const float sv[2][4] = {{acc[rt][0][0], acc[rt][0][1], acc[rt][0][2], acc[rt][0][3]},
                                   {acc[rt][1][0], acc[rt][1][1], acc[rt][1][2], acc[rt][1][3]}};
+          // a row's reference follows its own sums only, whatever the wave's other rows do
+          const bool own = max_xor32(max_xor16(sum[rt] > sum_limit[rt] ? 1.0f : 0.0f)) > 0.0f;
           const float m_tile = maxima.of_groups(maxima.of8(sv)) * scale_log2(rt);
-          const bool raise = m_tile > m_run[rt];
+          const bool raise = own && m_tile > m_run[rt];
           const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;
           l_run[rt] *= alpha;
 #pragma unroll

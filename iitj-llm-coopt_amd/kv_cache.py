@@ -336,7 +336,7 @@ def qkv_norm_rope_and_cache(qkv, q_weight, k_weight, eps, positions, cos, sin, k
         index, _lib.entry("coopt_qkv_norm_epilogue"), code, 0 if part is not None else x.data_ptr(), stride,
         0 if part is None else x.data_ptr(), 0 if part is None else part.ks,
         0 if part is None else part.rows_padded * part.n, q_weight.data_ptr(), k_weight.data_ptr(),
-        eps, positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), tab[0], rows, q_out.data_ptr(), q0,
+        float(eps), positions.data_ptr(), cos.data_ptr(), sin.data_ptr(), tab[0], rows, q_out.data_ptr(), q0,
         q1, k_cache.data_ptr(), v_cache.data_ptr(), c0, c1, c2, ks, vs, s0, s1, s2,
         slot_mapping.data_ptr(), T, Hq, Hkv, D, bs, NB, _lib.raw_stream(index)),
         "coopt_qkv_norm_epilogue")

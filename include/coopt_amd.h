@@ -96,7 +96,9 @@ int coopt_hip_runtime_version(int* version);
  *                              (engine/kv_tier_manager.py:21-31), codes and scales bit-exact.
  *               COOPT_DT_I4:   k_cache/v_cache are uint8 [NB, block_size, Hkv, D/2], two codes a
  *                              byte, as kv_tier_manager.quantize(x, 4) gives them, with the same
- *                              fp16 scales; cache strides count bytes, rows 4-byte aligned.
+ *                              fp16 scales; cache strides count bytes, rows 4-byte aligned;
+ *                              strides and num_blocks below 2^31.  A vector with a NaN
+ *                              gets a NaN for its scale.
  *   cache strides (c_blk, c_tok, c_head, 1) may describe a strided per-layer view of a
  *   block-major buffer (engine/elastic.py:74-77); scale strides (s_blk, s_tok, s_head).
  *   slot_mapping [T] int64.  A slot < 0 or >= num_blocks * block_size is skipped (padding).
@@ -144,7 +146,8 @@ int coopt_qkv_epilogue(int cache_dtype, const void* qkv, int64_t qkv_tok_stride,
  * in fp32 and rounded to bf16 once, after the rotation; v goes to the cache as it is.  No
  * counterpart in the reference, whose models norm no heads.  INT8 / INT4 caches hold the codes
  * of the rounded z and v (coopt_kv_write).  The other arguments are coopt_qkv_epilogue's;
- * partials are reduced and rounded to bf16 before the norm.  D in {64, 128, 256}.
+ * partials are reduced and rounded to bf16 before the norm.  D in {64, 128, 256}; head strides below
+ * 2^31, T times ceil((Hq + 2 Hkv) D / 4096) below 2^22.
  */
 int coopt_qkv_norm_epilogue(int cache_dtype, const void* qkv, int64_t qkv_tok_stride,
                             const float* part, int ks, int64_t slice_stride,
