@@ -430,7 +430,7 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
 // scale multiplies the score, the row's power of two goes into its softmax scale.  At head dim 128 the
 // 128-term MFMA takes one part at a time, at 64 both at once (K twice in its operand).
 // 32 sequences of 5 rows over 8192 keys (280 MB, 32/8 heads of 128): 70.3 us with K as bf16 16 + n (eight
-// instructions per 8 codes, two q loads a step), 61.5 like this, 58.5 with the maxima taken rarely (kLazy);
+// instructions per 8 codes, two q loads a step), 61.5 like this, 58.5 to 60.8 with the maxima taken rarely (kLazy);
 // its loads alone take 55, a copy of the bytes 44.5.  What bounds it: the memory stream and, at 28 % of the
 // matrix cores' cycles, ten VALU instructions a MFMA beside it.
 constexpr float kI4Bias = 8.0f, kI4VUnit = 0x1p20f;
@@ -1256,9 +1256,8 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
           }
         }
       };
-      const bool first = !ref_set;  // uniform
-      bool raise_any = first;
-      if (!first) {
+      bool raise_any = !ref_set;  // uniform
+      if (ref_set) {
         probabilities();
         bool over = false;
 #pragma unroll
@@ -1269,10 +1268,8 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
         ref_set = true;
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
-          // a row's reference follows its own sums only, whatever the block's other rows do
-          const bool own = first || max_xor32(max_xor16(sum[rt] > sum_limit[rt] ? 1.0f : 0.0f)) > 0.0f;
           const float m_tile = maxima.of_groups(maxima.of8(sv[rt])) * scale_log2(rt);
-          const bool raise = own && m_tile > m_run[rt];
+          const bool raise = m_tile > m_run[rt];
           const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;  // 0 when raised from -inf
           l_run[rt] *= alpha;
 #pragma unroll
@@ -2196,8 +2193,9 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
     if constexpr (WIN) {
       // The probabilities against the reference as it is, and the tile's maxima only if a lane's sum
       // of them passes 2^8: no maximum, and no exchange between lanes, stands between most tiles'
-      // scores and their exponents (the measured window case 82.4 -> 79.6 us).  A lane adds 8 probabilities,
-      // so none passes 2^8: the slack of 8 of a test of the maxima.
+      // scores and their exponents (the measured window case 82.4 -> 79.6 us).  Then every row moves up to
+      // its maximum: where only rows of their own sums do, each in its turn, the INT4 batch above takes 85 us,
+      // not 78.
       float sum[2];
       auto probabilities = [&]() {
 #pragma unroll
@@ -2224,10 +2222,8 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
         for (int rt = 0; rt < 2; ++rt) {
           const float sv[2][4] = {{acc[rt][0][0], acc[rt][0][1], acc[rt][0][2], acc[rt][0][3]},
                                   {acc[rt][1][0], acc[rt][1][1], acc[rt][1][2], acc[rt][1][3]}};
-          // a row's reference follows its own sums only, whatever the wave's other rows do
-          const bool own = max_xor32(max_xor16(sum[rt] > sum_limit[rt] ? 1.0f : 0.0f)) > 0.0f;
           const float m_tile = maxima.of_groups(maxima.of8(sv)) * scale_log2(rt);
-          const bool raise = own && m_tile > m_run[rt];
+          const bool raise = m_tile > m_run[rt];
           const float alpha = raise ? exp2_fast(m_run[rt] - m_tile) : 1.0f;
           l_run[rt] *= alpha;
 #pragma unroll

@@ -356,7 +356,8 @@ def test_scores_that_climb_over_the_keys(dev, kv):
 @pytest.mark.parametrize("kv", KINDS)
 @pytest.mark.parametrize("rows,Hq,Hkv", [(3, 8, 2), (40, 8, 2), (300, 64, 8)])
 def test_a_row_that_is_not_finite_is_its_own(dev, kv, rows, Hq, Hkv):
-    """A query with a NaN or an infinity among its elements: NaN, and every other row the same bits."""
+    """A query with a NaN or an infinity among its elements: NaN, and every other row as before (the
+    rows of a block share the moments at which references move, so not to the bit)."""
     s = Setup(dev, [(rows, rows + 100)], Hq, Hkv, 128, kv, 90, 4, seed=31)
     clean = s.run().clone()
     for value in (float("nan"), float("inf"), float("-inf")):
@@ -366,7 +367,7 @@ def test_a_row_that_is_not_finite_is_its_own(dev, kv, rows, Hq, Hkv):
         s.q.copy_(kept)
         assert torch.isnan(got[rows // 2, 1].float()).all(), value
         got[rows // 2, 1] = clean[rows // 2, 1]
-        assert torch.equal(got, clean), value
+        s.check(got, f"beside {value}")
 
 
 def test_two_threads_on_one_stream(dev):
