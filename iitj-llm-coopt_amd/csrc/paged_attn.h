@@ -477,9 +477,10 @@ __device__ __forceinline__ QBytes q_bytes_i4(u32x4_t q, int exponent) {
   }
   return r;
 }
-// What turns a row's sums into scores in the log2 domain.
+// What turns a row's sums into scores in the log2 domain; not 0, which would make the masked scores,
+// -inf, NaN.  (The sums times the keys' scales are below 2^27 of it: scores the size of its floor are 0.)
 __device__ __forceinline__ float row_scale_i4(float scale_log2, int exponent) {
-  return __builtin_ldexpf(scale_log2, 9 - exponent);
+  return fmaxf(__builtin_ldexpf(scale_log2, 9 - exponent), 0x1p-126f);
 }
 // K of code 0 everywhere
 __device__ __forceinline__ F8Operand k_zero_i4() {
@@ -2753,7 +2754,9 @@ int attention_impl(const char* who, const FusedQkv* fz, int window, int sinks, i
   a.bs_shift = shift;
   a.max_seqlen_k = max_seqlen_k;
   a.num_blocks = num_blocks;
-  a.scale_log2 = softmax_scale * kLog2e;
+  // A scale of 0 weighs every visible key the same.  The smallest number stands for it: a masked score,
+  // -inf, stays it when multiplied (the kernels keep subnormal numbers).
+  a.scale_log2 = softmax_scale == 0.0f ? 0x1p-149f : softmax_scale * kLog2e;
   a.out = static_cast<uint16_t*>(out);
   a.o_ts = o_tok_stride;
   a.o_hs = o_head_stride;

@@ -1,0 +1,57 @@
+"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large.
+
+Against the closed form in float64, with the tolerances of the window operator's own tests.
+"""
+import numpy as np
+import pytest
+import torch
+
+import iitj_llm_coopt_amd as M
+from test_gpu_window_attention import KINDS, Setup, closed_form
+
+pytestmark = pytest.mark.gpu
+
+
+def call(s, scale, **kw):
+    """s's call with a softmax scale of its own; two rows behind the last sequence stay."""
+    out = torch.full_like(s.q, 7.0)
+    args = dict(window=s.window, sink_tokens=s.sinks, out=out)
+    return M.flash_attn_varlen_func(
+        q=s.q, k=s.caches[0], v=s.caches[1], cu_seqlens_q=s.cu, max_seqlen_q=s.max_q, seqused_k=s.lens,
+        max_seqlen_k=s.max_k, softmax_scale=scale, causal=True, block_table=s.table, k_scale=s.scales[0],
+        v_scale=s.scales[1], **dict(args, **kw))
+
+
+def check(s, out, scale, note):
+    o, q, row = out.double().cpu().numpy(), s.q.double().cpu().numpy(), 0
+    assert (o[s.T:] == 7.0).all(), f"{note}: rows behind the last sequence were written"
+    for b, (n, L) in enumerate(s.seqs):
+        ref, tol = closed_form(q[row:row + n], s.K[b], s.V[b], scale, s.window, s.sinks, s.kv, s.sk[b], s.sv[b])
+        d = np.abs(o[row:row + n] - ref)
+        assert (d <= tol).all(), f"{note} sequence {b}: {np.isnan(d).sum()} NaN, {np.nanmax(d - tol)} over"
+        row += n
+
+
+# sequences, heads, window: short items in one block each, contexts in several blocks that are joined,
+# windows that fill the GPU
+SHAPES = [([(1, 1), (5, 100), (3, 300), (2, 1)], 8, 2, 90), ([(40, 300), (1, 77)], 8, 2, 90),
+          ([(2, 5000)], 8, 2, 4000), ([(300, 420), (2, 64)], 64, 8, 90)]
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("scale,D", [(0.0, 64), (0.0, 128), (1e-40, 128), (2.0 ** -40, 128), (1.0, 64)])
+def test_softmax_scales(dev, kv, scale, D):
+    """0 weighs every visible key the same; queries of zeros do so at any scale."""
+    for seqs, Hq, Hkv, window in SHAPES:
+        s = Setup(dev, seqs, Hq, Hkv, D, kv, window, 5, seed=window)
+        s.q[::2, ::3] = 0
+        check(s, call(s, scale), scale, f"window {window}, {seqs}")
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("scale", [0.0, 2.0 ** -40])
+def test_softmax_scales_without_a_window(dev, kv, scale):
+    for seqs, Hq, Hkv, _ in SHAPES[:3]:
+        s = Setup(dev, seqs, Hq, Hkv, 128, kv, poison=False, seed=3)
+        s.q[::2, ::3] = 0
+        check(s, call(s, scale), scale, f"{seqs}")
