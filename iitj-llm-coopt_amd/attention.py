@@ -22,6 +22,7 @@ k < sink_tokens).  Pages without a visible key are not read, so they may be free
 INT4 caches (reshape_and_cache_flash(..., "int4")) are attended over as INT8 ones, with or
 without a window; their keys and values are code * scale, unrounded.
 """
+import contextlib
 import functools
 import math
 import operator
@@ -35,8 +36,10 @@ __all__ = ["flash_attn_varlen_func", "paged_attention", "paged_attention_qkv",
            "qkv_attention_supported", "window_workspace_bytes", "workspace_bytes"]
 
 _WS = _lib.WorkspaceCache()
-# held over a window or INT4 call's launches where they share _WS with another thread's on its stream
+# held over the launches of every call that takes its workspace from _WS: another thread's call on the same
+# stream would write its own partial sums between a call's two launches
 _WS_LOCK = threading.Lock()
+_NO_LOCK = contextlib.nullcontext()
 
 
 @functools.lru_cache(maxsize=1024)   # a pure function of the sizes; 0.9 us through ctypes
@@ -133,20 +136,22 @@ def paged_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, ma
     sl = seq_lens.contiguous()
     lib = _lib.load()
     need = _workspace_bytes(B, Hq, Hkv, D, int(max_seqlen_q), int(max_seqlen_k))
-    if workspace is None:
-        workspace = _WS.get(need, q.device)
-    elif workspace.numel() * workspace.element_size() < need:
+    shared = workspace is None
+    if not shared and workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} "
                          f"bytes, {need} needed")
     cs = k_cache.stride()
-    _lib.check(lib.coopt_verify_attention_rows(
-        code, _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k_cache), _lib.ptr(v_cache),
-        cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1], sstr[2],
-        _lib.ptr(block_table), block_table.stride(0), _lib.ptr(cu), _lib.ptr(sl),
-        B, Hq, Hkv, D, bs, NB, int(max_seqlen_q), int(max_seqlen_k), T, float(softmax_scale),
-        _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size(), _lib.stream_handle(q.device)),
-        "coopt_verify_attention")
+    with _WS_LOCK if shared else _NO_LOCK:
+        if shared:
+            workspace = _WS.get(need, q.device)
+        rc = lib.coopt_verify_attention_rows(
+            code, _lib.ptr(q), q.stride(0), q.stride(1), _lib.ptr(k_cache), _lib.ptr(v_cache),
+            cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1], sstr[2],
+            _lib.ptr(block_table), block_table.stride(0), _lib.ptr(cu), _lib.ptr(sl),
+            B, Hq, Hkv, D, bs, NB, int(max_seqlen_q), int(max_seqlen_k), T, float(softmax_scale),
+            _lib.ptr(out), out.stride(0), out.stride(1), _lib.ptr(workspace),
+            workspace.numel() * workspace.element_size(), _lib.stream_handle(q.device))
+    _lib.check(rc, "coopt_verify_attention")
     return out
 
 
@@ -217,30 +222,28 @@ def _window_attention(q, k_cache, v_cache, cu_seqlens_q, seq_lens, block_table, 
         return out
     stream = _lib.raw_stream(index)
     need = _window_workspace_bytes(B, Hq, Hkv, D, max_q, max_k, win, sinks)
-    shared = False
-    if workspace is None:
+    shared = workspace is None
+    if shared and torch.cuda.is_current_stream_capturing():
         # a graph under capture gets a workspace of its own (from its memory pool), so that two
         # graphs captured on one stream may replay at the same time
-        shared = not torch.cuda.is_current_stream_capturing()
-        workspace = _WS.get(need, q.device) if shared else q.new_empty((max(need, 256),), dtype=torch.uint8)
-        have = workspace.numel()
-    else:
+        shared, workspace = False, q.new_empty((max(need, 256),), dtype=torch.uint8)
+    if not shared:
         have = workspace.numel() * workspace.element_size()
         if have < need or not workspace.is_contiguous():
             raise ValueError(f"workspace holds {have} bytes, {need} needed, contiguous")
     cu = cu_seqlens_q if cu_seqlens_q.is_contiguous() else cu_seqlens_q.contiguous()
     sl = seq_lens if seq_lens.is_contiguous() else seq_lens.contiguous()
     o0, o1, _ = out.stride()
-    call = (index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
+    with _WS_LOCK if shared else _NO_LOCK:
+        if shared:
+            workspace = _WS.get(need, q.device)
+            have = workspace.numel()
+        rc = _lib.call_on(
+            index, _lib.entry("coopt_window_attention"), code, q.data_ptr(), q0, q1, k_cache.data_ptr(),
             v_cache.data_ptr(), cs[0], cs[1], cs[2], ks, vs, s0, s1, s2, block_table.data_ptr(),
             block_table.stride(0), cu.data_ptr(), sl.data_ptr(), B, Hq, Hkv, D, bs, NB, max_q, max_k, T,
             win, sinks, 1.0 / math.sqrt(D) if softmax_scale is None else float(softmax_scale), out.data_ptr(),
             o0, o1, workspace.data_ptr(), have, stream)
-    if shared:
-        with _WS_LOCK:
-            rc = _lib.call_on(*call)
-    else:
-        rc = _lib.call_on(*call)
     _lib.check(rc, "coopt_window_attention")
     return out
 
@@ -327,26 +330,29 @@ def paged_attention_qkv(qkv, positions, cos, sin, slot_mapping, k_cache, v_cache
     if B == 0 or T == 0:
         return out
     need = _workspace_bytes(B, Hq, Hkv, D, int(max_seqlen_q), int(max_seqlen_k))
-    if workspace is None:
-        workspace = _WS.get(need, dev)
-    elif workspace.numel() * workspace.element_size() < need:
+    shared = workspace is None
+    if not shared and workspace.numel() * workspace.element_size() < need:
         raise ValueError(f"workspace holds {workspace.numel() * workspace.element_size()} "
                          f"bytes, {need} needed")
     positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
     cu, sl = cu_seqlens_q.contiguous(), seq_lens.contiguous()
     cs = k_cache.stride()
-    _lib.check(_lib.load().coopt_verify_attention_qkv(
-        code, _lib.ptr(qkv_t), 0 if qkv_t is None else qkv_t.stride(0),
-        None if part is None else _lib.ptr(part.buf), 0 if part is None else part.ks,
-        0 if part is None else part.rows_padded * part.n,
-        _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), cos.stride(0), cos.shape[0],
-        _lib.ptr(slot_mapping), _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2],
-        _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1], sstr[2], _lib.ptr(block_table),
-        block_table.stride(0), _lib.ptr(cu), _lib.ptr(sl), B, Hq, Hkv, D, bs, NB,
-        int(max_seqlen_q), int(max_seqlen_k), float(softmax_scale), _lib.ptr(out),
-        out.stride(0), out.stride(1), _lib.ptr(workspace),
-        workspace.numel() * workspace.element_size(), _lib.stream_handle(dev)),
-        "coopt_verify_attention_qkv")
+    lib = _lib.load()
+    with _WS_LOCK if shared else _NO_LOCK:
+        if shared:
+            workspace = _WS.get(need, dev)
+        rc = lib.coopt_verify_attention_qkv(
+            code, _lib.ptr(qkv_t), 0 if qkv_t is None else qkv_t.stride(0),
+            None if part is None else _lib.ptr(part.buf), 0 if part is None else part.ks,
+            0 if part is None else part.rows_padded * part.n,
+            _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), cos.stride(0), cos.shape[0],
+            _lib.ptr(slot_mapping), _lib.ptr(k_cache), _lib.ptr(v_cache), cs[0], cs[1], cs[2],
+            _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1], sstr[2], _lib.ptr(block_table),
+            block_table.stride(0), _lib.ptr(cu), _lib.ptr(sl), B, Hq, Hkv, D, bs, NB,
+            int(max_seqlen_q), int(max_seqlen_k), float(softmax_scale), _lib.ptr(out),
+            out.stride(0), out.stride(1), _lib.ptr(workspace),
+            workspace.numel() * workspace.element_size(), _lib.stream_handle(dev))
+    _lib.check(rc, "coopt_verify_attention_qkv")
     return out
 
 

@@ -1,7 +1,10 @@
-"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large.
+"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large; calls of
+several kinds from several threads.
 
 Against the closed form in float64, with the tolerances of the window operator's own tests.
 """
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -55,3 +58,29 @@ def test_softmax_scales_without_a_window(dev, kv, scale):
         s = Setup(dev, seqs, Hq, Hkv, 128, kv, poison=False, seed=3)
         s.q[::2, ::3] = 0
         check(s, call(s, scale), scale, f"{seqs}")
+
+
+def test_threads_with_and_without_a_window_on_one_stream(dev):
+    """Split calls of three kinds, which share the stream's workspace, from a thread each."""
+    sets = [Setup(dev, [(2, 5000)], 8, 2, 128, "int4", seed=20), Setup(dev, [(1, 6000)], 8, 2, 128, "auto", 3000, 4, seed=21),
+            Setup(dev, [(2, 4800)], 8, 2, 128, "auto", poison=False, seed=22)]
+    runs = [lambda s=s, kw=kw: call(s, 0.09, **kw) for s, kw in zip(sets, ({}, {}, dict(window=None, sink_tokens=0)))]
+    want = [r().clone() for r in runs]
+    torch.cuda.synchronize(dev)
+    bad, failed = [], []
+
+    def work(i):
+        try:
+            for _ in range(150):
+                if not torch.equal(runs[i](), want[i]):
+                    bad.append(i)
+        except Exception as e:  # noqa: BLE001 -- shown by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(3)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+    assert not bad, f"{len(bad)} of 450 calls"
