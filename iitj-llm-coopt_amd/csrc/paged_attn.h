@@ -59,9 +59,10 @@
 // Windows and INT4 (WIN).  Row p sees key k iff k <= p and (k > p - window or k < sinks).  The keys no row
 // of a block sees lie in one gap: tiles are counted without it (Visible), so a call's time follows the keys
 // in sight, not the context, and pages inside the gap are not read.  Tiles that every row sees whole take
-// no mask.  A partly visible tile may hold keys that were never written: values and scales that are not
-// finite are taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly,
-// into the rows that do see them (add_not_finite).  INT4 operands: below.
+// no mask.  A partly visible tile may hold keys that were never written: values that are not finite are
+// taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly, into the
+// rows that do see them (add_not_finite).  Values' scales that are not finite are taken out of every tile
+// (the bias of an INT4 code times infinity would be left of its products otherwise).  INT4 operands: below.
 // Measured, 32/8 heads of 128: 32 sequences of 5 rows, 512-8192 keys, window 2048, bf16: 43.7 us, the
 // bytes at 5.8 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.7 (17.2 and a merge of
 // 3.5: four tiles a wave, each waiting for its own loads); 1 row, window 1024, bf16: 14.2, the host's time
@@ -349,47 +350,57 @@ __device__ __forceinline__ void load_words(const unsigned char* p, uint32_t* dst
 // What take_out_not_finite took out of tiles, for the rows that see it: walks the wave's tiles once
 // more (rare, after its loop, when the loop's registers are free) and adds infinities and NaN to the
 // sums o.  tile(t): the first key of its t-th tile, or -1 to pass over it; page(key); row_sees(rt,
-// key): whether the lane's row of row tile rt does.  bf16 values: a positive infinity is
-// counted per row and element by a product of twos where V holds one (or NaN) with ones where the row
-// sees the key, a negative one likewise; NaN is both.
+// key): whether the lane's row of row tile rt does.  A positive infinity is counted per row and element
+// by a product of twos where V holds one (or NaN) with ones where the row sees the key, a negative one
+// likewise; NaN is both.  A code times an infinite scale is an infinity of its sign, 0 times it NaN.
+// (A key whose weight is under 2^-126 of the row's largest may leave NaN in place of its infinity: the
+// waves' sums are scaled by such weights where they meet.)
 template <int D, int KV, int RT, int ACC, typename Tile, typename Page, typename Sees>
 __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L, int ntiles, Tile tile, Page page,
                                                Sees row_sees, f32x4_t (&o)[RT][ACC]) {
-  constexpr int kDt = D / 16;
+  using Raw = RawTile<D, KV>;
+  constexpr int kDt = D / 16, kElt = Raw::kElt;
   const int grp = (threadIdx.x & 63) >> 4, l16 = threadIdx.x & 15, bs_mask = (1 << a.bs_shift) - 1;
 #pragma unroll 1
   for (int t = 0; t < ntiles; ++t) {
     const int kb = tile(t);
     if (kb < 0) continue;
-    if constexpr (KV != kBf16) {  // a scale: every element of a row that sees the key is NaN
-      uint32_t bad = 0;           // bit j: of the lane's key j
+    uint32_t scale[8];  // codes: of the lane's keys
+    if constexpr (KV != kBf16) {
+      uint32_t bad = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int sub = kb + 16 * (j >> 2), key = min(sub + grp * 4 + (j & 3), L - 1);
-        const uint32_t s = a.vs[page(sub) * a.s_bs + hkv * a.s_hs + (key & bs_mask) * a.s_ts];
-        bad |= ((s & 0x7fffu) >= 0x7c00u ? 1u : 0u) << j;
+        scale[j] = a.vs[page(sub) * a.s_bs + hkv * a.s_hs + (key & bs_mask) * a.s_ts];
+        bad |= not_finite2<kF16Step>(scale[j]);
       }
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float hit = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if ((bad >> j & 1u) && row_sees(rt, kb + 16 * (j >> 2) + grp * 4 + (j & 3))) hit = 1.0f;
-        hit = max_xor32(max_xor16(hit));
-#pragma unroll
-        for (int dt = 0; dt < kDt; ++dt) o[rt][dt] += hit > 0.0f ? NAN : 0.0f;
-      }
-      continue;
+      if (!__builtin_amdgcn_ballot_w64(bad != 0)) continue;
     }
-    const uint16_t* v0 = static_cast<const uint16_t*>(a.vc) + hkv * a.c_hs;
+    const unsigned char* v0 = static_cast<const unsigned char*>(a.vc) + kElt * (hkv * a.c_hs) + l16 * Raw::kVBytes;
     const int64_t c_bs = a.c_bs, c_ts = a.c_ts;
-    uint32_t v[8][kDt / 2];
+    uint32_t v[8][Raw::kVWords];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int sub = kb + 16 * (j >> 2), key = min(sub + grp * 4 + (j & 3), L - 1);
-      load_words<2 * kDt>(reinterpret_cast<const unsigned char*>(v0 + page(sub) * c_bs + (key & bs_mask) * c_ts + l16 * kDt),
-                          v[j]);
+      load_words<Raw::kVBytes>(v0 + kElt * (page(sub) * c_bs + (key & bs_mask) * c_ts), v[j]);
     }
+    // the value of code c, key j, as bf16: 0 where it is finite
+    auto value = [&](int j, int c) -> uint32_t {
+      const uint32_t s = scale[j] & 0x7fffu;
+      const uint32_t x = s > 0x7c00u || c == 0 ? 0x7fc0u : (c < 0) != (scale[j] > 0x7fffu) ? 0xff80u : 0x7f80u;
+      return s < 0x7c00u ? 0u : x;
+    };
+    auto pair = [&](int w, int dt) -> uint32_t {  // element dt of the lane's keys 2 w and 2 w + 1
+      if constexpr (KV == kBf16) {
+        return __builtin_amdgcn_perm(v[2 * w + 1][dt >> 1], v[2 * w][dt >> 1], (dt & 1) ? 0x07060302u : 0x05040100u);
+      } else {
+        auto code = [&](int j) {
+          if constexpr (KV == kI4) return static_cast<int>(v[j][0] >> (4 * dt) & 15u) - 8;
+          else return static_cast<int>(static_cast<int8_t>(v[j][dt >> 2] >> (8 * (dt & 3))));
+        };
+        return value(2 * w, code(2 * w)) | (value(2 * w + 1, code(2 * w + 1)) << 16);
+      }
+    };
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       u32x4_t see;
@@ -403,8 +414,7 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
         u32x4_t up, down;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-          const uint32_t x = __builtin_amdgcn_perm(v[2 * w + 1][dt >> 1], v[2 * w][dt >> 1],
-                                                   (dt & 1) ? 0x07060302u : 0x05040100u);
+          const uint32_t x = pair(w, dt);
           const uint32_t bad = not_finite2<kBf16Step>(x), nan = ((x & 0x7fff7fffu) + 0x007f007fu) & 0x80008000u;
           up[w] = (nan | (bad & ~x)) >> 1;  // 0x4000: bf16 2
           down[w] = (nan | (bad & x)) >> 1;
@@ -1013,7 +1023,9 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
   // per wave).  Scales are non-negative fp16, so their bit patterns order them; non-finite
   // patterns count as the largest finite scale.  Run on a tile before it is computed, at the
   // end of the previous tile's compute, where that tile's registers are free.
-  // WIN: a scale that is not finite, or of a key that no row of the block sees, does not count.
+  // WIN: a scale that is negative, or of a key that no row of the block sees, does not count; one that is
+  // not finite is taken out here (0x7bff, the largest finite one, is the highest threshold) and left to
+  // add_not_finite.
   auto counted_scale = [&](const Raw& raw, int t) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
     uint32_t most = 0;
@@ -1027,16 +1039,21 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
       }
     return most;
   };
-  auto vcheck = [&](const Raw& raw, int t) {
+  auto vcheck = [&](Raw& raw, int t) {
     if constexpr (CODES) {
       const uint32_t wv = max_u16x2(max_u16x2(raw.vs[0][0], raw.vs[0][1]),
                                     max_u16x2(raw.vs[1][0], raw.vs[1][1]));
       const uint32_t smax = WIN ? max(wv & 0xffffu, wv >> 16) : min(max(wv & 0xffffu, wv >> 16), 0x7bffu);
       const uint32_t thr = !ev_set ? 0u
-                           : (e_v + 7 >= 16 ? 0x7c00u : static_cast<uint32_t>(e_v + 7 + 15) << 10);
+                           : (e_v + 7 >= 16 ? (WIN ? 0x7bffu : 0x7c00u) : static_cast<uint32_t>(e_v + 7 + 15) << 10);
       if (__builtin_amdgcn_ballot_w64(smax > thr)) {
         uint32_t wm = smax;
-        if constexpr (WIN) wm = counted_scale(raw, t);
+        if constexpr (WIN) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            raw.vs[w >> 1][w & 1] = take_out_not_finite<kF16Step>(raw.vs[w >> 1][w & 1], not_finite);
+          wm = counted_scale(raw, t);
+        }
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1)
           wm = max(wm, static_cast<uint32_t>(__shfl_xor(static_cast<int>(wm), off, 64)));
@@ -1067,14 +1084,10 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
     const int kb = vis.key_of(k_begin + t * kTileKeys);
     // every key of the tile inside the split and visible to every row: no masking
     const bool open = WIN ? tile_open(kb) : kb + kTileKeys <= k_end && kb + kTileKeys - 1 <= min_lim;
-    // values (INT8, INT4: their scales) that are not finite, in a tile that not every row sees whole:
-    // 0 * inf would reach the other rows, so they wait for add_not_finite
-    if (WIN && !open) {
-      if constexpr (CODES) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          raw.vs[w >> 1][w & 1] = take_out_not_finite<kF16Step>(raw.vs[w >> 1][w & 1], not_finite);
-      } else {
+    // bf16 values that are not finite, in a tile that not every row sees whole: 0 * inf would reach the
+    // other rows, so they wait for add_not_finite
+    if constexpr (WIN && !CODES) {
+      if (!open) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -1452,7 +1465,7 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
           a, hkv, L, (ntiles - wave + kWaves - 1) / kWaves,
           [&](int t) {
             const int kb = vis.key_of(k_begin + (wave + t * kWaves) * kTileKeys);
-            return tile_open(kb) ? -1 : kb;
+            return !CODES && tile_open(kb) ? -1 : kb;
           },
           page_of, [&](int rt, int key) { return sees(a, lim[rt], key); }, o);
   }
@@ -2002,11 +2015,11 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           if (j >= left) vx[j][e] = INT8 ? 0x80808080u : 0u;
     }
     u32x2_t vs = st.vs;
-    if (WIN && !block_open(stage_key(s) + 32 * tile)) {  // as verify_attn_kernel
-      if constexpr (CODES) {
-        vs[0] = take_out_not_finite<kF16Step>(vs[0], not_finite);
-        vs[1] = take_out_not_finite<kF16Step>(vs[1], not_finite);
-      } else {
+    if constexpr (WIN && CODES) {  // as verify_attn_kernel
+      vs[0] = take_out_not_finite<kF16Step>(vs[0], not_finite);
+      vs[1] = take_out_not_finite<kF16Step>(vs[1], not_finite);
+    } else if constexpr (WIN) {
+      if (!block_open(stage_key(s) + 32 * tile)) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -2140,7 +2153,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
                            : (e_v + 7 >= 16 ? 0x7c00u : static_cast<uint32_t>(e_v + 7 + 15) << 10);
       if (__builtin_amdgcn_ballot_w64(smax > thr)) {
         uint32_t wm = smax;
-        if constexpr (WIN) {  // finite ones of keys that some row of the window sees
+        if constexpr (WIN) {  // of keys that some row of the window sees, not negative
           wm = 0;
 #pragma unroll
           for (int kt = 0; kt < kSub; ++kt)
@@ -2364,7 +2377,7 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           a, hkv, L, pair ? stages : 2 * stages,
           [&](int t) {
             const int kb = pair ? stage_key(t) + 32 * tile : stage_key(t >> 1) + 32 * (t & 1);
-            return tile_seen(kb) && !block_open(kb) ? kb : -1;
+            return tile_seen(kb) && (CODES || !block_open(kb)) ? kb : -1;
           },
           [&](int key) { return clamp_page(table[min(key, L - 1) >> a.bs_shift], a.num_blocks); },
           [&](int rt, int key) { return sees(a, lim[rt], key); }, o);

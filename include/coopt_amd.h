@@ -332,7 +332,8 @@ int coopt_verify_attention_window_rows(int kv_dtype, int B, int Hq, int Hkv, int
  *   total_q      query rows of the call (0: unknown); decides how long items are cut, nothing else
  * Pages that hold no visible key are not read: their block ids may be anything (ids outside the
  * pool are clamped to it), and what a key or value that a row does not see holds, infinities and NaN
- * included, does not reach that row.  Rows that see no key are written as zeros.  Scores
+ * included, does not reach that row.  Rows that see no key are written as zeros.  A value that is not
+ * finite (over codes: code * scale with such a scale) is one in every row that sees it.  Scores
  * (softmax_scale q . k) are below 2^30 in magnitude; softmax_scale is finite and not negative (0: every
  * visible key weighs the same).
  * The other arguments, and the limits on shapes and alignment, are coopt_verify_attention's.

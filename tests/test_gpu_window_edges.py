@@ -1,5 +1,5 @@
-"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large; calls of
-several kinds from several threads.
+"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large; values'
+scales that are not finite; calls of several kinds from several threads.
 
 Against the closed form in float64, with the tolerances of the window operator's own tests.
 """
@@ -58,6 +58,47 @@ def test_softmax_scales_without_a_window(dev, kv, scale):
         s = Setup(dev, seqs, Hq, Hkv, 128, kv, poison=False, seed=3)
         s.q[::2, ::3] = 0
         check(s, call(s, scale), scale, f"{seqs}")
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kv", ["int8", "int4"])
+@pytest.mark.parametrize("rows,L,Hq,Hkv,window", [(4, 400, 8, 2, 300), (16, 400, 8, 2, 300), (40, 400, 8, 2, 300),
+                                                  (300, 600, 64, 8, 250), (2, 5000, 8, 2, 4000)])
+def test_scales_that_are_not_finite(dev, kv, D, rows, L, Hq, Hkv, window):
+    """A value of code c and scale s is c * s: an infinite scale makes infinities of the codes' signs
+    and NaN of zeros, a NaN one NaN, for every row that sees the key and for no other, wherever the
+    key stands: in tiles that all rows see, and at the windows' edges."""
+    s = Setup(dev, [(rows, L)], Hq, Hkv, D, kv, window, 3, seed=rows)
+    q = s.q.double().cpu().numpy()[:rows]
+    ref, tol = closed_form(q, s.K[0], s.V[0], D ** -0.5, window, 3, kv, s.sk[0], s.sv[0])
+    first = L - rows
+    low = first - window + 1                     # the first key of the first row's window
+    inf, nan = float("inf"), float("nan")
+    far = low + 140                              # seen by the first rows at least
+    for bad in ({far: inf}, {far: nan}, {far: inf, far + 5: inf}, {low + 1: inf}, {L - 1: nan}, {first + 1: inf, low: inf},
+                {1: inf}):
+        kept = {}
+        values = s.V[0].copy()
+        for key, x in bad.items():
+            page, off = int(s.table[0, key // 16]), key % 16
+            kept[page, off] = s.scales[1][page, off].clone()
+            s.scales[1][page, off] = x
+            codes = np.rint(s.V[0][key] / s.sv[0][key][:, None])
+            with np.errstate(invalid="ignore"):
+                values[key] = codes * x
+        got = s.run().double().cpu().numpy()[:rows]
+        for (page, off), x in kept.items():
+            s.scales[1][page, off] = x
+        for j in range(rows):
+            p = first + j
+            seen = [k for k in bad if k <= p and (k > p - window or k < 3)]
+            if not seen:
+                assert (np.abs(got[j] - ref[j]) <= tol[j]).all(), (bad, j)
+                continue
+            with np.errstate(invalid="ignore"):
+                want = sum(values[k] for k in seen)      # [Hkv, D]
+            want = np.repeat(want, Hq // Hkv, 0)
+            assert np.array_equal(got[j], want, equal_nan=True), (bad, j)
 
 
 def test_threads_with_and_without_a_window_on_one_stream(dev):
