@@ -1105,48 +1105,48 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
     // at 48 rows and more they are built after the softmax, which keeps them out of the
     // score phase's registers ----
     u32x4_t va[kDt];
-    auto build_va_i4 = [&]() {
-      I4Nibbles x[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = i4_nibbles(raw.v[j][0]);
-      each<kDt>([&](auto dt) {
-        constexpr int DT = decltype(dt)::value;
-#pragma unroll
-        for (int e2 = 0; e2 < 4; ++e2)
-          va[DT][e2] = v_pair_i4<DT>(x[2 * e2], x[2 * e2 + 1]);
-      });
-    };
     auto build_va = [&]() {
-      if constexpr (INT4) return build_va_i4();
-      uint32_t vx[8][Raw::kVWords];
+      if constexpr (INT4) {
+        I4Nibbles x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j) x[j] = i4_nibbles(raw.v[j][0]);
+        each<kDt>([&](auto dt) {
+          constexpr int DT = decltype(dt)::value;
 #pragma unroll
-        for (int w = 0; w < Raw::kVWords; ++w) vx[j][w] = INT8 ? (raw.v[j][w] ^ 0x80808080u) : raw.v[j][w];
-      if constexpr (INT8) {
-        // exact fp16 codes; the V scales go into P (below).  Two byte selects interleave
-        // keys j0, j1 over four d's, two more place each pair under the 0x64 exponent bytes.
-#pragma unroll
-        for (int w = 0; w < Raw::kVWords; ++w)
-#pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            const int j0 = 2 * e2, j1 = 2 * e2 + 1;  // keys of k-elements 2*e2, 2*e2+1
-            const uint32_t lo = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], 0x05010400u);
-            const uint32_t hi = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], 0x07030602u);
-            va[4 * w + 0][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, lo, 0x04010400u));
-            va[4 * w + 1][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, lo, 0x04030402u));
-            va[4 * w + 2][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, hi, 0x04010400u));
-            va[4 * w + 3][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, hi, 0x04030402u));
-          }
+          for (int e2 = 0; e2 < 4; ++e2)
+            va[DT][e2] = v_pair_i4<DT>(x[2 * e2], x[2 * e2 + 1]);
+        });
       } else {
+        uint32_t vx[8][Raw::kVWords];
 #pragma unroll
-        for (int dt = 0; dt < kDt; ++dt)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-          for (int e2 = 0; e2 < 4; ++e2) {
-            const int j0 = 2 * e2, j1 = 2 * e2 + 1;  // keys of k-elements 2*e2, 2*e2+1
-            const int w = INT4 ? 0 : dt >> 1;
-            va[dt][e2] = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], (dt & 1) ? 0x07060302u : 0x05040100u);
-          }
+          for (int w = 0; w < Raw::kVWords; ++w) vx[j][w] = INT8 ? (raw.v[j][w] ^ 0x80808080u) : raw.v[j][w];
+        if constexpr (INT8) {
+          // exact fp16 codes; the V scales go into P (below).  Two byte selects interleave
+          // keys j0, j1 over four d's, two more place each pair under the 0x64 exponent bytes.
+#pragma unroll
+          for (int w = 0; w < Raw::kVWords; ++w)
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) {
+              const int j0 = 2 * e2, j1 = 2 * e2 + 1;  // keys of k-elements 2*e2, 2*e2+1
+              const uint32_t lo = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], 0x05010400u);
+              const uint32_t hi = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], 0x07030602u);
+              va[4 * w + 0][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, lo, 0x04010400u));
+              va[4 * w + 1][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, lo, 0x04030402u));
+              va[4 * w + 2][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, hi, 0x04010400u));
+              va[4 * w + 3][e2] = codes_f16x2(__builtin_amdgcn_perm(k64, hi, 0x04030402u));
+            }
+        } else {
+#pragma unroll
+          for (int dt = 0; dt < kDt; ++dt)
+#pragma unroll
+            for (int e2 = 0; e2 < 4; ++e2) {
+              const int j0 = 2 * e2, j1 = 2 * e2 + 1;  // keys of k-elements 2*e2, 2*e2+1
+              const int w = dt >> 1;
+              va[dt][e2] = __builtin_amdgcn_perm(vx[j1][w], vx[j0][w], (dt & 1) ? 0x07060302u : 0x05040100u);
+            }
+        }
       }
     };
     constexpr bool kVFirst = RT <= 2 && !(WIN && KV == kBf16 && D == 128 && RT == 2);
@@ -1177,44 +1177,40 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
 #pragma unroll
           for (int kt = 0; kt < 2; ++kt) acc[rt][kt] = mfma_f8(kop[kt], qop, acc[rt][kt]);
         }
-    }
-#pragma unroll
-    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks) {
-      u32x4_t qop[RT];
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        qop[rt] = *reinterpret_cast<const u32x4_t*>(qlds + rt * 16 * kQPitch + q_byte(ks));
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-        u32x4_t kop;
-        if constexpr (INT8) {
-          // the lane's key l16 of sub-tile kt: codes 8*(ks%2) .. +8 of its load ks/2
-          const u32x4_t& c4 = raw.k[kt][ks >> 1];
-          const float sk = f16_to_f32(static_cast<uint16_t>(raw.ks[kt]));
-          const float skb = -1152.0f * sk;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t ux = c4[(ks & 1) * 2 + h] ^ 0x80808080u;
-            kop[2 * h] = dequant_pair(__builtin_amdgcn_perm(k64, ux, 0x04010400u), sk, skb);
-            kop[2 * h + 1] = dequant_pair(__builtin_amdgcn_perm(k64, ux, 0x04030402u), sk, skb);
-          }
-        } else if constexpr (INT4) {
-          kop = u32x4_t{0, 0, 0, 0};  // not reached: no steps
-        } else {
-          kop = raw.k[kt][ks];
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = mfma_bf16(kop, qop[rt], acc[rt][kt]);
-      }
-    }
-
-    if constexpr (INT4) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) acc[rt][kt][i] = times_f16(acc[rt][kt][i], raw.ks4[kt][i >> 1], i & 1);
+    } else {
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks) {
+        u32x4_t qop[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          qop[rt] = *reinterpret_cast<const u32x4_t*>(qlds + rt * 16 * kQPitch + q_byte(ks));
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+          u32x4_t kop;
+          if constexpr (INT8) {
+            // the lane's key l16 of sub-tile kt: codes 8*(ks%2) .. +8 of its load ks/2
+            const u32x4_t& c4 = raw.k[kt][ks >> 1];
+            const float sk = f16_to_f32(static_cast<uint16_t>(raw.ks[kt]));
+            const float skb = -1152.0f * sk;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t ux = c4[(ks & 1) * 2 + h] ^ 0x80808080u;
+              kop[2 * h] = dequant_pair(__builtin_amdgcn_perm(k64, ux, 0x04010400u), sk, skb);
+              kop[2 * h + 1] = dequant_pair(__builtin_amdgcn_perm(k64, ux, 0x04030402u), sk, skb);
+            }
+          } else {
+            kop = raw.k[kt][ks];
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) acc[rt][kt] = mfma_bf16(kop, qop[rt], acc[rt][kt]);
+        }
+      }
     }
 
     // ---- online softmax (log2 domain) ----
@@ -2108,21 +2104,22 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
 #pragma unroll
           for (int rt = 0; rt < 2; ++rt) acc[rt][kt] = mfma_f8(kop, q8[rt][part], acc[rt][kt]);
       }
-    }
+    } else {
 #pragma unroll
-    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks)
+      for (int ks = 0; ks < kKs; ++ks)
 #pragma unroll
-      for (int kt = 0; kt < kSub; ++kt) {
-        const u32x4_t kop = fk[(kt * kKs + ks) * 64];
+        for (int kt = 0; kt < kSub; ++kt) {
+          const u32x4_t kop = fk[(kt * kKs + ks) * 64];
 #pragma unroll
-        for (int rt = 0; rt < 2; ++rt) acc[rt][kt] = mfma_bf16(kop, qop[rt][ks], acc[rt][kt]);
+          for (int rt = 0; rt < 2; ++rt) acc[rt][kt] = mfma_bf16(kop, qop[rt][ks], acc[rt][kt]);
+        }
+      // two k-steps' fragments ahead of the MFMAs that take them (0x100: LDS reads, 8: MFMAs)
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * kSub, 0);
+#pragma unroll
+      for (int ks = 0; ks < kKs; ++ks) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * kSub, 0);
+        if (ks + 2 < kKs) __builtin_amdgcn_sched_group_barrier(0x100, kSub, 0);
       }
-    // two k-steps' fragments ahead of the MFMAs that take them (0x100: LDS reads, 8: MFMAs)
-    if constexpr (!INT4) __builtin_amdgcn_sched_group_barrier(0x100, 2 * kSub, 0);
-#pragma unroll
-    for (int ks = 0; ks < (INT4 ? 0 : kKs); ++ks) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 2 * kSub, 0);
-      if (ks + 2 < kKs) __builtin_amdgcn_sched_group_barrier(0x100, kSub, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     // V's fragments, read under the softmax
