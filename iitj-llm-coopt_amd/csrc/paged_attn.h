@@ -170,11 +170,12 @@ struct Visible {
 
 // verify_attn_kernel's leading scalar arguments: the fields its first load round needs (row
 // range, key count, the first tile's pages) and the launch mode (0 a grid of (split, KV head,
-// sequence), 1 ordered items (plan), 2 query windows).  As scalars ahead of the AttnArgs they are
+// sequence), 1 ordered items (plan), 2 query windows), and the last entry of a table row that max_seqlen_k
+// keys need (a row's stride may be more than what is its own).  As scalars ahead of the AttnArgs they are
 // preloaded into SGPRs (the build's kernarg-preload option), so that round does not wait for a
 // kernel-argument load; the rest of AttnArgs loads alongside it.
 #define ATTN_LEAD(a) (a).cu, (a).seq_lens, (a).bt, (a).bt_stride, (a).split, (a).bs_shift, \
-                     ((a).plan ? 1 : ((a).nwin > 0 ? 2 : 0))
+                     ((a).plan ? 1 : ((a).nwin > 0 ? 2 : 0)), ((a).max_seqlen_k - 1) >> (a).bs_shift
 
 // Partials of a fused epilogue are reduced with a compile-time slice bound (every load
 // unconditional, see Partials4); launches with more slices are rejected on the host.
@@ -563,7 +564,7 @@ __device__ void plan_item(const AttnArgs& a, int lane, int* out) {
 template <int D, int KV, int RT, bool SC, int FUSED, bool WIN>
 __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, WIN)) void verify_attn_kernel(
     const int32_t* cu_p, const int32_t* sl_p, const int32_t* bt_p, int64_t bt_stride, int split,
-    int bs_shift, int mode, AttnArgs a) {
+    int bs_shift, int mode, int bt_last, AttnArgs a) {
   using Raw = RawTile<D, KV>;
   constexpr bool INT8 = KV == kI8, INT4 = KV == kI4, CODES = KV != kBf16;
   constexpr int kWaves = waves_for(RT);
@@ -607,15 +608,14 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
   // the wave-uniform page lookups be scalar loads, which do not wait behind (or drain) the
   // wave's outstanding K/V vector loads.
   typedef const __attribute__((address_space(4))) int32_t* const_i32_ptr;
-  const int64_t bt_last = bt_stride - 1;
   // The pages of the wave's first tile of piece sidx of sequence b, looked up before L is
   // known: they are used only if that tile is full, i.e. all its keys are < L, where no
-  // clamp to L - 1 applies (the index is kept inside the table row regardless).
+  // clamp to L - 1 applies (the index is kept inside the row's needed entries regardless).
   auto first_pages = [&](int b, int sidx, int32_t& p0, int32_t& p1) {
     const const_i32_ptr tb = (const_i32_ptr)(bt_p + static_cast<int64_t>(b) * bt_stride);
     const int kb = sidx * split + wave * kTileKeys;
-    p0 = tb[min<int64_t>(kb >> bs_shift, bt_last)];
-    p1 = tb[min<int64_t>((kb + 16) >> bs_shift, bt_last)];
+    p0 = tb[min(kb >> bs_shift, bt_last)];
+    p1 = tb[min((kb + 16) >> bs_shift, bt_last)];
   };
 
   // One piece: keys [sidx * split, min(L, (sidx + 1) * split)) of (sequence b, KV head hkv)

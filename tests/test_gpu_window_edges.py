@@ -1,5 +1,6 @@
-"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large; values'
-scales that are not finite; calls of several kinds from several threads.
+"""GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large;
+values' scales that are not finite; block tables whose rows are part of longer ones; calls of several kinds from
+several threads.
 
 Against the closed form in float64, with the tolerances of the window operator's own tests.
 """
@@ -99,6 +100,22 @@ def test_scales_that_are_not_finite(dev, kv, D, rows, L, Hq, Hkv, window):
                 want = sum(values[k] for k in seen)      # [Hkv, D]
             want = np.repeat(want, Hq // Hkv, 0)
             assert np.array_equal(got[j], want, equal_nan=True), (bad, j)
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("window", [None, 150])
+def test_block_tables_that_are_views(dev, kv, window):
+    """Columns [1:] of a wider table, the last row's end the end of its memory: as with a table of their own."""
+    for seqs, Hq, Hkv in (([(2, 40), (1, 33)], 8, 2), ([(1, 5000)], 8, 2), ([(40, 300), (1, 20)], 8, 2),
+                          ([(1, 100)] * 40, 64, 8)):
+        s = Setup(dev, seqs, Hq, Hkv, 128, kv, window, 5 if window else 0, poison=False, seed=4)
+        s.table = s.table[:, : -(-s.max_k // 16)].contiguous()
+        want = call(s, 0.09)
+        wide = torch.full((len(seqs), s.table.shape[1] + 1), 2 ** 30, dtype=torch.int32, device=dev)
+        wide[:, 1:] = s.table
+        s.table = wide[:, 1:]
+        assert torch.equal(call(s, 0.09), want), seqs
+        check(s, want, 0.09, f"{seqs}")
 
 
 def test_threads_with_and_without_a_window_on_one_stream(dev):
