@@ -18,7 +18,10 @@ the GPU, of 128/(Hq/Hkv) rows in a kernel that stages K and V in LDS for the win
 
 window=W limits a query at position p to the keys above p - W, beside the first sink_tokens keys
 of its sequence, which stay visible (attention sinks): key k is seen iff k <= p and (k > p - W or
-k < sink_tokens).  Pages without a visible key are not read, so they may be freed and reused.
+k < sink_tokens).  Pages without a visible key do not reach the output, whatever their table entries
+and contents are, so they may be freed and reused by others.  Keys go in steps of 32 or 64, so up to
+63 hidden keys before the window and behind the first tokens are loaded, from the pool's page that
+the table entry is clamped to; the pages between are not read.
 INT4 caches (reshape_and_cache_flash(..., "int4")) are attended over as INT8 ones, with or
 without a window; their keys and values are code * scale, unrounded.
 """

@@ -58,7 +58,8 @@
 // it cancels in o / l like the running max does.
 // Windows and INT4 (WIN).  Row p sees key k iff k <= p and (k > p - window or k < sinks).  The keys no row
 // of a block sees lie in one gap: tiles are counted without it (Visible), so a call's time follows the keys
-// in sight, not the context, and pages inside the gap are not read.  Tiles that every row sees whole take
+// in sight, not the context.  The gap's ends are whole tiles: hidden keys that share one with a visible key
+// are loaded, from a page clamped to the pool, and masked; the pages between are not read.  Tiles that every row sees whole take
 // no mask.  A partly visible tile may hold keys that were never written: values that are not finite are
 // taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly, into the
 // rows that do see them (add_not_finite).  Values' scales that are not finite are taken out of every tile

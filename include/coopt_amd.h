@@ -266,7 +266,8 @@ int coopt_kv_copy_blocks(const int64_t* regions, int num_regions, const int64_t*
  *                           in fp16's normal range for every fp16 scale).  The output is
  *                           therefore not bit-equal to the bf16 path on the dequantised
  *                           cache; it stays within the INT8 tolerance of attention over it.
- *   block_table [B, bt_stride] int32; entries past ceil(L/block_size) are never read.
+ *   block_table [B, bt_stride] int32; entries past ceil(L/block_size) are never used;
+ *               those up to ceil(max_seqlen_k/block_size) must be there.
  *   Supported: D in {64, 128}; Hq/Hkv <= 64; block_size a power of two >= 16; B <= 65535.
  *   Query rows: up to 64 rows per (sequence, KV head), i.e. (Hq/Hkv) * max_seqlen_q <= 64
  *   (speculative verify and decode), run on the tuned path (contexts split over blocks).
@@ -330,9 +331,10 @@ int coopt_verify_attention_window_rows(int kv_dtype, int B, int Hq, int Hkv, int
  *                coopt_verify_attention attends over them; INT4 keys and values are code * scale,
  *                unrounded.  INT4 caches are uint8 [NB, block_size, Hkv, D/2], strides in bytes.
  *   total_q      query rows of the call (0: unknown); decides how long items are cut, nothing else
- * Pages that hold no visible key are not read: their block ids may be anything (ids outside the
- * pool are clamped to it), and what a key or value that a row does not see holds, infinities and NaN
- * included, does not reach that row.  Rows that see no key are written as zeros.  A value that is not
+ * The block ids of pages that hold no visible key may be anything, and what a key or value that a row
+ * does not see holds, infinities and NaN included, does not reach that row.  Keys are walked in steps of
+ * 32 or 64: up to 63 hidden keys before the window and behind the first tokens are loaded, from the page
+ * that an id names (clamped to the pool); pages between them are not read.  Rows that see no key are written as zeros.  A value that is not
  * finite (over codes: code * scale with such a scale) is one in every row that sees it.  Scores
  * (softmax_scale q . k) are below 2^30 in magnitude; softmax_scale is finite and not negative (0: every
  * visible key weighs the same).
