@@ -163,8 +163,9 @@ __device__ __forceinline__ int64_t stride_mul(int64_t index, int64_t stride) {
 
 // The INT4 codes of the group's vector (element e of the chunk in nibble e, offset by +8, as
 // coopt_quantize packs them) at the lane's place, and its fp16 scale.
-// The write of 8191 tokens (8 heads of 128, K and V, 42 MB) takes 11.8-12.9 us, a copy of the bytes 6.7; 15.1
-// with codes by rint, clamp and conversion, and 64-bit address products.
+// The write of 8191 tokens (8 heads of 128, K and V, 42 MB) takes 11.7-12.4 us, 3.5 TB/s, a copy of the bytes
+// 6.7; 15.1 with codes by rint, clamp and conversion, and 64-bit address products.  A row is 64 bytes and
+// kv_write_kernel's blocks hold one head each, so in a token-major cache two blocks write each 128-byte line.
 template <int G>
 __device__ __forceinline__ void store_chunk_i4(const uint32_t (&w)[4], uint8_t* dst, uint16_t* scale, int c) {
   uint32_t amax = 0;

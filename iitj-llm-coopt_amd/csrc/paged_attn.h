@@ -59,15 +59,20 @@
 // Windows and INT4 (WIN).  Row p sees key k iff k <= p and (k > p - window or k < sinks).  The keys no row
 // of a block sees lie in one gap: tiles are counted without it (Visible), so a call's time follows the keys
 // in sight, not the context.  The gap's ends are whole tiles: hidden keys that share one with a visible key
-// are loaded, from a page clamped to the pool, and masked; the pages between are not read.  Tiles that every row sees whole take
-// no mask.  A partly visible tile may hold keys that were never written: values that are not finite are
-// taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly, into the
+// are loaded, from a page clamped to the pool, and masked; the pages between are not read.  Tiles that every
+// row sees whole take no mask.  A partly visible tile may hold keys that were never written: values that are
+// not finite are taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly, into the
 // rows that do see them (add_not_finite).  Values' scales that are not finite are taken out of every tile
 // (the bias of an INT4 code times infinity would be left of its products otherwise).  INT4 operands: below.
 // Measured, 32/8 heads of 128: 32 sequences of 5 rows, 512-8192 keys, window 2048, bf16: 43.7 us, the
-// bytes at 5.8 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.7 (17.2 and a merge of
-// 3.5: four tiles a wave, each waiting for its own loads); 1 row, window 1024, bf16: 14.2, the host's time
-// for two launches.
+// bytes at 5.8 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.5 (16.9 and a merge of
+// 3.6: some 4140 keys a sequence go in three pieces of 1280, five tiles a wave, and one of 300, a quarter
+// of the blocks with little to do); 1 row, window 1024, bf16: 13.8, the host's time for two launches.
+// Roundings to fewer than 32 bits, each for the matrix cores' operands: probabilities of bf16 caches to
+// bf16, as without a window (the instructions take no mix of types, and fp16 does not hold bf16's values):
+// outputs lie 2.1e-3 to 2.3e-3 from 64 bits, relative, where 32-bit probabilities leave the output's own
+// rounding, 1.6e-3 to 1.7e-3.  Over codes probability times scale to fp16 and q as two 4-bit numbers, which
+// the output's rounding hides (1.6e-3 to 1.8e-3 either way).
 #pragma once
 
 #include <math.h>
@@ -91,6 +96,11 @@ constexpr int kThreads = 256;  // merge kernel
 constexpr int waves_for(int RT) { return RT <= 3 ? 8 : 4; }
 // Waves a SIMD is to hold: two blocks a CU with 4 waves at head dim 64 and bf16 (79 KB of LDS, at most 256
 // registers asked for), where batches of many query windows take 0.63 to 0.8 of the time; see alone_lds.
+// And two with 8 waves for one row tile of heads of 64 over INT4 codes whose scales lie together (sc): the
+// form takes 131 registers unasked and 127 asked to stay under 128.  48 sequences of 500-4100 keys 30.3 ->
+// 26.1 us, 64 of 2048 33.1 -> 25.1, 256 of 200-2000 81.2 -> 60.5; up to one block a CU the same.
+// Strided scales take 144, and spill when asked: 1.04 to 1.16 of the time, so they are not.  INT8's form fits
+// by itself (112); at head dim 128, or with more row tiles, the accumulators and two tile buffers alone do not.
 constexpr int waves_per_simd(int D, int kv, int RT, bool sc, bool win) {
   if (win && D == 64 && RT == 1 && kv == kI4 && sc) return 4;
   return D == 64 && kv == kBf16 && RT == 4 ? 2 : 1;
@@ -442,9 +452,9 @@ __device__ __forceinline__ void add_not_finite(const AttnArgs& a, int hkv, int L
 // scale multiplies the score, the row's power of two goes into its softmax scale.  At head dim 128 the
 // 128-term MFMA takes one part at a time, at 64 both at once (K twice in its operand).
 // 32 sequences of 5 rows over 8192 keys (280 MB, 32/8 heads of 128): 70.3 us with K as bf16 16 + n (eight
-// instructions per 8 codes, two q loads a step), 61.5 like this, 58.5 to 60.8 with the maxima taken rarely (kLazy);
-// its loads alone take 55, a copy of the bytes 44.5.  What bounds it: the memory stream and, at 28 % of the
-// matrix cores' cycles, ten VALU instructions a MFMA beside it.
+// instructions per 8 codes, two q loads a step), 59.4 to 62 like this; its loads alone take 55 (5.1 TB/s: V
+// comes in four loads of 4 bytes a lane and sub-tile, of 2 at head dim 64), a copy of the bytes 44.5.  What
+// bounds it: the memory stream and, at 28 % of the matrix cores' cycles, ten VALU instructions a MFMA beside it.
 constexpr float kI4Bias = 8.0f, kI4VUnit = 0x1p20f;
 
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
@@ -1246,8 +1256,12 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
     if constexpr (kLazy) {
       // The probabilities against the reference as it is; the tile's maxima only if a lane's sum of
       // them passes 2^kSlack (each is at most that sum), so no exchange between lanes stands between
-      // most tiles' scores and their exponents.  Over INT4 codes 61.5 -> 58.5 us (32 sequences of 5
-      // rows and 8192 keys, 32/8 heads of 128), 20.1 -> 20.7 us at 4 tiles a wave; bf16 tiles have no registers for it (20 rows: 28 spilled).
+      // most tiles' scores and their exponents.  Alternated with maxima for every tile (32/8 heads): 32
+      // sequences of 5 rows and 8192 keys, INT4, 79.4 -> 77.1 us (128; inputs that no cache holds) and 56.4 ->
+      // 54.2 (64); 8 sequences over 4100 keys in sight 22.4 -> 22.5; at worst 24.0 -> 24.4 (INT4) and 25.0 ->
+      // 25.8 (INT8, both 4 sequences of 5 rows, 16000 keys, 64).  Three row tiles of 128 spill without it: 57.5 ->
+      // 32.9 (INT4), 54.0 -> 37.0 (INT8; 16 sequences of 9 rows, 3000 keys).  bf16 tiles have no registers
+      // for it (20 rows: 28 spilled).
       float sum[RT];
       auto probabilities = [&]() {
 #pragma unroll
@@ -2440,8 +2454,12 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
 // are not split however few the items are (1 sequence, 8 KV heads, bf16, 1 row, 400 keys: 9.0 us
 // whole, the merge launch alone costs 3); past that a split may be as short as one round (717
 // keys: 11.6 us whole, 11.8 in splits of two rounds, 9.8 of one; 4096 keys: 13.2 and 11.7).
-// INT4 contexts of up to kWholeRoundsI4 rounds are not split either (1 sequence, 8 KV heads, 1 row of 128:
-// 600 keys 8.9 us whole, 10.6 split; 1000 keys 11.4 and 10.4; the merge's launch costs the host 3 more).
+// INT4 contexts of up to kWholeRoundsI4 rounds (768 keys; 384 with 4 waves) are not split either.  530 and 700
+// keys, heads of 64 and 128, 32/8, 28/4, 8/8 and 64/8 of them, 1 to 8 sequences of 1 and 5 rows, replayed from a
+// graph: with one or two row tiles 0.82 to 1.03 of the split call's time (1 sequence, 8 KV heads, 1 row of 128:
+// 8.5 us whole, 10.1 split), with three 0.95 to 1.14 (5 rows of 7 heads, 700 keys: 16.3 and 14.4); called one by one
+// 0.82 to 1.05 of it, the merge's launch costing the host 3 us.  Four rounds: 1000 keys take 0.99 to 1.06 with
+// one row tile, 1.05 to 1.3 with more.
 constexpr int kWholeRounds = 2, kWholeRoundsI4 = 3;
 int target_blocks(int waves) { return waves == 8 ? 256 : 512; }
 

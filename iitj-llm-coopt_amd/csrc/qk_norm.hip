@@ -5,8 +5,12 @@
 // in fp32, rounded to bf16 once.  q goes to q_out, k to the cache; v goes to the cache unchanged.
 // An INT8 or INT4 cache holds the codes of the rounded k and v, as coopt_kv_write makes them.
 //
-// What bounds it: the memory stream at many rows (4093 rows of 32/8 heads of 64, 50.9 MB: 11.4 us, 4.5 TB/s;
-// a copy of the bytes 8.1), the call's host time at few (one row: 9.6 us, the kernel 2.8).  A vector
+// What bounds it: the loads in flight at many rows (4093 rows of 32/8 heads of 64, 50.9 MB: 11.5 us, 4.4 TB/s;
+// a copy of the bytes 8.1): a lane has one 16-byte load of its row out, beside 48 bytes of cos, sin and weight
+// that every head reads again from the caches.  At few rows the call's host time (one row: 9.5 us, the
+// kernel 2.8).  4093 rows of 128: 21.4 us into bf16, 20.7 into INT8, 20.8 into INT4 caches (101.7, 93.5 and
+// 89.3 MB); of 64 12.4, 13.9 and 14.2; 160 rows of 128 3.7 to 4.2, from four slices of partial sums 5.4 to 6.0.
+// A vector
 // stays in its lanes' registers: the sum of squares goes round the group by DPP, and so does the
 // other half that a rotation needs (through LDS shuffles, 8 a lane, the same rows took 14.1 us).  Token and
 // slot are uniform in a block: their page arithmetic is one shift, and cos, sin and the slot load beside
