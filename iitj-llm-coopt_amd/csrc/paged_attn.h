@@ -1726,7 +1726,7 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a) {
     float m_new = M;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (s0 + u * kSG + sg >= nsplit) ml[u].x = -INFINITY;
+      if (s0 + u * kSG + sg >= nsplit) ml[u] = make_float2(-INFINITY, 0.0f);
       m_new = fmaxf(m_new, ml[u].x);
     }
     const float f = M > -INFINITY ? exp2_fast(M - m_new) : 0.0f;
@@ -1735,8 +1735,9 @@ __global__ __launch_bounds__(kThreads) void merge_kernel(AttnArgs a) {
     acc1 *= f;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      // a split without a visible key has no sums worth reading (its maximum is -inf)
-      if (!(ml[u].x > -INFINITY)) continue;
+      // a split without a visible key has no sums worth reading (its maximum is -inf); one whose scores
+      // are all NaN has no maximum either, and NaN sums that the row takes on
+      if (!(ml[u].x > -INFINITY) && ml[u].y == 0.0f) continue;
       const float w = exp2_fast(ml[u].x - m_new);
       Lsum += ml[u].y * w;
       acc0 += x0[u] * w;

@@ -1,6 +1,6 @@
 """GPU: paged attention at the edges of its arguments: softmax scales of zero, tiny and large;
-values' scales that are not finite; block tables whose rows are part of longer ones; calls of several kinds from
-several threads.
+values' scales that are not finite; queries that are not finite in contexts that
+are split; block tables whose rows are part of longer ones; calls of several kinds from several threads.
 
 Against the closed form in float64, with the tolerances of the window operator's own tests.
 """
@@ -100,6 +100,23 @@ def test_scales_that_are_not_finite(dev, kv, D, rows, L, Hq, Hkv, window):
                 want = sum(values[k] for k in seen)      # [Hkv, D]
             want = np.repeat(want, Hq // Hkv, 0)
             assert np.array_equal(got[j], want, equal_nan=True), (bad, j)
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("window", [None, 4000])
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_row_that_is_not_finite_in_a_split_context(dev, kv, window, D):
+    """NaN, and the other rows of its pieces and of the other sequence as the closed form has them."""
+    s = Setup(dev, [(3, 6000), (2, 5000)], 8, 2, D, kv, window, 4 if window else 0, poison=window is not None, seed=41)
+    clean = call(s, 0.09)
+    for value in (float("nan"), float("inf"), float("-inf")):
+        kept = s.q.clone()
+        s.q[1, 1, 5] = value
+        got = call(s, 0.09)
+        s.q.copy_(kept)
+        assert torch.isnan(got[1, 1].float()).all(), (value, got[1, 1])
+        got[1, 1] = clean[1, 1]
+        check(s, got, 0.09, f"beside {value}")
 
 
 @pytest.mark.parametrize("kv", KINDS)
