@@ -2638,14 +2638,14 @@ int launch_rt(const char* who, int RT, const AttnArgs& a, dim3 grid, hipStream_t
   if (rc != COOPT_OK || a.max_splits <= 1) return rc;
   const int rows = a.Hkv * a.rmax, per = kThreads / 64;
   hipLaunchKernelGGL((merge_kernel<D, WIN>), dim3((rows + per - 1) / per, a.B), dim3(kThreads), 0, s, a);
-  return coopt::check_launch((std::string(who) + "/merge").c_str());
+  return coopt::check_launch(WIN ? "coopt_window_attention/merge" : "coopt_verify_attention/merge");
 }
 
 template <int D, int KV, bool WIN>
 int launch_kv(const char* who, bool sc, int RT, const AttnArgs& a, dim3 grid, hipStream_t s) {
   if (a.prefill) {
     hipLaunchKernelGGL((prefill_attn_kernel<D, KV, WIN>), grid, dim3(256), 0, s, a);
-    return coopt::check_launch((std::string(who) + "/prefill").c_str());
+    return coopt::check_launch(WIN ? "coopt_window_attention/prefill" : "coopt_verify_attention/prefill");
   }
   if constexpr (KV == kBf16) return launch_rt<D, KV, false, WIN>(who, RT, a, grid, s);
   else return sc ? launch_rt<D, KV, true, WIN>(who, RT, a, grid, s) : launch_rt<D, KV, false, WIN>(who, RT, a, grid, s);
