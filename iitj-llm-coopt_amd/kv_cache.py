@@ -60,7 +60,7 @@ def dequantize(q: torch.Tensor, scale, bits: int, dtype=torch.bfloat16):
         raise ValueError(f"bits must be 16, 8 or 4, got {bits}")
     index = q.get_device()
     if index < 0 or index != scale.get_device():
-        _lib.require_cuda(q, scale)
+        _lib.require_one_device(q, scale)
     qc, sc = q.contiguous(), scale.contiguous()
     *lead, width = qc.shape
     D = width * (2 if bits == 4 else 1)
@@ -204,14 +204,17 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
     if part is not None:
         if part.n != width:
             raise ValueError(f"partials are {part.n} wide, expected {width}")
-        T, dev = part.rows, part.device
-        qkv_t = None
+        T, src, qkv_t = part.rows, part.buf, None
     else:
         _lib.require_cuda(qkv)
         if qkv.dtype != torch.bfloat16 or qkv.dim() != 2 or qkv.shape[1] != width or qkv.stride(1) != 1:
             raise ValueError(f"qkv must be bf16 [T, {width}] with contiguous rows")
-        T, dev, qkv_t = qkv.shape[0], qkv.device, qkv
-    _lib.require_cuda(positions, cos, sin, k_cache, v_cache, slot_mapping)
+        T, src, qkv_t = qkv.shape[0], qkv, qkv
+    index = src.get_device()
+    if not (index >= 0 and index == positions.get_device() == cos.get_device() == sin.get_device() ==
+            k_cache.get_device() == v_cache.get_device() == slot_mapping.get_device() ==
+            (index if q_out is None else q_out.get_device())):
+        _lib.require_one_device(src, positions, cos, sin, k_cache, v_cache, slot_mapping, q_out)
     _check_cache_pair(k_cache, v_cache)
     NB, bs, cH, cD = k_cache.shape
     if (cH, cD) != (Hkv, D // 2 if kv_cache_dtype == "int4" else D):
@@ -228,27 +231,30 @@ def qkv_rope_and_cache(qkv, positions, cos, sin, k_cache, v_cache, slot_mapping,
     elif kv_cache_dtype == "int8":
         if k_scale is None or v_scale is None or k_scale.stride() != v_scale.stride():
             raise ValueError("'int8' caches need alike k_scale and v_scale scale caches")
+        if not index == k_scale.get_device() == v_scale.get_device():
+            _lib.require_one_device(k_cache, k_scale, v_scale)
         code, ks, vs, sstr = _lib.DT_I8, k_scale, v_scale, k_scale.stride()
     elif kv_cache_dtype == "int4":
         _check_int4(k_cache, v_cache)
         sstr = _scale_args(k_cache, k_scale, v_scale, "int4")
-        _lib.require_cuda(k_scale, v_scale)
+        if not index == k_scale.get_device() == v_scale.get_device():
+            _lib.require_one_device(k_cache, k_scale, v_scale)
         code, ks, vs = _lib.DT_I4, k_scale, v_scale
     else:
         raise ValueError(f"kv_cache_dtype must be 'auto', 'int8' or 'int4', got {kv_cache_dtype!r}")
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=dev)
+        q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=src.device)
     positions, slot_mapping = positions.contiguous(), slot_mapping.contiguous()
     cs = k_cache.stride()
-    _lib.check(_lib.load().coopt_qkv_epilogue(
-        code, _lib.ptr(qkv_t), 0 if qkv_t is None else qkv_t.stride(0),
+    _lib.check(_lib.call_on(
+        index, _lib.entry("coopt_qkv_epilogue"), code, _lib.ptr(qkv_t), 0 if qkv_t is None else qkv_t.stride(0),
         None if part is None else _lib.ptr(part.buf), 0 if part is None else part.ks,
         0 if part is None else part.rows_padded * part.n,
         _lib.ptr(positions), _lib.ptr(cos), _lib.ptr(sin), cos.stride(0),
         cos.shape[0], _lib.ptr(q_out), q_out.stride(0), q_out.stride(1), _lib.ptr(k_cache),
         _lib.ptr(v_cache), cs[0], cs[1], cs[2], _lib.ptr(ks), _lib.ptr(vs), sstr[0], sstr[1],
         sstr[2], _lib.ptr(slot_mapping), T, Hq, Hkv, D, bs, NB,
-        _lib.stream_handle(dev)), "coopt_qkv_epilogue")
+        _lib.raw_stream(index)), "coopt_qkv_epilogue")
     return q_out
 
 
