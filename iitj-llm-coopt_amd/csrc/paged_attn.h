@@ -99,7 +99,7 @@ constexpr int waves_for(int RT) { return RT <= 3 ? 8 : 4; }
 // And two with 8 waves for one row tile of heads of 64 over INT4 codes whose scales lie together (sc): the
 // form takes 131 registers unasked and 127 asked to stay under 128.  48 sequences of 500-4100 keys 30.3 ->
 // 26.1 us, 64 of 2048 33.1 -> 25.1, 256 of 200-2000 81.2 -> 60.5; up to one block a CU the same.
-// Strided scales take 144, and spill when asked: 1.04 to 1.16 of the time, so they are not.  INT8's form fits
+// Strided scales take 146, and spill when asked: 1.04 to 1.16 of the time, so they are not.  INT8's form fits
 // by itself (112); at head dim 128, or with more row tiles, the accumulators and two tile buffers alone do not.
 constexpr int waves_per_simd(int D, int kv, int RT, bool sc, bool win) {
   if (win && D == 64 && RT == 1 && kv == kI4 && sc) return 4;
@@ -1035,19 +1035,23 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
   // patterns count as the largest finite scale.  Run on a tile before it is computed, at the
   // end of the previous tile's compute, where that tile's registers are free.
   // WIN: a scale that is negative, or of a key that no row of the block sees, does not count; one that is
-  // not finite is taken out here (0x7bff, the largest finite one, is the highest threshold) and left to
-  // add_not_finite.
+  // not finite is taken out here (0x7bff, the largest finite one, is the highest threshold) and, where some
+  // row may see its key, left to add_not_finite.
   auto counted_scale = [&](const Raw& raw, int t) {
     const int kb = vis.key_of(k_begin + t * kTileKeys);
     uint32_t most = 0;
+    bool bad = false;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint32_t s = raw.vs[kt][i >> 1] >> (16 * (i & 1)) & 0xffffu;
         const int key = kb + kt * 16 + grp * 4 + i;
-        if (s < 0x7c00u && (key < a.sinks || key > min_lim - a.window)) most = max(most, s);
+        if (!(key < a.sinks || key > min_lim - a.window)) continue;
+        if (s < 0x7c00u) most = max(most, s);
+        else bad = true;
       }
+    not_finite |= __builtin_amdgcn_ballot_w64(bad) ? 1u : 0u;  // uniform: a scalar register
     return most;
   };
   auto vcheck = [&](Raw& raw, int t) {
@@ -1060,10 +1064,11 @@ __global__ __launch_bounds__(64 * waves_for(RT), waves_per_simd(D, KV, RT, SC, W
       if (__builtin_amdgcn_ballot_w64(smax > thr)) {
         uint32_t wm = smax;
         if constexpr (WIN) {
+          wm = counted_scale(raw, t);
+          uint32_t any = 0;
 #pragma unroll
           for (int w = 0; w < 4; ++w)
-            raw.vs[w >> 1][w & 1] = take_out_not_finite<kF16Step>(raw.vs[w >> 1][w & 1], not_finite);
-          wm = counted_scale(raw, t);
+            raw.vs[w >> 1][w & 1] = take_out_not_finite<kF16Step>(raw.vs[w >> 1][w & 1], any);
         }
 #pragma unroll
         for (int off = 1; off < 64; off <<= 1)
@@ -2027,9 +2032,22 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
           if (j >= left) vx[j][e] = INT8 ? 0x80808080u : 0u;
     }
     u32x2_t vs = st.vs;
+    if constexpr (CODES) {
+      vs[0] &= (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
+      vs[1] &= (left > 2 ? 0xffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
+    }
     if constexpr (WIN && CODES) {  // as verify_attn_kernel
-      vs[0] = take_out_not_finite<kF16Step>(vs[0], not_finite);
-      vs[1] = take_out_not_finite<kF16Step>(vs[1], not_finite);
+      uint32_t any = 0;
+      const u32x2_t finite = {take_out_not_finite<kF16Step>(vs[0], any), take_out_not_finite<kF16Step>(vs[1], any)};
+      if (__builtin_amdgcn_ballot_w64(any != 0)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = stage_key(s) + wave * 16 + grp * 4 + i;
+          const bool bad = (vs[i >> 1] >> (16 * (i & 1)) & 0x7fffu) >= 0x7c00u;
+          if (bad && (key < a.sinks || key > L - n - a.window)) not_finite = 1;
+        }
+        vs = finite;
+      }
     } else if constexpr (WIN) {
       if (!block_open(stage_key(s) + 32 * tile)) {
 #pragma unroll
@@ -2039,8 +2057,6 @@ __global__ __launch_bounds__(256, 2) void prefill_attn_kernel(AttnArgs a) {
       }
     }
     if constexpr (CODES) {
-      vs[0] &= (left > 0 ? 0xffffu : 0u) | (left > 1 ? 0xffff0000u : 0u);
-      vs[1] &= (left > 2 ? 0xffffu : 0u) | (left > 3 ? 0xffff0000u : 0u);
       if (l16 == 0) *reinterpret_cast<u32x2_t*>(&lsv[buf][wave * 16 + grp * 4]) = vs;
     }
     // fragment dt of the tile: 8 keys of d-tile dt per lane, this wave's 4 in its half's 8 bytes
