@@ -64,13 +64,13 @@
 // not finite are taken out of it before the products (0 * NaN is NaN) and put back after the loop, exactly, into the
 // rows that do see them (add_not_finite).  Values' scales that are not finite are taken out of every tile
 // (the bias of an INT4 code times infinity would be left of its products otherwise).  INT4 operands: below.
-// Measured, 32/8 heads of 128: 32 sequences of 5 rows, 512-8192 keys, window 2048, bf16: 43.7 us, the
-// bytes at 5.8 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.5 (16.9 and a merge of
-// 3.6: some 4140 keys a sequence go in three pieces of 1280, five tiles a wave, and one of 300, a quarter
-// of the blocks with little to do); 1 row, window 1024, bf16: 13.8, the host's time for two launches.
+// Measured, 32/8 heads of 128: 32 sequences of 5 rows, 512-8192 keys, window 2048, bf16: 44 us, the
+// bytes at 5.7 TB/s of 6.3; 8 sequences of 8000-16000 keys, window 4096, INT4: 20.9 (17.0 and a merge of
+// 3.9: some 4140 keys a sequence go in three pieces of 1280, five tiles a wave, and one of 300, a quarter
+// of the blocks with little to do); 1 row, window 1024, bf16: 13.6, the host's time for two launches.
 // Roundings to fewer than 32 bits, each for the matrix cores' operands: probabilities of bf16 caches to
 // bf16, as without a window (the instructions take no mix of types, and fp16 does not hold bf16's values):
-// outputs lie 2.1e-3 to 2.3e-3 from 64 bits, relative, where 32-bit probabilities leave the output's own
+// outputs lie 2.0e-3 to 2.3e-3 from 64 bits, relative, where 32-bit probabilities leave the output's own
 // rounding, 1.6e-3 to 1.7e-3.  Over codes probability times scale to fp16 and q as two 4-bit numbers, which
 // the output's rounding hides (1.6e-3 to 1.8e-3 either way).
 #pragma once
