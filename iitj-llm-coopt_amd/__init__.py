@@ -9,10 +9,11 @@ surface of mohsinmubarak/iitj-llm-coopt's engine:
                 131; engine/block_manager.py:165-187)
   attention     flash_attn_varlen_func-compatible paged verification attention (model.py:244)
   block_manager BlockManager slot / block-table contract (engine/block_manager.py)
+  mxfp4         microscaled 4-bit rows and weights, for fused.linear
   batch         WorkItem / Batch / build_batch varlen layout (engine/batch.py)
 """
 from . import _lib  # noqa: F401  (imports torch first, then binds the library lazily)
-from . import fused  # noqa: F401  (rms_norm / rope_ / silu_and_mul forward stages)
+from . import fused  # noqa: F401  (rms_norm / residual_norm / rope_ / silu_and_mul / linear forward stages)
 from .attention import (flash_attn_varlen_func, paged_attention, paged_attention_qkv,
                         qkv_attention_supported)
 from .batch import Batch, WorkItem, build_batch, build_padded_batch
@@ -22,6 +23,8 @@ from .kv_cache import (allocate_kv_cache, dequantize, qkv_norm_rope_and_cache, q
                        quantize, reshape_and_cache_flash)
 from .kv_tier import (KVTierManager, SwappedKV, swap_in_blocks, swap_in_caches, swap_out_blocks,
                       swap_out_caches)
+from .mxfp4 import (MXFP4Weight, dequantize_mxfp4, pack_mxfp4_weight, quantize_mxfp4,
+                    quantize_mxfp4_weight)
 from .spec_decode import AcceptResult, accept, sample, softmax, verify
 
 __all__ = [
@@ -31,5 +34,6 @@ __all__ = [
     "verify", "KVTierManager", "SwappedKV", "swap_in_blocks", "swap_out_blocks",
     "allocate_block_major_kv", "copy_blocks", "migrate_out_of", "qkv_rope_and_cache",
     "qkv_norm_rope_and_cache",
-    "swap_out_caches", "swap_in_caches",
+    "swap_out_caches", "swap_in_caches", "MXFP4Weight", "quantize_mxfp4", "dequantize_mxfp4",
+    "pack_mxfp4_weight", "quantize_mxfp4_weight",
 ]

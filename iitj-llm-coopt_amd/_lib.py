@@ -89,6 +89,16 @@ SIGNATURES = {
     "coopt_sample_probs": (_i, [_i, _p, _i64, _i, _i, _f, _p, _sz, _p, _i64, _p]),
     "coopt_sample": (_i, [_i, _p, _i64, _i, _i, _f, _p, _p, _p, _p, _i64, _p, _sz, _p]),
     "coopt_sample64": (_i, [_i, _p, _i64, _i, _i, _f, _p, _p, _p, _p, _i64, _p, _sz, _p]),
+    "coopt_mxfp4_quantize": (_i, [_i, _p, _i64, _i, _p, _p, _p]),
+    "coopt_mxfp4_dequantize": (_i, [_p, _p, _i64, _i, _i, _p, _p]),
+    "coopt_mxfp4_packed_bytes": (_sz, [_i, _i]),
+    "coopt_mxfp4_pack_weight": (_i, [_p, _p, _i, _i, _p, _p]),
+    "coopt_mxfp4_linear_workspace": (_sz, [_i, _i, _i, _i, _i]),
+    "coopt_mxfp4_linear_split": (_i, [_i, _i, _i, _i, _p, _p]),
+    "coopt_mxfp4_linear": (_i, [_p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _sz, _p]),
+    "coopt_mxfp4_linear_partials": (_i, [_p, _i64, _p, _i, _i, _i, _i, _p, _sz, _p]),
+    "coopt_residual_norm": (_i, [_p, _p, _i, _i64, _p, _p, _p, _p, _i64, _p, _p, _i64, _i, _f, _f,
+                                 _f, _p]),
     "coopt_rms_norm": (_i, [_p, _p, _p, _p, _i64, _i, _f, _p]),
     "coopt_rope": (_i, [_p, _i64, _i64, _p, _i64, _i64, _p, _p, _p, _i64, _i, _i, _i, _i, _i, _p]),
     "coopt_silu_mul": (_i, [_p, _p, _i64, _i, _p]),

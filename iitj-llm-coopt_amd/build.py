@@ -19,7 +19,8 @@ LIB_NAME = "libcoopt_amd.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 
 SOURCES = ["abi.hip", "kv_cache.hip", "kv_blocks.hip", "accept.hip", "verify_attn.hip", "fused.hip",
-           "linear.hip", "spec_step.hip", "qk_norm.hip", "window_attn.hip"]
+           "linear.hip", "spec_step.hip", "qk_norm.hip", "window_attn.hip", "mxfp4.hip", "mxfp4_linear.hip",
+           "residual_norm.hip"]
 
 ARCH = "gfx950"
 # -packed-fp32-ops: keep hipcc from forming packed fp32 VALU ops (the pool's known hazard).

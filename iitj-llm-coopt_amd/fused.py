@@ -6,20 +6,31 @@ Counterparts of the vLLM ops the reference's forward calls (engine/model.py:234-
   silu_and_mul(gate_up, out=None)                      torch.ops._C.silu_and_mul
   linear(x, weight, out=None)                          F.linear projections (model.py:238-253)
   pack_linear_weight(weight)                           the weight in tile-packed form, for linear
+Beside them, for models that the reference does not run:
+  residual_norm(x, residual, weight, eps, ...)         norm, gate and scale of a block's output, residual
+                                                       sum and the next norm
+  linear(x, MXFP4Weight)                               a projection by a 4-bit weight (mxfp4)
 """
+import contextlib
 import ctypes
+import functools
+import threading
 
 import torch
 import torch.nn.functional as F
 
 from . import _lib
+from .mxfp4 import MXFP4Weight
 
-__all__ = ["rms_norm", "rope_", "silu_and_mul", "linear", "LinearPartials", "LINEAR_MAX_ROWS",
+__all__ = ["rms_norm", "residual_norm", "rope_", "silu_and_mul", "linear", "LinearPartials", "LINEAR_MAX_ROWS",
            "PackedWeight", "pack_linear_weight", "pack_gate_up_weight", "linear_silu",
            "row_major"]
 
 LINEAR_MAX_ROWS = 256
 _WS = _lib.WorkspaceCache()
+# held over the launches of a 4-bit product that takes its workspace from _WS: another thread's call on the
+# same stream would write its own between them
+_WS_LOCK = threading.Lock()
 
 
 def _bf16_rows(t, name):
@@ -82,6 +93,58 @@ def _rms_norm_partials(xp, weight, eps, residual, out):
         _lib.ptr(xp.buf), xp.ks, xp.rows_padded * xp.n, _lib.ptr(residual), _lib.ptr(weight),
         _lib.ptr(out), xp.rows, xp.n, float(eps), _lib.stream_handle(xp.device)),
         "coopt_rms_norm_partials")
+    return out
+
+
+def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_scale=1.0, residual_scale=1.0,
+                  residual_out=None, out=None):
+    """The step between two blocks of a model that norms its blocks' outputs:
+        b = x, or rms(x) * post_weight;  b *= gate;  r = residual_scale * residual + branch_scale * b
+        residual_out = r;  out = rms(r) * weight
+    with rms(v) = v * rsqrt(mean(v^2) + eps), computed in fp32: residual_out and out are rounded to bf16
+    once each, out from the unrounded r.  Without post_weight, gate and scales this is rms_norm with a
+    residual, which rounds r and the normed values on its way.
+
+    x [..., H] bf16 or the LinearPartials of the projection that made it (summed here), residual of its
+    shape; gate [H], or of x's shape (rows may be strided); H a multiple of 8 up to 16384.  residual_out: where r
+    goes, by default into `residual`.  Returns out (a new tensor by default)."""
+    part = x if isinstance(x, LinearPartials) else None
+    shape, H = tuple(x.shape), x.shape[-1]
+    index = residual.get_device()
+    same = [t for t in (None if part is not None else x, residual, weight, post_weight, gate, residual_out, out)
+            if t is not None]
+    if index < 0 or any(t.get_device() != index for t in same) or \
+            (part is not None and part.buf.get_device() != index):
+        _lib.require_one_device(*same, None if part is None else part.buf)
+    for name, t in (("x", None if part is not None else x), ("residual", residual), ("residual_out", residual_out),
+                    ("out", out)):
+        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous bf16 {shape}")
+    for name, t in (("weight", weight), ("post_weight", post_weight)):
+        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (H,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous bf16 [{H}]")
+    gate_stride = 0
+    if gate is not None:
+        if gate.dtype != torch.bfloat16 or tuple(gate.shape) not in ((H,), shape):
+            raise ValueError(f"gate must be bf16 [{H}] or {shape}")
+        if gate.dim() > 1:
+            gate = gate.reshape(-1, H)
+            if gate.stride(1) != 1 or gate.stride(0) < H or gate.stride(0) % 8:
+                gate = gate.contiguous()
+            gate_stride = gate.stride(0) if gate.shape[0] > 1 else 0
+        elif gate.stride(0) != 1:
+            gate = gate.contiguous()
+    if out is None:
+        out = torch.empty_like(residual)
+    if residual_out is None:
+        residual_out = residual
+    rows = residual.numel() // H if H else 0
+    _lib.check(_lib.call_on(
+        index, _lib.entry("coopt_residual_norm"), 0 if part is not None else x.data_ptr(),
+        0 if part is None else part.buf.data_ptr(), 0 if part is None else part.ks,
+        0 if part is None else part.rows_padded * part.n, residual.data_ptr(), residual_out.data_ptr(),
+        _lib.ptr(post_weight), _lib.ptr(gate), gate_stride, weight.data_ptr(), out.data_ptr(), rows, H, float(eps),
+        float(branch_scale), float(residual_scale), _lib.raw_stream(index)), "coopt_residual_norm")
     return out
 
 
@@ -155,7 +218,10 @@ class PackedWeight:
 
 
 def row_major(weight):
-    """The row-major [N, K] tensor of a weight (a PackedWeight's first copy, else itself)."""
+    """The row-major [N, K] tensor of a weight (a PackedWeight's first copy, the values of an MXFP4Weight,
+    else itself)."""
+    if isinstance(weight, MXFP4Weight):
+        return weight.dequantize()
     return weight.weight if isinstance(weight, PackedWeight) else weight
 
 
@@ -232,7 +298,13 @@ def linear(x, weight, out=None, defer_reduce=False):
     the tensor.
 
     `weight` may be a PackedWeight: the kernel path then streams its tile-packed copy
-    (coopt_linear_packed), torch's path its row-major one."""
+    (coopt_linear_packed), torch's path its row-major one.
+
+    `weight` may be an MXFP4Weight (K a multiple of 32, any N and row count): coopt_mxfp4_linear, with
+    bf16 rows or, where the weight says activations "mxfp4", rows quantised to 4 bits in the call.
+    defer_reduce returns LinearPartials where K is split."""
+    if isinstance(weight, MXFP4Weight):
+        return _linear_mxfp4(x, weight, out, defer_reduce)
     packed = weight.packed if isinstance(weight, PackedWeight) and not weight.gate_up else None
     if isinstance(weight, PackedWeight):
         weight = weight.weight
@@ -279,4 +351,63 @@ def linear(x, weight, out=None, defer_reduce=False):
             _lib.ptr(x2), x2.stride(0), _lib.ptr(packed), M, N, K, _lib.ptr(y2), y2.stride(0),
             _lib.ptr(ws), 0 if ws is None else ws.numel(), _lib.stream_handle(x.device)),
             "coopt_linear_packed")
+    return out
+
+
+@functools.lru_cache(maxsize=1024)   # pure functions of the sizes
+def _mxfp4_workspace(M, N, K, act4, partials):
+    return int(_lib.load().coopt_mxfp4_linear_workspace(M, N, K, act4, partials))
+
+
+@functools.lru_cache(maxsize=1024)
+def _mxfp4_split(M, N, K, act4):
+    ks, rp = ctypes.c_int(0), ctypes.c_int(0)
+    _lib.check(_lib.load().coopt_mxfp4_linear_split(M, N, K, act4, ctypes.byref(ks), ctypes.byref(rp)),
+               "coopt_mxfp4_linear_split")
+    return ks.value, rp.value
+
+
+def _linear_mxfp4(x, weight, out, defer_reduce):
+    """linear() with an MXFP4Weight."""
+    N, K = weight.shape
+    index = x.get_device()
+    if index < 0 or index != weight.packed.get_device() or (out is not None and out.get_device() != index):
+        _lib.require_one_device(x, weight.packed, out)
+    if x.dtype is not torch.bfloat16 or x.dim() == 0 or x.shape[-1] != K:
+        raise ValueError(f"x must be bf16 [..., {K}], got {x.dtype} {tuple(x.shape)}")
+    shape = (*x.shape[:-1], N)
+    if out is not None and (out.dtype is not torch.bfloat16 or tuple(out.shape) != shape or out.stride(-1) != 1):
+        raise ValueError(f"out must be bf16 {shape} with contiguous rows")
+    x2 = x.reshape(-1, K)
+    M = x2.shape[0]
+    if x2.stride(1) != 1 or x2.stride(0) % 8 or (M > 1 and x2.stride(0) < K) or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    act4 = 1 if weight.activations == "mxfp4" else 0
+    partials = False
+    if defer_reduce and out is None and N % 16 == 0 and M > 0:
+        ks, rows_padded = _mxfp4_split(M, N, K, act4)
+        partials = ks > 1
+    if not partials and out is None:
+        out = x.new_empty(shape)
+    need = _mxfp4_workspace(M, N, K, act4, 1 if partials else 0)
+    # a graph under capture gets a workspace of its own (from its memory pool), so that two graphs captured on
+    # one stream may replay at the same time
+    shared = need > 0 and not torch.cuda.is_current_stream_capturing()
+    ws = None if shared or not need else x.new_empty((need,), dtype=torch.uint8)
+    ldx = x2.stride(0) if M > 1 else max(K, x2.stride(0))
+    with _WS_LOCK if shared else contextlib.nullcontext():
+        if shared:
+            ws = _WS.get(need, x.device)
+        have, wsp = (0, 0) if ws is None else (ws.numel(), ws.data_ptr())
+        if partials:
+            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear_partials"), x2.data_ptr(), ldx,
+                              weight.packed.data_ptr(), M, N, K, act4, wsp, have, _lib.raw_stream(index))
+        else:
+            y2 = out.view(-1, N)
+            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear"), x2.data_ptr(), ldx, weight.packed.data_ptr(),
+                              M, N, K, act4, y2.data_ptr(), max(N, y2.stride(0)), wsp, have,
+                              _lib.raw_stream(index))
+    _lib.check(rc, "coopt_mxfp4_linear")
+    if partials:
+        return LinearPartials(ws, ks, M, rows_padded, N, torch.Size(shape), x.device)
     return out

@@ -1,0 +1,122 @@
+"""Microscaled 4-bit rows (the OCP format MXFP4) and weights, on gfx950 kernels.
+
+  quantize_mxfp4(x) / dequantize_mxfp4(codes, scales, dtype)   the codec, beside quantize / dequantize
+  pack_mxfp4_weight(codes, scales, activations)                a weight for fused.linear
+  quantize_mxfp4_weight(weight, activations)                   the same from a bf16 weight
+
+A row of K elements (K a multiple of 32) is K / 2 code bytes, the even element in the low half, and K / 32
+scale bytes.  A code is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; an element is code * 2^(s - 127) with its
+block's scale byte s, NaN where s is 255.  Quantisation takes s - 127 = floor(log2 amax) - 2 (at least
+-127) and the nearest code, ties to the even one, 6 for everything above; a block that is not finite gets 255.
+The reference has no such weights; its codes for swapped caches are kv_cache.quantize's.
+"""
+import torch
+
+from . import _lib
+
+__all__ = ["quantize_mxfp4", "dequantize_mxfp4", "MXFP4Weight", "pack_mxfp4_weight",
+           "quantize_mxfp4_weight"]
+
+BLOCK = 32
+
+
+def _aligned(t, nbytes):
+    """Contiguous, at an address that is a multiple of nbytes."""
+    t = t.contiguous()
+    return t if t.data_ptr() % nbytes == 0 else t.clone()
+
+
+def quantize_mxfp4(x: torch.Tensor):
+    """x [..., K] (bf16, fp16 or fp32) -> (codes uint8 [..., K / 2], scales uint8 [..., K / 32])."""
+    index = x.get_device()
+    if index < 0:
+        _lib.require_cuda(x)
+    if x.dim() == 0 or x.shape[-1] % BLOCK:
+        raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {tuple(x.shape)}")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
+    *lead, K = x.shape
+    xc = _aligned(x, 16)
+    codes = xc.new_empty((*lead, K // 2), dtype=torch.uint8)
+    scales = xc.new_empty((*lead, K // BLOCK), dtype=torch.uint8)
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_quantize"), _lib.dt_code(x.dtype), xc.data_ptr(),
+                            xc.numel() // K if K else 0, K, codes.data_ptr(), scales.data_ptr(),
+                            _lib.raw_stream(index)), "coopt_mxfp4_quantize")
+    return codes, scales
+
+
+def _check_rows(codes, scales):
+    """K of codes [..., K / 2] and scales [..., K / 32]."""
+    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise ValueError("codes and scales must be uint8")
+    if codes.dim() == 0 or codes.shape[-1] % (BLOCK // 2) or \
+            scales.shape != (*codes.shape[:-1], codes.shape[-1] // (BLOCK // 2)):
+        raise ValueError(f"codes [..., K / 2] and scales [..., K / {BLOCK}] disagree: {tuple(codes.shape)}, "
+                         f"{tuple(scales.shape)}")
+    return 2 * codes.shape[-1]
+
+
+def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16):
+    """The values [..., K] of 4-bit rows: exact in bf16 and fp32, rounded in fp16."""
+    index = codes.get_device()
+    if index < 0 or index != scales.get_device():
+        _lib.require_one_device(codes, scales)
+    K = _check_rows(codes, scales)
+    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
+    cc, sc = _aligned(codes, 4), scales.contiguous()
+    out = cc.new_empty((*codes.shape[:-1], K), dtype=dtype)
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_dequantize"), cc.data_ptr(), sc.data_ptr(),
+                            out.numel() // K if K else 0, K, _lib.dt_code(dtype), out.data_ptr(),
+                            _lib.raw_stream(index)), "coopt_mxfp4_dequantize")
+    return out
+
+
+class MXFP4Weight:
+    """A projection weight [N, K] in microscaled 4 bits: `codes` and `scales` as they were given, and
+    `packed`, the copy that fused.linear streams (coopt_mxfp4_pack_weight's layout).
+
+    activations "bf16": products with the rows as they are.  "mxfp4": rows are quantised to 4 bits in the call and
+    both operands go to the scaled matrix instructions (4 bits by 4 bits)."""
+
+    def __init__(self, codes, scales, packed, activations="bf16"):
+        self.codes, self.scales, self.packed, self.activations = codes, scales, packed, activations
+        self.shape = torch.Size((codes.shape[0], 2 * codes.shape[1]))
+
+    @property
+    def dtype(self):
+        return torch.bfloat16   # of the values it stands for
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def dequantize(self, dtype=torch.bfloat16):
+        """The values [N, K], row-major."""
+        return dequantize_mxfp4(self.codes, self.scales, dtype)
+
+
+def pack_mxfp4_weight(codes, scales, activations="bf16"):
+    """MXFP4Weight of codes [N, K / 2] and scales [N, K / 32] on the GPU: one launch at model load."""
+    if activations not in ("bf16", "mxfp4"):
+        raise ValueError(f"activations must be 'bf16' or 'mxfp4', got {activations!r}")
+    index = codes.get_device()
+    if index < 0 or index != scales.get_device():
+        _lib.require_one_device(codes, scales)
+    if codes.dim() != 2:
+        raise ValueError(f"codes must be [N, K / 2], got {tuple(codes.shape)}")
+    K = _check_rows(codes, scales)
+    N = codes.shape[0]
+    cc, sc = _aligned(codes, 16), scales.contiguous()
+    nbytes = int(_lib.entry("coopt_mxfp4_packed_bytes")(N, K))
+    packed = cc.new_empty(nbytes)
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_pack_weight"), cc.data_ptr(), sc.data_ptr(), N, K,
+                            packed.data_ptr(), _lib.raw_stream(index)), "coopt_mxfp4_pack_weight")
+    return MXFP4Weight(cc, sc, packed, activations)
+
+
+def quantize_mxfp4_weight(weight, activations="bf16"):
+    """MXFP4Weight of a weight [N, K] on the GPU, quantised by quantize_mxfp4."""
+    if weight.dim() != 2:
+        raise ValueError(f"weight must be [N, K], got {tuple(weight.shape)}")
+    return pack_mxfp4_weight(*quantize_mxfp4(weight), activations=activations)

@@ -524,6 +524,57 @@ int coopt_rms_norm_partials(const float* part, int ks, int64_t slice_stride, voi
                             coopt_stream_t stream);
 
 /*
+ * The norm behind a block, its gate and scale, the residual sum and the next block's norm, for models that
+ * norm their blocks' outputs too (the reference's forward has none).  With h the block's output,
+ *   b = h, or h * rsqrt(mean(h^2) + eps) * post_weight;  b *= gate;
+ *   r = residual_scale * residual + branch_scale * b;    out = r * rsqrt(mean(r^2) + eps) * weight
+ * in fp32; residual_out = bf16(r) (it may be `residual` itself), out is rounded once, from the unrounded r.
+ *   h: x [rows, hidden] bf16, or (x null) part: the fp32 split-K partials of the projection that made it, as
+ *      coopt_rms_norm_partials takes them (rounded to bf16 when summed).  post_weight, gate: bf16 or null.
+ *      gate_stride 0: one gate [hidden] for all rows, else row r's gate is gate + r * gate_stride.
+ *   hidden a multiple of 8, at most 16384; every row 16-byte aligned.
+ */
+int coopt_residual_norm(const void* x, const float* part, int ks, int64_t slice_stride, const void* residual,
+                        void* residual_out, const void* post_weight, const void* gate, int64_t gate_stride,
+                        const void* weight, void* out, int64_t rows, int hidden, float eps, float branch_scale,
+                        float residual_scale, coopt_stream_t stream);
+
+/*
+ * Microscaled 4-bit rows (the OCP format MXFP4), beside the caches' codec: per 32 elements along K a scale
+ * byte s, per element a code of sign and {0, 0.5, 1, 1.5, 2, 3, 4, 6}; the value is code * 2^(s - 127), NaN where
+ * s = 255.  codes [rows, K / 2], the even element in the low half of its byte; scales [rows, K / 32].
+ *   coopt_mxfp4_quantize: x [rows, K] contiguous (BF16 / F16 / F32).  With a the largest magnitude of a
+ *     block, s = max(floor(log2 a) + 125, 0) and a code is the nearest to x / 2^(s - 127), ties to the even
+ *     code, 6 for all above; a block that is not finite has s = 255 and codes 0.
+ *   coopt_mxfp4_dequantize: out [rows, K] (BF16 and F32 exact, F16 rounded).
+ * K a multiple of 32; x and out 16-byte, codes 4-byte aligned.
+ */
+int coopt_mxfp4_quantize(int in_dtype, const void* x, int64_t rows, int K, void* codes, void* scales,
+                         coopt_stream_t stream);
+int coopt_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, int K, int out_dtype, void* out,
+                           coopt_stream_t stream);
+/*
+ * Projections by a microscaled 4-bit weight: y [M, N] = x [M, K] w [N, K]^T, bf16 in and out, fp32 sums.
+ *   coopt_mxfp4_pack_weight: codes [N, K / 2] and scales [N, K / 32] into out (coopt_mxfp4_packed_bytes(N, K)
+ *     bytes) in the order the kernels load them; once a model load.  codes and out 16-byte aligned.
+ *   coopt_mxfp4_linear: act4 = 0: x as it is (every weight is a bf16 number, products are those of bf16);
+ *     act4 = 1: x is quantised first, as coopt_mxfp4_quantize does, and the 4-bit operands are multiplied.
+ *     K a multiple of 32, N any, M up to 2^19; x rows 16-byte aligned (ldx a multiple of 8).
+ *     workspace: coopt_mxfp4_linear_workspace(M, N, K, act4, 0) bytes (0: none), 16-byte aligned.
+ *   coopt_mxfp4_linear_split / _partials: as coopt_linear_split / coopt_linear_partials: ks fp32 slices
+ *     [rows_padded, N] at the workspace's start, whose sum in order is the output before its rounding.  N a
+ *     multiple of 16; coopt_mxfp4_linear_workspace(M, N, K, act4, 1) bytes.
+ */
+size_t coopt_mxfp4_packed_bytes(int N, int K);
+int coopt_mxfp4_pack_weight(const void* codes, const void* scales, int N, int K, void* out, coopt_stream_t stream);
+size_t coopt_mxfp4_linear_workspace(int M, int N, int K, int act4, int partials);
+int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, int* rows_padded);
+int coopt_mxfp4_linear(const void* x, int64_t ldx, const void* w_packed, int M, int N, int K, int act4, void* y,
+                       int64_t ldy, void* workspace, size_t workspace_bytes, coopt_stream_t stream);
+int coopt_mxfp4_linear_partials(const void* x, int64_t ldx, const void* w_packed, int M, int N, int K, int act4,
+                                void* workspace, size_t workspace_bytes, coopt_stream_t stream);
+
+/*
  * Paged addressing of a batch of row runs on the device -- BlockManager.slot_mapping
  * (engine/block_manager.py:216-220: slot = table[p / bs] * bs + p % bs) and the positions and
  * seq_lens of build_batch (engine/batch.py:23-55), for the padded verify layout

@@ -1,0 +1,279 @@
+"""GPU: microscaled 4-bit rows and products with 4-bit weights, against the definition in 64 bits.
+
+Codes, scales and dequantised values are compared bit for bit.  Products are compared twice: on small
+integers, whose sums any order of fp32 additions gives exactly, so that the bf16 output is the exact sum rounded
+once; and on values of all sizes, within half a bf16 step (2^-8) and the fp32 sums' bound.  That bound: a
+sum of K products is a chain of at most K / 32 + 32 additions of partial sums, each of at most 32 (bf16) or
+128 (4-bit) products formed by one instruction, so it is off by at most (K / 32 + 32 + 128) * 2^-23 * sum |x w|.
+"""
+import numpy as np
+import pytest
+import torch
+
+import iitj_llm_coopt_amd as M
+from iitj_llm_coopt_amd import fused
+
+pytestmark = pytest.mark.gpu
+
+GRID = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+
+
+def reference_quantize(x):
+    """(codes [..., K] as 0..15, scale bytes [..., K / 32]) of a float64 array, element by element."""
+    y = x.reshape(*x.shape[:-1], -1, 32)
+    amax = np.abs(y).max(-1)
+    finite = np.isfinite(amax)
+    e = np.full(amax.shape, -127)
+    pos = finite & (amax > 0)
+    e[pos] = np.maximum(np.frexp(amax[pos])[1] - 1 - 2, -127)
+    with np.errstate(invalid="ignore", over="ignore"):
+        q = np.abs(y) * np.exp2(-e.astype(np.float64))[..., None]
+    # the nearest of the grid; between two, the even code
+    code = np.zeros(y.shape, np.int64)
+    for c in range(1, 8):
+        mid = (GRID[c - 1] + GRID[c]) / 2
+        code += (q > mid) | ((q == mid) & (c % 2 == 0))
+    code |= np.signbit(y).astype(np.int64) << 3
+    code[~finite] = 0
+    s = np.where(finite, e + 127, 255)
+    return code.reshape(x.shape), s
+
+
+def reference_values(code, s):
+    v = GRID[code & 7] * np.where(code & 8, -1.0, 1.0)
+    v = v.reshape(*s.shape, 32) * np.where(s == 255, np.nan, np.exp2(s.astype(np.float64) - 127))[..., None]
+    return v.reshape(code.shape)
+
+
+def unpack(codes):
+    c = codes.cpu().numpy().astype(np.int64)
+    return np.stack([c & 15, c >> 4], -1).reshape(*c.shape[:-1], -1)
+
+
+def pack(code):
+    return torch.from_numpy((code[..., 0::2] | (code[..., 1::2] << 4)).astype(np.uint8))
+
+
+def quantizer_input(shape, dtype, seed):
+    """Values over the whole range of the type, ties and borders among them, blocks of zeros, of one value."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal(shape)
+    y = x.reshape(-1, 32)
+    top = 13 if dtype == torch.float16 else 100
+    y *= np.exp2(rng.integers(-top, top, (len(y), 1)))
+    k = np.arange(len(y))
+    ties = np.array([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5, 6, 7, -0.25, -2.5, -5, 0.5, 4, 3, 0])
+    y[k % 4 == 1] = np.tile(ties, 2) * np.exp2(rng.integers(-8, 9, (np.sum(k % 4 == 1), 1)))
+    y[k % 16 == 2] = 0
+    y[k % 16 == 6, 1:] *= 1e-6
+    return torch.from_numpy(x).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("shape", [(1, 32), (3, 64), (7, 5, 96), (129, 4096), (1000, 1504)])
+def test_quantize_is_the_definition(dev, shape, dtype):
+    x = quantizer_input(shape, dtype, len(shape) + shape[-1])
+    codes, scales = M.quantize_mxfp4(x.to(dev))
+    code, s = reference_quantize(x.double().numpy())
+    assert np.array_equal(scales.cpu().numpy(), s)
+    assert np.array_equal(unpack(codes), code)
+    for out in (torch.bfloat16, torch.float32, torch.float16):
+        got = M.dequantize_mxfp4(codes, scales, out)
+        want = torch.from_numpy(reference_values(code, s)).to(out)
+        assert got.dtype == out and torch.equal(got.cpu(), want)
+
+
+def test_quantize_extremes(dev):
+    """Blocks of subnormals, of the largest values, and blocks that are not finite."""
+    rows = []
+    for v in (2.0 ** -126, 2.0 ** -127, 2.0 ** -133, 3.0 * 2.0 ** -128, 2.0 ** -124, 1.5 * 2.0 ** 127, 2.0 ** 127):
+        r = np.linspace(-1, 1, 32) * v
+        rows.append(r)
+    x = torch.tensor(np.stack(rows)).to(torch.bfloat16)
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        r = torch.ones(32, dtype=torch.bfloat16)
+        r[17] = bad
+        x = torch.cat([x, r[None]])
+    for dtype in (torch.bfloat16, torch.float32):
+        xt = x.to(dtype)
+        codes, scales = M.quantize_mxfp4(xt.to(dev))
+        code, s = reference_quantize(xt.double().numpy())
+        assert np.array_equal(scales.cpu().numpy(), s) and np.array_equal(unpack(codes), code)
+        got = M.dequantize_mxfp4(codes, scales).double().cpu().numpy()
+        want = reference_values(code, s)
+        assert np.array_equal(got, want, equal_nan=True)
+        assert np.isnan(got[-3:]).all() and np.isfinite(got[:-3]).all()
+
+
+def test_every_byte_pair_dequantizes(dev):
+    """All 256 scales by all 16 codes."""
+    code = np.tile(np.arange(16), (256, 2))
+    s = np.arange(256)[:, None]
+    got = M.dequantize_mxfp4(pack(code).to(dev), torch.from_numpy(s.astype(np.uint8)).to(dev), torch.float32)
+    with np.errstate(over="ignore"):
+        want = reference_values(code, s).astype(np.float32)   # 6 * 2^127 and 4 * 2^127 are past fp32
+    assert np.array_equal(got.cpu().numpy(), want, equal_nan=True)
+
+
+def test_codec_views_and_empty(dev):
+    x = quantizer_input((64, 256), torch.bfloat16, 3).to(dev)
+    base = M.quantize_mxfp4(x)
+    flat = torch.empty(64 * 256 + 1, dtype=torch.bfloat16, device=dev)
+    flat[1:] = x.flatten()
+    for view in (flat[1:].view(64, 256), x.t().contiguous().t(), torch.cat([x, x], 1)[:, :256]):
+        assert all(torch.equal(a, b) for a, b in zip(M.quantize_mxfp4(view), base))
+    for shape in ((0, 32), (4, 0)):
+        c, s = M.quantize_mxfp4(torch.empty(shape, dtype=torch.bfloat16, device=dev))
+        assert M.dequantize_mxfp4(c, s).shape == shape
+
+
+# ---- products ----------------------------------------------------------------------------------
+
+def make_weight(dev, N, K, seed, activations="bf16", integers=False):
+    """(MXFP4Weight, float64 values [N, K])."""
+    rng = np.random.default_rng(seed)
+    code = rng.integers(0, 16, (N, K))
+    s = np.full((N, K // 32), 128) if integers else rng.integers(118, 126, (N, K // 32))
+    w = M.pack_mxfp4_weight(pack(code).to(dev), torch.from_numpy(s.astype(np.uint8)).to(dev), activations)
+    return w, reference_values(code, s)
+
+
+def half_up_to_even(v):
+    return torch.from_numpy(v).to(torch.bfloat16)
+
+
+def quantized(x):
+    return reference_values(*reference_quantize(x))
+
+
+# row counts around the row tiles, widths with and without a whole tile, lengths with and without a whole step
+# of 128 and a whole quad of 512
+SHAPES = [(1, 16, 32), (1, 4096, 4096), (2, 17, 64), (5, 100, 96), (15, 33, 160), (16, 64, 128), (17, 64, 512),
+          (31, 130, 544), (32, 2048, 2048), (33, 48, 640), (48, 1000, 1024), (63, 16, 4096), (64, 257, 480),
+          (65, 512, 992), (80, 272, 2048), (96, 1023, 256), (127, 64, 1536), (128, 4096, 1024), (129, 640, 1024), (160, 6144, 512),
+          (200, 96, 14336), (256, 1000, 736), (300, 4096, 4096), (513, 514, 1056), (1000, 2048, 512)]
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_products_of_integers_are_exact(dev, shape, activations):
+    """|x| <= 6 in steps a 4-bit code has, weights up to 12: sums below 2^24, exact in fp32 in any order."""
+    m, N, K = shape
+    w, vals = make_weight(dev, N, K, m + N + K, activations, integers=True)
+    rng = np.random.default_rng(K)
+    x = rng.choice([-6, -4, -3, -2, -1, 0, 1, 2, 3, 4, 6], (m, K)).astype(np.float64)
+    x[:, ::32] = 6   # every block's scale is 1
+    assert K * 6 * 12 < 2 ** 24
+    want = half_up_to_even(x @ vals.T)
+    xt = torch.from_numpy(x).to(dev, torch.bfloat16)
+    got = fused.linear(xt, w)
+    assert got.shape == (m, N) and torch.equal(got.cpu(), want)
+    part = fused.linear(xt, w, defer_reduce=True)
+    if isinstance(part, fused.LinearPartials):
+        part = part.reduce()
+    assert torch.equal(part.cpu(), want)
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("shape", [(1, 4096, 4096), (7, 300, 1504), (32, 2048, 2048), (77, 1024, 14336),
+                                   (160, 4096, 1024), (333, 512, 2080)])
+def test_products_of_values(dev, shape, activations):
+    m, N, K = shape
+    w, vals = make_weight(dev, N, K, 3 * m + N, activations)
+    g = torch.Generator().manual_seed(K)
+    xt = (torch.randn(m, K, generator=g) * torch.exp2(torch.randint(-3, 4, (1, K), generator=g).float()))
+    xt = xt.to(torch.bfloat16)
+    x = xt.double().numpy()
+    if activations == "mxfp4":
+        x = quantized(x)
+    ref, mag = x @ vals.T, np.abs(x) @ np.abs(vals).T
+    tol = 2.0 ** -8 * np.abs(ref) + (K / 32 + 160) * 2.0 ** -23 * (1 + 2.0 ** -8) * mag
+    got = fused.linear(xt.to(dev), w).double().cpu().numpy()
+    assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_strides_and_outputs(dev, activations):
+    """Rows of a wider matrix, rows that start off a 16-byte border, three dimensions, given outputs; what
+    lies around a given output's rows stays."""
+    w, _ = make_weight(dev, 130, 160, 5, activations)
+    x = torch.randn(6, 160, device=dev).to(torch.bfloat16)
+    base = fused.linear(x, w)
+    wide = torch.randn(6, 400, device=dev).to(torch.bfloat16)
+    for off in (0, 8, 3, 40):
+        wide[:, off:off + 160] = x
+        assert torch.equal(fused.linear(wide[:, off:off + 160], w), base)
+    assert torch.equal(fused.linear(x.view(2, 3, 160), w), base.view(2, 3, 130))
+    assert torch.equal(fused.linear(x[0], w), base[0])
+    assert fused.linear(x[:0], w).shape == (0, 130)
+    for width, off in ((200, 8), (201, 5), (130, 0), (132, 1)):
+        room = torch.full((8, width), 7.0, dtype=torch.bfloat16, device=dev)
+        out = room[1:7, off:off + 130]
+        assert fused.linear(x, w, out=out) is out and torch.equal(out, base)
+        room[1:7, off:off + 130] = 7.0
+        assert (room == 7.0).all()
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_values_that_are_not_finite(dev, activations):
+    """A row with an infinity or NaN leaves the other rows as they are; a weight block of scale 255 makes its
+    row's outputs NaN and no other's."""
+    N, K = 48, 288
+    w, vals = make_weight(dev, N, K, 8, activations)
+    x = torch.randn(20, K, device=dev).to(torch.bfloat16)
+    base = fused.linear(x, w)
+    y = x.clone()
+    y[3, 100], y[7, K - 1] = float("nan"), float("inf")
+    got = fused.linear(y, w)
+    keep = [i for i in range(20) if i not in (3, 7)]
+    assert torch.equal(got[keep], base[keep]) and got[3].isnan().all() and not got[7].isfinite().any()
+    s = w.scales.clone()
+    s[5, 2] = 255
+    bad = fused.linear(x, M.pack_mxfp4_weight(w.codes, s, activations))
+    assert bad[:, 5].isnan().all()
+    others = [i for i in range(N) if i != 5]
+    assert torch.equal(bad[:, others], base[:, others])
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_streams_graphs_and_repeats(dev, activations):
+    """The same bits each time: on another stream, and from two graphs captured on one stream and replayed in
+    turns with eager work between."""
+    shapes = [(9, 2048, 4096), (160, 1024, 4096)]
+    ws = [make_weight(dev, N, K, i, activations)[0] for i, (_, N, K) in enumerate(shapes)]
+    xs = [torch.randn(m, K, device=dev).to(torch.bfloat16) for m, _, K in shapes]
+    want = [fused.linear(x, w) for x, w in zip(xs, ws)]
+    side = torch.cuda.Stream(device=dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        again = [fused.linear(x, w) for x, w in zip(xs, ws)]
+    torch.cuda.current_stream(dev).wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    graphs = []
+    for x, w in zip(xs, ws):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = fused.linear(x, w)
+        graphs.append((g, out))
+    for i in range(4):
+        for (g, out), x, w in zip(graphs, xs, ws):
+            x.copy_(torch.randn_like(x))
+            out.zero_()
+            g.replay()
+        for (_, out), x, w in zip(graphs, xs, ws):
+            assert torch.equal(out, fused.linear(x, w)), i
+
+
+def test_weight_helpers(dev):
+    w0 = (0.02 * torch.randn(96, 256, device=dev)).to(torch.bfloat16)
+    w = M.quantize_mxfp4_weight(w0, "mxfp4")
+    code, s = reference_quantize(w0.double().cpu().numpy())
+    assert torch.equal(w.dequantize().cpu().double(), torch.from_numpy(reference_values(code, s)))
+    assert torch.equal(fused.row_major(w), w.dequantize()) and w.shape == (96, 256)
+    # the values of a quantised weight quantise to themselves
+    again = M.quantize_mxfp4_weight(w.dequantize())
+    assert torch.equal(again.dequantize(), w.dequantize())
+    # gate_up: silu_and_mul of the projection
+    gu = M.quantize_mxfp4_weight(torch.randn(128, 256, device=dev).to(torch.bfloat16))
+    x = torch.randn(9, 256, device=dev).to(torch.bfloat16)
+    assert torch.equal(fused.linear_silu(x, gu), fused.silu_and_mul(fused.linear(x, gu)))
