@@ -17,16 +17,15 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const void* __
   if (i >= eighths) return;   // whole groups of four lanes: a block has four eighths
   uint32_t code, s;
   if constexpr (DT == COOPT_DT_BF16) {
-    const uint4 v = reinterpret_cast<const uint4*>(x)[i];
+    const mxfp4::u32x4_t v = reinterpret_cast<const mxfp4::u32x4_t*>(x)[i];
     s = mxfp4::scale_byte(group_max_u32<4>(mxfp4::amax_bits(v)));
     code = mxfp4::codes_of(v, s);
   } else {
     float f[8];
     if constexpr (DT == COOPT_DT_F16) {
-      const uint4 v = reinterpret_cast<const uint4*>(x)[i];
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      const mxfp4::u32x4_t v = reinterpret_cast<const mxfp4::u32x4_t*>(x)[i];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = f16_to_f32(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
+      for (int e = 0; e < 8; ++e) f[e] = f16_to_f32(static_cast<uint16_t>(v[e / 2] >> (16 * (e & 1))));
     } else {
       const float4 a = reinterpret_cast<const float4*>(x)[2 * i], b = reinterpret_cast<const float4*>(x)[2 * i + 1];
       f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w;
@@ -53,14 +52,13 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const uint32
   const int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (i >= eighths) return;
   const uint32_t s = scales[i >> 2];
-  const uint4 b = mxfp4::bf16_of(codes[i], mxfp4::scale_operand(s));
+  const mxfp4::u32x4_t b = mxfp4::bf16_of(codes[i], mxfp4::scale_operand(s));
   if constexpr (DT == COOPT_DT_BF16) {
-    reinterpret_cast<uint4*>(out)[i] = b;
+    reinterpret_cast<mxfp4::u32x4_t*>(out)[i] = b;
   } else {
-    const uint32_t w[4] = {b.x, b.y, b.z, b.w};
     float f[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f[e] = bf16_to_f32(static_cast<uint16_t>(w[e / 2] >> (16 * (e & 1))));
+    for (int e = 0; e < 8; ++e) f[e] = bf16_to_f32(static_cast<uint16_t>(b[e / 2] >> (16 * (e & 1))));
     if constexpr (DT == COOPT_DT_F32) {
       reinterpret_cast<float4*>(out)[2 * i] = make_float4(f[0], f[1], f[2], f[3]);
       reinterpret_cast<float4*>(out)[2 * i + 1] = make_float4(f[4], f[5], f[6], f[7]);
@@ -79,14 +77,14 @@ __global__ __launch_bounds__(kThreads) void mxfp4_dequantize_kernel(const uint32
 // u % 4 = 0 the dword of four scales.
 __global__ __launch_bounds__(kThreads) void mxfp4_pack_kernel(const uint8_t* __restrict__ codes,
                                                               const uint8_t* __restrict__ scales, int N, int K,
-                                                              int ksteps, int kquads, int64_t chunks,
+                                                              int kquads, int64_t chunks,
                                                               uint4* __restrict__ tiles, uint32_t* __restrict__ packed_scales) {
   const int64_t o = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
   if (o >= chunks) return;
   const int l = static_cast<int>(o & 63);
-  const int64_t tu = o >> 6, t = tu / ksteps;
-  const int u = static_cast<int>(tu - t * ksteps);
-  const int64_t row = 16 * t + (l & 15);
+  const int64_t tu = o >> 6, t = tu / (4 * kquads);
+  const int u = static_cast<int>(tu - t * 4 * kquads);
+  const int64_t row = mxfp4::weight_row(t, l & 15);
   const int block = 4 * u + (l >> 4), blocks = K / mxfp4::kBlock;
   uint4 c = make_uint4(0, 0, 0, 0);
   if (row < N && block < blocks)
@@ -159,7 +157,7 @@ extern "C" int coopt_mxfp4_dequantize(const void* codes, const void* scales, int
 
 extern "C" size_t coopt_mxfp4_packed_bytes(int N, int K) {
   if (N <= 0 || K <= 0 || K % mxfp4::kBlock) return 0;
-  return static_cast<size_t>(mxfp4::packed_bytes(N, K));
+  return static_cast<size_t>(mxfp4::packed_bytes(mxfp4::weight_tiles(N), K));
 }
 
 extern "C" int coopt_mxfp4_pack_weight(const void* codes, const void* scales, int N, int K, void* out,
@@ -169,12 +167,12 @@ extern "C" int coopt_mxfp4_pack_weight(const void* codes, const void* scales, in
   if (N == 0 || K == 0) return COOPT_OK;
   COOPT_REQUIRE(codes && scales && out, "null pointer");
   COOPT_REQUIRE(coopt::aligned16(codes) && coopt::aligned16(out), "codes and out must be 16-byte aligned");
-  const int64_t chunks = mxfp4::tile_bytes(N, K) / 16;
+  const int64_t chunks = mxfp4::tile_bytes(mxfp4::weight_tiles(N), K) / 16;
   COOPT_REQUIRE(blocks_fit(chunks), "weight too large");
   hipLaunchKernelGGL(mxfp4_pack_kernel, grid_for(chunks), dim3(kThreads), 0, reinterpret_cast<hipStream_t>(stream),
                      static_cast<const uint8_t*>(codes), static_cast<const uint8_t*>(scales), N, K,
-                     static_cast<int>(mxfp4::steps(K)), static_cast<int>(mxfp4::quads(K)), chunks,
+                     static_cast<int>(mxfp4::quads(K)), chunks,
                      static_cast<uint4*>(out),
-                     reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + mxfp4::tile_bytes(N, K)));
+                     reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(out) + mxfp4::tile_bytes(mxfp4::weight_tiles(N), K)));
   return coopt::check_launch("coopt_mxfp4_pack_weight");
 }

@@ -17,7 +17,9 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 
+using mxfp4::kQuad;
 using mxfp4::kStep;
+using mxfp4::u32x4_t;
 using mxfp4::kTile;
 
 struct Args {
@@ -28,7 +30,7 @@ struct Args {
   const uint8_t* w;            // packed weight and its scales
   const uint32_t* ws;
   int M, N, K;
-  int ksteps, kquads;
+  int kquads;                  // K in quads of 512 elements
   int slice_quads;             // K quads (512 elements) of a K slice
   uint16_t* y;                 // part == nullptr: the outputs
   int64_t ldy;
@@ -37,17 +39,23 @@ struct Args {
   int pitch;
 };
 
-__device__ __forceinline__ f32x4_t mfma_bf16(const uint4& a, const uint4& b, f32x4_t c) {
+__device__ __forceinline__ f32x4_t mfma_bf16(const u32x4_t& a, const u32x4_t& b, f32x4_t c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
                                                  c, 0, 0, 0);
 }
 
 template <int J>
-__device__ __forceinline__ f32x4_t mfma_fp4(const uint4& a, uint32_t sa, const uint4& b, uint32_t sb, f32x4_t c) {
+__device__ __forceinline__ f32x4_t mfma_fp4(const u32x4_t& a, uint32_t sa, const u32x4_t& b, uint32_t sb, f32x4_t c) {
   const i32x8_t av = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
   const i32x8_t bv = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, J, static_cast<int>(sa), J,
                                                           static_cast<int>(sb));
+}
+
+// Two fp32 -> packed bf16, round to nearest even (v_cvt_pk_bf16_f32).
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+  typedef float f32x2_t __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), mxfp4::bf16x2_t));
 }
 
 template <int J>
@@ -55,28 +63,60 @@ __device__ __forceinline__ float step_scale(uint32_t quad) {
   return mxfp4::scale_operand((quad >> (8 * J)) & 255u);
 }
 
-__device__ __forceinline__ uint32_t dword(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
-
-// Four consecutive outputs n .. n + 3 of row m.
-__device__ __forceinline__ void store4(const Args& a, int m, int n, f32x4_t v) {
+// C consecutive outputs n .. of row m (C = 4 or 8: a lane's of one weight tile, or of a pair).
+template <int C>
+__device__ __forceinline__ void store(const Args& a, int m, int n, const float (&v)[C]) {
   if (m >= a.M || n >= a.N) return;
   if (a.part) {
-    float* p = a.part + blockIdx.y * a.part_slice + static_cast<int64_t>(m) * a.pitch + n;
-    *reinterpret_cast<f32x4_t*>(p) = v;   // pitch is a multiple of 16
+    float* p = a.part + blockIdx.y * a.part_slice + static_cast<int64_t>(m) * a.pitch + n;   // pitch: whole tiles
+#pragma unroll
+    for (int i = 0; i < C; i += 4) *reinterpret_cast<f32x4_t*>(p + i) = f32x4_t{v[i], v[i + 1], v[i + 2], v[i + 3]};
     return;
   }
   uint16_t* o = a.y + static_cast<int64_t>(m) * a.ldy + n;
-  const uint32_t lo = f32_to_bf16(v[0]) | (static_cast<uint32_t>(f32_to_bf16(v[1])) << 16);
-  const uint32_t hi = f32_to_bf16(v[2]) | (static_cast<uint32_t>(f32_to_bf16(v[3])) << 16);
-  if (n + 3 < a.N && (reinterpret_cast<uintptr_t>(o) & 7) == 0) {
-    *reinterpret_cast<uint2*>(o) = make_uint2(lo, hi);
-  } else {
-    const uint16_t e[4] = {static_cast<uint16_t>(lo), static_cast<uint16_t>(lo >> 16), static_cast<uint16_t>(hi),
-                           static_cast<uint16_t>(hi >> 16)};
+  uint32_t w[C / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) o[i] = e[i];
+  for (int i = 0; i < C / 2; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  if (n + C <= a.N && (reinterpret_cast<uintptr_t>(o) & (2 * C - 1)) == 0) {
+    if constexpr (C == 8) *reinterpret_cast<u32x4_t*>(o) = u32x4_t{w[0], w[1], w[2], w[3]};
+    else *reinterpret_cast<uint2*>(o) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (n + i < a.N) o[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
   }
+}
+
+// The outputs of a wave's tiles (column tiles from t0 on, rows from m on), lane (g, l16).
+template <int NT>
+__device__ __forceinline__ void store_row(const Args& a, int m, int t0, int g, const f32x4_t (&acc)[NT]) {
+#pragma unroll
+  for (int nt = 0; nt < NT; nt += 2) {
+    if constexpr (NT % 2 == 0) {
+      const f32x4_t lo = acc[nt], hi = acc[nt + 1];
+      const float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      store<8>(a, m, static_cast<int>(mxfp4::weight_row(t0 + nt, 4 * g)), v);
+    } else {
+      const float v[4] = {acc[0][0], acc[0][1], acc[0][2], acc[0][3]};
+      store<4>(a, m, static_cast<int>(mxfp4::weight_row(t0, 4 * g)), v);
+    }
+  }
+}
+
+// Block `id` of a grid of mblocks x nblocks.  Consecutive ids go to the eight XCDs in turn, each with an L2 of its
+// own: an XCD gets a run of blocks that lie next to one another, eight blocks of rows by as many of columns
+// as it has, so that they share rows and weights there.
+__device__ __forceinline__ void block_of(int id, int mblocks, int nblocks, int& mb, int& nb) {
+  const int total = mblocks * nblocks;
+  const int per = total / 8, extra = total % 8;
+  const int xcd = id % 8, at = id / 8;
+  const int t = xcd * per + (xcd < extra ? xcd : extra) + at;
+  constexpr int kRun = 8;
+  const int band = t / (kRun * nblocks);
+  const int rows = mblocks - band * kRun < kRun ? mblocks - band * kRun : kRun;
+  const int in = t - band * kRun * nblocks;
+  mb = band * kRun + in % rows;
+  nb = in / rows;
 }
 
 // Few rows: every wave of a block has the same NT column tiles and its own K quads, reads X where it lies
@@ -86,8 +126,8 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
   __shared__ f32x4_t red[KW][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int l16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * (NT * 16), m0 = blockIdx.z * (MT * 16);
-  const int ntiles = (a.N + 15) / 16, mtiles = (a.M + 15) / 16;
+  const int t0 = blockIdx.x * NT, m0 = blockIdx.z * (MT * 16);
+  const int ntiles = (a.N + 31) / 32 * 2, mtiles = (a.M + 15) / 16;
   const int qbeg = blockIdx.y * a.slice_quads;
   const int qend = qbeg + a.slice_quads < a.kquads ? qbeg + a.slice_quads : a.kquads;
 
@@ -95,9 +135,9 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
   const uint32_t* wsc[NT];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    int t = n0 / 16 + nt;
+    int t = t0 + nt;
     t = t < ntiles ? t : ntiles - 1;   // tiles past the weight: computed, not stored
-    wt[nt] = a.w + static_cast<int64_t>(t) * a.ksteps * kTile + lane * 16;
+    wt[nt] = a.w + static_cast<int64_t>(t) * a.kquads * (4 * kTile) + lane * 16;
     wsc[nt] = a.ws + static_cast<int64_t>(t) * a.kquads * 64 + lane;
   }
   const uint16_t* xr[MT];
@@ -108,7 +148,7 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
     if constexpr (A4) {
       int t = m0 / 16 + mt;
       t = t < mtiles ? t : mtiles - 1;
-      xt[mt] = a.xt + static_cast<int64_t>(t) * a.ksteps * kTile + lane * 16;
+      xt[mt] = a.xt + static_cast<int64_t>(t) * a.kquads * (4 * kTile) + lane * 16;
       xsc[mt] = a.xs + static_cast<int64_t>(t) * a.kquads * 64 + lane;
     } else {
       int m = m0 + mt * 16 + l16;
@@ -123,9 +163,8 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
     for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
   for (int q = qbeg + wave; q < qend; q += KW) {
-    uint4 w[4][NT];
+    u32x4_t w[4][NT];
     uint32_t sw[NT], sx[MT];
-    const int left = a.ksteps - 4 * q;   // steps from this quad's first on
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sw[nt] = wsc[nt][q * 64];
     if constexpr (A4) {
@@ -133,40 +172,38 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
       for (int mt = 0; mt < MT; ++mt) sx[mt] = xsc[mt][q * 64];
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int u = 4 * q + (j < left ? j : left - 1);
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) w[j][nt] = *reinterpret_cast<const uint4*>(wt[nt] + static_cast<int64_t>(u) * kTile);
-    }
+      for (int nt = 0; nt < NT; ++nt)
+        w[j][nt] = *reinterpret_cast<const u32x4_t*>(wt[nt] + (static_cast<int64_t>(4 * q + j)) * kTile);
     auto step = [&](auto J) {
       constexpr int j = J.value;
-      if (j >= left) return;
-      const int u = 4 * q + j;
       if constexpr (A4) {
-        uint4 xv[MT];
+        u32x4_t xv[MT];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) xv[mt] = *reinterpret_cast<const uint4*>(xt[mt] + static_cast<int64_t>(u) * kTile);
+        for (int mt = 0; mt < MT; ++mt)
+          xv[mt] = *reinterpret_cast<const u32x4_t*>(xt[mt] + (static_cast<int64_t>(4 * q + j)) * kTile);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[nt], xv[mt], sx[mt], acc[mt][nt]);
       } else {
-        const int k = u * kStep + 32 * g;
+        const int k = q * kQuad + j * kStep + 32 * g;
         const bool live = !TAIL || k < a.K;
-        uint4 xv[MT][4];
+        u32x4_t xv[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            xv[mt][i] = *reinterpret_cast<const uint4*>(xr[mt] + (live ? k : 0) + 8 * i);
-            if (TAIL && !live) xv[mt][i] = make_uint4(0, 0, 0, 0);
+            xv[mt][i] = *reinterpret_cast<const u32x4_t*>(xr[mt] + (live ? k : 0) + 8 * i);
+            if (TAIL && !live) xv[mt][i] = u32x4_t{0, 0, 0, 0};
           }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float s = step_scale<j>(sw[nt]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint4 b = mxfp4::bf16_of(dword(w[j][nt], i), s);
+            const u32x4_t b = mxfp4::bf16_of(w[j][nt][i], s);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_bf16(b, xv[mt][i], acc[mt][nt]);
           }
@@ -184,17 +221,286 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) red[wave][mt * NT + nt][lane] = acc[mt][nt];
   __syncthreads();
-  for (int t = wave; t < MT * NT; t += KW) {
-    f32x4_t s = red[0][t][lane];
+  constexpr int kSide = NT % 2 == 0 ? 2 : 1;   // tiles side by side that a wave adds and stores
+  for (int p = wave; p < MT * NT / kSide; p += KW) {
+    const int mt = p / (NT / kSide), nt = p % (NT / kSide) * kSide;
+    f32x4_t s[kSide];
 #pragma unroll
-    for (int k = 1; k < KW; ++k) s += red[k][t][lane];
-    store4(a, m0 + (t / NT) * 16 + l16, n0 + (t % NT) * 16 + 4 * g, s);
+    for (int i = 0; i < kSide; ++i) {
+      s[i] = red[0][mt * NT + nt + i][lane];
+#pragma unroll
+      for (int k = 1; k < KW; ++k) s[i] += red[k][mt * NT + nt + i][lane];
+    }
+    store_row<kSide>(a, m0 + mt * 16 + l16, t0 + nt, g, s);
   }
+}
+
+// Between two scheduling barriers: MFMAS products with the CVTS conversions spread among them.
+template <int MFMAS, int CVTS>
+__device__ __forceinline__ void spread() {
+  constexpr int kEach = (CVTS + MFMAS - 1) / MFMAS;
+#pragma unroll
+  for (int i = 0; i < MFMAS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x002, kEach, 0);
+  }
+}
+
+// 16-byte reads of a wave go to the 64 LDS banks in four groups of lanes, of which the first is 0-3, 12-15 and
+// 20-27: with this key the operand reads (16 rows, one chunk of each of four blocks) touch each bank once a group, as
+// consecutive lanes' reads do (5.5 cycles a read; keys of r alone, r % 8 or r % 4: 9.1, no key: 33).  A store of
+// a row's 16 chunks touches each bank once with any key.
+__device__ __forceinline__ int chunk_key(int r) { return (r >> 2) ^ ((r & 3) << 2); }
+
+// Many rows: a block has WM x WN waves, a wave MT x NT tiles of 16 x 16.  gridDim.y blocks split K.
+//
+// K goes in stages: 128 elements of bf16 rows, a quad of 512 of 4-bit ones, 4 KB of LDS a row tile in both, and four
+// operands (of 32 or 128 elements) a stage.  X goes through LDS, three stages' buffers: in stage s, behind its
+// barrier, stage s + 2 is stored (loaded from global memory since stage s - 2) and s + 1 is complete, so
+// that the first operand of s + 1 is read before the next barrier and the matrix cores have work on both sides of
+// it.  Every wave loads its weight tiles straight into registers, 512 elements ahead, and with bf16 rows converts
+// an operand while the one before it is multiplied.
+//   LDS: bf16 rows of 256 bytes, 16-byte chunk c of row r at place c ^ chunk_key(r % 16); 4-bit tiles as they are.
+template <bool A4, bool TAIL, int MT, int NT, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) {
+  constexpr int kThreads = 64 * WM * WN;
+  constexpr int kTiles = MT * WM;                      // row tiles of the block
+  constexpr int kChunks = kTiles * 256;                // 16-byte chunks of X in a stage
+  constexpr int kRounds = (kChunks + kThreads - 1) / kThreads;
+  static_assert(WM * WN % 4 == 0, "a wave's chunks of 4-bit rows lie in one tile");
+  constexpr int kBuf = kRounds * kThreads;
+  __shared__ u32x4_t xs[3 * kBuf];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave % WM, wn = wave / WM;
+  const int l16 = lane & 15, g = lane >> 4;
+  const int mblocks = (a.M + 16 * kTiles - 1) / (16 * kTiles), nblocks = (a.N + 16 * NT * WN - 1) / (16 * NT * WN);
+  int mb, nb;
+  block_of(blockIdx.x, mblocks, nblocks, mb, nb);
+  const int t0 = (nb * WN + wn) * NT, m0 = (mb * WM + wm) * MT * 16;
+  const int ntiles = (a.N + 31) / 32 * 2, mtiles = (a.M + 15) / 16;
+  const int qbeg = blockIdx.y * a.slice_quads;
+  const int qend = qbeg + a.slice_quads < a.kquads ? qbeg + a.slice_quads : a.kquads;
+  const int ksteps = (a.K + kStep - 1) / kStep;
+  const int nsteps = (4 * qend < ksteps ? 4 * qend : ksteps) - 4 * qbeg;
+  const int nst = A4 ? qend - qbeg : nsteps, last = nst - 1;
+
+  const uint8_t* wt[NT];
+  const uint32_t* wsc[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    int t = t0 + nt;
+    t = t < ntiles ? t : ntiles - 1;   // tiles past the weight: computed, not stored
+    wt[nt] = a.w + (static_cast<int64_t>(t) * a.kquads + qbeg) * (4 * kTile);
+    wsc[nt] = a.ws + (static_cast<int64_t>(t) * a.kquads + qbeg) * 64;
+  }
+  const uint32_t* xsc[MT];
+  if constexpr (A4) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      int t = m0 / 16 + mt;
+      t = t < mtiles ? t : mtiles - 1;
+      xsc[mt] = a.xs + (static_cast<int64_t>(t) * a.kquads + qbeg) * 64;
+    }
+  }
+  // The thread's chunks of X: round r, chunk id r * kThreads + threadIdx.x.
+  const uint8_t* xg[kRounds];
+  const int xk = (threadIdx.x & 15) * 8;   // bf16: the chunks' first element within a step
+#pragma unroll
+  for (int r = 0; r < kRounds; ++r) {
+    if constexpr (A4) {                    // the wave's chunks lie in one tile
+      int t = mb * kTiles + (r * WM * WN + wave) / 4;
+      t = t < mtiles ? t : mtiles - 1;     // past the last, also of the block: stored behind all
+      xg[r] = a.xt + (static_cast<int64_t>(t) * a.kquads + qbeg) * (4 * kTile);
+    } else {
+      const int c = r * kThreads + threadIdx.x;
+      int m = mb * kTiles * 16 + c / 16;
+      m = m < a.M ? m : a.M - 1;           // rows past the last repeat it, and are not stored
+      xg[r] = reinterpret_cast<const uint8_t*>(a.x + static_cast<int64_t>(m) * a.ldx + qbeg * kQuad + xk);
+    }
+  }
+  // TAIL: the bytes by which the last step's chunks lie past the row's end and are moved back, to be stored as zeros.
+  const int past = TAIL && qbeg * kQuad + last * kStep + xk >= a.K ? 2 * xk : 0;
+  u32x4_t xq[2][kRounds];
+  auto load_x = [&](int s, u32x4_t (&v)[kRounds]) {
+    s = s < last ? s : last;               // stages past the last repeat it, so that no load is conditional
+    if constexpr (A4) {
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) v[r] = reinterpret_cast<const u32x4_t*>(xg[r] + static_cast<int64_t>(s) * (4 * kTile))[threadIdx.x & 255];
+    } else {
+      const int off = 2 * s * kStep - (TAIL && s == last ? past : 0);   // K <= 2^24; negative in a slice of one step
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) v[r] = *reinterpret_cast<const u32x4_t*>(xg[r] + off);
+    }
+  };
+  auto store_x = [&](int s, int buf, const u32x4_t (&v)[kRounds]) {
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int c = r * kThreads + threadIdx.x;
+      u32x4_t t = v[r];
+      if (TAIL && s >= last && past) t = u32x4_t{0, 0, 0, 0};
+      xs[buf + (A4 ? c : (c & ~15) | ((c & 15) ^ chunk_key((c >> 4) & 15)))] = t;
+    }
+  };
+  const int key = chunk_key(l16);
+  auto frag = [&](int buf, int i, u32x4_t (&f)[MT]) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      f[mt] = xs[buf + (A4 ? ((wm * MT + mt) * 4 + i) * 64 + lane : ((wm * MT + mt) * 16 + l16) * 16 + ((4 * g + i) ^ key))];
+  };
+  u32x4_t w[4][NT];                        // bf16: stages s .. s + 3; 4-bit: the stage's four steps
+  auto load_w = [&](int u, u32x4_t (&v)[NT]) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) v[nt] = reinterpret_cast<const u32x4_t*>(wt[nt] + static_cast<int64_t>(u) * kTile)[lane];
+  };
+  uint32_t sw[NT], sx[MT], sw_next[NT], sx_next[MT];
+  auto load_scales = [&](int q) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sw_next[nt] = wsc[nt][q * 64 + lane];
+    if constexpr (A4) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sx_next[mt] = xsc[mt][q * 64 + lane];
+    }
+  };
+  auto take_scales = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) sw[nt] = sw_next[nt];
+    if constexpr (A4) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) sx[mt] = sx_next[mt];
+    }
+  };
+
+  f32x4_t acc[MT][NT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  const int lastq = qend - qbeg - 1;
+  {
+    u32x4_t xa[kRounds], xb[kRounds];       // everything in flight before the first wait
+    load_x(0, xa);
+    load_scales(0);
+    load_w(0, w[0]);
+    load_x(1, xb);
+#pragma unroll
+    for (int j = 1; j < 4; ++j) load_w(j, w[j]);
+    load_x(2, xq[0]);
+    load_x(3, xq[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    store_x(0, 0, xa);
+    take_scales();
+    store_x(1, kBuf, xb);
+    load_scales(lastq < 1 ? lastq : 1);
+  }
+  __syncthreads();
+  u32x4_t f0[MT], f1[MT];
+  frag(0, 0, f0);
+  int cur = 0, nxt = kBuf, far = 2 * kBuf;   // buffers of stages s, s + 1, s + 2
+  auto rotate = [&]() {
+    const int t = cur;
+    cur = nxt;
+    nxt = far;
+    far = t;
+  };
+  // What is common to a stage's begin: its barrier, the operand behind the one in hand, X of later stages.
+  auto begin = [&](auto P, int s) {   // P: s % 2
+    __syncthreads();
+    frag(cur, 1, f1);
+    store_x(s + 2, far, xq[P.value]);
+    load_x(s + 4, xq[P.value]);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if constexpr (A4) {
+    auto products = [&](auto J, const u32x4_t (&f)[MT]) {
+      constexpr int j = J.value;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[nt], f[mt], sx[mt], acc[mt][nt]);
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto stage = [&](auto P, int s) {
+      const int un = 4 * (s < last ? s + 1 : s);
+      begin(P, s);
+      products(std::integral_constant<int, 0>{}, f0);
+      frag(cur, 2, f0);
+      load_w(un, w[0]);
+      __builtin_amdgcn_sched_barrier(0);
+      products(std::integral_constant<int, 1>{}, f1);
+      frag(cur, 3, f1);
+      load_w(un + 1, w[1]);
+      __builtin_amdgcn_sched_barrier(0);
+      products(std::integral_constant<int, 2>{}, f0);
+      frag(nxt, 0, f0);
+      load_w(un + 2, w[2]);
+      __builtin_amdgcn_sched_barrier(0);
+      products(std::integral_constant<int, 3>{}, f1);
+      load_w(un + 3, w[3]);
+      take_scales();
+      load_scales(s + 2 < lastq ? s + 2 : lastq);
+      rotate();
+    };
+    for (int s0 = 0; s0 < nst; s0 += 2) {
+      stage(std::integral_constant<int, 0>{}, s0);
+      if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
+    }
+  } else {
+    u32x4_t b0[NT], b1[NT];
+    auto weights = [&](auto J, const uint32_t (&sc)[NT], int i, u32x4_t (&b)[NT]) {
+      constexpr int j = J.value;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) b[nt] = mxfp4::bf16_of(w[j][nt][i], step_scale<j>(sc[nt]));
+    };
+    // Products of one operand, the conversion of the next spread among them.
+    auto products = [&](const u32x4_t (&f)[MT], const u32x4_t (&b)[NT]) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_bf16(b[nt], f[mt], acc[mt][nt]);
+      spread<MT * NT, 4 * NT + 1>();
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    weights(std::integral_constant<int, 0>{}, sw, 0, b0);
+    auto stage = [&](auto J, int s) {
+      constexpr int j = J.value;
+      begin(std::integral_constant<int, j & 1>{}, s);
+      weights(J, sw, 1, b1);
+      products(f0, b0);
+      frag(cur, 2, f0);
+      __builtin_amdgcn_sched_barrier(0);
+      weights(J, sw, 2, b0);
+      products(f1, b1);
+      frag(cur, 3, f1);
+      __builtin_amdgcn_sched_barrier(0);
+      weights(J, sw, 3, b1);
+      products(f0, b0);
+      frag(nxt, 0, f0);
+      // the quad's tile of the next one: K is padded to whole quads
+      load_w(s - j + 4 <= 4 * lastq ? s + 4 : 4 * lastq + j, w[j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (j < 3) weights(std::integral_constant<int, (j + 1) & 3>{}, sw, 0, b0);
+      else weights(std::integral_constant<int, 0>{}, sw_next, 0, b0);
+      products(f1, b1);
+      rotate();
+    };
+    for (int s0 = 0; s0 < nst; s0 += 4) {
+      stage(std::integral_constant<int, 0>{}, s0);
+      if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
+      if (s0 + 2 < nst) stage(std::integral_constant<int, 2>{}, s0 + 2);
+      if (s0 + 3 < nst) stage(std::integral_constant<int, 3>{}, s0 + 3);
+      take_scales();
+      const int q = s0 / 4 + 2;
+      load_scales(q < lastq ? q : lastq);
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) store_row<NT>(a, m0 + mt * 16 + l16, t0, g, acc[mt]);
 }
 
 // Rows of X to packed 4-bit tiles.  A block is a tile, a wave its block g of 32 elements, four lanes a row of it.
 __global__ __launch_bounds__(256) void mxfp4_pack_rows_kernel(const uint16_t* __restrict__ x, int64_t ldx, int M, int K,
-                                                              int ksteps, int kquads, uint32_t* __restrict__ tiles,
+                                                              int kquads, uint32_t* __restrict__ tiles,
                                                               uint8_t* __restrict__ scales) {
   const int u = blockIdx.x, t = blockIdx.y, g = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int r = lane >> 2, q = lane & 3;
@@ -203,12 +509,12 @@ __global__ __launch_bounds__(256) void mxfp4_pack_rows_kernel(const uint16_t* __
   const int k = u * kStep + 32 * g + 8 * q;
   uint32_t code = 0, s = 127;
   if (k < K) {   // the same for a block's four lanes
-    const uint4 v = *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(row) * ldx + k);
+    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(x + static_cast<int64_t>(row) * ldx + k);
     s = mxfp4::scale_byte(group_max_u32<4>(mxfp4::amax_bits(v)));
     code = mxfp4::codes_of(v, s);
   }
   const int l = 16 * g + r;
-  tiles[((static_cast<int64_t>(t) * ksteps + u) * 64 + l) * 4 + q] = code;
+  tiles[((static_cast<int64_t>(t) * 4 * kquads + u) * 64 + l) * 4 + q] = code;
   if (q == 0) scales[((static_cast<int64_t>(t) * kquads + u / 4) * 64 + l) * 4 + (u & 3)] = static_cast<uint8_t>(s);
 }
 
@@ -224,25 +530,89 @@ __global__ __launch_bounds__(256) void mxfp4_reduce_kernel(const float* __restri
   const float4 s = sum_partials4(part + m * pitch + n, ks, slice);
   Args a{};
   a.M = M; a.N = N; a.y = y; a.ldy = ldy;
-  store4(a, static_cast<int>(m), n, f32x4_t{s.x, s.y, s.z, s.w});
+  const float v[4] = {s.x, s.y, s.z, s.w};
+  store<4>(a, static_cast<int>(m), n, v);
 }
 
+// ---- which kernel ------------------------------------------------------------------------------
+// Tile kernels, smallest first: MT, NT, WM, WN, and the us that a stage takes one block a CU (bf16 rows; a
+// stage of 512 elements of 4-bit ones), measured at 4096 and 28672 columns, K = 4096.
+struct TileConfig {
+  int mt, nt, wm, wn;
+  float us, us4;
+  int rows() const { return 16 * mt * wm; }
+  int cols() const { return 16 * nt * wn; }
+};
+constexpr TileConfig kTile2x1{2, 1, 1, 4, 0.36f, 0.f}, kTile2x2{2, 2, 1, 4, 0.44f, 0.f}, kTile4{4, 2, 1, 4, 0.56f, 0.f},
+    kTile5{5, 2, 1, 4, 0.62f, 0.85f}, kTile6{3, 2, 2, 4, 0.80f, 1.05f}, kTile8{4, 2, 2, 4, 0.93f, 1.30f},
+    kTile10{5, 2, 2, 4, 1.12f, 1.55f}, kTileWide{8, 2, 1, 8, 1.50f, 2.40f};
+constexpr TileConfig kTiles[] = {kTile2x1, kTile2x2, kTile4, kTile5, kTile6, kTile8, kTile10, kTileWide};
+constexpr int kFirstTile4 = 3;   // 4-bit rows: up to 64 go to the stream kernel
+
 struct Plan {
-  int mt, nt, kw;
+  bool stream;
+  int tile;          // index in kTiles
+  int mt, nt, kw;    // stream
   int ks, slice_quads;
   int rows_padded, pitch;
 };
 
-Plan plan_for(int M, int N, int K, bool a4) {
+void split_k(Plan& p, int quads, int ks) {
+  p.slice_quads = (quads + ks - 1) / ks;
+  p.ks = (quads + p.slice_quads - 1) / p.slice_quads;
+}
+
+// The plan for a product.  `partials`: a consumer adds the K slices.
+Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   Plan p{};
   const int mtiles = static_cast<int>(mxfp4::row_tiles(M)), quads = static_cast<int>(mxfp4::quads(K));
-  p.mt = mtiles <= 1 ? 1 : mtiles <= 2 ? 2 : 4;
-  p.nt = 2;
-  p.kw = 4;
-  p.ks = 1;
-  p.slice_quads = (quads + p.ks - 1) / p.ks;
+  const int ntiles = static_cast<int>(mxfp4::weight_tiles(N));
   p.rows_padded = mtiles * 16;
-  p.pitch = static_cast<int>(mxfp4::row_tiles(N)) * 16;
+  p.pitch = ntiles * 16;
+  if (mtiles <= (a4 ? 4 : 1)) {
+    // Stream kernel.  Blocks enough for every CU first, then columns: X is read once for NT tiles.  us, NT = 1, 2, 4:
+    // 16 bf16 rows of 4096 x 4096 5.9, 6.8, 8.1, of 16384 x 2048 8.6, 7.3, 6.3; 32 4-bit rows 4.0, 4.6, 5.5 and 5.8,
+    // 5.3, 6.3; 64 of 28672 x 4096 21.5, 19.0, 16.9.  Eight waves take long K, four leave room for more blocks.
+    p.stream = true;
+    p.mt = mtiles <= 2 ? mtiles : 4;
+    const int enough = p.mt == 4 ? 128 : a4 && p.mt == 1 ? 1 << 30 : 512;   // column tiles for NT = 2
+    p.nt = ntiles >= (a4 ? 3 * enough + (p.mt == 4 ? 1024 : 0) : 2 * enough) ? 4 : ntiles >= enough ? 2 : 1;
+    if (a4 && p.mt == 2) p.nt = ntiles >= 1024 ? 2 : 1;
+    p.kw = p.nt == 4 || quads < 8 ? 4 : 8;
+    if (!a4 && p.nt == 1 && quads > 8) p.kw = 4;
+    int ks = 1;
+    if (partials)
+      while (ks < 4 && ks * 2 * p.kw <= quads && 2 * ks * ((ntiles + p.nt - 1) / p.nt) <= 512) ks *= 2;
+    split_k(p, quads, ks);
+    return p;
+  }
+  // Tile kernels: the cheapest of all tiles and K splits by this estimate.  A round is a block on each of the 256
+  // CUs (two of the four-wave ones); 6 us lie before its first and behind its last product; a reduction
+  // costs a launch where no consumer does it, and its bytes.
+  float best = 1e30f;
+  const int steps = static_cast<int>((K + kStep - 1) / kStep);
+  for (int t = a4 ? kFirstTile4 : 0; t < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
+    const TileConfig& c = kTiles[t];
+    const int64_t blocks = static_cast<int64_t>((M + c.rows() - 1) / c.rows()) * ((ntiles * 16 + c.cols() - 1) / c.cols());
+    for (int ks = 1; ks <= 16 && ks <= quads; ++ks) {
+      Plan q = p;
+      split_k(q, quads, ks);
+      if (q.ks != ks) continue;
+      const int64_t grid = blocks * ks, rounds = (grid + 255) / 256;
+      const float stages = a4 ? static_cast<float>(q.slice_quads) : static_cast<float>(steps < 4 * q.slice_quads ? steps : 4 * q.slice_quads);
+      const float block = 6.0f + stages * (a4 ? c.us4 : c.us);
+      float us = rounds * block;
+      if (c.wm * c.wn == 4 && rounds > 1) us = (rounds + 1) / 2 * block * 1.6f;
+      if (ks > 1) us += (partials ? 0.0f : 2.5f) + 2e-6f * ks * M * static_cast<float>(p.pitch);
+      if (us < best) {
+        best = us;
+        q.tile = t;
+        p.tile = t;
+        p.ks = q.ks;
+        p.slice_quads = q.slice_quads;
+      }
+    }
+  }
   return p;
 }
 
@@ -250,13 +620,68 @@ int64_t part_bytes(const Plan& p, bool partials) {
   return p.ks > 1 || partials ? int64_t{4} * p.ks * p.rows_padded * p.pitch : 0;
 }
 
-template <bool A4, bool TAIL>
-void launch_product(const Plan& p, const Args& a, hipStream_t s) {
-  const dim3 grid((a.N + 16 * p.nt - 1) / (16 * p.nt), p.ks, (a.M + 16 * p.mt - 1) / (16 * p.mt));
-  switch (p.mt) {
-    case 1: hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, 1, 2, 4>), grid, dim3(256), 0, s, a); break;
-    case 2: hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, 2, 2, 4>), grid, dim3(256), 0, s, a); break;
-    default: hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, 4, 2, 4>), grid, dim3(256), 0, s, a); break;
+template <bool A4, bool TAIL, int MT, int NT>
+void launch_stream(const Plan& p, const Args& a, hipStream_t s) {
+  const dim3 grid((static_cast<int>(mxfp4::weight_tiles(a.N)) + NT - 1) / NT, p.ks, (a.M + 16 * MT - 1) / (16 * MT));
+  if constexpr (NT < 4) {
+    if (p.kw == 8) {
+      hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, MT, NT, 8>), grid, dim3(512), 0, s, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, MT, NT, 4>), grid, dim3(256), 0, s, a);
+}
+
+template <bool A4, bool TAIL, int MT>
+void launch_stream_rows(const Plan& p, const Args& a, hipStream_t s) {
+  switch (p.nt) {
+    case 1: launch_stream<A4, TAIL, MT, 1>(p, a, s); break;
+    case 2: launch_stream<A4, TAIL, MT, 2>(p, a, s); break;
+    default: launch_stream<A4, TAIL, MT, 4>(p, a, s); break;
+  }
+}
+
+template <bool A4, bool TAIL, int T>
+void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
+  constexpr TileConfig c = kTiles[T];
+  const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
+  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(blocks, p.ks), dim3(64 * c.wm * c.wn), 0, s, a);
+}
+
+template <bool A4, bool TAIL>   // TAIL: K is not whole quads
+void launch_streams(const Plan& p, const Args& a, hipStream_t s) {
+  if constexpr (A4) {
+    if (p.mt == 2) return launch_stream_rows<A4, TAIL, 2>(p, a, s);
+    if (p.mt == 4) return launch_stream_rows<A4, TAIL, 4>(p, a, s);
+  }
+  launch_stream_rows<A4, TAIL, 1>(p, a, s);
+}
+
+template <bool A4, bool TAIL>   // TAIL: K is not whole steps
+void launch_tiles(const Plan& p, const Args& a, hipStream_t s) {
+  switch (p.tile) {
+    case 3: return launch_tile<A4, TAIL, 3>(p, a, s);
+    case 4: return launch_tile<A4, TAIL, 4>(p, a, s);
+    case 5: return launch_tile<A4, TAIL, 5>(p, a, s);
+    case 6: return launch_tile<A4, TAIL, 6>(p, a, s);
+    case 7: return launch_tile<A4, TAIL, 7>(p, a, s);
+  }
+  if constexpr (!A4) {
+    if (p.tile == 0) return launch_tile<A4, TAIL, 0>(p, a, s);
+    if (p.tile == 1) return launch_tile<A4, TAIL, 1>(p, a, s);
+    return launch_tile<A4, TAIL, 2>(p, a, s);
+  }
+}
+
+void launch_product(const Plan& p, const Args& a, bool a4, hipStream_t s) {
+  if (p.stream) {
+    if (a4) launch_streams<true, false>(p, a, s);
+    else if (a.K % kQuad) launch_streams<false, true>(p, a, s);
+    else launch_streams<false, false>(p, a, s);
+  } else {
+    if (a4) launch_tiles<true, false>(p, a, s);
+    else if (a.K % kStep) launch_tiles<false, true>(p, a, s);
+    else launch_tiles<false, false>(p, a, s);
   }
 }
 
@@ -279,15 +704,15 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
     else if (!coopt::aligned16(x) || !coopt::aligned16(w)) bad = "x and w must be 16-byte aligned";
     else if (ldx < K || ldx % 8) bad = "row stride of x must be >= K and a multiple of 8";
     else if (!partials && (ldy < N || (reinterpret_cast<uintptr_t>(y) & 1))) bad = "row stride of y must be >= N";
-    else if (partials && N % 16) bad = "partial sums need N a multiple of 16";
+    else if (partials && N % 32) bad = "partial sums need N a multiple of 32";
   }
   if (bad) {
     coopt::set_error(std::string(who) + ": " + bad);
     return COOPT_EINVAL;
   }
   if (M == 0 || N == 0) return COOPT_OK;
-  const Plan p = plan_for(M, N, K, act4 != 0);
-  const int64_t pb = part_bytes(p, partials), need = pb + (act4 ? mxfp4::packed_bytes(M, K) : 0);
+  const Plan p = plan_for(M, N, K, act4 != 0, partials);
+  const int64_t pb = part_bytes(p, partials), need = pb + (act4 ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0);
   if (need && (static_cast<int64_t>(workspace_bytes) < need || !workspace || !coopt::aligned16(workspace))) {
     coopt::set_error(std::string(who) + ": workspace smaller than required (or misaligned)");
     return COOPT_EWORKSPACE;
@@ -297,9 +722,8 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   a.x = static_cast<const uint16_t*>(x);
   a.ldx = ldx;
   a.w = static_cast<const uint8_t*>(w);
-  a.ws = reinterpret_cast<const uint32_t*>(a.w + mxfp4::tile_bytes(N, K));
+  a.ws = reinterpret_cast<const uint32_t*>(a.w + mxfp4::tile_bytes(mxfp4::weight_tiles(N), K));
   a.M = M; a.N = N; a.K = K;
-  a.ksteps = static_cast<int>(mxfp4::steps(K));
   a.kquads = static_cast<int>(mxfp4::quads(K));
   a.slice_quads = p.slice_quads;
   a.y = static_cast<uint16_t*>(y);
@@ -309,17 +733,13 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   a.pitch = p.pitch;
   if (act4) {
     uint8_t* tiles = static_cast<uint8_t*>(workspace) + pb;
-    uint8_t* scales = tiles + mxfp4::tile_bytes(M, K);
+    uint8_t* scales = tiles + mxfp4::tile_bytes(mxfp4::row_tiles(M), K);
     a.xt = tiles;
     a.xs = reinterpret_cast<const uint32_t*>(scales);
-    hipLaunchKernelGGL(mxfp4_pack_rows_kernel, dim3(a.ksteps, static_cast<unsigned>(mxfp4::row_tiles(M))), dim3(256), 0, s,
-                       a.x, ldx, M, K, a.ksteps, a.kquads, reinterpret_cast<uint32_t*>(tiles), scales);
-    launch_product<true, false>(p, a, s);
-  } else if (K % kStep) {
-    launch_product<false, true>(p, a, s);
-  } else {
-    launch_product<false, false>(p, a, s);
+    hipLaunchKernelGGL(mxfp4_pack_rows_kernel, dim3(4 * a.kquads, static_cast<unsigned>(mxfp4::row_tiles(M))), dim3(256), 0, s,
+                       a.x, ldx, M, K, a.kquads, reinterpret_cast<uint32_t*>(tiles), scales);
   }
+  launch_product(p, a, act4 != 0, s);
   if (pb && !partials) {
     const int64_t n = static_cast<int64_t>(M) * (p.pitch / 4);
     hipLaunchKernelGGL(mxfp4_reduce_kernel, dim3(static_cast<unsigned>((n + 255) / 256)), dim3(256), 0, s, a.part, p.ks,
@@ -332,15 +752,15 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
 
 extern "C" size_t coopt_mxfp4_linear_workspace(int M, int N, int K, int act4, int partials) {
   if (shape_error(M, N, K) || M == 0 || N == 0) return 0;
-  const Plan p = plan_for(M, N, K, act4 != 0);
-  return static_cast<size_t>(part_bytes(p, partials != 0) + (act4 ? mxfp4::packed_bytes(M, K) : 0));
+  const Plan p = plan_for(M, N, K, act4 != 0, partials != 0);
+  return static_cast<size_t>(part_bytes(p, partials != 0) + (act4 ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0));
 }
 
 extern "C" int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, int* rows_padded) {
   coopt::clear_error();
   COOPT_REQUIRE(ks && rows_padded, "null output pointer");
   COOPT_REQUIRE(!shape_error(M, N, K) && M > 0 && N > 0, "unsupported shape");
-  const Plan p = plan_for(M, N, K, act4 != 0);
+  const Plan p = plan_for(M, N, K, act4 != 0, true);
   *ks = p.ks;
   *rows_padded = p.rows_padded;
   return COOPT_OK;

@@ -384,7 +384,7 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
         x2 = x2.clone(memory_format=torch.contiguous_format)
     act4 = 1 if weight.activations == "mxfp4" else 0
     partials = False
-    if defer_reduce and out is None and N % 16 == 0 and M > 0:
+    if defer_reduce and out is None and N % 32 == 0 and M > 0:
         ks, rows_padded = _mxfp4_split(M, N, K, act4)
         partials = ks > 1
     if not partials and out is None:

@@ -563,7 +563,7 @@ int coopt_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, 
  *     workspace: coopt_mxfp4_linear_workspace(M, N, K, act4, 0) bytes (0: none), 16-byte aligned.
  *   coopt_mxfp4_linear_split / _partials: as coopt_linear_split / coopt_linear_partials: ks fp32 slices
  *     [rows_padded, N] at the workspace's start, whose sum in order is the output before its rounding.  N a
- *     multiple of 16; coopt_mxfp4_linear_workspace(M, N, K, act4, 1) bytes.
+ *     multiple of 32; coopt_mxfp4_linear_workspace(M, N, K, act4, 1) bytes.
  */
 size_t coopt_mxfp4_packed_bytes(int N, int K);
 int coopt_mxfp4_pack_weight(const void* codes, const void* scales, int N, int K, void* out, coopt_stream_t stream);
