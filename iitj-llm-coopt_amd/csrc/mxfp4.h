@@ -53,9 +53,10 @@ __device__ __forceinline__ float scale_operand(uint32_t byte) { return __uint_as
 __device__ __forceinline__ bf16x2_t pair(uint32_t v) { return __builtin_bit_cast(bf16x2_t, v); }
 
 // The codes of eight bf16 values (four dwords of two), nearest with ties to the even code, saturated at 6
-// (v_cvt_scalef32_pk_fp4_bf16).  A block of scale byte 255 has codes 0.
+// (v_cvt_scalef32_pk_fp4_bf16).  CLEAR: a block of scale byte 255 has codes 0 (any others stand for NaN too).
+template <bool CLEAR = true>
 __device__ __forceinline__ uint32_t codes_of(const u32x4_t& x, uint32_t s) {
-  if (s == 255) return 0;
+  if (CLEAR && s == 255) return 0;
   const float f = scale_operand(s);
   uint32_t r = 0;
   r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, pair(x[0]), f, 0);
@@ -77,16 +78,20 @@ __device__ __forceinline__ uint32_t codes_of(const float (&x)[8], uint32_t s) {
   return r;
 }
 
-// Bits of the largest magnitude of eight bf16 values.
-__device__ __forceinline__ uint32_t amax_bits(const u32x4_t& x) {
-  uint32_t m = 0;
+// Bits (of fp32) of the largest magnitude of 8 N bf16 values.
+template <int N>
+__device__ __forceinline__ uint32_t amax_bits(const u32x4_t (&x)[N]) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t m = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = (x[i] << 16) & 0x7fffffffu, hi = x[i] & 0x7fff0000u;
-    m = m > lo ? m : lo;
-    m = m > hi ? m : hi;
-  }
-  return m;
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t v = x[i][e] & 0x7fff7fffu;
+      m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2_t, v));
+    }
+  const uint32_t lo = m[0], hi = m[1];
+  return (lo > hi ? lo : hi) << 16;
 }
 
 // Eight elements of one block as bf16 (exact), from their four code bytes.

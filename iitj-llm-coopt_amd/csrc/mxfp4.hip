@@ -17,9 +17,9 @@ __global__ __launch_bounds__(kThreads) void mxfp4_quantize_kernel(const void* __
   if (i >= eighths) return;   // whole groups of four lanes: a block has four eighths
   uint32_t code, s;
   if constexpr (DT == COOPT_DT_BF16) {
-    const mxfp4::u32x4_t v = reinterpret_cast<const mxfp4::u32x4_t*>(x)[i];
+    const mxfp4::u32x4_t v[1] = {reinterpret_cast<const mxfp4::u32x4_t*>(x)[i]};
     s = mxfp4::scale_byte(group_max_u32<4>(mxfp4::amax_bits(v)));
-    code = mxfp4::codes_of(v, s);
+    code = mxfp4::codes_of(v[0], s);
   } else {
     float f[8];
     if constexpr (DT == COOPT_DT_F16) {

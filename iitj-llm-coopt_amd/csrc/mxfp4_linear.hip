@@ -44,11 +44,12 @@ __device__ __forceinline__ f32x4_t mfma_bf16(const u32x4_t& a, const u32x4_t& b,
                                                  c, 0, 0, 0);
 }
 
-template <int J>
+// J, JX: the bytes of sa and sb that are the operands' scales.
+template <int J, int JX = J>
 __device__ __forceinline__ f32x4_t mfma_fp4(const u32x4_t& a, uint32_t sa, const u32x4_t& b, uint32_t sb, f32x4_t c) {
   const i32x8_t av = {static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(a.z), static_cast<int>(a.w), 0, 0, 0, 0};
   const i32x8_t bv = {static_cast<int>(b.x), static_cast<int>(b.y), static_cast<int>(b.z), static_cast<int>(b.w), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, J, static_cast<int>(sa), J,
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, J, static_cast<int>(sa), JX,
                                                           static_cast<int>(sb));
 }
 
@@ -119,9 +120,15 @@ __device__ __forceinline__ void block_of(int id, int mblocks, int nblocks, int& 
   nb = in / rows;
 }
 
+// X of the stream kernel: bf16 rows multiplied as they are, packed 4-bit rows, or bf16 rows quantised as they are read.
+enum { kRows, kPacked, kQuantize };
+
 // Few rows: every wave of a block has the same NT column tiles and its own K quads, reads X where it lies
 // (caches serve it to the blocks) and the block adds the waves' sums in LDS, in order.  No barrier before that.
-template <bool A4, bool TAIL, int MT, int NT, int KW>
+// kQuantize: a lane's 32 elements of a step are one block of the format, so that it finds their scale and codes by
+// itself, some 55 instructions a step and row tile in every block, where that takes less than the launch that packs
+// them (in_kernel).
+template <int X, bool TAIL, int MT, int NT, int KW>
 __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
   __shared__ f32x4_t red[KW][MT * NT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -145,7 +152,7 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
   const uint32_t* xsc[MT];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    if constexpr (A4) {
+    if constexpr (X == kPacked) {
       int t = m0 / 16 + mt;
       t = t < mtiles ? t : mtiles - 1;
       xt[mt] = a.xt + static_cast<int64_t>(t) * a.kquads * (4 * kTile) + lane * 16;
@@ -167,7 +174,7 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
     uint32_t sw[NT], sx[MT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) sw[nt] = wsc[nt][q * 64];
-    if constexpr (A4) {
+    if constexpr (X == kPacked) {
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) sx[mt] = xsc[mt][q * 64];
     }
@@ -176,28 +183,28 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         w[j][nt] = *reinterpret_cast<const u32x4_t*>(wt[nt] + (static_cast<int64_t>(4 * q + j)) * kTile);
-    auto step = [&](auto J) {
-      constexpr int j = J.value;
-      if constexpr (A4) {
-        u32x4_t xv[MT];
+    // X of the whole quad too before anything waits: step by step, each would wait for the caches' latency.
+    u32x4_t xv[4][MT][X == kPacked ? 1 : 4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-          xv[mt] = *reinterpret_cast<const u32x4_t*>(xt[mt] + (static_cast<int64_t>(4 * q + j)) * kTile);
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[nt], xv[mt], sx[mt], acc[mt][nt]);
-      } else {
-        const int k = q * kQuad + j * kStep + 32 * g;
-        const bool live = !TAIL || k < a.K;
-        u32x4_t xv[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (X == kPacked) {
+          xv[j][mt][0] = *reinterpret_cast<const u32x4_t*>(xt[mt] + (static_cast<int64_t>(4 * q + j)) * kTile);
+        } else {
+          const int k = q * kQuad + j * kStep + 32 * g;
+          const bool live = !TAIL || k < a.K;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            xv[mt][i] = *reinterpret_cast<const u32x4_t*>(xr[mt] + (live ? k : 0) + 8 * i);
-            if (TAIL && !live) xv[mt][i] = u32x4_t{0, 0, 0, 0};
+            xv[j][mt][i] = *reinterpret_cast<const u32x4_t*>(xr[mt] + (live ? k : 0) + 8 * i);
+            if (TAIL && !live) xv[j][mt][i] = u32x4_t{0, 0, 0, 0};
           }
+        }
+      }
+    __builtin_amdgcn_sched_barrier(0);
+    auto step = [&](auto J) {
+      constexpr int j = J.value;
+      if constexpr (X == kRows) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           const float s = step_scale<j>(sw[nt]);
@@ -205,8 +212,22 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
           for (int i = 0; i < 4; ++i) {
             const u32x4_t b = mxfp4::bf16_of(w[j][nt][i], s);
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_bf16(b, xv[mt][i], acc[mt][nt]);
+            for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_bf16(b, xv[j][mt][i], acc[mt][nt]);
           }
+        }
+        return;
+      }
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (X == kPacked) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[nt], xv[j][mt][0], sx[mt], acc[mt][nt]);
+        } else {
+          const uint32_t s = mxfp4::scale_byte(mxfp4::amax_bits(xv[j][mt]));
+          const u32x4_t c = {mxfp4::codes_of<false>(xv[j][mt][0], s), mxfp4::codes_of<false>(xv[j][mt][1], s),
+                             mxfp4::codes_of<false>(xv[j][mt][2], s), mxfp4::codes_of<false>(xv[j][mt][3], s)};
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j, 0>(w[j][nt], sw[nt], c, s, acc[mt][nt]);
         }
       }
     };
@@ -509,9 +530,9 @@ __global__ __launch_bounds__(256) void mxfp4_pack_rows_kernel(const uint16_t* __
   const int k = u * kStep + 32 * g + 8 * q;
   uint32_t code = 0, s = 127;
   if (k < K) {   // the same for a block's four lanes
-    const u32x4_t v = *reinterpret_cast<const u32x4_t*>(x + static_cast<int64_t>(row) * ldx + k);
+    const u32x4_t v[1] = {*reinterpret_cast<const u32x4_t*>(x + static_cast<int64_t>(row) * ldx + k)};
     s = mxfp4::scale_byte(group_max_u32<4>(mxfp4::amax_bits(v)));
-    code = mxfp4::codes_of(v, s);
+    code = mxfp4::codes_of(v[0], s);
   }
   const int l = 16 * g + r;
   tiles[((static_cast<int64_t>(t) * 4 * kquads + u) * 64 + l) * 4 + q] = code;
@@ -551,7 +572,8 @@ constexpr int kFirstTile4 = 3;   // 4-bit rows: up to 64 go to the stream kernel
 
 struct Plan {
   bool stream;
-  int tile;          // index in kTiles
+  int x;             // stream: kRows, kPacked, kQuantize
+  int tile;          // else index in kTiles
   int mt, nt, kw;    // stream
   int ks, slice_quads;
   int rows_padded, pitch;
@@ -562,6 +584,11 @@ void split_k(Plan& p, int quads, int ks) {
   p.ks = (quads + p.slice_quads - 1) / p.slice_quads;
 }
 
+// Whether the stream kernel quantises X itself.  us, it / packed without the 2 us and the host's 3 of the launch that
+// packs: 16 rows of 4096 x 4096 6.7 / 3.4, of 16384 x 2048 7.1 / 4.9, but of 28672 x 4096 17.5 / 12.4 and of 4096 x 14336
+// 17.5 / 7.4; one row 4.1, 5.7, 13.8, 9.8.
+bool in_kernel(int M, int ntiles, int quads) { return M <= 8 || (M <= 16 && ntiles <= 1024 && quads <= 8); }
+
 // The plan for a product.  `partials`: a consumer adds the K slices.
 Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   Plan p{};
@@ -570,16 +597,17 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   p.rows_padded = mtiles * 16;
   p.pitch = ntiles * 16;
   if (mtiles <= (a4 ? 4 : 1)) {
-    // Stream kernel.  Blocks enough for every CU first, then columns: X is read once for NT tiles.  us, NT = 1, 2, 4:
-    // 16 bf16 rows of 4096 x 4096 5.9, 6.8, 8.1, of 16384 x 2048 8.6, 7.3, 6.3; 32 4-bit rows 4.0, 4.6, 5.5 and 5.8,
-    // 5.3, 6.3; 64 of 28672 x 4096 21.5, 19.0, 16.9.  Eight waves take long K, four leave room for more blocks.
+    // Stream kernel.  Blocks enough for every CU first, then column tiles, for which X is read once.  us, NT = 1, 2, 4:
+    // 16 bf16 rows of 4096 x 4096 6.3, 6.8, 8.1, of 6144 x 4096 8.4, 7.3, 8.1, of 28672 x 4096 35, 23.3, 18.7 (one row 14.5,
+    // 13.7, 14.4); packed ones of 4096 x 4096 3.4, 3.8, 6.6; 32 of 16384 x 2048 5.8, 5.5, 7.1; 64 of 28672 x 4096 21.5, 19.0,
+    // 16.9.  Eight waves where each has a quad.
     p.stream = true;
+    p.x = !a4 ? kRows : in_kernel(M, ntiles, quads) ? kQuantize : kPacked;
     p.mt = mtiles <= 2 ? mtiles : 4;
-    const int enough = p.mt == 4 ? 128 : a4 && p.mt == 1 ? 1 << 30 : 512;   // column tiles for NT = 2
-    p.nt = ntiles >= (a4 ? 3 * enough + (p.mt == 4 ? 1024 : 0) : 2 * enough) ? 4 : ntiles >= enough ? 2 : 1;
-    if (a4 && p.mt == 2) p.nt = ntiles >= 1024 ? 2 : 1;
+    if (p.x != kPacked) p.nt = ntiles >= 1024 && M > 4 ? 4 : ntiles >= 384 ? 2 : 1;
+    else if (p.mt == 4) p.nt = ntiles >= 1408 ? 4 : ntiles >= 192 ? 2 : 1;
+    else p.nt = ntiles >= 1024 ? 2 : 1;
     p.kw = p.nt == 4 || quads < 8 ? 4 : 8;
-    if (!a4 && p.nt == 1 && quads > 8) p.kw = 4;
     int ks = 1;
     if (partials)
       while (ks < 4 && ks * 2 * p.kw <= quads && 2 * ks * ((ntiles + p.nt - 1) / p.nt) <= 512) ks *= 2;
@@ -599,6 +627,7 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
       split_k(q, quads, ks);
       if (q.ks != ks) continue;
       const int64_t grid = blocks * ks, rounds = (grid + 255) / 256;
+      if (ks > 1 && grid > 512) break;   // enough for every CU
       const float stages = a4 ? static_cast<float>(q.slice_quads) : static_cast<float>(steps < 4 * q.slice_quads ? steps : 4 * q.slice_quads);
       const float block = 6.0f + stages * (a4 ? c.us4 : c.us);
       float us = rounds * block;
@@ -620,25 +649,25 @@ int64_t part_bytes(const Plan& p, bool partials) {
   return p.ks > 1 || partials ? int64_t{4} * p.ks * p.rows_padded * p.pitch : 0;
 }
 
-template <bool A4, bool TAIL, int MT, int NT>
+template <int X, bool TAIL, int MT, int NT>
 void launch_stream(const Plan& p, const Args& a, hipStream_t s) {
   const dim3 grid((static_cast<int>(mxfp4::weight_tiles(a.N)) + NT - 1) / NT, p.ks, (a.M + 16 * MT - 1) / (16 * MT));
   if constexpr (NT < 4) {
     if (p.kw == 8) {
-      hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, MT, NT, 8>), grid, dim3(512), 0, s, a);
+      hipLaunchKernelGGL((mxfp4_stream_kernel<X, TAIL, MT, NT, 8>), grid, dim3(512), 0, s, a);
       return;
     }
   }
-  hipLaunchKernelGGL((mxfp4_stream_kernel<A4, TAIL, MT, NT, 4>), grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((mxfp4_stream_kernel<X, TAIL, MT, NT, 4>), grid, dim3(256), 0, s, a);
 }
 
-template <bool A4, bool TAIL, int MT>
+template <int X, bool TAIL, int MT>
 void launch_stream_rows(const Plan& p, const Args& a, hipStream_t s) {
-  switch (p.nt) {
-    case 1: launch_stream<A4, TAIL, MT, 1>(p, a, s); break;
-    case 2: launch_stream<A4, TAIL, MT, 2>(p, a, s); break;
-    default: launch_stream<A4, TAIL, MT, 4>(p, a, s); break;
+  if constexpr (X != kPacked || MT == 4) {
+    if (p.nt == 4) return launch_stream<X, TAIL, MT, 4>(p, a, s);
   }
+  if (p.nt == 2) launch_stream<X, TAIL, MT, 2>(p, a, s);
+  else launch_stream<X, TAIL, MT, 1>(p, a, s);
 }
 
 template <bool A4, bool TAIL, int T>
@@ -646,15 +675,6 @@ void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
   constexpr TileConfig c = kTiles[T];
   const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
   hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(blocks, p.ks), dim3(64 * c.wm * c.wn), 0, s, a);
-}
-
-template <bool A4, bool TAIL>   // TAIL: K is not whole quads
-void launch_streams(const Plan& p, const Args& a, hipStream_t s) {
-  if constexpr (A4) {
-    if (p.mt == 2) return launch_stream_rows<A4, TAIL, 2>(p, a, s);
-    if (p.mt == 4) return launch_stream_rows<A4, TAIL, 4>(p, a, s);
-  }
-  launch_stream_rows<A4, TAIL, 1>(p, a, s);
 }
 
 template <bool A4, bool TAIL>   // TAIL: K is not whole steps
@@ -675,9 +695,18 @@ void launch_tiles(const Plan& p, const Args& a, hipStream_t s) {
 
 void launch_product(const Plan& p, const Args& a, bool a4, hipStream_t s) {
   if (p.stream) {
-    if (a4) launch_streams<true, false>(p, a, s);
-    else if (a.K % kQuad) launch_streams<false, true>(p, a, s);
-    else launch_streams<false, false>(p, a, s);
+    const bool tail = a.K % kQuad != 0;
+    if (p.x == kPacked) {
+      if (p.mt == 1) launch_stream_rows<kPacked, false, 1>(p, a, s);
+      else if (p.mt == 2) launch_stream_rows<kPacked, false, 2>(p, a, s);
+      else launch_stream_rows<kPacked, false, 4>(p, a, s);
+    } else if (p.x == kQuantize) {
+      if (tail) launch_stream_rows<kQuantize, true, 1>(p, a, s);
+      else launch_stream_rows<kQuantize, false, 1>(p, a, s);
+    } else {
+      if (tail) launch_stream_rows<kRows, true, 1>(p, a, s);
+      else launch_stream_rows<kRows, false, 1>(p, a, s);
+    }
   } else {
     if (a4) launch_tiles<true, false>(p, a, s);
     else if (a.K % kStep) launch_tiles<false, true>(p, a, s);
@@ -712,7 +741,8 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   }
   if (M == 0 || N == 0) return COOPT_OK;
   const Plan p = plan_for(M, N, K, act4 != 0, partials);
-  const int64_t pb = part_bytes(p, partials), need = pb + (act4 ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0);
+  const bool pack = act4 && p.x != kQuantize;
+  const int64_t pb = part_bytes(p, partials), need = pb + (pack ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0);
   if (need && (static_cast<int64_t>(workspace_bytes) < need || !workspace || !coopt::aligned16(workspace))) {
     coopt::set_error(std::string(who) + ": workspace smaller than required (or misaligned)");
     return COOPT_EWORKSPACE;
@@ -731,7 +761,7 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   a.part = pb ? static_cast<float*>(workspace) : nullptr;
   a.part_slice = static_cast<int64_t>(p.rows_padded) * p.pitch;
   a.pitch = p.pitch;
-  if (act4) {
+  if (pack) {
     uint8_t* tiles = static_cast<uint8_t*>(workspace) + pb;
     uint8_t* scales = tiles + mxfp4::tile_bytes(mxfp4::row_tiles(M), K);
     a.xt = tiles;
@@ -753,7 +783,8 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
 extern "C" size_t coopt_mxfp4_linear_workspace(int M, int N, int K, int act4, int partials) {
   if (shape_error(M, N, K) || M == 0 || N == 0) return 0;
   const Plan p = plan_for(M, N, K, act4 != 0, partials != 0);
-  return static_cast<size_t>(part_bytes(p, partials != 0) + (act4 ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0));
+  return static_cast<size_t>(part_bytes(p, partials != 0) +
+                             (act4 && p.x != kQuantize ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0));
 }
 
 extern "C" int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, int* rows_padded) {

@@ -13,7 +13,7 @@ Beside them, for models that the reference does not run:
 """
 import contextlib
 import ctypes
-import functools
+import math
 import threading
 
 import torch
@@ -31,6 +31,7 @@ _WS = _lib.WorkspaceCache()
 # held over the launches of a 4-bit product that takes its workspace from _WS: another thread's call on the
 # same stream would write its own between them
 _WS_LOCK = threading.Lock()
+_NO_LOCK = contextlib.nullcontext()
 
 
 def _bf16_rows(t, name):
@@ -108,43 +109,59 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
     x [..., H] bf16 or the LinearPartials of the projection that made it (summed here), residual of its
     shape; gate [H], or of x's shape (rows may be strided); H a multiple of 8 up to 16384.  residual_out: where r
     goes, by default into `residual`.  Returns out (a new tensor by default)."""
-    part = x if isinstance(x, LinearPartials) else None
-    shape, H = tuple(x.shape), x.shape[-1]
+    part = x if type(x) is LinearPartials else None
+    shape = x.shape
+    H = shape[-1] if shape else 0
     index = residual.get_device()
-    same = [t for t in (None if part is not None else x, residual, weight, post_weight, gate, residual_out, out)
-            if t is not None]
-    if index < 0 or any(t.get_device() != index for t in same) or \
-            (part is not None and part.buf.get_device() != index):
-        _lib.require_one_device(*same, None if part is None else part.buf)
-    for name, t in (("x", None if part is not None else x), ("residual", residual), ("residual_out", residual_out),
-                    ("out", out)):
-        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != shape or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous bf16 {shape}")
-    for name, t in (("weight", weight), ("post_weight", post_weight)):
-        if t is not None and (t.dtype != torch.bfloat16 or tuple(t.shape) != (H,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must be contiguous bf16 [{H}]")
-    gate_stride = 0
+    source = x if part is None else part.buf
+    alike = index >= 0 and index == source.get_device() == weight.get_device()
+    if part is None and (x.dtype is not torch.bfloat16 or not x.is_contiguous()):
+        raise ValueError(f"x must be contiguous bf16 or LinearPartials, got {x.dtype} {tuple(shape)}")
+    if residual.dtype is not torch.bfloat16 or residual.shape != shape or not residual.is_contiguous():
+        raise ValueError(f"residual must be contiguous bf16 {tuple(shape)}")
+    if weight.dtype is not torch.bfloat16 or weight.shape != (H,) or not weight.is_contiguous():
+        raise ValueError(f"weight must be contiguous bf16 [{H}]")
+    pp = gp = gate_stride = 0
+    if post_weight is not None:
+        if post_weight.dtype is not torch.bfloat16 or post_weight.shape != (H,) or not post_weight.is_contiguous():
+            raise ValueError(f"post_weight must be contiguous bf16 [{H}]")
+        alike = alike and index == post_weight.get_device()
+        pp = post_weight.data_ptr()
     if gate is not None:
-        if gate.dtype != torch.bfloat16 or tuple(gate.shape) not in ((H,), shape):
-            raise ValueError(f"gate must be bf16 [{H}] or {shape}")
-        if gate.dim() > 1:
-            gate = gate.reshape(-1, H)
-            if gate.stride(1) != 1 or gate.stride(0) < H or gate.stride(0) % 8:
-                gate = gate.contiguous()
-            gate_stride = gate.stride(0) if gate.shape[0] > 1 else 0
-        elif gate.stride(0) != 1:
+        rows_of = gate.dim() > 1
+        if gate.dtype is not torch.bfloat16 or gate.shape != (shape if rows_of else (H,)):
+            raise ValueError(f"gate must be bf16 [{H}] or {tuple(shape)}")
+        alike = alike and index == gate.get_device()
+        if rows_of:
+            if gate.is_contiguous():
+                gate_stride = H
+            else:
+                gate = gate.reshape(-1, H)
+                gate_stride, along = gate.stride()
+                if along != 1 or gate_stride < H or gate_stride % 8:
+                    gate, gate_stride = gate.contiguous(), H
+        elif not gate.is_contiguous():
             gate = gate.contiguous()
+        gp = gate.data_ptr()
+    for name, t in (("out", out), ("residual_out", residual_out)):
+        if t is not None:
+            if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous bf16 {tuple(shape)}")
+            alike = alike and index == t.get_device()
+    if not alike:
+        _lib.require_one_device(source, residual, weight, post_weight, gate, residual_out, out)
     if out is None:
         out = torch.empty_like(residual)
-    if residual_out is None:
-        residual_out = residual
+    rp = residual.data_ptr()
     rows = residual.numel() // H if H else 0
-    _lib.check(_lib.call_on(
-        index, _lib.entry("coopt_residual_norm"), 0 if part is not None else x.data_ptr(),
-        0 if part is None else part.buf.data_ptr(), 0 if part is None else part.ks,
-        0 if part is None else part.rows_padded * part.n, residual.data_ptr(), residual_out.data_ptr(),
-        _lib.ptr(post_weight), _lib.ptr(gate), gate_stride, weight.data_ptr(), out.data_ptr(), rows, H, float(eps),
-        float(branch_scale), float(residual_scale), _lib.raw_stream(index)), "coopt_residual_norm")
+    rc = _lib.call_on(
+        index, _lib.entry("coopt_residual_norm"), x.data_ptr() if part is None else 0,
+        0 if part is None else source.data_ptr(), 0 if part is None else part.ks,
+        0 if part is None else part.rows_padded * part.n, rp, rp if residual_out is None else residual_out.data_ptr(),
+        pp, gp, gate_stride, weight.data_ptr(), out.data_ptr(), rows, H, eps, branch_scale, residual_scale,
+        _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc, "coopt_residual_norm")
     return out
 
 
@@ -303,7 +320,7 @@ def linear(x, weight, out=None, defer_reduce=False):
     `weight` may be an MXFP4Weight (K a multiple of 32, any N and row count): coopt_mxfp4_linear, with
     bf16 rows or, where the weight says activations "mxfp4", rows quantised to 4 bits in the call.
     defer_reduce returns LinearPartials where K is split."""
-    if isinstance(weight, MXFP4Weight):
+    if type(weight) is MXFP4Weight:
         return _linear_mxfp4(x, weight, out, defer_reduce)
     packed = weight.packed if isinstance(weight, PackedWeight) and not weight.gate_up else None
     if isinstance(weight, PackedWeight):
@@ -354,60 +371,64 @@ def linear(x, weight, out=None, defer_reduce=False):
     return out
 
 
-@functools.lru_cache(maxsize=1024)   # pure functions of the sizes
-def _mxfp4_workspace(M, N, K, act4, partials):
-    return int(_lib.load().coopt_mxfp4_linear_workspace(M, N, K, act4, partials))
-
-
-@functools.lru_cache(maxsize=1024)
-def _mxfp4_split(M, N, K, act4):
-    ks, rp = ctypes.c_int(0), ctypes.c_int(0)
-    _lib.check(_lib.load().coopt_mxfp4_linear_split(M, N, K, act4, ctypes.byref(ks), ctypes.byref(rp)),
-               "coopt_mxfp4_linear_split")
-    return ks.value, rp.value
-
-
 def _linear_mxfp4(x, weight, out, defer_reduce):
     """linear() with an MXFP4Weight."""
     N, K = weight.shape
-    index = x.get_device()
-    if index < 0 or index != weight.packed.get_device() or (out is not None and out.get_device() != index):
-        _lib.require_one_device(x, weight.packed, out)
-    if x.dtype is not torch.bfloat16 or x.dim() == 0 or x.shape[-1] != K:
-        raise ValueError(f"x must be bf16 [..., {K}], got {x.dtype} {tuple(x.shape)}")
-    shape = (*x.shape[:-1], N)
-    if out is not None and (out.dtype is not torch.bfloat16 or tuple(out.shape) != shape or out.stride(-1) != 1):
-        raise ValueError(f"out must be bf16 {shape} with contiguous rows")
-    x2 = x.reshape(-1, K)
-    M = x2.shape[0]
-    if x2.stride(1) != 1 or x2.stride(0) % 8 or (M > 1 and x2.stride(0) < K) or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    act4 = 1 if weight.activations == "mxfp4" else 0
-    partials = False
-    if defer_reduce and out is None and N % 32 == 0 and M > 0:
-        ks, rows_padded = _mxfp4_split(M, N, K, act4)
-        partials = ks > 1
-    if not partials and out is None:
-        out = x.new_empty(shape)
-    need = _mxfp4_workspace(M, N, K, act4, 1 if partials else 0)
-    # a graph under capture gets a workspace of its own (from its memory pool), so that two graphs captured on
-    # one stream may replay at the same time
-    shared = need > 0 and not torch.cuda.is_current_stream_capturing()
-    ws = None if shared or not need else x.new_empty((need,), dtype=torch.uint8)
-    ldx = x2.stride(0) if M > 1 else max(K, x2.stride(0))
-    with _WS_LOCK if shared else contextlib.nullcontext():
-        if shared:
-            ws = _WS.get(need, x.device)
-        have, wsp = (0, 0) if ws is None else (ws.numel(), ws.data_ptr())
-        if partials:
-            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear_partials"), x2.data_ptr(), ldx,
-                              weight.packed.data_ptr(), M, N, K, act4, wsp, have, _lib.raw_stream(index))
-        else:
-            y2 = out.view(-1, N)
-            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear"), x2.data_ptr(), ldx, weight.packed.data_ptr(),
-                              M, N, K, act4, y2.data_ptr(), max(N, y2.stride(0)), wsp, have,
-                              _lib.raw_stream(index))
-    _lib.check(rc, "coopt_mxfp4_linear")
+    packed = weight.packed
+    index = packed.get_device()
+    if x.get_device() != index or index < 0 or (out is not None and out.get_device() != index):
+        _lib.require_one_device(x, packed, out)
+    lead = x.shape
+    if x.dtype is not torch.bfloat16 or not lead or lead[-1] != K:
+        raise ValueError(f"x must be bf16 [..., {K}], got {x.dtype} {tuple(lead)}")
+    lead = lead[:-1]
+    if out is not None and (out.dtype is not torch.bfloat16 or out.shape != (*lead, N) or out.stride(-1) != 1):
+        raise ValueError(f"out must be bf16 {(*lead, N)} with contiguous rows")
+    M, ldx = (lead[0] if len(lead) == 1 else math.prod(lead)), K
+    if not x.is_contiguous():
+        x = x.reshape(-1, K)
+        ldx, along = x.stride()
+        if along != 1 or ldx % 8 or ldx < K:
+            x, ldx = x.contiguous(), K
+    if x.data_ptr() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), K
+    if M == 0:
+        return x.new_empty((*lead, N)) if out is None else out
+    need, ks, rows_padded, need_partials = weight.plan(M)
+    partials = defer_reduce and out is None and ks > 1
     if partials:
-        return LinearPartials(ws, ks, M, rows_padded, N, torch.Size(shape), x.device)
+        need = need_partials
+    if not need:
+        wsp = have = 0
+        lock = _NO_LOCK
+    elif torch.cuda.is_current_stream_capturing():
+        # a graph under capture gets a workspace of its own (from its memory pool), so that two graphs captured
+        # on one stream may replay at the same time
+        ws, lock = x.new_empty((need,), dtype=torch.uint8), _NO_LOCK
+        wsp, have = ws.data_ptr(), need
+    else:
+        lock, wsp = _WS_LOCK, None
+    if partials:
+        yp = ldy = None
+    else:
+        if out is None:
+            out = x.new_empty(M, N) if len(lead) == 1 else x.new_empty((*lead, N))
+        y = out if out.dim() == 2 else out.view(-1, N)
+        yp, ldy = y.data_ptr(), y.stride(0)
+        if ldy < N:   # one row
+            ldy = N
+    with lock:
+        if wsp is None:
+            ws = _WS.get(need, packed.device)
+            wsp, have = ws.data_ptr(), ws.numel()
+        if partials:
+            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear_partials"), x.data_ptr(), ldx, packed.data_ptr(), M, N,
+                              K, weight.act4, wsp, have, _lib.raw_stream(index))
+        else:
+            rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear"), x.data_ptr(), ldx, packed.data_ptr(), M, N, K,
+                              weight.act4, yp, ldy, wsp, have, _lib.raw_stream(index))
+    if rc:
+        _lib.check(rc, "coopt_mxfp4_linear")
+    if partials:
+        return LinearPartials(ws, ks, M, rows_padded, N, torch.Size((*lead, N)), x.device)
     return out

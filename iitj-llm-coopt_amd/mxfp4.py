@@ -10,6 +10,8 @@ block's scale byte s, NaN where s is 255.  Quantisation takes s - 127 = floor(lo
 -127) and the nearest code, ties to the even one, 6 for everything above; a block that is not finite gets 255.
 The reference has no such weights; its codes for swapped caches are kv_cache.quantize's.
 """
+import ctypes
+
 import torch
 
 from . import _lib
@@ -26,34 +28,40 @@ def _aligned(t, nbytes):
     return t if t.data_ptr() % nbytes == 0 else t.clone()
 
 
+_KINDS = {torch.bfloat16: _lib.DT_BF16, torch.float16: _lib.DT_F16, torch.float32: _lib.DT_F32}
+
+
 def quantize_mxfp4(x: torch.Tensor):
     """x [..., K] (bf16, fp16 or fp32) -> (codes uint8 [..., K / 2], scales uint8 [..., K / 32])."""
     index = x.get_device()
     if index < 0:
         _lib.require_cuda(x)
-    if x.dim() == 0 or x.shape[-1] % BLOCK:
-        raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {tuple(x.shape)}")
-    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    kind = _KINDS.get(x.dtype)
+    if kind is None:
         raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
-    *lead, K = x.shape
-    xc = _aligned(x, 16)
-    codes = xc.new_empty((*lead, K // 2), dtype=torch.uint8)
-    scales = xc.new_empty((*lead, K // BLOCK), dtype=torch.uint8)
-    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_quantize"), _lib.dt_code(x.dtype), xc.data_ptr(),
-                            xc.numel() // K if K else 0, K, codes.data_ptr(), scales.data_ptr(),
-                            _lib.raw_stream(index)), "coopt_mxfp4_quantize")
+    shape = x.shape
+    K = shape[-1] if shape else 1
+    if K % BLOCK:
+        raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {tuple(shape)}")
+    if not x.is_contiguous() or x.data_ptr() % 16:
+        x = _aligned(x, 16)
+    lead = shape[:-1]
+    codes = x.new_empty((*lead, K // 2), dtype=torch.uint8)
+    scales = x.new_empty((*lead, K // BLOCK), dtype=torch.uint8)
+    rows = x.numel() // K if K else 0
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_quantize"), kind, x.data_ptr(), rows, K, codes.data_ptr(),
+                            scales.data_ptr(), _lib.raw_stream(index)), "coopt_mxfp4_quantize")
     return codes, scales
 
 
 def _check_rows(codes, scales):
     """K of codes [..., K / 2] and scales [..., K / 32]."""
-    if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+    cs, ss = codes.shape, scales.shape
+    if codes.dtype is not torch.uint8 or scales.dtype is not torch.uint8:
         raise ValueError("codes and scales must be uint8")
-    if codes.dim() == 0 or codes.shape[-1] % (BLOCK // 2) or \
-            scales.shape != (*codes.shape[:-1], codes.shape[-1] // (BLOCK // 2)):
-        raise ValueError(f"codes [..., K / 2] and scales [..., K / {BLOCK}] disagree: {tuple(codes.shape)}, "
-                         f"{tuple(scales.shape)}")
-    return 2 * codes.shape[-1]
+    if not cs or len(ss) != len(cs) or cs[:-1] != ss[:-1] or cs[-1] != ss[-1] * (BLOCK // 2):
+        raise ValueError(f"codes [..., K / 2] and scales [..., K / {BLOCK}] disagree: {tuple(cs)}, {tuple(ss)}")
+    return 2 * cs[-1]
 
 
 def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16):
@@ -62,13 +70,17 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bflo
     if index < 0 or index != scales.get_device():
         _lib.require_one_device(codes, scales)
     K = _check_rows(codes, scales)
-    if dtype not in (torch.bfloat16, torch.float16, torch.float32):
+    kind = _KINDS.get(dtype)
+    if kind is None:
         raise ValueError(f"dtype must be bf16, fp16 or fp32, got {dtype}")
-    cc, sc = _aligned(codes, 4), scales.contiguous()
-    out = cc.new_empty((*codes.shape[:-1], K), dtype=dtype)
-    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_dequantize"), cc.data_ptr(), sc.data_ptr(),
-                            out.numel() // K if K else 0, K, _lib.dt_code(dtype), out.data_ptr(),
-                            _lib.raw_stream(index)), "coopt_mxfp4_dequantize")
+    if not codes.is_contiguous() or codes.data_ptr() % 4:
+        codes = _aligned(codes, 4)
+    if not scales.is_contiguous():
+        scales = scales.contiguous()
+    out = codes.new_empty((*codes.shape[:-1], K), dtype=dtype)
+    rows = out.numel() // K if K else 0
+    _lib.check(_lib.call_on(index, _lib.entry("coopt_mxfp4_dequantize"), codes.data_ptr(), scales.data_ptr(), rows, K,
+                            kind, out.data_ptr(), _lib.raw_stream(index)), "coopt_mxfp4_dequantize")
     return out
 
 
@@ -82,6 +94,25 @@ class MXFP4Weight:
     def __init__(self, codes, scales, packed, activations="bf16"):
         self.codes, self.scales, self.packed, self.activations = codes, scales, packed, activations
         self.shape = torch.Size((codes.shape[0], 2 * codes.shape[1]))
+        self.act4 = 1 if activations == "mxfp4" else 0
+        self._plans = {}   # rows: what plan() returns, a pure function of the sizes
+
+    def plan(self, rows):
+        """(workspace bytes, K slices a consumer would add, padded rows and workspace bytes of those) of a
+        product of `rows` rows."""
+        p = self._plans.get(rows)
+        if p is None:
+            lib, (N, K) = _lib.load(), self.shape
+            ks, padded = ctypes.c_int(0), ctypes.c_int(0)
+            _lib.check(lib.coopt_mxfp4_linear_split(rows, N, K, self.act4, ctypes.byref(ks), ctypes.byref(padded)),
+                       "coopt_mxfp4_linear_split")
+            size = lib.coopt_mxfp4_linear_workspace
+            p = (int(size(rows, N, K, self.act4, 0)), ks.value if N % 32 == 0 else 1, padded.value,
+                 int(size(rows, N, K, self.act4, 1)))
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            self._plans[rows] = p
+        return p
 
     @property
     def dtype(self):

@@ -64,15 +64,15 @@ def test_products_refuse(lib, partials):
         refused(product(lib, True, wsb=8), _lib.COOPT_EWORKSPACE)
     else:
         assert "null" in refused(product(lib, y=None)) and "row stride of y" in refused(product(lib, ldy=63))
-    assert "workspace" in refused(product(lib, partials, act4=1, wsb=8), _lib.COOPT_EWORKSPACE)
-    assert "workspace" in refused(product(lib, partials, act4=1, ws=8), _lib.COOPT_EWORKSPACE)
+    assert "workspace" in refused(product(lib, partials, M=20, act4=1, wsb=8), _lib.COOPT_EWORKSPACE)
+    assert "workspace" in refused(product(lib, partials, M=20, act4=1, ws=8), _lib.COOPT_EWORKSPACE)
     assert product(lib, partials, M=0) == product(lib, partials, N=0) == _lib.COOPT_OK
 
 
 def test_product_workspaces(lib):
     import ctypes
     ws, split = lib.coopt_mxfp4_linear_workspace, lib.coopt_mxfp4_linear_split
-    for M, N, K in ((1, 4096, 4096), (32, 2048, 8192), (77, 4096, 14336), (160, 6144, 4096), (2000, 4096, 14336)):
+    for M, N, K in ((17, 4096, 4096), (32, 2048, 8192), (77, 4096, 14336), (160, 6144, 4096), (2000, 4096, 14336)):
         for act4 in (0, 1):
             ks, rows = ctypes.c_int(), ctypes.c_int()
             assert split(M, N, K, act4, ctypes.byref(ks), ctypes.byref(rows)) == _lib.COOPT_OK
@@ -120,7 +120,7 @@ def test_wrappers_refuse():
         M.pack_mxfp4_weight(u8(2, 16), u8(2, 1), "int8")
     with pytest.raises(ValueError, match="must be .N, K."):
         M.quantize_mxfp4_weight(bf(32))
-    w = M.MXFP4Weight(u8(16, 16), u8(16, 1), u8(2048))
+    w = M.MXFP4Weight(u8(16, 16), u8(16, 1), u8(8704))
     with pytest.raises(_lib.CooptError, match="no CPU fallback"):
         fused.linear(bf(2, 32), w)
     with pytest.raises(_lib.CooptError, match="no CPU fallback"):
