@@ -30,8 +30,9 @@ from .attention import (paged_attention, paged_attention_qkv, qkv_attention_supp
                         window_workspace_bytes, workspace_bytes)
 from .batch import row_slots
 from .fused import (LinearPartials, linear, linear_silu, pack_gate_up_weight, pack_linear_weight,
-                    rms_norm, rope_,
+                    residual_norm, rms_norm, rope_,
                     row_major, silu_and_mul)
+from .mxfp4 import MXFP4Weight, quantize_mxfp4_weight
 from .kv_cache import (allocate_kv_cache, qkv_norm_rope_and_cache, qkv_rope_and_cache,
                        reshape_and_cache_flash)
 from .spec_decode import AcceptResult, accept
@@ -55,12 +56,22 @@ class LlamaShape:
     window: int | None = None    # attention sees the last `window` keys ...
     sink_tokens: int = 0         # ... and these first ones
     qk_norm: bool = False        # RMS norms of the query and key heads before the rotation
+    post_norm: bool = False      # RMS norms of the attention's and the MLP's outputs, before the residual sum ...
+    branch_gate: bool = False    # ... a gate [hidden] on each ...
+    branch_scale: float = 1.0    # ... and the sum is residual_scale * x + branch_scale * output
+    residual_scale: float = 1.0
+
+    @property
+    def scaled_branches(self) -> bool:
+        """Whether the residual sums are more than x + output (fused.residual_norm instead of rms_norm)."""
+        return self.post_norm or self.branch_gate or self.branch_scale != 1.0 or self.residual_scale != 1.0
 
     def params(self) -> int:
         qkv = (self.heads + 2 * self.kv_heads) * self.head_dim * self.hidden
         o = self.heads * self.head_dim * self.hidden
         mlp = 3 * self.ffn * self.hidden
         per_layer = qkv + o + mlp + 2 * self.hidden + (2 * self.head_dim if self.qk_norm else 0)
+        per_layer += 2 * self.hidden * (self.post_norm + self.branch_gate)
         emb = self.vocab * self.hidden
         return self.layers * per_layer + emb * (1 if self.tie_embeddings else 2) + self.hidden
 
@@ -70,11 +81,22 @@ DRAFT_LLAMA32_1B = LlamaShape(2048, 8192, 16, 32, 8, 64, 128256, 500000.0, tie_e
 
 
 class RandomLlama:
-    """Llama decoder with N(0, std^2) weights (unit norms), bf16 on `device`."""
+    """Llama decoder with N(0, std^2) weights (unit norms), bf16 on `device`.
+
+    weights="mxfp4": the projections named in `packed` are microscaled 4-bit weights (mxfp4.MXFP4Weight;
+    4.25 bits a weight are streamed instead of 16); activations="mxfp4": rows are quantised to 4 bits
+    on their way into them, too.  Needs a GPU; a copy on the CPU (to) holds the same values in bf16."""
 
     def __init__(self, shape: LlamaShape, device, seed=0, std=0.02, max_pos=8192,
-                 dtype=torch.bfloat16, packed=None):
+                 dtype=torch.bfloat16, packed=None, weights="bf16", activations="bf16"):
         self.s, self.device, self.dtype = shape, torch.device(device), dtype
+        if weights not in ("bf16", "mxfp4") or activations not in ("bf16", "mxfp4"):
+            raise ValueError(f"weights and activations must be 'bf16' or 'mxfp4', got {weights!r}, {activations!r}")
+        if activations == "mxfp4" and weights != "mxfp4":
+            raise ValueError("4-bit activations need 4-bit weights")
+        if weights == "mxfp4" and self.device.type != "cuda":
+            raise ValueError("4-bit weights need a GPU")
+        self.weights, self.activations = weights, activations
         self.packed = tuple(self.PACKED if packed is None else packed)
         g = torch.Generator(device=self.device).manual_seed(seed)
 
@@ -99,6 +121,9 @@ class RandomLlama:
             if shape.qk_norm:
                 self.layers[-1].update({k: torch.ones(D, device=self.device, dtype=dtype)
                                         for k in ("q_norm", "k_norm")})
+            names = [f"{b}_{k}" for b in ("attn", "mlp")
+                     for k, has in (("post", shape.post_norm), ("gate", shape.branch_gate)) if has]
+            self.layers[-1].update({k: torch.ones(H, device=self.device, dtype=dtype) for k in names})
         if self.device.type == "cuda":
             self._pack()
         inv = 1.0 / (shape.rope_theta ** (torch.arange(0, D, 2, dtype=torch.float32) / D))
@@ -118,6 +143,14 @@ class RandomLlama:
     PACKED = ("qkv", "o", "gate_up", "down")
 
     def _pack(self):
+        if self.weights == "mxfp4":
+            for L in self.layers:
+                for k in self.packed:
+                    if k in L:
+                        L[k] = quantize_mxfp4_weight(L[k], self.activations)
+            if "lm_head" in self.packed:
+                self.lm_head = quantize_mxfp4_weight(self.lm_head, self.activations)
+            return
         ok = lambda w, r=16: w.shape[0] % r == 0 and w.shape[1] % 128 == 0  # tile granularity
         for L in self.layers:
             for k in self.packed:
@@ -131,9 +164,10 @@ class RandomLlama:
         """A copy of the weights on another device (same values)."""
         other = object.__new__(RandomLlama)
         other.s, other.device, other.dtype = self.s, torch.device(device), self.dtype
-        other.packed = self.packed
+        other.packed, other.weights, other.activations = self.packed, self.weights, self.activations
         other.embed = self.embed.to(device)
-        other.lm_head = other.embed if self.s.tie_embeddings else row_major(self.lm_head).to(device)
+        tied = self.s.tie_embeddings and not isinstance(self.lm_head, MXFP4Weight)
+        other.lm_head = other.embed if tied else row_major(self.lm_head).to(device)
         other.norm = self.norm.to(device)
         other.layers = [{k: row_major(v).to(device) for k, v in L.items()} for L in self.layers]
         if other.device.type == "cuda":
@@ -155,7 +189,7 @@ class RandomLlama:
         x = F.embedding(ids, self.embed)                       # residual stream
         d = None
         for li, L in enumerate(self.layers):
-            h = ops.rms_norm(x if d is None else d, None if d is None else x, L["ln1"], s.eps)
+            h = self.add_norm(ops, d, x, L["ln1"], self.layers[li - 1], "mlp")
             # qkv projection, RoPE, the KV write and attention (engine/model.py:238-247):
             # split-K partials straight into one launch that reduces them, writes the paged
             # cache and attends (ops.attend_qkv), or into the epilogue launch that writes q
@@ -170,12 +204,23 @@ class RandomLlama:
             # otherwise gate_up feed only the fused add + norm or SiLU, which reduce their
             # split-K partials as they read them
             o = ops.linear(attn.reshape(T, H * D), L["o"], defer_reduce=True)
-            h = ops.rms_norm(o, x, L["ln2"], s.eps)
+            h = self.add_norm(ops, o, x, L["ln2"], L, "attn")
             d = ops.linear(ops.linear_silu(h, L["gate_up"]), L["down"], defer_reduce=True)
-        h = ops.rms_norm(d, x, self.norm, s.eps)
+        h = self.add_norm(ops, d, x, self.norm, self.layers[-1], "mlp")
         if keep_rows is not None:
             h = h.index_select(0, keep_rows)
         return ops.linear(h, self.lm_head, out=logits_out)
+
+    def add_norm(self, ops, d, x, weight, L, branch):
+        """The output d of `branch` ("attn" or "mlp") of layer L into the residual stream x, in place, and the
+        norm of that by `weight`; the norm alone where there is no d yet."""
+        s = self.s
+        if d is None:
+            return ops.rms_norm(x, None, weight, s.eps)
+        if not s.scaled_branches:
+            return ops.rms_norm(d, x, weight, s.eps)
+        return ops.residual_norm(d, x, weight, s.eps, L.get(branch + "_post"), L.get(branch + "_gate"), s.branch_scale,
+                                 s.residual_scale)
 
     def attend(self, ops, kv, li, L, qkv, pos, slots, meta):
         """The epilogue of layer li's qkv projection (rotation, with the head norms where the shape
@@ -259,6 +304,9 @@ class HipOps:
 
     def rms_norm(self, x, residual, w, eps):
         return rms_norm(x, w, eps, residual=residual)
+
+    def residual_norm(self, x, residual, w, eps, post_weight, gate, branch_scale, residual_scale):
+        return residual_norm(x, residual, w, eps, post_weight, gate, branch_scale, residual_scale)
 
     def rope(self, q, k, pos, cos, sin):
         rope_(q, k, pos, cos, sin)
@@ -562,8 +610,8 @@ class SpecDecoder:
         if s.qk_norm or s.window is not None:
             meta = (self._meta(B, P), torch.full((B,), P, dtype=torch.int32, device=ids.device), P, P)
         for li, L in enumerate(model.layers):
-            h = self.ops.rms_norm(x if d is None else d, None if d is None else x, L["ln1"], s.eps)
-            qkv = F.linear(h, row_major(L["qkv"]))
+            h = model.add_norm(self.ops, d, x, L["ln1"], model.layers[li - 1], "mlp")
+            qkv = self._prompt_linear(h, L["qkv"])
             if meta is not None:
                 attn = model.attend(self.ops, kv, li, L, qkv, flat_pos, slots, meta).reshape(T, H * D)
             else:
@@ -579,13 +627,18 @@ class SpecDecoder:
                 a = F.scaled_dot_product_attention(qf.contiguous(), kf.contiguous(), vf.contiguous(),
                                                    is_causal=True, scale=model.scale)
                 attn = a.transpose(1, 2).reshape(T, H * D).to(x.dtype)
-            o = F.linear(attn, row_major(L["o"]))
-            h = self.ops.rms_norm(o, x, L["ln2"], s.eps)
-            d = F.linear(self.ops.silu_mul(F.linear(h, row_major(L["gate_up"]))), row_major(L["down"]))
+            o = self._prompt_linear(attn, L["o"])
+            h = model.add_norm(self.ops, o, x, L["ln2"], L, "attn")
+            d = self._prompt_linear(self.ops.silu_mul(self._prompt_linear(h, L["gate_up"])), L["down"])
         last_d = d.view(B, P, -1)[:, -1].contiguous()
         last_x = x.view(B, P, -1)[:, -1].contiguous()
-        h = self.ops.rms_norm(last_d, last_x, model.norm, s.eps)
-        return F.linear(h, row_major(model.lm_head))
+        h = model.add_norm(self.ops, last_d, last_x, model.norm, model.layers[-1], "mlp")
+        return self._prompt_linear(h, model.lm_head)
+
+    def _prompt_linear(self, x, weight):
+        if isinstance(weight, MXFP4Weight):
+            return self.ops.linear(x, weight)
+        return F.linear(x, row_major(weight))
 
     # ---- buckets ----------------------------------------------------------------------
     def bucket(self):
