@@ -116,8 +116,8 @@ __device__ __forceinline__ void block_of(int id, int mblocks, int nblocks, int& 
   const int band = t / (kRun * nblocks);
   const int rows = mblocks - band * kRun < kRun ? mblocks - band * kRun : kRun;
   const int in = t - band * kRun * nblocks;
-  mb = band * kRun + in % rows;
-  nb = in / rows;
+  mb = __builtin_amdgcn_readfirstlane(band * kRun + in % rows);   // divisions leave their results in vector registers
+  nb = __builtin_amdgcn_readfirstlane(in / rows);
 }
 
 // X of the stream kernel: bf16 rows multiplied as they are, packed 4-bit rows, or bf16 rows quantised as they are read.
@@ -281,9 +281,16 @@ __device__ __forceinline__ int chunk_key(int r) { return (r >> 2) ^ ((r & 3) << 
 // that the first operand of s + 1 is read before the next barrier and the matrix cores have work on both sides of
 // it.  Every wave loads its weight tiles straight into registers, 512 elements ahead, and with bf16 rows converts
 // an operand while the one before it is multiplied.
+//
+// With 4-bit rows a block takes the tiles blockIdx.x, blockIdx.x + gridDim.x, ... .  Loads run into the next tile (its
+// first stages behind this one's last), so that between tiles nothing waits but the stores: 4093 x 28672 x 4096, 14
+// tiles a CU, takes 304 us (3.2 PFLOP/s), 347 with a block for each tile.  The launch gives a block more than one only
+// where stages come in pairs, four or more.  (bf16 rows: the addresses of a next tile do not fit beside the operands of
+// the widest tile.)
 //   LDS: bf16 rows of 256 bytes, 16-byte chunk c of row r at place c ^ chunk_key(r % 16); 4-bit tiles as they are.
+// Two waves a SIMD at least: above 256 registers a CU holds one four-wave block, 394 us there for 327.
 template <bool A4, bool TAIL, int MT, int NT, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args a) {
   constexpr int kThreads = 64 * WM * WN;
   constexpr int kTiles = MT * WM;                      // row tiles of the block
   constexpr int kChunks = kTiles * 256;                // 16-byte chunks of X in a stage
@@ -295,9 +302,9 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
   const int wm = wave % WM, wn = wave / WM;
   const int l16 = lane & 15, g = lane >> 4;
   const int mblocks = (a.M + 16 * kTiles - 1) / (16 * kTiles), nblocks = (a.N + 16 * NT * WN - 1) / (16 * NT * WN);
-  int mb, nb;
-  block_of(blockIdx.x, mblocks, nblocks, mb, nb);
-  const int t0 = (nb * WN + wn) * NT, m0 = (mb * WM + wm) * MT * 16;
+  const int total = mblocks * nblocks;
+  int id = blockIdx.x, mb, nb;
+  block_of(id, mblocks, nblocks, mb, nb);
   const int ntiles = (a.N + 31) / 32 * 2, mtiles = (a.M + 15) / 16;
   const int qbeg = blockIdx.y * a.slice_quads;
   const int qend = qbeg + a.slice_quads < a.kquads ? qbeg + a.slice_quads : a.kquads;
@@ -305,52 +312,54 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
   const int nsteps = (4 * qend < ksteps ? 4 * qend : ksteps) - 4 * qbeg;
   const int nst = A4 ? qend - qbeg : nsteps, last = nst - 1;
 
-  const uint8_t* wt[NT];
-  const uint32_t* wsc[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    int t = t0 + nt;
-    t = t < ntiles ? t : ntiles - 1;   // tiles past the weight: computed, not stored
-    wt[nt] = a.w + (static_cast<int64_t>(t) * a.kquads + qbeg) * (4 * kTile);
-    wsc[nt] = a.ws + (static_cast<int64_t>(t) * a.kquads + qbeg) * 64;
-  }
-  const uint32_t* xsc[MT];
-  if constexpr (A4) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      int t = m0 / 16 + mt;
-      t = t < mtiles ? t : mtiles - 1;
-      xsc[mt] = a.xs + (static_cast<int64_t>(t) * a.kquads + qbeg) * 64;
-    }
-  }
-  // The thread's chunks of X: round r, chunk id r * kThreads + threadIdx.x.
-  const uint8_t* xg[kRounds];
-  const int xk = (threadIdx.x & 15) * 8;   // bf16: the chunks' first element within a step
-#pragma unroll
-  for (int r = 0; r < kRounds; ++r) {
-    if constexpr (A4) {                    // the wave's chunks lie in one tile
-      int t = mb * kTiles + (r * WM * WN + wave) / 4;
-      t = t < mtiles ? t : mtiles - 1;     // past the last, also of the block: stored behind all
-      xg[r] = a.xt + (static_cast<int64_t>(t) * a.kquads + qbeg) * (4 * kTile);
+  // Where the loads are: each of these moves to the next tile as its own run ahead passes this tile's last stage.
+  // (First tiles in scalar registers, addresses formed at each load: as pointers they took the registers of the tiles.)
+  int w_tile, sw_tile, sx_tile, x_tile;
+  const uint16_t* x_base;                  // bf16: the tile's first row; the thread's chunks of X (round r, chunk id
+  uint32_t x_off[kRounds];                 // r * kThreads + threadIdx.x) in bytes behind it: at most 160 rows of 2^22
+  const int xk = (threadIdx.x & 15) * 8;   // and their first element within a step
+  auto tile_at = [&](const uint8_t* base, int t, int tiles, int bytes) {   // tiles past the last: computed, not stored
+    return base + (static_cast<int64_t>(t < tiles ? t : tiles - 1) * a.kquads + qbeg) * bytes;
+  };
+  auto weights_of = [&](int nb) { w_tile = (nb * WN + wn) * NT; };
+  auto scales_of = [&](int mb, int nb) {
+    sw_tile = (nb * WN + wn) * NT;
+    sx_tile = (mb * WM + wm) * MT;
+  };
+  auto rows_of = [&](int mb) {
+    if constexpr (A4) {
+      x_tile = mb * kTiles;
     } else {
-      const int c = r * kThreads + threadIdx.x;
-      int m = mb * kTiles * 16 + c / 16;
-      m = m < a.M ? m : a.M - 1;           // rows past the last repeat it, and are not stored
-      xg[r] = reinterpret_cast<const uint8_t*>(a.x + static_cast<int64_t>(m) * a.ldx + qbeg * kQuad + xk);
+      const int m0 = mb * kTiles * 16;
+      x_base = a.x + static_cast<int64_t>(m0) * a.ldx + qbeg * kQuad;
+#pragma unroll
+      for (int r = 0; r < kRounds; ++r) {
+        const int c = r * kThreads + threadIdx.x;
+        int m = c / 16;
+        m = m < a.M - m0 ? m : a.M - m0 - 1;   // rows past the last repeat it, and are not stored
+        x_off[r] = 2 * (static_cast<uint32_t>(m) * static_cast<uint32_t>(a.ldx) + xk);
+      }
     }
-  }
+  };
+  rows_of(mb);
+  weights_of(nb);
+  scales_of(mb, nb);
   // TAIL: the bytes by which the last step's chunks lie past the row's end and are moved back, to be stored as zeros.
-  const int past = TAIL && qbeg * kQuad + last * kStep + xk >= a.K ? 2 * xk : 0;
+  const uint32_t past = TAIL && qbeg * kQuad + last * kStep + xk >= a.K ? 2 * xk : 0;
   u32x4_t xq[2][kRounds];
   auto load_x = [&](int s, u32x4_t (&v)[kRounds]) {
     s = s < last ? s : last;               // stages past the last repeat it, so that no load is conditional
     if constexpr (A4) {
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) v[r] = reinterpret_cast<const u32x4_t*>(xg[r] + static_cast<int64_t>(s) * (4 * kTile))[threadIdx.x & 255];
+      for (int r = 0; r < kRounds; ++r) {  // the wave's chunks lie in one tile
+        const uint8_t* t = tile_at(a.xt, x_tile + (r * WM * WN + wave) / 4, mtiles, 4 * kTile);
+        v[r] = reinterpret_cast<const u32x4_t*>(t + static_cast<int64_t>(s) * (4 * kTile))[threadIdx.x & 255];
+      }
     } else {
-      const int off = 2 * s * kStep - (TAIL && s == last ? past : 0);   // K <= 2^24; negative in a slice of one step
+      const uint8_t* at = reinterpret_cast<const uint8_t*>(x_base + s * kStep);
+      const uint32_t back = TAIL && s == last ? past : 0;   // of the chunk's own 2 * xk
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) v[r] = *reinterpret_cast<const u32x4_t*>(xg[r] + off);
+      for (int r = 0; r < kRounds; ++r) v[r] = *reinterpret_cast<const u32x4_t*>(at + (x_off[r] - back));
     }
   };
   auto store_x = [&](int s, int buf, const u32x4_t (&v)[kRounds]) {
@@ -358,7 +367,7 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
     for (int r = 0; r < kRounds; ++r) {
       const int c = r * kThreads + threadIdx.x;
       u32x4_t t = v[r];
-      if (TAIL && s >= last && past) t = u32x4_t{0, 0, 0, 0};
+      if (TAIL && s >= last && past) t = u32x4_t{0, 0, 0, 0};   // (with one tile only)
       xs[buf + (A4 ? c : (c & ~15) | ((c & 15) ^ chunk_key((c >> 4) & 15)))] = t;
     }
   };
@@ -371,37 +380,33 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
   u32x4_t w[4][NT];                        // bf16: stages s .. s + 3; 4-bit: the stage's four steps
   auto load_w = [&](int u, u32x4_t (&v)[NT]) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) v[nt] = reinterpret_cast<const u32x4_t*>(wt[nt] + static_cast<int64_t>(u) * kTile)[lane];
+    for (int nt = 0; nt < NT; ++nt)
+      v[nt] = reinterpret_cast<const u32x4_t*>(tile_at(a.w, w_tile + nt, ntiles, 4 * kTile) + static_cast<int64_t>(u) * kTile)[lane];
   };
-  uint32_t sw[NT], sx[MT], sw_next[NT], sx_next[MT];
-  auto load_scales = [&](int q) {
+  // Scales of even and odd quads: a register that is copied waits for its load, and that for all loads before it.
+  uint32_t sw[2][NT], sx[2][MT];
+  const int lastq = qend - qbeg - 1;
+  auto load_scales = [&](auto P, int q) {
+    q = q < lastq ? q : lastq;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sw_next[nt] = wsc[nt][q * 64 + lane];
+    for (int nt = 0; nt < NT; ++nt)
+      sw[P.value][nt] = reinterpret_cast<const uint32_t*>(
+          tile_at(reinterpret_cast<const uint8_t*>(a.ws), sw_tile + nt, ntiles, 256) + q * 256)[lane];
     if constexpr (A4) {
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sx_next[mt] = xsc[mt][q * 64 + lane];
+      for (int mt = 0; mt < MT; ++mt)
+        sx[P.value][mt] = reinterpret_cast<const uint32_t*>(
+            tile_at(reinterpret_cast<const uint8_t*>(a.xs), sx_tile + mt, mtiles, 256) + q * 256)[lane];
     }
   };
-  auto take_scales = [&]() {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) sw[nt] = sw_next[nt];
-    if constexpr (A4) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) sx[mt] = sx_next[mt];
-    }
-  };
+  constexpr std::integral_constant<int, 0> kEven{};
+  constexpr std::integral_constant<int, 1> kOdd{};
 
   f32x4_t acc[MT][NT];
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  const int lastq = qend - qbeg - 1;
   {
     u32x4_t xa[kRounds], xb[kRounds];       // everything in flight before the first wait
     load_x(0, xa);
-    load_scales(0);
+    load_scales(kEven, 0);
     load_w(0, w[0]);
     load_x(1, xb);
 #pragma unroll
@@ -410,9 +415,8 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
     load_x(3, xq[1]);
     __builtin_amdgcn_sched_barrier(0);
     store_x(0, 0, xa);
-    take_scales();
     store_x(1, kBuf, xb);
-    load_scales(lastq < 1 ? lastq : 1);
+    load_scales(kOdd, 1);
   }
   __syncthreads();
   u32x4_t f0[MT], f1[MT];
@@ -425,98 +429,124 @@ __global__ __launch_bounds__(64 * WM * WN) void mxfp4_tile_kernel(const Args a) 
     far = t;
   };
   // What is common to a stage's begin: its barrier, the operand behind the one in hand, X of later stages.
+  int mb_next, nb_next;               // the next tile, if there is one
+  bool more = false;
   auto begin = [&](auto P, int s) {   // P: s % 2
     __syncthreads();
     frag(cur, 1, f1);
     store_x(s + 2, far, xq[P.value]);
-    load_x(s + 4, xq[P.value]);
+    if (A4 && P.value == 0 && s + 4 == nst) rows_of(mb_next);   // (stages come in pairs where there is a next tile)
+    load_x(s + 4 < nst || !more ? s + 4 : s + 4 - nst, xq[P.value]);
     __builtin_amdgcn_sched_barrier(0);
   };
-  if constexpr (A4) {
-    auto products = [&](auto J, const u32x4_t (&f)[MT]) {
-      constexpr int j = J.value;
+  // The scales of quad q of this tile, or of the next one's first two.
+  auto scales_ahead = [&](auto P, int q) {
+    if (A4 && q == lastq + 1) scales_of(mb_next, nb_next);
+    load_scales(P, q <= lastq || !more ? q : q - lastq - 1);
+  };
+  u32x4_t b0[NT], b1[NT];
+  auto weights = [&](auto J, const uint32_t (&sc)[NT], int i, u32x4_t (&b)[NT]) {
+    constexpr int j = J.value;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[nt], f[mt], sx[mt], acc[mt][nt]);
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    auto stage = [&](auto P, int s) {
-      const int un = 4 * (s < last ? s + 1 : s);
-      begin(P, s);
-      products(std::integral_constant<int, 0>{}, f0);
-      frag(cur, 2, f0);
-      load_w(un, w[0]);
-      __builtin_amdgcn_sched_barrier(0);
-      products(std::integral_constant<int, 1>{}, f1);
-      frag(cur, 3, f1);
-      load_w(un + 1, w[1]);
-      __builtin_amdgcn_sched_barrier(0);
-      products(std::integral_constant<int, 2>{}, f0);
-      frag(nxt, 0, f0);
-      load_w(un + 2, w[2]);
-      __builtin_amdgcn_sched_barrier(0);
-      products(std::integral_constant<int, 3>{}, f1);
-      load_w(un + 3, w[3]);
-      take_scales();
-      load_scales(s + 2 < lastq ? s + 2 : lastq);
-      rotate();
-    };
-    for (int s0 = 0; s0 < nst; s0 += 2) {
-      stage(std::integral_constant<int, 0>{}, s0);
-      if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
+    for (int nt = 0; nt < NT; ++nt) b[nt] = mxfp4::bf16_of(w[j][nt][i], step_scale<j>(sc[nt]));
+  };
+  if constexpr (!A4) weights(std::integral_constant<int, 0>{}, sw[0], 0, b0);
+  for (;;) {
+    int id_next = id;
+    if constexpr (A4) {
+      id_next = id + static_cast<int>(gridDim.x) < total ? id + static_cast<int>(gridDim.x) : id;
+      block_of(id_next, mblocks, nblocks, mb_next, nb_next);
+      more = id_next != id;
     }
-  } else {
-    u32x4_t b0[NT], b1[NT];
-    auto weights = [&](auto J, const uint32_t (&sc)[NT], int i, u32x4_t (&b)[NT]) {
-      constexpr int j = J.value;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) b[nt] = mxfp4::bf16_of(w[j][nt][i], step_scale<j>(sc[nt]));
-    };
-    // Products of one operand, the conversion of the next spread among them.
-    auto products = [&](const u32x4_t (&f)[MT], const u32x4_t (&b)[NT]) {
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if constexpr (A4) {
+      auto products = [&](auto P, auto J, const u32x4_t (&f)[MT]) {
+        constexpr int j = J.value, p = P.value;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_bf16(b[nt], f[mt], acc[mt][nt]);
-      spread<MT * NT, 4 * NT + 1>();
-      __builtin_amdgcn_sched_barrier(0);
-    };
-    weights(std::integral_constant<int, 0>{}, sw, 0, b0);
-    auto stage = [&](auto J, int s) {
-      constexpr int j = J.value;
-      begin(std::integral_constant<int, j & 1>{}, s);
-      weights(J, sw, 1, b1);
-      products(f0, b0);
-      frag(cur, 2, f0);
-      __builtin_amdgcn_sched_barrier(0);
-      weights(J, sw, 2, b0);
-      products(f1, b1);
-      frag(cur, 3, f1);
-      __builtin_amdgcn_sched_barrier(0);
-      weights(J, sw, 3, b1);
-      products(f0, b0);
-      frag(nxt, 0, f0);
-      // the quad's tile of the next one: K is padded to whole quads
-      load_w(s - j + 4 <= 4 * lastq ? s + 4 : 4 * lastq + j, w[j]);
-      __builtin_amdgcn_sched_barrier(0);
-      if constexpr (j < 3) weights(std::integral_constant<int, (j + 1) & 3>{}, sw, 0, b0);
-      else weights(std::integral_constant<int, 0>{}, sw_next, 0, b0);
-      products(f1, b1);
-      rotate();
-    };
-    for (int s0 = 0; s0 < nst; s0 += 4) {
-      stage(std::integral_constant<int, 0>{}, s0);
-      if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
-      if (s0 + 2 < nst) stage(std::integral_constant<int, 2>{}, s0 + 2);
-      if (s0 + 3 < nst) stage(std::integral_constant<int, 3>{}, s0 + 3);
-      take_scales();
-      const int q = s0 / 4 + 2;
-      load_scales(q < lastq ? q : lastq);
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[p][nt], f[mt], sx[p][mt], acc[mt][nt]);
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto stage = [&](auto P, int s) {
+        if (s == last) weights_of(nb_next);
+        const int un = s < last ? 4 * (s + 1) : more ? 0 : 4 * last;
+        begin(P, s);
+        products(P, std::integral_constant<int, 0>{}, f0);
+        frag(cur, 2, f0);
+        load_w(un, w[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(P, std::integral_constant<int, 1>{}, f1);
+        frag(cur, 3, f1);
+        load_w(un + 1, w[1]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(P, std::integral_constant<int, 2>{}, f0);
+        frag(nxt, 0, f0);
+        load_w(un + 2, w[2]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(P, std::integral_constant<int, 3>{}, f1);
+        load_w(un + 3, w[3]);
+        scales_ahead(P, s + 2);
+        rotate();
+      };
+      for (int s0 = 0; s0 < nst; s0 += 2) {
+        stage(std::integral_constant<int, 0>{}, s0);
+        if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
+      }
+    } else {
+      // Products of one operand, the conversion of the next spread among them.
+      auto products = [&](const u32x4_t (&f)[MT], const u32x4_t (&b)[NT]) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_bf16(b[nt], f[mt], acc[mt][nt]);
+        spread<MT * NT, 4 * NT + 1>();
+        __builtin_amdgcn_sched_barrier(0);
+      };
+      auto stage = [&](auto P, auto J, int s) {   // P: the quad's parity, J: the stage in it
+        constexpr int j = J.value, p = P.value;
+        begin(std::integral_constant<int, j & 1>{}, s);
+        weights(J, sw[p], 1, b1);
+        products(f0, b0);
+        frag(cur, 2, f0);
+        __builtin_amdgcn_sched_barrier(0);
+        weights(J, sw[p], 2, b0);
+        products(f1, b1);
+        frag(cur, 3, f1);
+        __builtin_amdgcn_sched_barrier(0);
+        weights(J, sw[p], 3, b1);
+        products(f0, b0);
+        frag(nxt, 0, f0);
+        load_w(s - j < 4 * lastq ? s + 4 : 4 * lastq + j, w[j]);   // the next quad's: K is padded to whole ones
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (j < 3) weights(std::integral_constant<int, (j + 1) & 3>{}, sw[p], 0, b0);
+        else weights(std::integral_constant<int, 0>{}, sw[p ^ 1], 0, b0);
+        products(f1, b1);
+        rotate();
+      };
+      auto quad = [&](auto P, int s) {
+        stage(P, std::integral_constant<int, 0>{}, s);
+        if (s + 1 < nst) stage(P, std::integral_constant<int, 1>{}, s + 1);
+        if (s + 2 < nst) stage(P, std::integral_constant<int, 2>{}, s + 2);
+        if (s + 3 < nst) stage(P, std::integral_constant<int, 3>{}, s + 3);
+        scales_ahead(P, s / 4 + 2);
+      };
+      for (int s = 0; s < nst; s += 8) {
+        quad(kEven, s);
+        if (s + 4 < nst) quad(kOdd, s + 4);
+      }
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+      store_row<NT>(a, ((mb * WM + wm) * MT + mt) * 16 + l16, (nb * WN + wn) * NT, g, acc[mt]);
+    if (!more) return;
+    id = id_next;
+    mb = mb_next;
+    nb = nb_next;
   }
-#pragma unroll
-  for (int mt = 0; mt < MT; ++mt) store_row<NT>(a, m0 + mt * 16 + l16, t0, g, acc[mt]);
 }
 
 // Rows of X to packed 4-bit tiles.  A block is a tile, a wave its block g of 32 elements, four lanes a row of it.
@@ -674,7 +704,11 @@ template <bool A4, bool TAIL, int T>
 void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
   constexpr TileConfig c = kTiles[T];
   const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
-  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(blocks, p.ks), dim3(64 * c.wm * c.wn), 0, s, a);
+  // 4-bit rows: one block a CU, two of four waves, where a block's loads may run from one tile into the next.
+  const bool persistent = A4 && p.ks == 1 && a.kquads % 2 == 0 && a.kquads >= 4;
+  const unsigned slots = c.wm * c.wn == 4 ? 512 : 256;
+  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(persistent && blocks > slots ? slots : blocks, p.ks),
+                     dim3(64 * c.wm * c.wn), 0, s, a);
 }
 
 template <bool A4, bool TAIL>   // TAIL: K is not whole steps
@@ -714,13 +748,14 @@ void launch_product(const Plan& p, const Args& a, bool a4, hipStream_t s) {
   }
 }
 
+constexpr int kMaxRow = 1 << 22;    // elements from one row of X to the next: 160 rows' bytes are counted in 32 bits
 constexpr int kMaxRows = 1 << 19;   // the grids count row tiles in a dimension of 65535
 
 const char* shape_error(int M, int N, int K) {
   if (M < 0 || N < 0 || K < 0) return "negative size";
   if (K % mxfp4::kBlock || (K == 0 && M && N)) return "K must be a positive multiple of 32";
   if (M > kMaxRows) return "M must be at most 2^19";
-  if (N > (1 << 24) || K > (1 << 24)) return "N and K must be at most 2^24";
+  if (N > (1 << 24) || K > kMaxRow) return "N must be at most 2^24 and K at most 2^22";
   return nullptr;
 }
 
@@ -731,7 +766,7 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   if (!bad && M && N) {
     if (!x || !w || (!y && !partials)) bad = "null pointer";
     else if (!coopt::aligned16(x) || !coopt::aligned16(w)) bad = "x and w must be 16-byte aligned";
-    else if (ldx < K || ldx % 8) bad = "row stride of x must be >= K and a multiple of 8";
+    else if (ldx < K || ldx % 8 || ldx > kMaxRow) bad = "row stride of x must be >= K, a multiple of 8, at most 2^22";
     else if (!partials && (ldy < N || (reinterpret_cast<uintptr_t>(y) & 1))) bad = "row stride of y must be >= N";
     else if (partials && N % 32) bad = "partial sums need N a multiple of 32";
   }

@@ -388,7 +388,7 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
     if not x.is_contiguous():
         x = x.reshape(-1, K)
         ldx, along = x.stride()
-        if along != 1 or ldx % 8 or ldx < K:
+        if along != 1 or ldx % 8 or ldx < K or ldx > 1 << 22:   # (what the library refuses)
             x, ldx = x.contiguous(), K
     if x.data_ptr() % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), K

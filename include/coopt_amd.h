@@ -559,7 +559,8 @@ int coopt_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, 
  *     bytes) in the order the kernels load them; once a model load.  codes and out 16-byte aligned.
  *   coopt_mxfp4_linear: act4 = 0: x as it is (every weight is a bf16 number, products are those of bf16);
  *     act4 = 1: x is quantised first, as coopt_mxfp4_quantize does, and the 4-bit operands are multiplied.
- *     K a multiple of 32, N any, M up to 2^19; x rows 16-byte aligned (ldx a multiple of 8).
+ *     K a multiple of 32 up to 2^22, N up to 2^24, M up to 2^19; x rows 16-byte aligned (ldx a
+ *     multiple of 8, at most 2^22).
  *     workspace: coopt_mxfp4_linear_workspace(M, N, K, act4, 0) bytes (0: none), 16-byte aligned.
  *   coopt_mxfp4_linear_split / _partials: as coopt_linear_split / coopt_linear_partials: ks fp32 slices
  *     [rows_padded, N] at the workspace's start, whose sum in order is the output before its rounding.  N a

@@ -175,6 +175,23 @@ def test_products_of_integers_are_exact(dev, shape, activations):
 
 
 @pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("shape", [(1500, 9001, 2048), (1025, 18000, 1536), (2100, 8200, 3584), (700, 33000, 1024),
+                                   (1300, 16400, 2016)])
+def test_more_tiles_than_blocks(dev, shape, activations):
+    """Products of so many tiles that a block takes several, at lengths of an even and an odd number of quads, with a
+    ragged last tile on both sides.  Whole-number sums, as above; the reference is a product in 64 bits."""
+    m, N, K = shape
+    w, vals = make_weight(dev, N, K, m + N + K, activations, integers=True)
+    rng = np.random.default_rng(K)
+    x = rng.choice([-6, -4, -3, -2, -1, 0, 1, 2, 3, 4, 6], (m, K)).astype(np.float64)
+    x[:, ::32] = 6
+    assert K * 6 * 12 < 2 ** 24
+    xd = torch.from_numpy(x).to(dev)
+    want = torch.matmul(xd, torch.from_numpy(vals).to(dev).T.contiguous()).to(torch.bfloat16)
+    assert torch.equal(fused.linear(xd.to(torch.bfloat16), w), want)
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
 @pytest.mark.parametrize("shape", [(1, 4096, 4096), (7, 300, 1504), (32, 2048, 2048), (77, 1024, 14336),
                                    (160, 4096, 1024), (333, 512, 2080)])
 def test_products_of_values(dev, shape, activations):

@@ -57,7 +57,7 @@ def test_products_refuse(lib, partials):
     for kw, what in ((dict(K=200), "multiple of 32"), (dict(K=0), "multiple of 32"), (dict(M=-1), "negative"),
                      (dict(N=-4), "negative"), (dict(M=(1 << 19) + 1), "2^19"), (dict(N=(1 << 24) + 16), "2^24"),
                      (dict(x=None), "null"), (dict(w=None), "null"), (dict(x=8), "aligned"), (dict(w=8), "aligned"),
-                     (dict(ldx=255), "row stride of x"), (dict(ldx=260), "row stride of x")):
+                     (dict(K=(1 << 22) + 32), "2^22"), (dict(ldx=(1 << 22) + 8), "row stride of x"), (dict(K=(1 << 22) + 32), "2^22"), (dict(ldx=(1 << 22) + 8), "row stride of x"), (dict(ldx=255), "row stride of x"), (dict(ldx=260), "row stride of x")):
         assert what in refused(product(lib, partials, **kw)), kw
     if partials:
         assert "multiple of 32" in refused(product(lib, True, N=80))
