@@ -101,7 +101,8 @@ __global__ __launch_bounds__(kThreads) void mxfp4_pack_kernel(const uint8_t* __r
   }
 }
 
-bool blocks_fit(int64_t threads) { return (threads + kThreads - 1) / kThreads <= 0x7fffffff; }
+// A grid counts its threads in 32 bits.
+bool blocks_fit(int64_t threads) { return threads <= 0xffffffffll - kThreads; }
 
 dim3 grid_for(int64_t threads) { return dim3(static_cast<unsigned>((threads + kThreads - 1) / kThreads)); }
 

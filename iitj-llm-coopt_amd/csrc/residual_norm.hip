@@ -132,9 +132,21 @@ __global__ __launch_bounds__(64 * WAVES) void residual_norm_kernel(const Row a) 
   }
 }
 
+// A grid counts its threads in 32 bits: more rows than these go in several launches.
+constexpr int64_t kLaunchRows = 1 << 21;
+
 template <int WAVES, int CPT>
-void launch(const Row& a, int64_t rows, hipStream_t s) {
-  hipLaunchKernelGGL((residual_norm_kernel<WAVES, CPT>), dim3(static_cast<unsigned>(rows)), dim3(64 * WAVES), 0, s, a);
+void launch(Row a, int64_t rows, hipStream_t s) {
+  for (; rows > 0; rows -= kLaunchRows) {
+    const int64_t n = rows < kLaunchRows ? rows : kLaunchRows, past = n * a.H;
+    hipLaunchKernelGGL((residual_norm_kernel<WAVES, CPT>), dim3(static_cast<unsigned>(n)), dim3(64 * WAVES), 0, s, a);
+    if (a.x) a.x += past;
+    if (a.part) a.part += past;
+    if (a.gate) a.gate += n * a.gate_stride;
+    a.residual += past;
+    a.residual_out += past;
+    a.out += past;
+  }
 }
 
 constexpr int kMaxHidden = 16384;
@@ -146,7 +158,7 @@ extern "C" int coopt_residual_norm(const void* x, const float* part, int ks, int
                                    int64_t gate_stride, const void* weight, void* out, int64_t rows, int hidden,
                                    float eps, float branch_scale, float residual_scale, coopt_stream_t stream) {
   coopt::clear_error();
-  COOPT_REQUIRE(rows >= 0 && rows <= 0x7fffffff && hidden > 0 && hidden % 8 == 0 && hidden <= kMaxHidden,
+  COOPT_REQUIRE(rows >= 0 && rows <= (int64_t(1) << 40) && hidden > 0 && hidden % 8 == 0 && hidden <= kMaxHidden,
                 "hidden must be a multiple of 8, at most 16384");
   COOPT_REQUIRE(eps >= 0.0f && eps <= 3.0e38f, "eps must be finite and not negative");
   if (rows == 0) return COOPT_OK;

@@ -108,13 +108,16 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
 
     x [..., H] bf16 or the LinearPartials of the projection that made it (summed here), residual of its
     shape; gate [H], or of x's shape (rows may be strided); H a multiple of 8 up to 16384.  residual_out: where r
-    goes, by default into `residual`.  Returns out (a new tensor by default)."""
+    goes, by default into `residual`.  Returns out (a new tensor by default).  out may be x, residual (with another
+    residual_out) or a gate of x's shape itself, and overlaps no input otherwise; nor does residual_out."""
     part = x if type(x) is LinearPartials else None
     shape = x.shape
     H = shape[-1] if shape else 0
     index = residual.get_device()
     source = x if part is None else part.buf
     alike = index >= 0 and index == source.get_device() == weight.get_device()
+    if H > 16384:   # (the library takes 32 bits of it)
+        raise ValueError(f"rows of at most 16384 elements, got {H}")
     if part is None and (x.dtype is not torch.bfloat16 or not x.is_contiguous()):
         raise ValueError(f"x must be contiguous bf16 or LinearPartials, got {x.dtype} {tuple(shape)}")
     if residual.dtype is not torch.bfloat16 or residual.shape != shape or not residual.is_contiguous():
@@ -152,14 +155,16 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
         _lib.require_one_device(source, residual, weight, post_weight, gate, residual_out, out)
     if out is None:
         out = torch.empty_like(residual)
-    rp = residual.data_ptr()
+    rp, op = residual.data_ptr(), out.data_ptr()
+    sp = rp if residual_out is None else residual_out.data_ptr()
     rows = residual.numel() // H if H else 0
+    if op == sp and rows:
+        raise ValueError("out and residual_out are the same rows")
     rc = _lib.call_on(
         index, _lib.entry("coopt_residual_norm"), x.data_ptr() if part is None else 0,
         0 if part is None else source.data_ptr(), 0 if part is None else part.ks,
-        0 if part is None else part.rows_padded * part.n, rp, rp if residual_out is None else residual_out.data_ptr(),
-        pp, gp, gate_stride, weight.data_ptr(), out.data_ptr(), rows, H, eps, branch_scale, residual_scale,
-        _lib.raw_stream(index))
+        0 if part is None else part.rows_padded * part.n, rp, sp, pp, gp, gate_stride, weight.data_ptr(), op, rows, H, eps,
+        branch_scale, residual_scale, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "coopt_residual_norm")
     return out
@@ -319,7 +324,7 @@ def linear(x, weight, out=None, defer_reduce=False):
 
     `weight` may be an MXFP4Weight (K a multiple of 32, any N and row count): coopt_mxfp4_linear, with
     bf16 rows or, where the weight says activations "mxfp4", rows quantised to 4 bits in the call.
-    defer_reduce returns LinearPartials where K is split."""
+    defer_reduce returns LinearPartials where K is split (in memory of their own).  out overlaps no input."""
     if type(weight) is MXFP4Weight:
         return _linear_mxfp4(x, weight, out, defer_reduce)
     packed = weight.packed if isinstance(weight, PackedWeight) and not weight.gate_up else None
@@ -392,7 +397,7 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
             x, ldx = x.contiguous(), K
     if x.data_ptr() % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), K
-    if M == 0:
+    if M == 0 or N == 0:
         return x.new_empty((*lead, N)) if out is None else out
     need, ks, rows_padded, need_partials = weight.plan(M)
     partials = defer_reduce and out is None and ks > 1
@@ -401,9 +406,9 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
     if not need:
         wsp = have = 0
         lock = _NO_LOCK
-    elif torch.cuda.is_current_stream_capturing():
-        # a graph under capture gets a workspace of its own (from its memory pool), so that two graphs captured
-        # on one stream may replay at the same time
+    elif partials or torch.cuda.is_current_stream_capturing():
+        # partial sums live as long as their LinearPartials; a graph under capture gets a workspace of its own
+        # (from its memory pool), so that two graphs captured on one stream may replay at the same time
         ws, lock = x.new_empty((need,), dtype=torch.uint8), _NO_LOCK
         wsp, have = ws.data_ptr(), need
     else:
@@ -415,7 +420,9 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
             out = x.new_empty(M, N) if len(lead) == 1 else x.new_empty((*lead, N))
         y = out if out.dim() == 2 else out.view(-1, N)
         yp, ldy = y.data_ptr(), y.stride(0)
-        if ldy < N:   # one row
+        if ldy < N:
+            if M > 1:
+                raise ValueError(f"out's rows overlap: {ldy} apart")
             ldy = N
     with lock:
         if wsp is None:

@@ -20,6 +20,7 @@ __all__ = ["quantize_mxfp4", "dequantize_mxfp4", "MXFP4Weight", "pack_mxfp4_weig
            "quantize_mxfp4_weight"]
 
 BLOCK = 32
+MAX_ROWS, MAX_N, MAX_K = 1 << 19, 1 << 24, 1 << 22   # of a product
 
 
 def _aligned(t, nbytes):
@@ -41,8 +42,8 @@ def quantize_mxfp4(x: torch.Tensor):
         raise ValueError(f"x must be bf16, fp16 or fp32, got {x.dtype}")
     shape = x.shape
     K = shape[-1] if shape else 1
-    if K % BLOCK:
-        raise ValueError(f"the last dimension must be a multiple of {BLOCK}, got {tuple(shape)}")
+    if K % BLOCK or K >> 31:
+        raise ValueError(f"the last dimension must be a multiple of {BLOCK} below 2^31, got {tuple(shape)}")
     if not x.is_contiguous() or x.data_ptr() % 16:
         x = _aligned(x, 16)
     lead = shape[:-1]
@@ -61,6 +62,8 @@ def _check_rows(codes, scales):
         raise ValueError("codes and scales must be uint8")
     if not cs or len(ss) != len(cs) or cs[:-1] != ss[:-1] or cs[-1] != ss[-1] * (BLOCK // 2):
         raise ValueError(f"codes [..., K / 2] and scales [..., K / {BLOCK}] disagree: {tuple(cs)}, {tuple(ss)}")
+    if cs[-1] >> 30:
+        raise ValueError(f"rows of less than 2^31 elements, got {2 * cs[-1]}")
     return 2 * cs[-1]
 
 
@@ -86,7 +89,8 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bflo
 
 class MXFP4Weight:
     """A projection weight [N, K] in microscaled 4 bits: `codes` and `scales` as they were given, and
-    `packed`, the copy that fused.linear streams (coopt_mxfp4_pack_weight's layout).
+    `packed`, the copy that fused.linear streams (coopt_mxfp4_pack_weight's layout; it does not see
+    later changes of the codes).
 
     activations "bf16": products with the rows as they are.  "mxfp4": rows are quantised to 4 bits in the call and
     both operands go to the scaled matrix instructions (4 bits by 4 bits)."""
@@ -102,6 +106,8 @@ class MXFP4Weight:
         product of `rows` rows."""
         p = self._plans.get(rows)
         if p is None:
+            if rows > MAX_ROWS:
+                raise ValueError(f"at most {MAX_ROWS} rows, got {rows}")
             lib, (N, K) = _lib.load(), self.shape
             ks, padded = ctypes.c_int(0), ctypes.c_int(0)
             _lib.check(lib.coopt_mxfp4_linear_split(rows, N, K, self.act4, ctypes.byref(ks), ctypes.byref(padded)),
@@ -138,6 +144,8 @@ def pack_mxfp4_weight(codes, scales, activations="bf16"):
         raise ValueError(f"codes must be [N, K / 2], got {tuple(codes.shape)}")
     K = _check_rows(codes, scales)
     N = codes.shape[0]
+    if N > MAX_N or K > MAX_K:
+        raise ValueError(f"a weight of at most {MAX_N} x {MAX_K}, got {N} x {K}")
     cc, sc = _aligned(codes, 16), scales.contiguous()
     nbytes = int(_lib.entry("coopt_mxfp4_packed_bytes")(N, K))
     packed = cc.new_empty(nbytes)

@@ -281,6 +281,98 @@ def test_streams_graphs_and_repeats(dev, activations):
             assert torch.equal(out, fused.linear(x, w)), i
 
 
+def small_numbers(dev, shape, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return torch.randint(-2, 3, shape, generator=g, device=dev).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_offsets_past_32_bits(dev, activations):
+    """Weights of more than 4 GB, rows and outputs that lie more than 4 GB behind the first.  Whole numbers, so that
+    a product of the last part alone has to give the same bits."""
+    g = torch.Generator(device=dev).manual_seed(1)
+    N, K, part = (1 << 21) + 64, 4224, 4160
+    codes = torch.randint(0, 256, (N, K // 2), generator=g, device=dev, dtype=torch.uint8)
+    scales = torch.full((N, K // 32), 127, device=dev, dtype=torch.uint8)
+    whole = M.pack_mxfp4_weight(codes, scales, activations)
+    end = M.pack_mxfp4_weight(codes[-part:].contiguous(), scales[-part:].contiguous(), activations)
+    for m in (1, 20, 70):
+        x = small_numbers(dev, (m, K), m)
+        assert torch.equal(fused.linear(x, whole)[:, -part:], fused.linear(x, end))
+    del whole, codes, scales
+    # rows 2^22 elements apart, and farther
+    for apart, m in ((1 << 22, 600), ((1 << 22) + 8, 600), (1 << 22, 40)):
+        wide = torch.empty((m, apart), device=dev, dtype=torch.bfloat16)
+        x = small_numbers(dev, (m, K), m)
+        wide[:, 64:64 + K] = x
+        assert torch.equal(fused.linear(wide[:, 64:64 + K], end), fused.linear(x, end))
+        del wide
+    # 2^19 rows of outputs of more than 8 GB
+    w, _ = make_weight(dev, 8200, 64, 1, activations, integers=True)
+    x = small_numbers(dev, (1 << 19, 64), 2)
+    y = fused.linear(x, w)
+    for rows in (slice(0, 300), slice((1 << 18) - 100, (1 << 18) + 100), slice((1 << 19) - 300, None)):
+        assert torch.equal(y[rows], fused.linear(x[rows], w))
+    with pytest.raises(ValueError, match="524288 rows"):
+        fused.linear(torch.empty(1, 64, device=dev, dtype=torch.bfloat16).expand((1 << 19) + 1, 64), w)
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_deferred_sums_live_on(dev, activations):
+    """The sums of one product stay while others run, and every consumer takes them."""
+    w, _ = make_weight(dev, 1024, 14336, 5, activations, integers=True)
+    xs = [small_numbers(dev, (77, 14336), i) for i in range(3)]
+    parts = [fused.linear(x, w, defer_reduce=True) for x in xs]
+    assert all(isinstance(p, fused.LinearPartials) for p in parts)
+    full = [fused.linear(x, w) for x in xs]
+    for p, y in zip(parts, full):
+        assert torch.equal(p.reduce(), y)
+        assert torch.equal(fused.silu_and_mul(p), fused.silu_and_mul(y))
+        norm = torch.ones(1024, device=dev, dtype=torch.bfloat16)
+        assert torch.equal(fused.rms_norm(p, norm, 1e-5), fused.rms_norm(y, norm, 1e-5))
+        assert torch.equal(fused.residual_norm(p, y.clone(), norm, 1e-5), fused.residual_norm(y, y.clone(), norm, 1e-5))
+    assert torch.equal(fused.linear_silu(xs[0], w), fused.silu_and_mul(full[0]))
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+def test_threads_on_one_stream(dev, activations):
+    """Two threads' products on one stream: each gets its own."""
+    import threading
+    w, _ = make_weight(dev, 4096, 4096, 6, activations, integers=True)
+    xs = [small_numbers(dev, (m, 4096), m) for m in (20, 70)]
+    want = [fused.linear(x, w) for x in xs]
+    wrong = []
+
+    def work(x, y):
+        for _ in range(100):
+            if not torch.equal(fused.linear(x, w), y):
+                wrong.append(x.shape)
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+def test_products_refuse_outputs(dev):
+    w, _ = make_weight(dev, 64, 128, 7)
+    x = small_numbers(dev, (4, 128), 7)
+    one = torch.zeros(1, 64, device=dev, dtype=torch.bfloat16)
+    flat = torch.zeros(4 * 64, device=dev, dtype=torch.bfloat16)
+    for out in (one.expand(4, 64), flat.as_strided((4, 64), (32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            fused.linear(x, w, out=out)
+    for out in (one, flat, one.float().expand(4, 64), flat.view(64, 4).T):
+        with pytest.raises(ValueError, match="out must be"):
+            fused.linear(x, w, out=out)
+    assert (one == 0).all() and (flat == 0).all()
+    assert fused.linear(x[:1], w, out=one) is one and torch.equal(one, fused.linear(x, w)[:1])
+    none = M.pack_mxfp4_weight(w.codes[:0], w.scales[:0])
+    assert fused.linear(x, none).shape == (4, 0)
+
+
 def test_weight_helpers(dev):
     w0 = (0.02 * torch.randn(96, 256, device=dev)).to(torch.bfloat16)
     w = M.quantize_mxfp4_weight(w0, "mxfp4")

@@ -118,3 +118,37 @@ def test_graph_replays(dev):
         new = torch.empty_like(start)
         want = fused.residual_norm(x, start, weight, 1e-5, pw, gv, 0.5, residual_out=new)
         assert torch.equal(out, want) and torch.equal(residual, new), i
+
+
+def test_more_rows_than_a_launch(dev):
+    """Past 2^21 rows the work goes in several launches: the same bits as of the rows alone."""
+    T, H = (1 << 21) + 5, 8
+    x, residual, weight, pw, gate = inputs(dev, T, H, "token", True)
+    new = torch.empty_like(residual)
+    got = fused.residual_norm(x, residual, weight, 1e-5, pw, gate, residual_out=new)
+    for rows in (slice(0, 100), slice((1 << 21) - 50, None)):
+        r = torch.empty_like(residual[rows])
+        o = fused.residual_norm(x[rows], residual[rows], weight, 1e-5, pw, gate[rows], residual_out=r)
+        assert torch.equal(o, got[rows]) and torch.equal(r, new[rows])
+
+
+def test_results_over_inputs(dev):
+    """out in the place of x, of the residual or of the gate, residual_out in that of x; both in one place are refused."""
+    x, residual, weight, pw, gate = inputs(dev, 9, 520, "token", True)
+    new = torch.empty_like(residual)
+    want = fused.residual_norm(x, residual, weight, 1e-5, pw, gate, residual_out=new)
+    for name in ("x", "gate", "residual"):
+        a = dict(x=x.clone(), residual=residual.clone(), gate=gate.clone())
+        other = torch.empty_like(residual)
+        fused.residual_norm(a["x"], a["residual"], weight, 1e-5, pw, a["gate"], residual_out=other, out=a[name])
+        assert torch.equal(a[name], want) and torch.equal(other, new)
+    a = x.clone()
+    assert torch.equal(fused.residual_norm(a, residual, weight, 1e-5, pw, gate, residual_out=a), want)
+    assert torch.equal(a, new)
+    before = residual.clone()
+    with pytest.raises(ValueError, match="same rows"):
+        fused.residual_norm(x, residual, weight, 1e-5, pw, gate, out=residual)
+    with pytest.raises(ValueError, match="16384"):
+        wide = torch.zeros(1, 16392, device=dev, dtype=torch.bfloat16)
+        fused.residual_norm(wide, wide.clone(), wide[0], 1e-5)
+    assert torch.equal(residual, before)

@@ -22,7 +22,8 @@ def test_codec_refuses(lib):
     for args, what in (((_lib.DT_I8, 16, 1, 32, 16, 16), "in_dtype"), ((_lib.DT_BF16, 16, 1, 48, 16, 16), "multiple of 32"),
                        ((_lib.DT_BF16, 16, -1, 32, 16, 16), "multiple of 32"), ((_lib.DT_BF16, 16, 1, -32, 16, 16), "multiple of 32"),
                        ((_lib.DT_BF16, None, 1, 32, 16, 16), "null"), ((_lib.DT_BF16, 8, 1, 32, 16, 16), "aligned"),
-                       ((_lib.DT_BF16, 16, 1, 32, 18, 16), "aligned"), ((_lib.DT_BF16, 16, 1 << 38, 32, 16, 16), "too large")):
+                       ((_lib.DT_BF16, 16, 1, 32, 18, 16), "aligned"), ((_lib.DT_BF16, 16, 1 << 38, 32, 16, 16), "too large"),
+                       ((_lib.DT_BF16, 16, 1 << 28, 128, 16, 16), "too large")):
         assert what in refused(q(*args, None)), args
     for args, what in (((16, 16, 1, 32, _lib.DT_I8, 16), "out_dtype"), ((16, 16, 1, 33, _lib.DT_F32, 16), "multiple of 32"),
                        ((16, None, 1, 32, _lib.DT_F32, 16), "null"), ((18, 16, 1, 32, _lib.DT_F32, 16), "aligned"),
@@ -57,7 +58,8 @@ def test_products_refuse(lib, partials):
     for kw, what in ((dict(K=200), "multiple of 32"), (dict(K=0), "multiple of 32"), (dict(M=-1), "negative"),
                      (dict(N=-4), "negative"), (dict(M=(1 << 19) + 1), "2^19"), (dict(N=(1 << 24) + 16), "2^24"),
                      (dict(x=None), "null"), (dict(w=None), "null"), (dict(x=8), "aligned"), (dict(w=8), "aligned"),
-                     (dict(K=(1 << 22) + 32), "2^22"), (dict(ldx=(1 << 22) + 8), "row stride of x"), (dict(K=(1 << 22) + 32), "2^22"), (dict(ldx=(1 << 22) + 8), "row stride of x"), (dict(ldx=255), "row stride of x"), (dict(ldx=260), "row stride of x")):
+                     (dict(K=(1 << 22) + 32), "2^22"), (dict(ldx=(1 << 22) + 8), "row stride of x"),
+                     (dict(ldx=255), "row stride of x"), (dict(ldx=260), "row stride of x")):
         assert what in refused(product(lib, partials, **kw)), kw
     if partials:
         assert "multiple of 32" in refused(product(lib, True, N=80))
