@@ -59,6 +59,13 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2_t{lo, hi}), mxfp4::bf16x2_t));
 }
 
+// A wave-uniform offset that stays in a scalar register: otherwise the compiler turns base + offset + lane into
+// a running address a lane of each tile, in vector registers that the products need.
+__device__ __forceinline__ uint32_t scalar(uint32_t off) {
+  asm("" : "+s"(off));
+  return off;
+}
+
 template <int J>
 __device__ __forceinline__ float step_scale(uint32_t quad) {
   return mxfp4::scale_operand((quad >> (8 * J)) & 255u);
@@ -273,6 +280,8 @@ __device__ __forceinline__ void spread() {
 // a row's 16 chunks touches each bank once with any key.
 __device__ __forceinline__ int chunk_key(int r) { return (r >> 2) ^ ((r & 3) << 2); }
 
+constexpr int kMostTiles = 10;   // row tiles of a block of 4-bit rows, at most
+
 // Many rows: a block has WM x WN waves, a wave MT x NT tiles of 16 x 16.  gridDim.y blocks split K.
 //
 // K goes in stages: 128 elements of bf16 rows, a quad of 512 of 4-bit ones, 4 KB of LDS a row tile in both, and four
@@ -284,11 +293,15 @@ __device__ __forceinline__ int chunk_key(int r) { return (r >> 2) ^ ((r & 3) << 
 //
 // With 4-bit rows a block takes the tiles blockIdx.x, blockIdx.x + gridDim.x, ... .  Loads run into the next tile (its
 // first stages behind this one's last), so that between tiles nothing waits but the stores: 4093 x 28672 x 4096, 14
-// tiles a CU, takes 304 us (3.2 PFLOP/s), 347 with a block for each tile.  The launch gives a block more than one only
-// where stages come in pairs, four or more.  (bf16 rows: the addresses of a next tile do not fit beside the operands of
-// the widest tile.)
+// tiles a CU, took 304 us for 347 with a block for each tile, and takes 285 now (3.4 PFLOP/s).  The launch gives a block
+// more than one only where stages come in pairs, four or more.  (bf16 rows: the addresses of a next tile do not fit
+// beside the operands of the widest tile.)
 //   LDS: bf16 rows of 256 bytes, 16-byte chunk c of row r at place c ^ chunk_key(r % 16); 4-bit tiles as they are.
 // Two waves a SIMD at least: above 256 registers a CU holds one four-wave block, 394 us there for 327.
+//
+// Scalar addresses: the tiles of a wave, or of a block's X, lie one row of tiles apart, so that a load costs two scalar
+// additions (ten operations where each tile had its own bound: 294 us for 285 on the same).  The packed rows are
+// therefore followed by room for what the last block reads past them.
 template <bool A4, bool TAIL, int MT, int NT, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args a) {
   constexpr int kThreads = 64 * WM * WN;
@@ -296,6 +309,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   constexpr int kChunks = kTiles * 256;                // 16-byte chunks of X in a stage
   constexpr int kRounds = (kChunks + kThreads - 1) / kThreads;
   static_assert(WM * WN % 4 == 0, "a wave's chunks of 4-bit rows lie in one tile");
+  static_assert(!A4 || (kChunks % kThreads == 0 && kTiles <= kMostTiles), "4-bit rows are read in whole tiles, up to the padding");
   constexpr int kBuf = kRounds * kThreads;
   __shared__ u32x4_t xs[3 * kBuf];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -305,30 +319,34 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   const int total = mblocks * nblocks;
   int id = blockIdx.x, mb, nb;
   block_of(id, mblocks, nblocks, mb, nb);
-  const int ntiles = (a.N + 31) / 32 * 2, mtiles = (a.M + 15) / 16;
+  const int ntiles = (a.N + 31) / 32 * 2;
   const int qbeg = blockIdx.y * a.slice_quads;
   const int qend = qbeg + a.slice_quads < a.kquads ? qbeg + a.slice_quads : a.kquads;
   const int ksteps = (a.K + kStep - 1) / kStep;
   const int nsteps = (4 * qend < ksteps ? 4 * qend : ksteps) - 4 * qbeg;
   const int nst = A4 ? qend - qbeg : nsteps, last = nst - 1;
 
-  // Where the loads are: each of these moves to the next tile as its own run ahead passes this tile's last stage.
-  // (First tiles in scalar registers, addresses formed at each load: as pointers they took the registers of the tiles.)
-  int w_tile, sw_tile, sx_tile, x_tile;
+  // Where the loads are, at the first of the tiles; each of these moves to the next tile as its own run ahead passes
+  // this tile's last stage.
+  const uint8_t *w_at, *sw_at, *sx_at, *x_at;
+  const uint32_t row_bytes = a.kquads * (4 * kTile), scale_bytes = a.kquads * 256;   // from a tile to the next
   const uint16_t* x_base;                  // bf16: the tile's first row; the thread's chunks of X (round r, chunk id
   uint32_t x_off[kRounds];                 // r * kThreads + threadIdx.x) in bytes behind it: at most 160 rows of 2^22
   const int xk = (threadIdx.x & 15) * 8;   // and their first element within a step
-  auto tile_at = [&](const uint8_t* base, int t, int tiles, int bytes) {   // tiles past the last: computed, not stored
-    return base + (static_cast<int64_t>(t < tiles ? t : tiles - 1) * a.kquads + qbeg) * bytes;
+  static_assert(NT <= 2 && (NT == 2 || !A4), "a wave's weight tiles are all of the weight or none");
+  auto first_tile = [&](int nb) {          // tiles past the weight: the last ones instead, computed and not stored
+    const int t = (nb * WN + wn) * NT;
+    return t < ntiles ? t : ntiles - NT;
   };
-  auto weights_of = [&](int nb) { w_tile = (nb * WN + wn) * NT; };
+  auto weights_of = [&](int nb) { w_at = a.w + (static_cast<int64_t>(first_tile(nb)) * a.kquads + qbeg) * (4 * kTile); };
   auto scales_of = [&](int mb, int nb) {
-    sw_tile = (nb * WN + wn) * NT;
-    sx_tile = (mb * WM + wm) * MT;
+    sw_at = reinterpret_cast<const uint8_t*>(a.ws) + (static_cast<int64_t>(first_tile(nb)) * a.kquads + qbeg) * 256;
+    if constexpr (A4)
+      sx_at = reinterpret_cast<const uint8_t*>(a.xs) + (static_cast<int64_t>((mb * WM + wm) * MT) * a.kquads + qbeg) * 256;
   };
   auto rows_of = [&](int mb) {
-    if constexpr (A4) {
-      x_tile = mb * kTiles;
+    if constexpr (A4) {                    // a wave's chunks of a round lie in one tile
+      x_at = a.xt + (static_cast<int64_t>(mb * kTiles + wave / 4) * a.kquads + qbeg) * (4 * kTile);
     } else {
       const int m0 = mb * kTiles * 16;
       x_base = a.x + static_cast<int64_t>(m0) * a.ldx + qbeg * kQuad;
@@ -350,10 +368,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   auto load_x = [&](int s, u32x4_t (&v)[kRounds]) {
     s = s < last ? s : last;               // stages past the last repeat it, so that no load is conditional
     if constexpr (A4) {
+      const uint8_t* at = x_at + scalar(s * (4 * kTile));
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) {  // the wave's chunks lie in one tile
-        const uint8_t* t = tile_at(a.xt, x_tile + (r * WM * WN + wave) / 4, mtiles, 4 * kTile);
-        v[r] = reinterpret_cast<const u32x4_t*>(t + static_cast<int64_t>(s) * (4 * kTile))[threadIdx.x & 255];
+      for (int r = 0; r < kRounds; ++r) {
+        v[r] = reinterpret_cast<const u32x4_t*>(at)[threadIdx.x & 255];
+        at += WM * WN / 4 * row_bytes;
       }
     } else {
       const uint8_t* at = reinterpret_cast<const uint8_t*>(x_base + s * kStep);
@@ -379,24 +398,31 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   };
   u32x4_t w[4][NT];                        // bf16: stages s .. s + 3; 4-bit: the stage's four steps
   auto load_w = [&](int u, u32x4_t (&v)[NT]) {
+    const uint8_t* at = w_at + scalar(u * kTile);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      v[nt] = reinterpret_cast<const u32x4_t*>(tile_at(a.w, w_tile + nt, ntiles, 4 * kTile) + static_cast<int64_t>(u) * kTile)[lane];
+    for (int nt = 0; nt < NT; ++nt) {
+      v[nt] = reinterpret_cast<const u32x4_t*>(at)[lane];
+      at += row_bytes;
+    }
   };
   // Scales of even and odd quads: a register that is copied waits for its load, and that for all loads before it.
   uint32_t sw[2][NT], sx[2][MT];
   const int lastq = qend - qbeg - 1;
   auto load_scales = [&](auto P, int q) {
-    q = q < lastq ? q : lastq;
+    const uint32_t off = scalar((q < lastq ? q : lastq) * 256);
+    const uint8_t* at = sw_at + off;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      sw[P.value][nt] = reinterpret_cast<const uint32_t*>(
-          tile_at(reinterpret_cast<const uint8_t*>(a.ws), sw_tile + nt, ntiles, 256) + q * 256)[lane];
+    for (int nt = 0; nt < NT; ++nt) {
+      sw[P.value][nt] = reinterpret_cast<const uint32_t*>(at)[lane];
+      at += scale_bytes;
+    }
     if constexpr (A4) {
+      at = sx_at + off;
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-        sx[P.value][mt] = reinterpret_cast<const uint32_t*>(
-            tile_at(reinterpret_cast<const uint8_t*>(a.xs), sx_tile + mt, mtiles, 256) + q * 256)[lane];
+      for (int mt = 0; mt < MT; ++mt) {
+        sx[P.value][mt] = reinterpret_cast<const uint32_t*>(at)[lane];
+        at += scale_bytes;
+      }
     }
   };
   constexpr std::integral_constant<int, 0> kEven{};
@@ -675,6 +701,9 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   return p;
 }
 
+// Row tiles of the packed X: what a tile kernel's last block reads past them is in the workspace, and not stored.
+int64_t x_tiles(const Plan& p) { return p.rows_padded / 16 + (p.stream ? 0 : kMostTiles - 1); }
+
 int64_t part_bytes(const Plan& p, bool partials) {
   return p.ks > 1 || partials ? int64_t{4} * p.ks * p.rows_padded * p.pitch : 0;
 }
@@ -777,7 +806,7 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   if (M == 0 || N == 0) return COOPT_OK;
   const Plan p = plan_for(M, N, K, act4 != 0, partials);
   const bool pack = act4 && p.x != kQuantize;
-  const int64_t pb = part_bytes(p, partials), need = pb + (pack ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0);
+  const int64_t pb = part_bytes(p, partials), need = pb + (pack ? mxfp4::packed_bytes(x_tiles(p), K) : 0);
   if (need && (static_cast<int64_t>(workspace_bytes) < need || !workspace || !coopt::aligned16(workspace))) {
     coopt::set_error(std::string(who) + ": workspace smaller than required (or misaligned)");
     return COOPT_EWORKSPACE;
@@ -798,7 +827,7 @@ int run(const void* x, int64_t ldx, const void* w, int M, int N, int K, int act4
   a.pitch = p.pitch;
   if (pack) {
     uint8_t* tiles = static_cast<uint8_t*>(workspace) + pb;
-    uint8_t* scales = tiles + mxfp4::tile_bytes(mxfp4::row_tiles(M), K);
+    uint8_t* scales = tiles + mxfp4::tile_bytes(x_tiles(p), K);
     a.xt = tiles;
     a.xs = reinterpret_cast<const uint32_t*>(scales);
     hipLaunchKernelGGL(mxfp4_pack_rows_kernel, dim3(4 * a.kquads, static_cast<unsigned>(mxfp4::row_tiles(M))), dim3(256), 0, s,
@@ -819,7 +848,7 @@ extern "C" size_t coopt_mxfp4_linear_workspace(int M, int N, int K, int act4, in
   if (shape_error(M, N, K) || M == 0 || N == 0) return 0;
   const Plan p = plan_for(M, N, K, act4 != 0, partials != 0);
   return static_cast<size_t>(part_bytes(p, partials != 0) +
-                             (act4 && p.x != kQuantize ? mxfp4::packed_bytes(mxfp4::row_tiles(M), K) : 0));
+                             (act4 && p.x != kQuantize ? mxfp4::packed_bytes(x_tiles(p), K) : 0));
 }
 
 extern "C" int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, int* rows_padded) {
