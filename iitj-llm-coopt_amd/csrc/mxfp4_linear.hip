@@ -62,6 +62,7 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 // A wave-uniform offset that stays in a scalar register: otherwise the compiler turns base + offset + lane into
 // a running address a lane of each tile, in vector registers that the products need.
 __device__ __forceinline__ uint32_t scalar(uint32_t off) {
+  off = __builtin_amdgcn_readfirstlane(off);
   asm("" : "+s"(off));
   return off;
 }
@@ -263,15 +264,20 @@ __global__ __launch_bounds__(64 * KW) void mxfp4_stream_kernel(const Args a) {
   }
 }
 
-// Between two scheduling barriers: MFMAS products with the CVTS conversions spread among them.
-template <int MFMAS, int CVTS>
+// Between two scheduling barriers: MFMAS products with VALUS conversions, READS and WRITES of LDS and LOADS of global
+// memory spread among them, reads with the first products (they are needed first), the rest with the last.
+template <int MFMAS, int VALUS, int READS, int WRITES, int LOADS>
 __device__ __forceinline__ void spread() {
-  constexpr int kEach = (CVTS + MFMAS - 1) / MFMAS;
 #pragma unroll
   for (int i = 0; i < MFMAS; ++i) {
+    auto share = [&](int n) { return (i + 1) * n / MFMAS - i * n / MFMAS; };
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-    __builtin_amdgcn_sched_group_barrier(0x002, kEach, 0);
+    if (i < READS) __builtin_amdgcn_sched_group_barrier(0x100, (READS + MFMAS - 1) / MFMAS, 0);
+    if (VALUS) __builtin_amdgcn_sched_group_barrier(0x002, (VALUS + MFMAS - 1) / MFMAS, 0);
+    if (share(WRITES)) __builtin_amdgcn_sched_group_barrier(0x200, 1, 0);
+    if (share(LOADS)) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
   }
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // 16-byte reads of a wave go to the 64 LDS banks in four groups of lanes, of which the first is 0-3, 12-15 and
@@ -289,7 +295,9 @@ constexpr int kMostTiles = 10;   // row tiles of a block of 4-bit rows, at most
 // barrier, stage s + 2 is stored (loaded from global memory since stage s - 2) and s + 1 is complete, so
 // that the first operand of s + 1 is read before the next barrier and the matrix cores have work on both sides of
 // it.  Every wave loads its weight tiles straight into registers, 512 elements ahead, and with bf16 rows converts
-// an operand while the one before it is multiplied.
+// an operand while the one before it is multiplied.  LDS reads and stores, loads and conversions lie among the
+// products (spread): with those of X together behind the barrier, no wave multiplied meanwhile, 41 us for 38.7 at
+// 160 x 28672 x 4096, 165 for 162 at 2000 x 4096 x 14336 (1.45 PFLOP/s).
 //
 // With 4-bit rows a block takes the tiles blockIdx.x, blockIdx.x + gridDim.x, ... .  Loads run into the next tile (its
 // first stages behind this one's last), so that between tiles nothing waits but the stores: 4093 x 28672 x 4096, 14
@@ -324,7 +332,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   const int qend = qbeg + a.slice_quads < a.kquads ? qbeg + a.slice_quads : a.kquads;
   const int ksteps = (a.K + kStep - 1) / kStep;
   const int nsteps = (4 * qend < ksteps ? 4 * qend : ksteps) - 4 * qbeg;
-  const int nst = A4 ? qend - qbeg : nsteps, last = nst - 1;
+  const int last = (A4 ? qend - qbeg : nsteps) - 1;
+  // Whole quads, zeros behind the last step: stages that may be skipped are waited for as if they had been (widest
+  // tile 716 us for 669 at 4093 x 28672 x 4096).  With the zeros' own test the widest tile spills, and skips.
+  constexpr bool kWhole = !A4 && (!TAIL || MT * NT <= 10);
+  const int nst = kWhole ? 4 * (qend - qbeg) : last + 1;
 
   // Where the loads are, at the first of the tiles; each of these moves to the next tile as its own run ahead passes
   // this tile's last stage.
@@ -375,19 +387,23 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
         at += WM * WN / 4 * row_bytes;
       }
     } else {
-      const uint8_t* at = reinterpret_cast<const uint8_t*>(x_base + s * kStep);
+      const uint8_t* at = reinterpret_cast<const uint8_t*>(x_base) + scalar(2 * s * kStep);
       const uint32_t back = TAIL && s == last ? past : 0;   // of the chunk's own 2 * xk
 #pragma unroll
-      for (int r = 0; r < kRounds; ++r) v[r] = *reinterpret_cast<const u32x4_t*>(at + (x_off[r] - back));
+      for (int r = 0; r < kRounds; ++r) {
+        asm volatile("" : "+v"(x_off[r]));   // 32 bits beside a scalar base: extended outside the loop it would be 64
+        v[r] = *reinterpret_cast<const u32x4_t*>(at + (x_off[r] - back));
+      }
     }
   };
+  static_assert(kThreads % 256 == 0, "a thread's chunks have one key");
+  const int place = A4 ? threadIdx.x : (threadIdx.x & ~15) | ((threadIdx.x & 15) ^ chunk_key((threadIdx.x >> 4) & 15));
   auto store_x = [&](int s, int buf, const u32x4_t (&v)[kRounds]) {
 #pragma unroll
     for (int r = 0; r < kRounds; ++r) {
-      const int c = r * kThreads + threadIdx.x;
       u32x4_t t = v[r];
-      if (TAIL && s >= last && past) t = u32x4_t{0, 0, 0, 0};   // (with one tile only)
-      xs[buf + (A4 ? c : (c & ~15) | ((c & 15) ^ chunk_key((c >> 4) & 15)))] = t;
+      if (TAIL && (s > last || (s == last && past))) t = u32x4_t{0, 0, 0, 0};
+      xs[buf + r * kThreads + place] = t;
     }
   };
   const int key = chunk_key(l16);
@@ -442,7 +458,6 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
     __builtin_amdgcn_sched_barrier(0);
     store_x(0, 0, xa);
     store_x(1, kBuf, xb);
-    load_scales(kOdd, 1);
   }
   __syncthreads();
   u32x4_t f0[MT], f1[MT];
@@ -454,21 +469,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
     nxt = far;
     far = t;
   };
-  // What is common to a stage's begin: its barrier, the operand behind the one in hand, X of later stages.
   int mb_next, nb_next;               // the next tile, if there is one
   bool more = false;
-  auto begin = [&](auto P, int s) {   // P: s % 2
-    __syncthreads();
-    frag(cur, 1, f1);
-    store_x(s + 2, far, xq[P.value]);
-    if (A4 && P.value == 0 && s + 4 == nst) rows_of(mb_next);   // (stages come in pairs where there is a next tile)
+  // X of stage s + 4, of this tile or the next (stages come in pairs where there is one).
+  auto rows_ahead = [&](auto P, int s) {   // P: s % 2
+    if (A4 && P.value == 0 && s + 4 == nst) rows_of(mb_next);
     load_x(s + 4 < nst || !more ? s + 4 : s + 4 - nst, xq[P.value]);
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  // The scales of quad q of this tile, or of the next one's first two.
-  auto scales_ahead = [&](auto P, int q) {
-    if (A4 && q == lastq + 1) scales_of(mb_next, nb_next);
-    load_scales(P, q <= lastq || !more ? q : q - lastq - 1);
   };
   u32x4_t b0[NT], b1[NT];
   auto weights = [&](auto J, const uint32_t (&sc)[NT], int i, u32x4_t (&b)[NT]) {
@@ -492,77 +498,91 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
       auto products = [&](auto P, auto J, const u32x4_t (&f)[MT]) {
         constexpr int j = J.value, p = P.value;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[p][nt], f[mt], sx[p][mt], acc[mt][nt]);
-        __builtin_amdgcn_sched_barrier(0);
+          for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = mfma_fp4<j>(w[j][nt], sw[p][nt], f[mt], sx[p][mt], acc[mt][nt]);
       };
       auto stage = [&](auto P, int s) {
-        if (s == last) weights_of(nb_next);
+        constexpr int p = P.value;
+        constexpr std::integral_constant<int, p ^ 1> kOther{};
         const int un = s < last ? 4 * (s + 1) : more ? 0 : 4 * last;
-        begin(P, s);
+        __syncthreads();
+        if (s == last) scales_of(mb_next, nb_next);
+        frag(cur, 1, f1);
+        load_scales(kOther, s < last || !more ? s + 1 : 0);
         products(P, std::integral_constant<int, 0>{}, f0);
+        spread<MT * NT, 0, MT, 0, MT + NT>();
+        if (s == last) weights_of(nb_next);
         frag(cur, 2, f0);
+        store_x(s + 2, far, xq[p]);
         load_w(un, w[0]);
-        __builtin_amdgcn_sched_barrier(0);
         products(P, std::integral_constant<int, 1>{}, f1);
+        spread<MT * NT, 0, MT, kRounds, NT>();
         frag(cur, 3, f1);
+        rows_ahead(P, s);
         load_w(un + 1, w[1]);
-        __builtin_amdgcn_sched_barrier(0);
         products(P, std::integral_constant<int, 2>{}, f0);
+        spread<MT * NT, 0, MT, 0, kRounds + NT>();
         frag(nxt, 0, f0);
         load_w(un + 2, w[2]);
-        __builtin_amdgcn_sched_barrier(0);
         products(P, std::integral_constant<int, 3>{}, f1);
         load_w(un + 3, w[3]);
-        scales_ahead(P, s + 2);
+        spread<MT * NT, 0, MT, 0, 2 * NT>();
         rotate();
       };
-      for (int s0 = 0; s0 < nst; s0 += 2) {
-        stage(std::integral_constant<int, 0>{}, s0);
-        if (s0 + 1 < nst) stage(std::integral_constant<int, 1>{}, s0 + 1);
+      for (int s = 0;;) {   // left at each stage's end: were stages skipped one by one, loads would be waited for
+        stage(kEven, s);    // as if any of them had been
+        if (++s >= nst) break;
+        stage(kOdd, s);
+        if (++s >= nst) break;
       }
     } else {
-      // Products of one operand, the conversion of the next spread among them.
+      // Products of one operand, the conversion of the next among them.
       auto products = [&](const u32x4_t (&f)[MT], const u32x4_t (&b)[NT]) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = mfma_bf16(b[nt], f[mt], acc[mt][nt]);
-        spread<MT * NT, 4 * NT + 1>();
-        __builtin_amdgcn_sched_barrier(0);
       };
+      constexpr int kCvts = 4 * NT + 1;
       auto stage = [&](auto P, auto J, int s) {   // P: the quad's parity, J: the stage in it
         constexpr int j = J.value, p = P.value;
-        begin(std::integral_constant<int, j & 1>{}, s);
+        constexpr std::integral_constant<int, j & 1> kSet{};
+        __syncthreads();
+        frag(cur, 1, f1);
+        if constexpr (j == 0) load_scales(std::integral_constant<int, p ^ 1>{}, s / 4 + 1);
         weights(J, sw[p], 1, b1);
         products(f0, b0);
+        spread<MT * NT, kCvts, MT, 0, j == 0 ? NT : 0>();
         frag(cur, 2, f0);
-        __builtin_amdgcn_sched_barrier(0);
+        store_x(s + 2, far, xq[kSet.value]);
         weights(J, sw[p], 2, b0);
         products(f1, b1);
+        spread<MT * NT, kCvts, MT, kRounds, 0>();
         frag(cur, 3, f1);
-        __builtin_amdgcn_sched_barrier(0);
+        rows_ahead(kSet, s);
         weights(J, sw[p], 3, b1);
         products(f0, b0);
+        spread<MT * NT, kCvts, MT, 0, kRounds>();
         frag(nxt, 0, f0);
         load_w(s - j < 4 * lastq ? s + 4 : 4 * lastq + j, w[j]);   // the next quad's: K is padded to whole ones
-        __builtin_amdgcn_sched_barrier(0);
         if constexpr (j < 3) weights(std::integral_constant<int, (j + 1) & 3>{}, sw[p], 0, b0);
         else weights(std::integral_constant<int, 0>{}, sw[p ^ 1], 0, b0);
         products(f1, b1);
+        spread<MT * NT, kCvts, MT, 0, NT>();
         rotate();
       };
       auto quad = [&](auto P, int s) {
         stage(P, std::integral_constant<int, 0>{}, s);
-        if (s + 1 < nst) stage(P, std::integral_constant<int, 1>{}, s + 1);
-        if (s + 2 < nst) stage(P, std::integral_constant<int, 2>{}, s + 2);
-        if (s + 3 < nst) stage(P, std::integral_constant<int, 3>{}, s + 3);
-        scales_ahead(P, s / 4 + 2);
+        if (kWhole || s + 1 < nst) stage(P, std::integral_constant<int, 1>{}, s + 1);
+        if (kWhole || s + 2 < nst) stage(P, std::integral_constant<int, 2>{}, s + 2);
+        if (kWhole || s + 3 < nst) stage(P, std::integral_constant<int, 3>{}, s + 3);
       };
-      for (int s = 0; s < nst; s += 8) {
+      for (int s = 0;;) {
         quad(kEven, s);
-        if (s + 4 < nst) quad(kOdd, s + 4);
+        if ((s += 4) >= nst) break;
+        quad(kOdd, s);
+        if ((s += 4) >= nst) break;
       }
     }
 #pragma unroll
@@ -612,17 +632,19 @@ __global__ __launch_bounds__(256) void mxfp4_reduce_kernel(const float* __restri
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-// Tile kernels, smallest first: MT, NT, WM, WN, and the us that a stage takes one block a CU (bf16 rows; a
-// stage of 512 elements of 4-bit ones), measured at 4096 and 28672 columns, K = 4096.
+// Tile kernels, smallest first: MT, NT, WM, WN; us before the first and behind the last product; us a stage with a block
+// on every CU (bf16 rows; a stage of 512 elements of 4-bit ones).  Fitted to 32 to 4093 rows of 4096, 6144, 16384 and 28672
+// columns, K = 2048 to 14336: estimates are within a fifth where a tile is in question, and the tile chosen within
+// 5 % of the best measured.
 struct TileConfig {
   int mt, nt, wm, wn;
-  float us, us4;
+  float start, us, us4;
   int rows() const { return 16 * mt * wm; }
   int cols() const { return 16 * nt * wn; }
 };
-constexpr TileConfig kTile2x1{2, 1, 1, 4, 0.36f, 0.f}, kTile2x2{2, 2, 1, 4, 0.44f, 0.f}, kTile4{4, 2, 1, 4, 0.56f, 0.f},
-    kTile5{5, 2, 1, 4, 0.62f, 0.85f}, kTile6{3, 2, 2, 4, 0.80f, 1.05f}, kTile8{4, 2, 2, 4, 0.93f, 1.30f},
-    kTile10{5, 2, 2, 4, 1.12f, 1.55f}, kTileWide{8, 2, 1, 8, 1.50f, 2.40f};
+constexpr TileConfig kTile2x1{2, 1, 1, 4, 2.7f, 0.27f, 0.f}, kTile2x2{2, 2, 1, 4, 3.7f, 0.30f, 0.f},
+    kTile4{4, 2, 1, 4, 4.4f, 0.58f, 0.f}, kTile5{5, 2, 1, 4, 4.8f, 0.68f, 1.30f}, kTile6{3, 2, 2, 4, 4.8f, 0.76f, 1.10f},
+    kTile8{4, 2, 2, 4, 5.0f, 0.80f, 1.30f}, kTile10{5, 2, 2, 4, 7.0f, 1.08f, 1.65f}, kTileWide{8, 2, 1, 8, 5.5f, 1.40f, 2.20f};
 constexpr TileConfig kTiles[] = {kTile2x1, kTile2x2, kTile4, kTile5, kTile6, kTile8, kTile10, kTileWide};
 constexpr int kFirstTile4 = 3;   // 4-bit rows: up to 64 go to the stream kernel
 
@@ -644,6 +666,9 @@ void split_k(Plan& p, int quads, int ks) {
 // packs: 16 rows of 4096 x 4096 6.7 / 3.4, of 16384 x 2048 7.1 / 4.9, but of 28672 x 4096 17.5 / 12.4 and of 4096 x 14336
 // 17.5 / 7.4; one row 4.1, 5.7, 13.8, 9.8.
 bool in_kernel(int M, int ntiles, int quads) { return M <= 8 || (M <= 16 && ntiles <= 1024 && quads <= 8); }
+
+// 4-bit rows: one block a CU, two of four waves, where a block's loads may run from one tile into the next.
+bool persistent(bool a4, int ks, int quads) { return a4 && ks == 1 && quads % 2 == 0 && quads >= 4; }
 
 // The plan for a product.  `partials`: a consumer adds the K slices.
 Plan plan_for(int M, int N, int K, bool a4, bool partials) {
@@ -670,11 +695,10 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
     split_k(p, quads, ks);
     return p;
   }
-  // Tile kernels: the cheapest of all tiles and K splits by this estimate.  A round is a block on each of the 256
-  // CUs (two of the four-wave ones); 6 us lie before its first and behind its last product; a reduction
-  // costs a launch where no consumer does it, and its bytes.
+  // Tile kernels: the cheapest of all tiles and K splits by this estimate.  A round is a block on each of the 256 CUs; with
+  // two four-wave blocks on a CU two rounds take the time of 1.45, and a stage takes less where CUs are free.  A
+  // reduction costs a launch where no consumer does it, and its bytes.
   float best = 1e30f;
-  const int steps = static_cast<int>((K + kStep - 1) / kStep);
   for (int t = a4 ? kFirstTile4 : 0; t < static_cast<int>(sizeof(kTiles) / sizeof(kTiles[0])); ++t) {
     const TileConfig& c = kTiles[t];
     const int64_t blocks = static_cast<int64_t>((M + c.rows() - 1) / c.rows()) * ((ntiles * 16 + c.cols() - 1) / c.cols());
@@ -684,11 +708,13 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
       if (q.ks != ks) continue;
       const int64_t grid = blocks * ks, rounds = (grid + 255) / 256;
       if (ks > 1 && grid > 512) break;   // enough for every CU
-      const float stages = a4 ? static_cast<float>(q.slice_quads) : static_cast<float>(steps < 4 * q.slice_quads ? steps : 4 * q.slice_quads);
-      const float block = 6.0f + stages * (a4 ? c.us4 : c.us);
+      const float stages = a4 ? static_cast<float>(q.slice_quads) : 4.0f * q.slice_quads;
+      const float share = grid < 256 ? static_cast<float>(grid) / 256.0f : 1.0f;
+      const float block = c.start + stages * (a4 ? c.us4 * (0.4f + 0.6f * share) : c.us * (0.65f + 0.35f * share));
       float us = rounds * block;
-      if (c.wm * c.wn == 4 && rounds > 1) us = (rounds + 1) / 2 * block * 1.6f;
-      if (ks > 1) us += (partials ? 0.0f : 2.5f) + 2e-6f * ks * M * static_cast<float>(p.pitch);
+      if (c.wm * c.wn == 4 && rounds > 1) us = (rounds + 1) / 2 * block * 1.45f;
+      if (persistent(a4, ks, quads)) us -= c.start * (us / block - 1.0f);   // loads run into the next tile
+      if (ks > 1) us += (partials ? 0.0f : 2.2f) + 0.7e-6f * ks * M * static_cast<float>(p.pitch);
       if (us < best) {
         best = us;
         q.tile = t;
@@ -733,14 +759,12 @@ template <bool A4, bool TAIL, int T>
 void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
   constexpr TileConfig c = kTiles[T];
   const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
-  // 4-bit rows: one block a CU, two of four waves, where a block's loads may run from one tile into the next.
-  const bool persistent = A4 && p.ks == 1 && a.kquads % 2 == 0 && a.kquads >= 4;
   const unsigned slots = c.wm * c.wn == 4 ? 512 : 256;
-  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(persistent && blocks > slots ? slots : blocks, p.ks),
+  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(persistent(A4, p.ks, a.kquads) && blocks > slots ? slots : blocks, p.ks),
                      dim3(64 * c.wm * c.wn), 0, s, a);
 }
 
-template <bool A4, bool TAIL>   // TAIL: K is not whole steps
+template <bool A4, bool TAIL>   // TAIL: K is not whole quads
 void launch_tiles(const Plan& p, const Args& a, hipStream_t s) {
   switch (p.tile) {
     case 3: return launch_tile<A4, TAIL, 3>(p, a, s);
@@ -772,7 +796,7 @@ void launch_product(const Plan& p, const Args& a, bool a4, hipStream_t s) {
     }
   } else {
     if (a4) launch_tiles<true, false>(p, a, s);
-    else if (a.K % kStep) launch_tiles<false, true>(p, a, s);
+    else if (a.K % kQuad) launch_tiles<false, true>(p, a, s);
     else launch_tiles<false, false>(p, a, s);
   }
 }
