@@ -6,7 +6,9 @@
 //   out = r * rsqrt(mean(r^2) + eps) * weight
 // Everything between the loads and the two stores is fp32: the residual (bf16) and out are rounded once
 // each, and the second norm is that of the unrounded r.  A row stays in its block's registers, so it is read
-// once and each result written once: 8 bytes an element (10 with a gate of rows).
+// once and each result written once: 8 bytes an element (10 with a gate of rows).  All loads of a row are issued before
+// its first sum, as many waves a row as leave a chunk a thread: 8191 rows of 4096 with a gate of rows 57 to 59 us
+// (5.7 to 5.9 TB/s, above the 5.1 of a large copy), one row 2.7, two sums through the block and one round trip.
 #include "common.h"
 
 namespace {
