@@ -176,7 +176,8 @@ def test_products_of_integers_are_exact(dev, shape, activations):
 
 @pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
 @pytest.mark.parametrize("shape", [(1500, 9001, 2048), (1025, 18000, 1536), (2100, 8200, 3584), (700, 33000, 1024),
-                                   (1300, 16400, 2016)])
+                                   (1300, 16400, 2016), (77, 70001, 2048), (90, 40000, 2048), (120, 40000, 2048),
+                                   (150, 40003, 2048)])
 def test_more_tiles_than_blocks(dev, shape, activations):
     """Products of so many tiles that a block takes several, at lengths of an even and an odd number of quads, with a
     ragged last tile on both sides.  Whole-number sums, as above; the reference is a product in 64 bits."""

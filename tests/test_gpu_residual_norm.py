@@ -75,6 +75,20 @@ def test_from_partial_sums(dev):
     check(got[0], new[0], reference(full, residual, weight, 1e-6, pw, gv, 0.5, 1.0))
 
 
+@pytest.mark.parametrize("ks", [1, 3, 4, 5, 8, 9, 16])
+@pytest.mark.parametrize("H", [8, 520, 4096, 8192, 16384])
+def test_any_number_of_slices(dev, H, ks):
+    """1 to 16 slices of partial sums at every block size: the bits of their sum in order, rounded once."""
+    T, padded = 5, 16
+    x, residual, weight, pw, gv = inputs(dev, T, H, "channel", True)
+    buf = torch.randn(ks * padded * H, device=dev)
+    part = fused.LinearPartials(buf.view(torch.uint8), ks, T, padded, H, x.shape, x.device)
+    want_new = torch.empty_like(residual)
+    want = fused.residual_norm(part.reduce(), residual, weight, 1e-6, pw, gv, 0.5, residual_out=want_new)
+    got = fused.residual_norm(part, residual, weight, 1e-6, pw, gv, 0.5)
+    assert torch.equal(got, want) and torch.equal(residual, want_new)
+
+
 def test_rows_are_their_own(dev):
     """A row that is not finite, a row of zeros and one of the largest values change no other row."""
     T, H = 6, 640
