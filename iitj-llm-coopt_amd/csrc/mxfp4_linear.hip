@@ -663,9 +663,11 @@ void split_k(Plan& p, int quads, int ks) {
 }
 
 // Whether the stream kernel quantises X itself.  us, it / packed without the 2 us and the host's 3 of the launch that
-// packs: 16 rows of 4096 x 4096 6.7 / 3.4, of 16384 x 2048 7.1 / 4.9, but of 28672 x 4096 17.5 / 12.4 and of 4096 x 14336
-// 17.5 / 7.4; one row 4.1, 5.7, 13.8, 9.8.
-bool in_kernel(int M, int ntiles, int quads) { return M <= 8 || (M <= 16 && ntiles <= 1024 && quads <= 8); }
+// packs: 16 rows of 4096 x 4096 6.5 / 3.4 (for a consumer 4.7 / 3.4), of 2048 x 8192 10.4 / 3.5 (5.2 / 3.5), of
+// 28672 x 4096 17.5 / 12.4, of 4096 x 14336 16.9 / 7.4; one row of that 10.1 / 7.3.
+bool in_kernel(int M, int ntiles, int quads, bool partials) {
+  return M <= 8 || (M <= 16 && ntiles <= 1024 && quads <= (partials ? 16 : 8));
+}
 
 // 4-bit rows: one block a CU, two of four waves, where a block's loads may run from one tile into the next.
 bool persistent(bool a4, int ks, int quads) { return a4 && ks == 1 && quads % 2 == 0 && quads >= 4; }
@@ -679,19 +681,29 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   p.pitch = ntiles * 16;
   if (mtiles <= (a4 ? 4 : 1)) {
     // Stream kernel.  Blocks enough for every CU first, then column tiles, for which X is read once.  us, NT = 1, 2, 4:
-    // 16 bf16 rows of 4096 x 4096 6.3, 6.8, 8.1, of 6144 x 4096 8.4, 7.3, 8.1, of 28672 x 4096 35, 23.3, 18.7 (one row 14.5,
-    // 13.7, 14.4); packed ones of 4096 x 4096 3.4, 3.8, 6.6; 32 of 16384 x 2048 5.8, 5.5, 7.1; 64 of 28672 x 4096 21.5, 19.0,
-    // 16.9.  Eight waves where each has a quad.
+    // 16 bf16 rows of 4096 x 4096 6.3, 6.9, 8.1, of 6144 x 4096 8.4, 7.3, 8.1, of 28672 x 4096 35, 23.3, 18.7 (one row 14.5,
+    // 13.7, 14.4); packed ones of 4096 x 4096 3.4, 3.8, 6.6; 32 of 16384 x 2048 5.9, 5.6, 7.1; 64 of 28672 x 4096 21.5, 16.7,
+    // 15.9.  Eight waves where each has a quad.
     p.stream = true;
-    p.x = !a4 ? kRows : in_kernel(M, ntiles, quads) ? kQuantize : kPacked;
+    p.x = !a4 ? kRows : in_kernel(M, ntiles, quads, partials) ? kQuantize : kPacked;
     p.mt = mtiles <= 2 ? mtiles : 4;
     if (p.x != kPacked) p.nt = ntiles >= 1024 && M > 4 ? 4 : ntiles >= 384 ? 2 : 1;
     else if (p.mt == 4) p.nt = ntiles >= 1408 ? 4 : ntiles >= 192 ? 2 : 1;
     else p.nt = ntiles >= 1024 ? 2 : 1;
     p.kw = p.nt == 4 || quads < 8 ? 4 : 8;
     int ks = 1;
-    if (partials)
-      while (ks < 4 && ks * 2 * p.kw <= quads && 2 * ks * ((ntiles + p.nt - 1) / p.nt) <= 512) ks *= 2;
+    auto blocks = [&]() { return (ntiles + p.nt - 1) / p.nt; };
+    if (p.x == kPacked) {
+      if (partials)
+        while (ks < 4 && ks * 2 * p.kw <= quads && 2 * ks * blocks() <= 512) ks *= 2;
+    } else if (partials || (M > 8 && quads >= 16 && ntiles < 1024)) {
+      // Slices instead of waves, and the tiles that leave blocks enough.  us for a consumer, against one slice: 5 rows of
+      // 4096 x 14336 8.9 / 10.1, of 6144 x 4096 4.9 / 5.3, 16 of 4096 x 4096 4.8 / 6.3, of 2048 x 8192 5.2 / 9.7, of 4096 x 14336
+      // 11.1 / 16.2 (for these two a launch that adds them pays as well).
+      p.nt = M > 8 ? (ntiles >= 256 ? 4 : ntiles >= 128 ? 2 : 1) : ntiles >= 192 ? 2 : 1;
+      p.kw = 4;
+      while (ks < 4 && ks * 4 <= quads && ks * blocks() < (M > 8 ? 256 : 512)) ks *= 2;
+    }
     split_k(p, quads, ks);
     return p;
   }
