@@ -28,9 +28,10 @@ __all__ = ["rms_norm", "residual_norm", "rope_", "silu_and_mul", "linear", "Line
 
 LINEAR_MAX_ROWS = 256
 _WS = _lib.WorkspaceCache()
-# held over the launches of a 4-bit product that takes its workspace from _WS: another thread's call on the
-# same stream would write its own between them
-_WS_LOCK = threading.Lock()
+# The same for 4-bit products, apart from those that others keep partial sums in, and held over a product's
+# launches: another thread's call on the same stream would write its own between them.
+_WS4 = _lib.WorkspaceCache()
+_WS4_LOCK = threading.Lock()
 _NO_LOCK = contextlib.nullcontext()
 
 
@@ -412,7 +413,7 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
         ws, lock = x.new_empty((need,), dtype=torch.uint8), _NO_LOCK
         wsp, have = ws.data_ptr(), need
     else:
-        lock, wsp = _WS_LOCK, None
+        lock, wsp = _WS4_LOCK, None
     if partials:
         yp = ldy = None
     else:
@@ -426,7 +427,7 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
             ldy = N
     with lock:
         if wsp is None:
-            ws = _WS.get(need, packed.device)
+            ws = _WS4.get(need, packed.device)
             wsp, have = ws.data_ptr(), ws.numel()
         if partials:
             rc = _lib.call_on(index, _lib.entry("coopt_mxfp4_linear_partials"), x.data_ptr(), ldx, packed.data_ptr(), M, N,

@@ -334,6 +334,13 @@ def test_deferred_sums_live_on(dev, activations):
         assert torch.equal(fused.rms_norm(p, norm, 1e-5), fused.rms_norm(y, norm, 1e-5))
         assert torch.equal(fused.residual_norm(p, y.clone(), norm, 1e-5), fused.residual_norm(y, y.clone(), norm, 1e-5))
     assert torch.equal(fused.linear_silu(xs[0], w), fused.silu_and_mul(full[0]))
+    dense = small_numbers(dev, (1024, 8192), 9)
+    part = fused.linear(xs[0][:40, :8192].contiguous(), dense, defer_reduce=True)
+    assert isinstance(part, fused.LinearPartials)
+    before = part.reduce()
+    for x in xs:
+        fused.linear(x, w)
+    assert torch.equal(part.reduce(), before)
 
 
 @pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
