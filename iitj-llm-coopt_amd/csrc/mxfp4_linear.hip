@@ -317,7 +317,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void mxfp4_tile_kernel(const Args 
   constexpr int kChunks = kTiles * 256;                // 16-byte chunks of X in a stage
   constexpr int kRounds = (kChunks + kThreads - 1) / kThreads;
   static_assert(WM * WN % 4 == 0, "a wave's chunks of 4-bit rows lie in one tile");
-  static_assert(!A4 || (kChunks % kThreads == 0 && kTiles <= kMostTiles), "4-bit rows are read in whole tiles, up to the padding");
+  static_assert(!A4 || (kChunks % kThreads == 0 && kTiles <= kMostTiles),
+                "4-bit rows are read in whole tiles, up to the padding");
   constexpr int kBuf = kRounds * kThreads;
   __shared__ u32x4_t xs[3 * kBuf];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -634,8 +635,7 @@ __global__ __launch_bounds__(256) void mxfp4_reduce_kernel(const float* __restri
 // ---- which kernel ------------------------------------------------------------------------------
 // Tile kernels, smallest first: MT, NT, WM, WN; us before the first and behind the last product; us a stage with a block
 // on every CU (bf16 rows; a stage of 512 elements of 4-bit ones).  Fitted to 32 to 4093 rows of 4096, 6144, 16384 and 28672
-// columns, K = 2048 to 14336, where the tile and split chosen take at most 8 % (one: 1.3 times, 256 x 6144 x 4096
-// for a consumer) more than the best measured.
+// columns, K = 2048 to 14336, where the tile and split chosen take at most 8 % more than the best measured.
 struct TileConfig {
   int mt, nt, wm, wn;
   float start, us, us4;
@@ -643,8 +643,9 @@ struct TileConfig {
   int cols() const { return 16 * nt * wn; }
 };
 constexpr TileConfig kTile2x1{2, 1, 1, 4, 2.7f, 0.27f, 0.f}, kTile2x2{2, 2, 1, 4, 3.7f, 0.33f, 0.f},
-    kTile4{4, 2, 1, 4, 4.4f, 0.56f, 0.f}, kTile5{5, 2, 1, 4, 4.8f, 0.68f, 1.30f}, kTile6{3, 2, 2, 4, 4.8f, 0.76f, 1.10f},
-    kTile8{4, 2, 2, 4, 5.0f, 0.80f, 1.30f}, kTile10{5, 2, 2, 4, 7.0f, 1.08f, 1.65f}, kTileWide{8, 2, 1, 8, 5.5f, 1.40f, 2.20f};
+    kTile4{4, 2, 1, 4, 4.4f, 0.50f, 0.f}, kTile5{5, 2, 1, 4, 4.8f, 0.68f, 1.30f}, kTile6{3, 2, 2, 4, 4.8f, 0.76f, 1.10f},
+    kTile8{4, 2, 2, 4, 5.0f, 0.80f, 1.30f}, kTile10{5, 2, 2, 4, 7.0f, 1.08f, 1.65f},
+    kTileWide{8, 2, 1, 8, 5.5f, 1.40f, 2.20f};
 constexpr TileConfig kTiles[] = {kTile2x1, kTile2x2, kTile4, kTile5, kTile6, kTile8, kTile10, kTileWide};
 constexpr int kFirstTile4 = 3;   // 4-bit rows: up to 64 go to the stream kernel
 
@@ -772,8 +773,8 @@ void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
   constexpr TileConfig c = kTiles[T];
   const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
   const unsigned slots = c.wm * c.wn == 4 ? 512 : 256;
-  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(persistent(A4, p.ks, a.kquads) && blocks > slots ? slots : blocks, p.ks),
-                     dim3(64 * c.wm * c.wn), 0, s, a);
+  const unsigned grid = persistent(A4, p.ks, a.kquads) && blocks > slots ? slots : blocks;
+  hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(grid, p.ks), dim3(64 * c.wm * c.wn), 0, s, a);
 }
 
 template <bool A4, bool TAIL>   // TAIL: K is not whole quads

@@ -150,7 +150,8 @@ def quantized(x):
 # of 128 and a whole quad of 512
 SHAPES = [(1, 16, 32), (1, 4096, 4096), (2, 17, 64), (5, 100, 96), (15, 33, 160), (16, 64, 128), (17, 64, 512),
           (31, 130, 544), (32, 2048, 2048), (33, 48, 640), (48, 1000, 1024), (63, 16, 4096), (64, 257, 480),
-          (65, 512, 992), (80, 272, 2048), (96, 1023, 256), (127, 64, 1536), (128, 4096, 1024), (129, 640, 1024), (160, 6144, 512),
+          (65, 512, 992), (80, 272, 2048), (96, 1023, 256), (127, 64, 1536), (128, 4096, 1024), (129, 640, 1024),
+          (160, 6144, 512),
           (200, 96, 14336), (256, 1000, 736), (5, 6144, 4096), (7, 4096, 14336), (12, 2100, 8224), (16, 300, 14336),
           (16, 4128, 8192), (300, 4096, 4096), (333, 512, 2080), (513, 514, 1056), (1000, 2048, 512)]
 
