@@ -95,6 +95,7 @@ SIGNATURES = {
     "coopt_mxfp4_pack_weight": (_i, [_p, _p, _i, _i, _p, _p]),
     "coopt_mxfp4_linear_workspace": (_sz, [_i, _i, _i, _i, _i]),
     "coopt_mxfp4_linear_split": (_i, [_i, _i, _i, _i, _p, _p]),
+    "coopt_mxfp4_linear_plan": (_i, [_i, _i, _i, _i, _i, _p]),
     "coopt_mxfp4_linear": (_i, [_p, _i64, _p, _i, _i, _i, _i, _p, _i64, _p, _sz, _p]),
     "coopt_mxfp4_linear_partials": (_i, [_p, _i64, _p, _i, _i, _i, _i, _p, _sz, _p]),
     "coopt_residual_norm": (_i, [_p, _p, _i, _i64, _p, _p, _p, _p, _i64, _p, _p, _i64, _i, _f, _f,

@@ -9,6 +9,8 @@
 // A4 = true.  A lane's 16 bytes are its operand of v_mfma_scale_f32_16x16x128_f8f6f4 as they are, with
 // their scale bytes: products and sums of a step are formed by the matrix core.
 // In both the weight is the A operand, so a lane ends with four consecutive outputs of one row.
+#include <algorithm>
+
 #include "mxfp4.h"
 
 namespace {
@@ -768,12 +770,20 @@ void launch_stream_rows(const Plan& p, const Args& a, hipStream_t s) {
   else launch_stream<X, TAIL, MT, 1>(p, a, s);
 }
 
+unsigned tiles_of(const TileConfig& c, int M, int N) {
+  return static_cast<unsigned>((M + c.rows() - 1) / c.rows()) * ((N + c.cols() - 1) / c.cols());
+}
+
+// Blocks along x of a tile kernel's grid.
+unsigned tile_blocks(const TileConfig& c, const Plan& p, bool a4, int M, int N, int quads) {
+  const unsigned tiles = tiles_of(c, M, N), slots = c.wm * c.wn == 4 ? 512 : 256;
+  return persistent(a4, p.ks, quads) && tiles > slots ? slots : tiles;
+}
+
 template <bool A4, bool TAIL, int T>
 void launch_tile(const Plan& p, const Args& a, hipStream_t s) {
   constexpr TileConfig c = kTiles[T];
-  const unsigned blocks = ((a.M + c.rows() - 1) / c.rows()) * ((a.N + c.cols() - 1) / c.cols());
-  const unsigned slots = c.wm * c.wn == 4 ? 512 : 256;
-  const unsigned grid = persistent(A4, p.ks, a.kquads) && blocks > slots ? slots : blocks;
+  const unsigned grid = tile_blocks(c, p, A4, a.M, a.N, a.kquads);
   hipLaunchKernelGGL((mxfp4_tile_kernel<A4, TAIL, c.mt, c.nt, c.wm, c.wn>), dim3(grid, p.ks), dim3(64 * c.wm * c.wn), 0, s, a);
 }
 
@@ -895,6 +905,24 @@ extern "C" int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, 
   const Plan p = plan_for(M, N, K, act4 != 0, true);
   *ks = p.ks;
   *rows_padded = p.rows_padded;
+  return COOPT_OK;
+}
+
+extern "C" int coopt_mxfp4_linear_plan(int M, int N, int K, int act4, int partials, int* plan) {
+  coopt::clear_error();
+  COOPT_REQUIRE(plan, "null output pointer");
+  COOPT_REQUIRE(!shape_error(M, N, K) && M > 0 && N > 0, "unsupported shape");
+  const Plan p = plan_for(M, N, K, act4 != 0, partials != 0);
+  if (p.stream) {
+    const int v[8] = {0, p.x, p.mt, p.nt, 1, p.kw, p.ks, 1};
+    std::copy(v, v + 8, plan);
+  } else {
+    const TileConfig& c = kTiles[p.tile];
+    const unsigned tiles = tiles_of(c, M, N);
+    const unsigned grid = tile_blocks(c, p, act4 != 0, M, N, static_cast<int>(mxfp4::quads(K)));
+    const int v[8] = {1, act4 ? kPacked : kRows, c.mt, c.nt, c.wm, c.wn, p.ks, static_cast<int>((tiles + grid - 1) / grid)};
+    std::copy(v, v + 8, plan);
+  }
   return COOPT_OK;
 }
 

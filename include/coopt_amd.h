@@ -565,11 +565,16 @@ int coopt_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, 
  *   coopt_mxfp4_linear_split / _partials: as coopt_linear_split / coopt_linear_partials: ks fp32 slices
  *     [rows_padded, N] at the workspace's start, whose sum in order is the output before its rounding.  N a
  *     multiple of 32; coopt_mxfp4_linear_workspace(M, N, K, act4, 1) bytes.
+ *   coopt_mxfp4_linear_plan: which kernel a product runs, for tests and traces: plan[0] 0 few rows, 1 tiles;
+ *     [1] rows as bf16 (0), packed by a launch before it (1) or quantised in it (2); [2], [3] row and column tiles of 16
+ *     a wave; [4], [5] waves along rows and columns (few rows: 1 and the waves along K); [6] K slices; [7] the
+ *     most tiles that a block takes.
  */
 size_t coopt_mxfp4_packed_bytes(int N, int K);
 int coopt_mxfp4_pack_weight(const void* codes, const void* scales, int N, int K, void* out, coopt_stream_t stream);
 size_t coopt_mxfp4_linear_workspace(int M, int N, int K, int act4, int partials);
 int coopt_mxfp4_linear_split(int M, int N, int K, int act4, int* ks, int* rows_padded);
+int coopt_mxfp4_linear_plan(int M, int N, int K, int act4, int partials, int* plan);
 int coopt_mxfp4_linear(const void* x, int64_t ldx, const void* w_packed, int M, int N, int K, int act4, void* y,
                        int64_t ldy, void* workspace, size_t workspace_bytes, coopt_stream_t stream);
 int coopt_mxfp4_linear_partials(const void* x, int64_t ldx, const void* w_packed, int M, int N, int K, int act4,
