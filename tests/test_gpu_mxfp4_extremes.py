@@ -1,0 +1,86 @@
+"""GPU: products with 4-bit weights at values that are not finite and at the ends of the scales' range, in every
+kernel that has a way of its own with them.
+
+Rows: 1, 8 and 16 (few rows, 4-bit ones quantised in the product), 20 (packed by a launch before it), 80 (tiles).
+Tolerance: half a bf16 step (2^-8) of the output; a sum of K products as a chain of K / 32 + 160 fp32 roundings at most,
+2^-23 each of the magnitudes' sum; and half of the smallest subnormal step, 2^-134 in the output.
+"""
+import numpy as np
+import pytest
+import torch
+
+import iitj_llm_coopt_amd as M
+from iitj_llm_coopt_amd import fused
+from test_gpu_mxfp4 import make_weight, pack, quantized, reference_values
+
+pytestmark = pytest.mark.gpu
+
+ROWS = [1, 8, 16, 20, 80]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("m", ROWS)
+def test_rows_that_are_not_finite(dev, m, activations, bad):
+    """One element of a row: with 4-bit rows its block is NaN and so is every output of the row, with bf16 rows each
+    output is that element times the weight (NaN where that is 0); other rows keep their bits."""
+    N, K = 208, 1184
+    w, vals = make_weight(dev, N, K, m, activations)
+    g = torch.Generator().manual_seed(m)
+    x = torch.randn(m, K, generator=g).to(torch.bfloat16)
+    base = fused.linear(x.to(dev), w).cpu()
+    for row, k in ((0, 0), (m // 2, 700), (m - 1, K - 1)):
+        y = x.clone()
+        y[row, k] = bad
+        got = fused.linear(y.to(dev), w).cpu()
+        others = [i for i in range(m) if i != row]
+        assert torch.equal(got[others], base[others])
+        if activations == "mxfp4" or np.isnan(bad):
+            assert got[row].isnan().all()
+        else:
+            with np.errstate(invalid="ignore"):
+                want = bad * vals[:, k]
+            assert np.array_equal(got[row].double().numpy(), want, equal_nan=True)
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("m", ROWS)
+def test_weight_blocks_that_are_not_numbers(dev, m, activations):
+    """A weight block of scale 255 makes its row's outputs NaN, whatever its codes, and no other's."""
+    N, K = 208, 1184
+    w, _ = make_weight(dev, N, K, m, activations)
+    x = torch.randn(m, K, generator=torch.Generator().manual_seed(m)).to(dev, torch.bfloat16)
+    base = fused.linear(x, w)
+    codes, scales = w.codes.clone(), w.scales.clone()
+    bad = [(0, 0), (77, 20), (N - 1, K // 32 - 1)]
+    for i, (n, b) in enumerate(bad):
+        scales[n, b] = 255
+        if i:
+            codes[n, 16 * b:16 * b + 16] = 0
+    got = fused.linear(x, M.pack_mxfp4_weight(codes, scales, activations))
+    rows = [n for n, _ in bad]
+    others = [n for n in range(N) if n not in rows]
+    assert got[:, rows].isnan().all() and torch.equal(got[:, others], base[:, others])
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("lo,hi,exponent", [(0, 4, 110), (0, 1, 0), (0, 30, 60), (248, 253, -120), (200, 253, -126),
+                                            (240, 253, -132), (120, 134, -131)])
+def test_scales_of_the_whole_range(dev, m, activations, lo, hi, exponent):
+    """Weight scale bytes lo .. hi - 1 by rows around 2^exponent: subnormal weights, subnormal rows, the largest of
+    both, products that underflow."""
+    N, K = 208, 1184
+    rng = np.random.default_rng(m + lo)
+    code, s = rng.integers(0, 16, (N, K)), rng.integers(lo, hi, (N, K // 32))
+    w = M.pack_mxfp4_weight(pack(code).to(dev), torch.from_numpy(s.astype(np.uint8)).to(dev), activations)
+    vals = reference_values(code, s)
+    xt = torch.from_numpy(rng.standard_normal((m, K)) * 2.0 ** exponent).to(torch.bfloat16)
+    x = xt.double().numpy()
+    assert (x != 0).any(1).all()
+    if activations == "mxfp4":
+        x = quantized(x)
+    ref, mag = x @ vals.T, np.abs(x) @ np.abs(vals).T
+    assert mag.max() < 2.0 ** 127
+    got = fused.linear(xt.to(dev), w).double().cpu().numpy()
+    assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + (K / 32 + 160) * 2.0 ** -23 * mag + 2.0 ** -134).all()
