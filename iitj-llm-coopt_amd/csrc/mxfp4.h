@@ -3,7 +3,9 @@
 //
 // A row of K elements is K / 2 code bytes (the even element in the low half) and K / 32 scale bytes.  A
 // code is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; an element of block b of 32 is code * 2^(s[b] - 127),
-// NaN where s[b] = 255.  Every such value is a bf16 number (two significant bits, bf16's exponents).
+// NaN where s[b] = 255.  Every value of a scale byte up to 252 is a bf16 number (two significant bits, bf16's
+// exponents), and quantisation gives no larger one; of 253 and 254 the codes whose value is 2^128 or more (4 and 6;
+// 2, 3, 4 and 6) are infinities as bf16 and fp32, while products of two 4-bit operands take them as they are.
 //
 // Packed layout, of a weight's rows or of quantised activations.  Tile (t, u) holds sixteen rows
 // of K elements 128 u .. 128 u + 127 as 64 chunks of 16 bytes: chunk l is the tile's row l % 16, block l / 16 --
@@ -94,7 +96,7 @@ __device__ __forceinline__ uint32_t amax_bits(const u32x4_t (&x)[N]) {
   return (lo > hi ? lo : hi) << 16;
 }
 
-// Eight elements of one block as bf16 (exact), from their four code bytes.
+// Eight elements of one block as bf16 (exact, infinity from 2^128 on), from their four code bytes.
 __device__ __forceinline__ u32x4_t bf16_of(uint32_t c, float scale) {
   u32x4_t o;
   o.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 0));

@@ -1,8 +1,8 @@
 // Products with microscaled 4-bit weights: Y[M, N] = X[M, K] W[N, K]^T, bf16 out, fp32 accumulation.
 // W is packed (mxfp4.h); X is bf16 (A4 = false) or quantised in the call to the same 4-bit format (A4 = true).
 //
-// A4 = false.  A weight is a bf16 number, so the product is exactly that of the bf16 matrix instructions
-// on code * 2^e: a lane's 16 bytes of a tile are 32 elements of one row and one block, four operands of
+// A4 = false.  A weight is a bf16 number (scale bytes up to 252, mxfp4.h), so the product is exactly that of the
+// bf16 matrix instructions on code * 2^e: a lane's 16 bytes of a tile are 32 elements of one row and one block, four operands of
 // v_mfma_f32_16x16x32_bf16 after 16 v_cvt_scalef32_pk_bf16_fp4 (two elements each, scale applied).  The K
 // order inside a step is any that both operands share: operand j of lane (row, g) holds elements
 // 32 g + 8 j .. + 7 of the step.

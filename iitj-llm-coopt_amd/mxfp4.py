@@ -8,6 +8,9 @@ A row of K elements (K a multiple of 32) is K / 2 code bytes, the even element i
 scale bytes.  A code is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6; an element is code * 2^(s - 127) with its
 block's scale byte s, NaN where s is 255.  Quantisation takes s - 127 = floor(log2 amax) - 2 (at least
 -127) and the nearest code, ties to the even one, 6 for everything above; a block that is not finite gets 255.
+Scales that others made may be 253 or 254, which quantisation never gives: their values from 2^128 on are past bf16
+and fp32, and are infinities in dequantize_mxfp4 and in products with bf16 rows (in products of 4-bit rows they
+are not).
 The reference has no such weights; its codes for swapped caches are kv_cache.quantize's.
 """
 import ctypes
@@ -68,7 +71,7 @@ def _check_rows(codes, scales):
 
 
 def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bfloat16):
-    """The values [..., K] of 4-bit rows: exact in bf16 and fp32, rounded in fp16."""
+    """The values [..., K] of 4-bit rows: exact in bf16 and fp32 (infinity from 2^128 on), rounded in fp16."""
     index = codes.get_device()
     if index < 0 or index != scales.get_device():
         _lib.require_one_device(codes, scales)

@@ -546,7 +546,8 @@ int coopt_residual_norm(const void* x, const float* part, int ks, int64_t slice_
  *   coopt_mxfp4_quantize: x [rows, K] contiguous (BF16 / F16 / F32).  With a the largest magnitude of a
  *     block, s = max(floor(log2 a) + 125, 0) and a code is the nearest to x / 2^(s - 127), ties to the even
  *     code, 6 for all above; a block that is not finite has s = 255 and codes 0.
- *   coopt_mxfp4_dequantize: out [rows, K] (BF16 and F32 exact, F16 rounded).
+ *   coopt_mxfp4_dequantize: out [rows, K] (BF16 and F32 exact, infinity for values from 2^128 on, which take a scale
+ *     byte of 253 or 254 and no quantised row has; F16 rounded).
  * K a multiple of 32; x and out 16-byte, codes 4-byte aligned.
  */
 int coopt_mxfp4_quantize(int in_dtype, const void* x, int64_t rows, int K, void* codes, void* scales,
@@ -557,7 +558,8 @@ int coopt_mxfp4_dequantize(const void* codes, const void* scales, int64_t rows, 
  * Projections by a microscaled 4-bit weight: y [M, N] = x [M, K] w [N, K]^T, bf16 in and out, fp32 sums.
  *   coopt_mxfp4_pack_weight: codes [N, K / 2] and scales [N, K / 32] into out (coopt_mxfp4_packed_bytes(N, K)
  *     bytes) in the order the kernels load them; once a model load.  codes and out 16-byte aligned.
- *   coopt_mxfp4_linear: act4 = 0: x as it is (every weight is a bf16 number, products are those of bf16);
+ *   coopt_mxfp4_linear: act4 = 0: x as it is (every weight is a bf16 number, infinity from 2^128 on; products are
+ *     those of bf16);
  *     act4 = 1: x is quantised first, as coopt_mxfp4_quantize does, and the 4-bit operands are multiplied.
  *     K a multiple of 32 up to 2^22, N up to 2^24, M up to 2^19; x rows 16-byte aligned (ldx a
  *     multiple of 8, at most 2^22).

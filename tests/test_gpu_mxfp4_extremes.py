@@ -84,3 +84,23 @@ def test_scales_of_the_whole_range(dev, m, activations, lo, hi, exponent):
     assert mag.max() < 2.0 ** 127
     got = fused.linear(xt.to(dev), w).double().cpu().numpy()
     assert (np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + (K / 32 + 160) * 2.0 ** -23 * mag + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("m", ROWS)
+@pytest.mark.parametrize("s", [252, 253, 254])
+def test_weights_past_bf16(dev, m, s, activations):
+    """Values from 2^128 on, of scale bytes 253 and 254 alone: infinities by bf16 rows and as bf16 values, numbers
+    by 4-bit rows.  Column n has code n % 16 throughout; 2^-120 * 512 * value is exact."""
+    N, K = 32, 512
+    code = np.tile((np.arange(N) % 16)[:, None], (1, K))
+    sc = np.full((N, K // 32), s)
+    w = M.pack_mxfp4_weight(pack(code).to(dev), torch.from_numpy(sc.astype(np.uint8)).to(dev), activations)
+    vals = reference_values(code, sc)
+    past = np.abs(vals[:, 0]) >= 2.0 ** 128
+    assert past.sum() == {252: 0, 253: 8, 254: 16}[s]
+    as_bf16 = np.where(np.abs(vals) >= 2.0 ** 128, np.sign(vals) * np.inf, vals)
+    assert np.array_equal(w.dequantize().double().cpu().numpy(), as_bf16)
+    got = fused.linear(torch.full((m, K), 2.0 ** -120, device=dev, dtype=torch.bfloat16), w).double().cpu().numpy()
+    want = 2.0 ** -120 * K * (as_bf16 if activations == "bf16" else vals)[:, 0]
+    assert np.array_equal(got, np.tile(want, (m, 1)))
