@@ -407,9 +407,10 @@ def _linear_mxfp4(x, weight, out, defer_reduce):
     if not need:
         wsp = have = 0
         lock = _NO_LOCK
-    elif partials or torch.cuda.is_current_stream_capturing():
-        # partial sums live as long as their LinearPartials; a graph under capture gets a workspace of its own
-        # (from its memory pool), so that two graphs captured on one stream may replay at the same time
+    elif partials or _lib.call_on(index, torch.cuda.is_current_stream_capturing):
+        # partial sums live as long as their LinearPartials; a graph under capture (of the stream that the product
+        # goes to: its GPU need not be the current one) gets a workspace of its own (from its memory pool), so that two
+        # graphs captured on one stream may replay at the same time
         ws, lock = x.new_empty((need,), dtype=torch.uint8), _NO_LOCK
         wsp, have = ws.data_ptr(), need
     else:
