@@ -236,18 +236,27 @@ class WorkspaceCache:
     """Device scratch buffers, grown on demand and reused (the kernels need no initialised
     workspace).  One buffer per (device, stream): calls that overlap in time must not share
     a workspace, and stream order keeps calls on one stream from overlapping.  An outgrown
-    buffer is kept alive, not freed: a HIP graph captured with it keeps its address."""
+    buffer is kept alive, not freed: a HIP graph captured with it keeps its address.
 
-    def __init__(self):
+    eager_only: no capture uses the buffers, and their sizes have no bound as small as a step's rows.
+    An outgrown one is freed (torch's allocator reuses it in its stream's order, behind the calls that use it),
+    and sizes are rounded up to eight a doubling, so that calls that grow little by little allocate seldom."""
+
+    def __init__(self, eager_only=False):
         self._bufs = {}
-        self._retired = []
+        self._retired = None if eager_only else []
 
     def get(self, nbytes: int, device) -> torch.Tensor:
         dev = device if isinstance(device, torch.device) else torch.device(device)
         key = (dev.index, stream_handle(dev))
         buf = self._bufs.get(key)
         if buf is None or buf.numel() < nbytes:
-            if buf is not None:
+            if self._retired is None:
+                self._bufs.pop(key, None)
+                buf = None
+                eighth = 1 << max(int(nbytes).bit_length() - 4, 0)
+                nbytes = -(-int(nbytes) // eighth) * eighth
+            elif buf is not None:
                 self._retired.append(buf)
             buf = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
             self._bufs[key] = buf

@@ -29,8 +29,8 @@ __all__ = ["rms_norm", "residual_norm", "rope_", "silu_and_mul", "linear", "Line
 LINEAR_MAX_ROWS = 256
 _WS = _lib.WorkspaceCache()
 # The same for 4-bit products, apart from those that others keep partial sums in, and held over a product's
-# launches: another thread's call on the same stream would write its own between them.
-_WS4 = _lib.WorkspaceCache()
+# launches: another thread's call on the same stream would write its own between them.  No graph holds them.
+_WS4 = _lib.WorkspaceCache(eager_only=True)
 _WS4_LOCK = threading.Lock()
 _NO_LOCK = contextlib.nullcontext()
 

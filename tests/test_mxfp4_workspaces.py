@@ -62,7 +62,7 @@ def gpu(monkeypatch):
         monkeypatch.setattr(_lib, name, lambda device=None: 0)
     monkeypatch.setattr(torch, "empty", cached)
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state.current in state.capturing)
-    monkeypatch.setattr(fused, "_WS4", type(fused._WS4)())
+    monkeypatch.setattr(fused._WS4, "_bufs", {})
     monkeypatch.setattr(Tensor, "gpu", state)
     return state
 
@@ -87,3 +87,16 @@ def test_a_capture_on_the_tensors_gpu_gets_a_workspace_of_its_own(gpu, current):
     gpu.capturing = {0}
     fused.linear(x, w)
     assert len(gpu.launches) == 2 and len(gpu.own) == 1 and len(gpu.cached) == 1
+
+
+def test_outgrown_workspaces_are_freed(gpu):
+    """Rows that grow 16 at a time, as prompts do: one workspace is alive, at most an eighth larger than the largest
+    need, and few were allocated."""
+    w = weight(64, 14336, 0)
+    for M in range(80, 4096, 16):
+        fused.linear(rows(M, 14336, 0), w)
+    alive = [n for ref, n in gpu.cached if ref() is not None]
+    need = w.plan(4080)[0]
+    assert len(alive) == 1 and need <= alive[0] <= need * 9 // 8
+    assert len(gpu.cached) <= 8 * 5   # eight sizes a doubling of the need, which grows 20-fold
+    assert not gpu.own
