@@ -63,9 +63,12 @@ class LinearPartials:
 def rms_norm(x, weight, eps, residual=None, out=None):
     """out = rmsnorm(x) * weight; with `residual`, first residual += x in place (fused add).
     x may be a LinearPartials (the split-K output of linear(..., defer_reduce=True)), reduced
-    in the same pass."""
+    in the same pass up to 8192 columns and ahead of it above."""
     if isinstance(x, LinearPartials):
-        return _rms_norm_partials(x, weight, eps, residual, out)
+        if x.n <= 8192 or weight.numel() != x.n:
+            return _rms_norm_partials(x, weight, eps, residual, out)
+        _lib.require_cuda(weight, residual, out)
+        x = x.reduce()
     _lib.require_cuda(x, weight, residual, out)
     for t, n in ((x, "x"), (weight, "weight")):
         _bf16_rows(t, n)
@@ -85,8 +88,8 @@ def rms_norm(x, weight, eps, residual=None, out=None):
 def _rms_norm_partials(xp, weight, eps, residual, out):
     _lib.require_cuda(weight, residual, out)
     _bf16_rows(weight, "weight")
-    if weight.numel() != xp.n or xp.n > 8192:
-        raise ValueError("weight must match the partials' width (at most 8192)")
+    if weight.numel() != xp.n:
+        raise ValueError("weight must match the partials' width")
     if residual is not None and (tuple(residual.shape) != tuple(xp.shape) or not residual.is_contiguous()):
         raise ValueError("residual must be contiguous with the layer output's shape")
     if out is None:

@@ -27,3 +27,32 @@ def test_rows_that_grow_keep_one_workspace(dev, activations):
     assert after - before <= max(w.plan(m)[0] for m in sizes) * 9 // 8 + 512
     for m, o in zip(sizes, out):
         assert torch.equal(o, want[:m])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("shape", [(160, 10240), (2, 3, 16384)])
+def test_rms_norm_takes_sums_of_any_width(dev, shape, residual):
+    """A wide product leaves its K slices to a consumer at some sizes and gives rows at others: the same norm of
+    both."""
+    H, ks = shape[-1], 3
+    rows, padded = 160 if len(shape) == 2 else 6, 160 if len(shape) == 2 else 16
+    buf = torch.randn(ks * padded * H, device=dev)
+    part = fused.LinearPartials(buf.view(torch.uint8), ks, rows, padded, H, torch.Size(shape), dev)
+    weight = (1 + 0.3 * torch.randn(H, device=dev)).to(torch.bfloat16)
+    r = [torch.randn(shape, device=dev).to(torch.bfloat16)] if residual else [None]
+    r.append(r[0].clone() if residual else None)
+    want = fused.rms_norm(part.reduce(), weight, 1e-5, residual=r[0])
+    out = torch.empty(shape, device=dev, dtype=torch.bfloat16)
+    assert fused.rms_norm(part, weight, 1e-5, residual=r[1], out=out) is out and torch.equal(out, want)
+    assert not residual or torch.equal(*r)
+    with pytest.raises(ValueError, match="width"):
+        fused.rms_norm(part, weight[:-8], 1e-5)
+
+
+def test_wide_products_feed_the_norm(dev):
+    w, _ = make_weight(dev, 8320, 14336, 4, integers=True)
+    x = small_numbers(dev, (20, 14336), 4)
+    part = fused.linear(x, w, defer_reduce=True)
+    assert isinstance(part, fused.LinearPartials)
+    norm = torch.ones(8320, device=dev, dtype=torch.bfloat16)
+    assert torch.equal(fused.rms_norm(part, norm, 1e-5), fused.rms_norm(fused.linear(x, w), norm, 1e-5))
