@@ -114,7 +114,7 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
     shape; gate [H], or of x's shape (rows may be strided); H a multiple of 8 up to 16384.  residual_out: where r
     goes, by default into `residual`.  Returns out (a new tensor by default).  out may be x, residual (with another
     residual_out) or a gate of x's shape itself, and overlaps no input otherwise; nor does residual_out."""
-    part = x if type(x) is LinearPartials else None
+    part = x if isinstance(x, LinearPartials) else None
     shape = x.shape
     H = shape[-1] if shape else 0
     index = residual.get_device()
@@ -329,7 +329,7 @@ def linear(x, weight, out=None, defer_reduce=False):
     `weight` may be an MXFP4Weight (K a multiple of 32, any N and row count): coopt_mxfp4_linear, with
     bf16 rows or, where the weight says activations "mxfp4", rows quantised to 4 bits in the call.
     defer_reduce returns LinearPartials where K is split (in memory of their own).  out overlaps no input."""
-    if type(weight) is MXFP4Weight:
+    if isinstance(weight, MXFP4Weight):
         return _linear_mxfp4(x, weight, out, defer_reduce)
     packed = weight.packed if isinstance(weight, PackedWeight) and not weight.gate_up else None
     if isinstance(weight, PackedWeight):
