@@ -90,6 +90,21 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, dtype=torch.bflo
     return out
 
 
+def _check_weight(codes, scales):
+    """(N, K) of a weight's codes [N, K / 2] and scales [N, K / 32]."""
+    if codes.dim() != 2:
+        raise ValueError(f"codes must be [N, K / 2], got {tuple(codes.shape)}")
+    N, K = codes.shape[0], _check_rows(codes, scales)
+    if N > MAX_N or K > MAX_K:
+        raise ValueError(f"a weight of at most {MAX_N} x {MAX_K}, got {N} x {K}")
+    return N, K
+
+
+def _check_activations(activations):
+    if activations not in ("bf16", "mxfp4"):
+        raise ValueError(f"activations must be 'bf16' or 'mxfp4', got {activations!r}")
+
+
 class MXFP4Weight:
     """A projection weight [N, K] in microscaled 4 bits: `codes` and `scales` as they were given, and
     `packed`, the copy that fused.linear streams (coopt_mxfp4_pack_weight's layout; it does not see
@@ -99,8 +114,17 @@ class MXFP4Weight:
     both operands go to the scaled matrix instructions (4 bits by 4 bits)."""
 
     def __init__(self, codes, scales, packed, activations="bf16"):
+        _check_activations(activations)
+        N, K = _check_weight(codes, scales)
+        if not codes.device == scales.device == packed.device:
+            raise ValueError(f"codes, scales and packed on {codes.device}, {scales.device}, {packed.device}: one device "
+                             "is needed")
+        size = int(_lib.entry("coopt_mxfp4_packed_bytes")(N, K))   # the kernels read all of it
+        if packed.dtype is not torch.uint8 or packed.numel() != size or not packed.is_contiguous() or \
+                packed.data_ptr() % 16:
+            raise ValueError(f"packed must be {size} contiguous bytes (uint8), 16-byte aligned")
         self.codes, self.scales, self.packed, self.activations = codes, scales, packed, activations
-        self.shape = torch.Size((codes.shape[0], 2 * codes.shape[1]))
+        self.shape = torch.Size((N, K))
         self.act4 = 1 if activations == "mxfp4" else 0
         self._plans = {}   # rows: what plan() returns, a pure function of the sizes
 
@@ -138,17 +162,11 @@ class MXFP4Weight:
 
 def pack_mxfp4_weight(codes, scales, activations="bf16"):
     """MXFP4Weight of codes [N, K / 2] and scales [N, K / 32] on the GPU: one launch at model load."""
-    if activations not in ("bf16", "mxfp4"):
-        raise ValueError(f"activations must be 'bf16' or 'mxfp4', got {activations!r}")
+    _check_activations(activations)
     index = codes.get_device()
     if index < 0 or index != scales.get_device():
         _lib.require_one_device(codes, scales)
-    if codes.dim() != 2:
-        raise ValueError(f"codes must be [N, K / 2], got {tuple(codes.shape)}")
-    K = _check_rows(codes, scales)
-    N = codes.shape[0]
-    if N > MAX_N or K > MAX_K:
-        raise ValueError(f"a weight of at most {MAX_N} x {MAX_K}, got {N} x {K}")
+    N, K = _check_weight(codes, scales)
     cc, sc = _aligned(codes, 16), scales.contiguous()
     nbytes = int(_lib.entry("coopt_mxfp4_packed_bytes")(N, K))
     packed = cc.new_empty(nbytes)

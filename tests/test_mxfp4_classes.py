@@ -1,4 +1,5 @@
-"""CPU: weights and partial sums of derived classes are taken as what they are."""
+"""CPU: weights and partial sums of derived classes are taken as what they are, and a weight's parts are held against
+one another."""
 import pytest
 import torch
 
@@ -24,3 +25,24 @@ def test_derived_classes():
     part = Partials(u8(4 * 16 * 64), 1, 2, 16, 64, torch.Size((2, 64)), torch.device("cpu"))
     with pytest.raises(_lib.CooptError, match="no CPU fallback"):
         fused.residual_norm(part, bf(2, 64), bf(64), 1e-5)
+
+
+def test_weights_refuse_parts_that_do_not_belong_together():
+    """The kernels read `packed` by the sizes of codes: a smaller one would be read past its end."""
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)
+    size = _lib.load().coopt_mxfp4_packed_bytes
+    assert size(16, 32) == 8704
+    MXFP4Weight(u8(16, 16), u8(16, 1), u8(8704))
+    MXFP4Weight(u8(0, 16), u8(0, 1), u8(0))
+    for codes, scales, packed, what in (
+            (u8(32, 16), u8(32, 1), u8(8700), "packed"), (u8(33, 16), u8(33, 1), u8(8704), "packed"),
+            (u8(16, 272), u8(16, 17), u8(8704), "packed"), (u8(16, 16), u8(16, 1), u8(8704).float(), "packed"),
+            (u8(16, 16), u8(16, 1), u8(2 * 8704)[::2], "packed"), (u8(16, 16), u8(16, 1), u8(8705)[1:], "packed"),
+            (u8(16, 16), u8(16, 2), u8(8704), "disagree"), (u8(16, 16), u8(8, 1), u8(8704), "disagree"),
+            (u8(16), u8(1), u8(8704), "must be .N, K / 2."), (u8(16, 16).int(), u8(16, 1), u8(8704), "uint8")):
+        with pytest.raises(ValueError, match=what):
+            MXFP4Weight(codes, scales, packed)
+    with pytest.raises(ValueError, match="activations"):
+        MXFP4Weight(u8(16, 16), u8(16, 1), u8(8704), "fp8")
+    with pytest.raises(ValueError, match="one device"):
+        MXFP4Weight(u8(16, 16), u8(16, 1), u8(8704).to("meta"))
