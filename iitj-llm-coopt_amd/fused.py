@@ -111,7 +111,7 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
     residual, which rounds r and the normed values on its way.
 
     x [..., H] bf16 or the LinearPartials of the projection that made it (summed here), residual of its
-    shape; gate [H], or of x's shape (rows may be strided); H a multiple of 8 up to 16384.  residual_out: where r
+    shape; gate [H], or of x's shape (any strides); H a multiple of 8 up to 16384.  residual_out: where r
     goes, by default into `residual`.  Returns out (a new tensor by default).  out may be x, residual (with another
     residual_out) or a gate of x's shape itself, and overlaps no input otherwise; nor does residual_out."""
     part = x if isinstance(x, LinearPartials) else None
@@ -150,6 +150,9 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
         elif not gate.is_contiguous():
             gate = gate.contiguous()
         gp = gate.data_ptr()
+        if gp % 16:   # a copy, as of rows that are not strided in whole 16 bytes
+            gate = gate.clone(memory_format=torch.contiguous_format)
+            gp, gate_stride = gate.data_ptr(), H if rows_of else 0
     for name, t in (("out", out), ("residual_out", residual_out)):
         if t is not None:
             if t.dtype is not torch.bfloat16 or t.shape != shape or not t.is_contiguous():
