@@ -170,8 +170,8 @@ def residual_norm(x, residual, weight, eps, post_weight=None, gate=None, branch_
     rc = _lib.call_on(
         index, _lib.entry("coopt_residual_norm"), x.data_ptr() if part is None else 0,
         0 if part is None else source.data_ptr(), 0 if part is None else part.ks,
-        0 if part is None else part.rows_padded * part.n, rp, sp, pp, gp, gate_stride, weight.data_ptr(), op, rows, H,
-        float(eps), float(branch_scale), float(residual_scale), _lib.raw_stream(index))
+        0 if part is None else part.rows_padded * part.n, rp, sp, pp, gp, gate_stride, weight.data_ptr(), op, rows, H, eps,
+        branch_scale, residual_scale, _lib.raw_stream(index))
     if rc:
         _lib.check(rc, "coopt_residual_norm")
     return out

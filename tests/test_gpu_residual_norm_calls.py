@@ -27,13 +27,3 @@ def test_gates_at_any_offset(dev, kind, off):
         other = torch.empty_like(residual)
         got = fused.residual_norm(x, residual, weight, 1e-5, pw, gate, residual_out=other)
         assert torch.equal(got, want) and torch.equal(other, new)
-
-
-@pytest.mark.parametrize("number", [np.float32, np.float64, torch.tensor], ids=["float32", "float64", "tensor"])
-def test_numbers_of_any_kind(dev, number):
-    """eps and the scales as NumPy numbers or tensors, as rms_norm takes its eps."""
-    x, residual, weight, pw, gv = inputs(dev, 3, 64, "channel", True)
-    new = [torch.empty_like(residual) for _ in range(2)]
-    want = fused.residual_norm(x, residual, weight, 2.0 ** -17, pw, gv, 0.25, 1.5, residual_out=new[0])
-    got = fused.residual_norm(x, residual, weight, number(2.0 ** -17), pw, gv, number(0.25), number(1.5), residual_out=new[1])
-    assert torch.equal(got, want) and torch.equal(*new)
