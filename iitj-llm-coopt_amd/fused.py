@@ -196,7 +196,7 @@ def rope_(q, k, positions, cos, sin):
 
 
 def silu_and_mul(gate_up, out=None):
-    """[T, 2F] -> [T, F]: silu(gate) * up.  gate_up may be a LinearPartials (the split-K output
+    """[..., 2F] -> [..., F]: silu(gate) * up.  gate_up may be a LinearPartials (the split-K output
     of linear(..., defer_reduce=True)), reduced in the same pass."""
     if isinstance(gate_up, LinearPartials):
         xp = gate_up
@@ -214,9 +214,10 @@ def silu_and_mul(gate_up, out=None):
     _bf16_rows(gate_up, "gate_up")
     if not gate_up.is_contiguous():
         raise ValueError("gate_up must be contiguous")
-    T, F2 = gate_up.shape
+    F2 = gate_up.shape[-1]
+    T = gate_up.numel() // F2 if F2 else 0
     if out is None:
-        out = torch.empty((T, F2 // 2), dtype=gate_up.dtype, device=gate_up.device)
+        out = torch.empty((*gate_up.shape[:-1], F2 // 2), dtype=gate_up.dtype, device=gate_up.device)
     _lib.check(_lib.load().coopt_silu_mul(_lib.ptr(gate_up), _lib.ptr(out), T, F2 // 2,
                                           _lib.stream_handle(gate_up.device)), "coopt_silu_mul")
     return out

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import iitj_llm_coopt_amd as M
 from iitj_llm_coopt_amd import fused
 from test_gpu_mxfp4 import make_weight, small_numbers
 
@@ -56,3 +57,25 @@ def test_wide_products_feed_the_norm(dev):
     assert isinstance(part, fused.LinearPartials)
     norm = torch.ones(8320, device=dev, dtype=torch.bfloat16)
     assert torch.equal(fused.rms_norm(part, norm, 1e-5), fused.rms_norm(fused.linear(x, w), norm, 1e-5))
+
+
+@pytest.mark.parametrize("activations", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("N,K", [(128, 256), (2048, 8192)])
+def test_linear_silu_of_any_shape(dev, N, K, activations):
+    """Rows in one, two and three dimensions, whether the product leaves sums behind or not."""
+    w, _ = make_weight(dev, N, K, 6, activations, integers=True)
+    x = small_numbers(dev, (20, K), 6)
+    want = fused.silu_and_mul(fused.linear(x, w))
+    assert torch.equal(fused.linear_silu(x, w), want)
+    assert torch.equal(fused.linear_silu(x.view(4, 5, K), w), want.view(4, 5, N // 2))
+    assert torch.equal(fused.linear_silu(x[3], w), fused.linear_silu(x[3:4], w)[0])
+    assert torch.equal(fused.silu_and_mul(fused.linear(x, w).view(4, 5, N)), want.view(4, 5, N // 2))
+    assert fused.linear_silu(x[:0], w).shape == (0, N // 2)
+
+
+def test_derived_weights(dev):
+    class Weight(M.MXFP4Weight):
+        pass
+    w, _ = make_weight(dev, 64, 256, 7)
+    x = small_numbers(dev, (5, 256), 7)
+    assert torch.equal(fused.linear(x, Weight(w.codes, w.scales, w.packed)), fused.linear(x, w))
