@@ -330,7 +330,7 @@ def linear(x, weight, out=None, defer_reduce=False):
     `weight` may be a PackedWeight: the kernel path then streams its tile-packed copy
     (coopt_linear_packed), torch's path its row-major one.
 
-    `weight` may be an MXFP4Weight (K a multiple of 32, any N and row count): coopt_mxfp4_linear, with
+    `weight` may be an MXFP4Weight (K a multiple of 32, any N, up to 2^19 rows): coopt_mxfp4_linear, with
     bf16 rows or, where the weight says activations "mxfp4", rows quantised to 4 bits in the call.
     defer_reduce returns LinearPartials where K is split (in memory of their own).  out overlaps no input."""
     if isinstance(weight, MXFP4Weight):

@@ -32,7 +32,7 @@ from .batch import row_slots
 from .fused import (LinearPartials, linear, linear_silu, pack_gate_up_weight, pack_linear_weight,
                     residual_norm, rms_norm, rope_,
                     row_major, silu_and_mul)
-from .mxfp4 import MXFP4Weight, quantize_mxfp4_weight
+from .mxfp4 import MAX_ROWS, MXFP4Weight, quantize_mxfp4_weight
 from .kv_cache import (allocate_kv_cache, qkv_norm_rope_and_cache, qkv_rope_and_cache,
                        reshape_and_cache_flash)
 from .spec_decode import AcceptResult, accept
@@ -636,9 +636,14 @@ class SpecDecoder:
         return self._prompt_linear(h, model.lm_head)
 
     def _prompt_linear(self, x, weight):
-        if isinstance(weight, MXFP4Weight):
+        if not isinstance(weight, MXFP4Weight):
+            return F.linear(x, row_major(weight))
+        if x.shape[0] <= MAX_ROWS:
             return self.ops.linear(x, weight)
-        return F.linear(x, row_major(weight))
+        out = x.new_empty(x.shape[0], weight.shape[0])
+        for i in range(0, x.shape[0], MAX_ROWS):   # a product takes no more rows
+            self.ops.linear(x[i:i + MAX_ROWS], weight, out=out[i:i + MAX_ROWS])
+        return out
 
     # ---- buckets ----------------------------------------------------------------------
     def bucket(self):
