@@ -732,7 +732,6 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
       if (ks > 1) us += (partials ? 0.8f : 2.2f) + 0.7e-6f * ks * M * static_cast<float>(p.pitch);
       if (us < best) {
         best = us;
-        q.tile = t;
         p.tile = t;
         p.ks = q.ks;
         p.slice_quads = q.slice_quads;
