@@ -1,11 +1,11 @@
 // Products with microscaled 4-bit weights: Y[M, N] = X[M, K] W[N, K]^T, bf16 out, fp32 accumulation.
 // W is packed (mxfp4.h); X is bf16 (A4 = false) or quantised in the call to the same 4-bit format (A4 = true).
 //
-// A4 = false.  A weight is a bf16 number (scale bytes up to 252, mxfp4.h), so the product is exactly that of the
-// bf16 matrix instructions on code * 2^e: a lane's 16 bytes of a tile are 32 elements of one row and one block, four operands of
-// v_mfma_f32_16x16x32_bf16 after 16 v_cvt_scalef32_pk_bf16_fp4 (two elements each, scale applied).  The K
-// order inside a step is any that both operands share: operand j of lane (row, g) holds elements
-// 32 g + 8 j .. + 7 of the step.
+// A4 = false.  A weight is a bf16 number (scale bytes up to 252, mxfp4.h), so the product is exactly that of the bf16
+// matrix instructions on code * 2^e: a lane's 16 bytes of a tile are 32 elements of one row and one block, four
+// operands of v_mfma_f32_16x16x32_bf16 after 16 v_cvt_scalef32_pk_bf16_fp4 (two elements each, scale applied).  The K
+// order inside a step is any that both operands share: operand j of lane (row, g) holds elements 32 g + 8 j .. + 7 of
+// the step.
 // A4 = true.  A lane's 16 bytes are its operand of v_mfma_scale_f32_16x16x128_f8f6f4 as they are, with
 // their scale bytes: products and sums of a step are formed by the matrix core.
 // In both the weight is the A operand, so a lane ends with four consecutive outputs of one row.
@@ -299,7 +299,7 @@ constexpr int kMostTiles = 10;   // row tiles of a block of 4-bit rows, at most
 // it.  Every wave loads its weight tiles straight into registers, 512 elements ahead, and with bf16 rows converts
 // an operand while the one before it is multiplied.  LDS reads and stores, loads and conversions lie among the
 // products (spread): with those of X together behind the barrier, no wave multiplied meanwhile, 41 us for 38.7 at
-// 160 x 28672 x 4096, 165 for 162 at 2000 x 4096 x 14336 (1.45 PFLOP/s).
+// 160 x 28672 x 4096, 165 for 162 at 2000 x 4096 x 14336 (a call of that takes 166, 1.41 PFLOP/s).
 //
 // With 4-bit rows a block takes the tiles blockIdx.x, blockIdx.x + gridDim.x, ... .  Loads run into the next tile (its
 // first stages behind this one's last), so that between tiles nothing waits but the stores: 4093 x 28672 x 4096, 14
@@ -635,9 +635,12 @@ __global__ __launch_bounds__(256) void mxfp4_reduce_kernel(const float* __restri
 }
 
 // ---- which kernel ------------------------------------------------------------------------------
-// Tile kernels, smallest first: MT, NT, WM, WN; us before the first and behind the last product; us a stage with a block
-// on every CU (bf16 rows; a stage of 512 elements of 4-bit ones).  Fitted to 32 to 4093 rows of 4096, 6144, 16384 and 28672
-// columns, K = 2048 to 14336, where the tile and split chosen take at most 8 % more than the best measured.
+// Tile kernels, smallest first: MT, NT, WM, WN; us before the first and behind the last product; us a stage with a
+// block on every CU (bf16 rows; a stage of 512 elements of 4-bit ones).  Every tile and split of 20 to 4093 rows of
+// seven sizes from 2048 x 2048 to 28672 x 4096 was timed in a graph, with the launch that adds slices.  bf16 rows: in
+// 93 of 98 products the choice takes at most 8 % more than the best measured, at worst 26.9 us for 21.7 (512 x 2048 x
+// 8192).  4-bit rows: in 35 of 77, the median 11 % more, at worst 19.5 us for 14.1 (the same size): the four-wave
+// tile of 80 rows is rated too dear, 11.1 us chosen for its 9.4 at 160 x 4096 x 4096.
 struct TileConfig {
   int mt, nt, wm, wn;
   float start, us, us4;
@@ -665,9 +668,13 @@ void split_k(Plan& p, int quads, int ks) {
   p.ks = (quads + p.slice_quads - 1) / p.slice_quads;
 }
 
-// Whether the stream kernel quantises X itself.  us, it / packed without the 2 us and the host's 3 of the launch that
-// packs: 16 rows of 4096 x 4096 6.5 / 3.4 (for a consumer 4.7 / 3.4), of 2048 x 8192 10.4 / 3.5 (5.2 / 3.5), of
-// 28672 x 4096 17.5 / 12.4, of 4096 x 14336 16.9 / 7.4; one row of that 10.1 / 7.3.
+// Whether the stream kernel quantises X itself.  us in a graph, it / with the launch that packs (3 us more of the host's
+// time where there is no graph): one row of 4096 x 4096 4.7 / 6.0, of 16384 x 2048 6.5 / 7.9, of 4096 x 14336
+// 10.9 / 10.3, of 28672 x 4096 17.6 / 15.1, of 128256 x 4096 61 / 46; 8 rows 5.8 / 5.8, 7.0 / 7.4, 13.6 / 10.4,
+// 16.2 / 15.3, 52 / 49; 16 rows of 2048 x 2048 4.7 / 4.9, of 4096 x 4096 7.1 / 5.9, of 4096 x 14336 18.5 / 10.7, of
+// 28672 x 4096 18.6 / 15.6; for a consumer that adds slices, 16 of 2048 x 8192 5.2 / 3.5 and the launch's 2.  Each block of
+// columns quantises the rows again, so that the widest and longest weights lose by the rule for up to eight rows,
+// which does not look at them.
 bool in_kernel(int M, int ntiles, int quads, bool partials) {
   return M <= 8 || (M <= 16 && ntiles <= 1024 && quads <= (partials ? 16 : 8));
 }
@@ -683,10 +690,11 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
   p.rows_padded = mtiles * 16;
   p.pitch = ntiles * 16;
   if (mtiles <= (a4 ? 4 : 1)) {
-    // Stream kernel.  Blocks enough for every CU first, then column tiles, for which X is read once.  us, NT = 1, 2, 4:
-    // 16 bf16 rows of 4096 x 4096 6.3, 6.9, 8.1, of 6144 x 4096 8.4, 7.3, 8.1, of 28672 x 4096 35, 23.3, 18.7 (one row 14.5,
-    // 13.7, 14.4); packed ones of 4096 x 4096 3.4, 3.8, 6.6; 32 of 16384 x 2048 5.9, 5.6, 7.1; 64 of 28672 x 4096 21.5, 16.7,
-    // 15.9.  Eight waves where each has a quad.
+    // Stream kernel.  Blocks enough for every CU first, then column tiles, for which X is read once.  us in a graph,
+    // NT = 1, 2, 4: 16 bf16 rows of 4096 x 4096 6.6, 7.2, 8.6, of 6144 x 4096 10.4, 7.8, 9.0, of 28672 x 4096 32,
+    // 25.5, 19.7; 5 rows of that 19.3, 18.5, 16.2; one 17.4, 17.1, 15.3, of 128256 x 4096 64, 57, 48 (up to four rows
+    // take NT = 2 there).  Packed: 16 rows of 4096 x 4096 3.9, 4.3, 32 of 16384 x 2048 6.6, 6.2, 64 of 28672 x 4096
+    // 24.5, 19.2, 17.0.  Eight waves where each has a quad.
     p.stream = true;
     p.x = !a4 ? kRows : in_kernel(M, ntiles, quads, partials) ? kQuantize : kPacked;
     p.mt = mtiles <= 2 ? mtiles : 4;
@@ -700,9 +708,10 @@ Plan plan_for(int M, int N, int K, bool a4, bool partials) {
       if (partials)
         while (ks < 4 && ks * 2 * p.kw <= quads && 2 * ks * blocks() <= 512) ks *= 2;
     } else if (partials || (M > 8 && quads >= 16 && ntiles < 1024)) {
-      // Slices instead of waves, and the tiles that leave blocks enough.  us for a consumer, against one slice: 5 rows of
-      // 4096 x 14336 8.9 / 10.1, of 6144 x 4096 4.9 / 5.3, 16 of 4096 x 4096 4.8 / 6.3, of 2048 x 8192 5.2 / 9.7, of 4096 x 14336
-      // 11.1 / 16.2 (for these two a launch that adds them pays as well).
+      // Slices instead of waves, and the tiles that leave blocks enough.  us for a consumer, against one slice: one
+      // row of 4096 x 4096 4.5 / 4.3, of 2048 x 8192 4.3 / 5.1, 5 rows of 4096 x 14336 9.8 / 11.1, of 6144 x 4096 5.4
+      // / 5.8, 16 of 4096 x 4096 5.4 / 6.8, of 2048 x 8192 5.7 / 10.3, of 4096 x 14336 11.9 / 17.6 (for these two a
+      // launch that adds them pays as well: 7.7, 14.0).
       p.nt = M > 8 ? (ntiles >= 256 ? 4 : ntiles >= 128 ? 2 : 1) : ntiles >= 192 ? 2 : 1;
       p.kw = 4;
       while (ks < 4 && ks * 4 <= quads && ks * blocks() < (M > 8 ? 256 : 512)) ks *= 2;

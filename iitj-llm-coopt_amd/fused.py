@@ -43,8 +43,8 @@ def _bf16_rows(t, name):
 class LinearPartials:
     """The unreduced output of linear(..., defer_reduce=True): `ks` fp32 slices of shape
     [rows_padded, N] in the linear workspace whose sum is the layer's output.  It is valid
-    until the next linear() call on the same stream (which reuses the workspace); rms_norm()
-    and silu_and_mul() reduce it while reading."""
+    until the next linear() call on the same stream (which reuses the workspace; those of an MXFP4Weight
+    have memory of their own); rms_norm(), residual_norm() and silu_and_mul() reduce it while reading."""
 
     def __init__(self, buf, ks, rows, rows_padded, n, shape, device):
         self.buf, self.ks, self.rows, self.rows_padded, self.n = buf, ks, rows, rows_padded, n
