@@ -99,7 +99,7 @@ def test_weights_past_bf16(dev, m, s, activations):
     vals = reference_values(code, sc)
     past = np.abs(vals[:, 0]) >= 2.0 ** 128
     assert past.sum() == {252: 0, 253: 8, 254: 16}[s]
-    as_bf16 = np.where(np.abs(vals) >= 2.0 ** 128, np.sign(vals) * np.inf, vals)
+    as_bf16 = np.where(np.abs(vals) >= 2.0 ** 128, np.copysign(np.inf, vals), vals)
     assert np.array_equal(w.dequantize().double().cpu().numpy(), as_bf16)
     got = fused.linear(torch.full((m, K), 2.0 ** -120, device=dev, dtype=torch.bfloat16), w).double().cpu().numpy()
     want = 2.0 ** -120 * K * (as_bf16 if activations == "bf16" else vals)[:, 0]
